@@ -184,6 +184,132 @@ int mxh_gemm_q_f16_noalloc(int type, const float *a, int64_t m, const void *w, i
 int mxh_attention_prefill(const float *q, const void *kc, const void *vc, float *att, int p0, int m, int nh, int nkv,
                           int hd);
 
+/* ---- paged K/V cache ----------------------------------------------------- */
+/* For runtimes that serve several sequences, fork them, or verify drafted
+ * tokens: K and V in pages of a pool, packed batches of tokens, and what fills,
+ * reads and moves the rows.  The reference has one contiguous cache per context
+ * (src/cache/kv_cache.cpp:50-75) and one sequence; the arithmetic per token is
+ * that of its layer (transformer.cpp:189-214, 529-629, rope.cpp:6-57).
+ * Everything here runs on the library stream, in order; nothing allocates,
+ * synchronizes or keeps state between calls, so every call may be recorded in
+ * a HIP graph and replayed (device arrays are read when the graph runs, host
+ * arrays when the call is made). */
+
+/* K and V in HBM: fp16, [n_layer][n_pages][page_rows][n_kv * head_dim] each,
+ * layer_stride elements from one layer to the next (0: dense).  page_rows a
+ * power of two from 16 to 1024; head_dim 32, 64 or 128; k and v 16-byte
+ * aligned, layer_stride a multiple of 8. */
+typedef struct {
+    void *k, *v;
+    int64_t layer_stride;
+    int n_layer, n_pages, page_rows, n_kv, head_dim;
+} mxh_kv_pool;
+
+/* A step's packed tokens.  Sequence s (0 .. n_seq-1, n_seq up to 4096) has the
+ * rows start[s] .. start[s+1]-1 of the token arrays (none: start[s+1] ==
+ * start[s]) and cached[s] rows in the cache before them; its i-th new token
+ * belongs in cache row cached[s] + i.  Cache row r of a sequence is row
+ * r % page_rows of page table[s * table_ld + r / page_rows].  parent[t] is the
+ * index, within its sequence's new tokens, of the token that t was drafted
+ * after (smaller than its own; -1: the last cached token), at most 64 new
+ * tokens a sequence; parent NULL: every token follows the one before it, any
+ * number of them.  The arrays are device memory that no call checks on the
+ * host, but no value in them makes a kernel leave the pool or the token
+ * arrays: rows of a page id outside 0 .. n_pages-1 or past table_ld are absent
+ * (never attended, never written), a parent that is not smaller than its token
+ * counts as -1, tokens past the 64th of a drafted tree and token rows outside
+ * start[0] .. start[n_seq]-1 or past n_tokens are left alone, lengths below
+ * zero count as zero.  start must not decrease. */
+typedef struct {
+    int n_seq, n_tokens;
+    const int *start;  /* [n_seq + 1] */
+    const int *cached; /* [n_seq] */
+    const int *table;  /* [n_seq][table_ld] */
+    int table_ld;
+    const int *parent; /* [n_tokens] or NULL */
+} mxh_kv_batch;
+
+/* From the projections of a batch's tokens, rows of [q | k | v] with ld floats
+ * from one to the next (nh + 2 n_kv heads): adds bias (that width, or NULL);
+ * norms every head of q and k, v / sqrt(mean(v^2) + eps) * w, with q_norm /
+ * k_norm (head_dim floats; NULL: no norm); rotates them to their positions;
+ * writes q as fp32 rows [n_tokens][nh * head_dim] and rounds k and v to fp16
+ * into the tokens' cache rows of `layer`.  A token's position is cached[s] plus
+ * the number of new tokens it follows (with parents: its ancestors).  Pair i
+ * turns by position * inv_freq[i] (head_dim / 2 doubles on the device,
+ * theta^(-2 i / head_dim) as rope.cpp:6-57 has them, or scaled ones); pairs are
+ * (2i, 2i+1), with neox (i, i + head_dim / 2).  Sums of squares, angles and the
+ * rotation are in double.  qkv, q, bias and norm weights 16-byte aligned, ld a
+ * multiple of 4; q must not overlap qkv; nh a multiple of n_kv, at most 8 per
+ * kv head.  Sequences whose new rows lie in the same page row race. */
+int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const float *qkv, int64_t ld,
+                       const float *bias, const float *q_norm, const float *k_norm, float eps, const double *inv_freq,
+                       int neox, int nh, float *q);
+
+/* Attention of a batch's tokens (q: [n_tokens][nh * head_dim] fp32, as
+ * mxh_qk_rope_append leaves it) over the paged cache of `layer`: softmax of
+ * q.k / sqrt(head_dim) over the cached rows of the token's sequence, the rows
+ * of the new tokens it follows and its own (all already in the cache), then
+ * the weighted sum of V rows into att, same shape as q.  What a token does not
+ * attend has no effect on it, infinities and NaN included; a token none of
+ * whose rows exist gets zeros.  Takes whole prompts, single tokens and drafted
+ * trees, mixed as they come.  Long rows of keys are split among workgroups,
+ * their parts in `work`: mxh_attention_paged_workspace sets *bytes to what a
+ * batch of this n_seq, n_tokens and table_ld needs at most, whatever its
+ * device arrays hold.  Calls that may run at the same time (a replayed graph
+ * beside the library stream) need work of their own.  q, att and work 16-byte
+ * aligned, not overlapping; nh as above. */
+int mxh_attention_paged(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const float *q, int nh,
+                        float *att, void *work, size_t work_bytes);
+int mxh_attention_paged_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, int nh, size_t *bytes);
+
+/* Copies page src[i] to page dst[i], K and V, in every layer (what a fork
+ * needs before both sequences write the page they share).  Host arrays; page
+ * ids in range, every dst once and no dst among the src, or MXH_ERR_ARG. */
+int mxh_kv_copy_pages(const mxh_kv_pool *pool, const int *src, const int *dst, int n);
+
+/* After the drafted tokens of a step were verified: moves the accepted rows of
+ * every sequence together, K and V, in every layer.  Sequence s keeps the new
+ * tokens keep[keep_start[s]] < ... < keep[keep_start[s+1] - 1] (indices within
+ * its new tokens); their cache rows move to rows cached[s], cached[s] + 1, ...
+ * Host arrays (table [n_seq][table_ld] as in mxh_kv_batch); kept indices
+ * ascending from 0 on, their rows in pages of the pool, and no row written
+ * that another move reads or writes, or MXH_ERR_ARG. */
+int mxh_kv_keep_rows(const mxh_kv_pool *pool, const int *table, int table_ld, const int *cached,
+                     const int *keep_start, const int *keep, int n_seq);
+
+/* The pages of a pool and who holds them (host memory only; works without a
+ * GPU).  A sequence is a list of pages and a length in rows; a forked sequence
+ * shares its parent's pages until one of them writes there.  Sequence ids are
+ * reused after mxh_pages_close. */
+typedef struct mxh_pages mxh_pages;
+int mxh_pages_create(int n_pages, int page_rows, int max_seqs, mxh_pages **out);
+void mxh_pages_destroy(mxh_pages *p);
+/* A new sequence of no rows. */
+int mxh_pages_open(mxh_pages *p, int *seq);
+/* A new sequence with the rows of `seq`, in the same pages. */
+int mxh_pages_fork(mxh_pages *p, int seq, int *child);
+/* Gives the sequence's pages back (those that no other sequence holds become free). */
+int mxh_pages_close(mxh_pages *p, int seq);
+/* Makes the `rows` rows behind the sequence's length its own to write.  Where
+ * the first of them lies in a page that another sequence also holds, a free
+ * page takes its place: *copies is then 1 and the caller copies page *src to
+ * *dst (mxh_kv_copy_pages) before it writes; otherwise *copies is 0.  On
+ * MXH_ERR_OOM (not enough free pages) nothing has changed. */
+int mxh_pages_extend(mxh_pages *p, int seq, int rows, int *src, int *dst, int *copies);
+/* Sets the sequence's length: fewer rows than it has (truncation), or more, up
+ * to those that the last mxh_pages_extend made (what a step wrote or kept).
+ * Pages behind the new length are given back. */
+int mxh_pages_set_length(mxh_pages *p, int seq, int rows);
+/* Rows of a sequence (MXH_ERR_ARG: no such sequence). */
+int mxh_pages_length(const mxh_pages *p, int seq);
+/* Pages that no sequence holds. */
+int mxh_pages_free(const mxh_pages *p);
+/* The batch's table and cached arrays (host): row i of `table` gets the page
+ * ids of sequence seqs[i], -1 behind them, and cached[i] its length (cached may
+ * be NULL).  MXH_ERR_ARG where one has more than table_ld pages. */
+int mxh_pages_table(const mxh_pages *p, const int *seqs, int n, int *table, int table_ld, int *cached);
+
 /* ---- per-op backend interface (host pointers) ------------------------- */
 /* These keep the reference op semantics for drop-in use: host pointers in
  * and out, one synchronous device round trip per call.  Quantized weights

@@ -53,6 +53,32 @@ class SynthArch(C.Structure):
                                        "ffn_down_type")]
 
 
+class KvPool(C.Structure):
+    """K and V pages in HBM (mxh_kv_pool): fp16, [n_layer][n_pages][page_rows][n_kv * head_dim] each, by address."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("layer_stride", C.c_int64)] + \
+               [(n, C.c_int) for n in ("n_layer", "n_pages", "page_rows", "n_kv", "head_dim")]
+
+    def __init__(self, k, v, *, n_layer: int, n_pages: int, page_rows: int, n_kv: int, head_dim: int,
+                 layer_stride: int = 0):
+        super().__init__(addr(k), addr(v), layer_stride, n_layer, n_pages, page_rows, n_kv, head_dim)
+
+
+class KvBatch(C.Structure):
+    """A step's packed tokens (mxh_kv_batch); int32 device arrays, by buffer or address."""
+
+    _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("start", C.c_void_p), ("cached", C.c_void_p),
+                ("table", C.c_void_p), ("table_ld", C.c_int), ("parent", C.c_void_p)]
+
+    def __init__(self, n_seq: int, n_tokens: int, start, cached, table, table_ld: int, parent=None):
+        super().__init__(n_seq, n_tokens, addr(start), addr(cached), addr(table), table_ld, addr(parent))
+
+
+def addr(b):
+    """The device address of a DeviceBuffer, or an address as it is (None: null)."""
+    return b.ptr if isinstance(b, DeviceBuffer) else b
+
+
 MODEL_ROPE_NEOX, MODEL_GGML_FORM, MODEL_NO_QK_NORM, MODEL_NO_GRAPH, MODEL_TOKEN_PREFILL, MODEL_GGUF_LAYOUT = 1, 4, 8, 16, 32, 64
 TILED_FLAG = 0x100
 MODEL_BF16_PREFILL = 128
@@ -109,6 +135,21 @@ def _load() -> C.CDLL:
         "mxh_model_set_token": (ip, [vp, ip]),
         "mxh_model_bench_gemv": (ip, [vp, ip, ip, C.POINTER(C.c_float), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
         "mxh_model_bench_attention": (ip, [vp, ip, C.POINTER(C.c_float), C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
+        "mxh_qk_rope_append": (ip, [vp, ip, vp, vp, i64, vp, vp, vp, C.c_float, vp, ip, ip, vp]),
+        "mxh_attention_paged": (ip, [vp, ip, vp, vp, ip, vp, vp, sz]),
+        "mxh_attention_paged_workspace": (ip, [vp, vp, ip, C.POINTER(sz)]),
+        "mxh_kv_copy_pages": (ip, [vp, vp, vp, ip]),
+        "mxh_kv_keep_rows": (ip, [vp, vp, ip, vp, vp, vp, ip]),
+        "mxh_pages_create": (ip, [ip, ip, ip, C.POINTER(vp)]),
+        "mxh_pages_destroy": (None, [vp]),
+        "mxh_pages_open": (ip, [vp, C.POINTER(C.c_int)]),
+        "mxh_pages_fork": (ip, [vp, ip, C.POINTER(C.c_int)]),
+        "mxh_pages_close": (ip, [vp, ip]),
+        "mxh_pages_extend": (ip, [vp, ip, ip, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int)]),
+        "mxh_pages_set_length": (ip, [vp, ip, ip]),
+        "mxh_pages_length": (ip, [vp, ip]),
+        "mxh_pages_free": (ip, [vp]),
+        "mxh_pages_table": (ip, [vp, vp, ip, vp, ip, vp]),
         "mxh_write_synthetic_gguf": (ip, [C.c_char_p, C.POINTER(SynthArch), C.c_uint64, ip]),
     }
     for name, (res, args) in sig.items():
@@ -125,7 +166,10 @@ EXPORTED = (
     "mxh_release_resources mxh_host_matmul_rhs_t mxh_host_matmul_f32 mxh_host_matmul_q mxh_host_matvec_strided "
     "mxh_host_vec_dot_rows mxh_host_vec_dot_rows_ring mxh_host_vec_mul_rows_cols mxh_model_open "
     "mxh_model_config_get mxh_model_reset mxh_model_position mxh_model_step mxh_model_prefill mxh_model_set_sampling mxh_model_set_logit_edits mxh_sample mxh_model_generate mxh_model_close "
-    "mxh_write_synthetic_gguf mxh_model_decode mxh_model_set_token mxh_model_bench_gemv mxh_model_bench_attention"
+    "mxh_write_synthetic_gguf mxh_model_decode mxh_model_set_token mxh_model_bench_gemv mxh_model_bench_attention "
+    "mxh_qk_rope_append mxh_attention_paged mxh_attention_paged_workspace mxh_kv_copy_pages mxh_kv_keep_rows "
+    "mxh_pages_create mxh_pages_destroy mxh_pages_open mxh_pages_fork mxh_pages_close mxh_pages_extend "
+    "mxh_pages_set_length mxh_pages_length mxh_pages_free mxh_pages_table"
 ).split()
 
 
@@ -224,6 +268,115 @@ def attention_prefill(q: DeviceBuffer, kc: DeviceBuffer, vc: DeviceBuffer, att: 
                       nh: int, nkv: int, hd: int) -> None:
     """Causal attention of m prompt tokens at positions p0.. over the fp16 K/V cache (matrix cores)."""
     check(lib.mxh_attention_prefill(q.ptr, kc.ptr, vc.ptr, att.ptr, p0, m, nh, nkv, hd), "mxh_attention_prefill")
+
+
+def qk_rope_append(pool: KvPool, layer: int, batch: KvBatch, qkv, ld: int, bias, q_norm, k_norm, eps: float, inv_freq,
+                   neox: bool, nh: int, q) -> None:
+    """Bias, norms of q and k, rotation to the tokens' positions; q to fp32 rows, k and v to their cache rows."""
+    check(lib.mxh_qk_rope_append(C.byref(pool), layer, C.byref(batch), addr(qkv), ld, addr(bias), addr(q_norm),
+                                 addr(k_norm), eps, addr(inv_freq), int(neox), nh, addr(q)), "mxh_qk_rope_append")
+
+
+def attention_paged_workspace(pool: KvPool, batch: KvBatch, nh: int) -> int:
+    """Bytes of work that attention_paged needs for batches of this n_seq, n_tokens and table_ld."""
+    n = C.c_size_t()
+    check(lib.mxh_attention_paged_workspace(C.byref(pool), C.byref(batch), nh, C.byref(n)),
+          "mxh_attention_paged_workspace")
+    return n.value
+
+
+def attention_paged(pool: KvPool, layer: int, batch: KvBatch, q, nh: int, att, work=None, work_bytes: int = 0) -> None:
+    """Attention of packed prompts, single tokens and drafted trees over the paged cache."""
+    check(lib.mxh_attention_paged(C.byref(pool), layer, C.byref(batch), addr(q), nh, addr(att), addr(work),
+                                  work_bytes), "mxh_attention_paged")
+
+
+def _ints(a) -> np.ndarray:
+    return np.ascontiguousarray(a, np.int32)
+
+
+def kv_copy_pages(pool: KvPool, src, dst) -> None:
+    """Pages src[i] to dst[i], K and V, in every layer."""
+    src, dst = _ints(src), _ints(dst)
+    if src.shape != dst.shape:
+        raise ValueError(f"{src.size} source pages for {dst.size}")
+    check(lib.mxh_kv_copy_pages(C.byref(pool), src.ctypes.data, dst.ctypes.data, src.size), "mxh_kv_copy_pages")
+
+
+def kv_keep_rows(pool: KvPool, table, cached, keep_start, keep) -> None:
+    """The accepted rows of every sequence's new tokens together behind its cached ones, K and V, in every layer."""
+    table, cached, keep_start, keep = _ints(table), _ints(cached), _ints(keep_start), _ints(keep)
+    n_seq = cached.size
+    if table.ndim != 2 or table.shape[0] != n_seq or keep_start.size != n_seq + 1 or \
+            (n_seq and keep.size < keep_start[-1]):
+        raise ValueError("kv_keep_rows: the arrays' sizes do not belong together")
+    check(lib.mxh_kv_keep_rows(C.byref(pool), table.ctypes.data, table.shape[1], cached.ctypes.data,
+                               keep_start.ctypes.data, keep.ctypes.data, n_seq), "mxh_kv_keep_rows")
+
+
+def rope_frequencies(theta: float, head_dim: int) -> np.ndarray:
+    """theta^(-2 i / head_dim), the double array that qk_rope_append turns by."""
+    return 1.0 / np.power(float(theta), 2.0 * np.arange(head_dim // 2) / head_dim)
+
+
+class Pages:
+    """Who holds which page of a pool (mxh_pages_*; host memory only)."""
+
+    def __init__(self, n_pages: int, page_rows: int, max_seqs: int):
+        h = C.c_void_p()
+        check(lib.mxh_pages_create(n_pages, page_rows, max_seqs, C.byref(h)), "mxh_pages_create")
+        self.h = h.value
+
+    def open(self) -> int:
+        s = C.c_int()
+        check(lib.mxh_pages_open(self.h, C.byref(s)), "mxh_pages_open")
+        return s.value
+
+    def fork(self, seq: int) -> int:
+        s = C.c_int()
+        check(lib.mxh_pages_fork(self.h, seq, C.byref(s)), "mxh_pages_fork")
+        return s.value
+
+    def release(self, seq: int) -> None:
+        """End a sequence; its pages that no other holds become free."""
+        check(lib.mxh_pages_close(self.h, seq), "mxh_pages_close")
+
+    def extend(self, seq: int, rows: int) -> list[tuple[int, int]]:
+        """Make `rows` rows behind the length writable; returns the page copies (src, dst) to do before writing."""
+        s, d, n = C.c_int(), C.c_int(), C.c_int()
+        check(lib.mxh_pages_extend(self.h, seq, rows, C.byref(s), C.byref(d), C.byref(n)), "mxh_pages_extend")
+        return [(s.value, d.value)] if n.value else []
+
+    def set_length(self, seq: int, rows: int) -> None:
+        check(lib.mxh_pages_set_length(self.h, seq, rows), "mxh_pages_set_length")
+
+    def length(self, seq: int) -> int:
+        n = lib.mxh_pages_length(self.h, seq)
+        check(min(n, 0), "mxh_pages_length")
+        return n
+
+    @property
+    def free(self) -> int:
+        return lib.mxh_pages_free(self.h)
+
+    def table(self, seqs, table_ld: int) -> tuple[np.ndarray, np.ndarray]:
+        """(page ids [n][table_ld], lengths [n]) of the sequences, for a KvBatch."""
+        seqs = _ints(seqs)
+        table, cached = np.empty((seqs.size, table_ld), np.int32), np.empty(seqs.size, np.int32)
+        check(lib.mxh_pages_table(self.h, seqs.ctypes.data, seqs.size, table.ctypes.data, table_ld,
+                                  cached.ctypes.data), "mxh_pages_table")
+        return table, cached
+
+    def close(self) -> None:
+        if self.h:
+            lib.mxh_pages_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def sample(logits: DeviceBuffer, n: int, top_k: int, temperature: float, top_p: float = 1.0, min_p: float = 0.0,
