@@ -72,15 +72,7 @@ constexpr int kThreads = 512;
 // keeps the loads of a region ahead of its arithmetic in the instruction order
 #define MXH_CODES_FENCE() __builtin_amdgcn_sched_barrier(0)
 
-// 16 bytes per lane from global memory into LDS (lane i writes lds + 16 i):
-// scalar base + lane offset, or a full lane address.  Inline assembly so that
-// the compiler does not wait for every such load before the next LDS read (it
-// cannot tell the stages apart); wait_vm waits for them.  The compiler does
-// not see a memory instruction here, so the wait states between a VALU write
-// of the base's SGPRs (5) or a write of M0 (1) and the load are in the asm.
-__device__ __forceinline__ void g2l_s(uint64_t base, uint32_t off, uint32_t lds) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
-}
+// 16 bytes per lane into LDS as g2l_s (mxh_device.h), from a full lane address
 __device__ __forceinline__ void g2l_v(const void* addr, uint32_t lds) {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(addr), "{m0}"(lds) : "memory");
 }
@@ -88,15 +80,6 @@ __device__ __forceinline__ void g2l_v(const void* addr, uint32_t lds) {
 __device__ __forceinline__ void g2l4_s(uint64_t base, uint32_t off, uint32_t lds) {
     asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
 }
-// a uniform address, held in SGPRs
-__device__ __forceinline__ uint64_t scalar_addr(const void* p) {
-    const uint64_t v = (uint64_t)p;
-    // (the builtin returns int: back to unsigned before widening)
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
-    return ((uint64_t)hi << 32) | lo;
-}
-
 template <int N>
 __device__ __forceinline__ void wait_vm() {
     static_assert(N >= 0 && N < 64, "vmcnt range");
