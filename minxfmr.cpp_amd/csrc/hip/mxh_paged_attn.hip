@@ -28,10 +28,9 @@
 //                    ds_read_b64_tr_b16
 //
 // Rows that a token does not attend must not reach it: their scores are
-// replaced, not added to, and since 0 times an infinity is none, blocks with
-// unattended rows look their V values over; where one is infinite or NaN the
-// products take the finite values alone, and two more products of 0 / 1
-// matrices tell which sums have an infinity or a NaN coming (blend_special).
+// replaced, not added to, and since 0 times an infinity is no zero, blocks with
+// unattended rows look their V values over; an item that meets an infinity or a
+// NaN there is computed again without products over such rows (redo_item).
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -49,15 +48,13 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kBlock = 32;                 // keys a wave takes at a time
-constexpr int kStage = kWaves * kBlock;    // keys a workgroup takes at a time
-constexpr int kSlots = 2;                  // blocks of a wave in LDS
+constexpr int kStage = 128;                // keys that splits are made of
+constexpr int kSlots = 2;                  // stages in LDS
 
-__host__ __device__ constexpr int slot_bytes(int hd) { return 2 * kBlock * hd * 2; }  // K and V rows
-// floats a wave leaves for the merge of one set: V sums [hd][32], references, sums
+// floats a wave leaves for the merge: V sums [hd][32], references, sums
 __host__ __device__ constexpr int merge_floats(int hd) { return hd * 32 + 64; }
 __host__ __device__ constexpr int lds_bytes(int hd, int rs) {
-    const int ring = kWaves * kSlots * slot_bytes(hd), merge = kWaves * rs * merge_floats(hd) * 4;
+    const int ring = kSlots * 2 * (kStage / rs) * hd * 2, merge = kWaves * merge_floats(hd) * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -166,95 +163,148 @@ struct AttnPagedArgs {
 // dims around in each 16 lanes.
 template <int HD>
 struct VRead {
-    uint32_t at[2][HD / 32];  // byte offsets in the V rows of a slot
+    uint32_t at;  // byte offset of t, d = 0 in the block's V rows
     __device__ __forceinline__ VRead() {
-        const int lane = threadIdx.x & 63, h = lane >> 5;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d) {
-                const int key = 8 * h + 4 * r + ((lane & 15) >> 2);
-                const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                at[r][d] = (uint32_t)(key * HD * 2 + 16 * (piece ^ v_swz(key)) + 8 * (lane & 1));
-            }
+        const int lane = threadIdx.x & 63, key = 8 * (lane >> 5) + ((lane & 15) >> 2);
+        const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        at = (uint32_t)(key * HD * 2 + 16 * (piece ^ v_swz(key)) + 8 * (lane & 1));
     }
     // pairs of 16-byte pieces rotated by the key, so that the four keys of a
     // read lie in different banks (the same for keys 16 apart)
     static __device__ __forceinline__ int v_swz(int key) {
         return HD == 128 ? 2 * (key & 7) : HD == 64 ? 2 * ((key >> 1) & 3) : 2 * ((key >> 2) & 1);
     }
+    // v0: the rows' place, a multiple of 256 bytes.  Dims 32 d on are 64 d bytes
+    // on; keys 4 on are 4 rows on, rotated by another HD bytes
     __device__ __forceinline__ f16x8 operator()(uint32_t v0, int t, int d) const {
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(v0 + at[0][d] + t * 16 * HD * 2));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(v0 + at[1][d] + t * 16 * HD * 2));
+        const uint32_t p = v0 + at;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((p ^ (64 * d)) + t * 32 * HD));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_s16x4*)(uintptr_t)(((p ^ (64 * d)) ^ HD) + t * 32 * HD + 8 * HD));
         return __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
 
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+
 // whether any V value of the block is infinite or NaN
 template <int HD>
 __device__ __forceinline__ bool any_special(uint32_t v0) {
-    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-    const int lane = threadIdx.x & 63;
-    bool bad = false;
+    uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < HD / 16; ++i) {
-        const u32x4 x = *(lds_u32x4*)(uintptr_t)(v0 + 1024 * i + 16 * lane);
+        const u32x4 x = *(lds_u32x4*)(uintptr_t)(v0 + 1024 * i + 16 * (threadIdx.x & 63));
 #pragma unroll
         for (int e = 0; e < 4; ++e) bad |= (x[e] & 0x7c00u) == 0x7c00u || (x[e] & 0x7c000000u) == 0x7c000000u;
     }
     return __any(bad);
 }
 
-// O^T += V^T P^T for one set where V has infinities or NaN: the finite values'
-// products, and +-inf / NaN into the sums of rows that attend such a value.  w:
-// this lane's row's attended keys, bit 16 t + u for key 16 t + 8 h + u.
-template <int HD>
-__device__ __forceinline__ void blend_special(const VRead<HD>& vr, uint32_t v0, uint32_t w, const f16x8 (&bh)[2],
-                                              const f16x8 (&bl)[2], f32x16 (&o)[HD / 32]) {
-    f16x8 on[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) on[t][u] = (w >> (16 * t + u)) & 1 ? (_Float16)1 : (_Float16)0;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d) {
-        f32x16 up, dn;
-#pragma unroll
-        for (int v = 0; v < 16; ++v) up[v] = dn[v] = 0.f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f16x8 a = vr(v0, t, d), pos, neg;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)a[u]);
-                const bool odd = (b & 0x7c00u) == 0x7c00u, nan = odd && (b & 0x3ffu);
-                pos[u] = nan || b == 0x7c00u ? (_Float16)1 : (_Float16)0;
-                neg[u] = nan || b == 0xfc00u ? (_Float16)1 : (_Float16)0;
-                if (odd) a[u] = (_Float16)0;
+// The item again with a wave a row and no product that meets a value its row
+// does not attend: a key a lane for the scores, then a dim a lane (or two) for
+// the sums.  For items that found such a value among rows that only some of
+// their tokens attend; the rest of the kernel pays no register for it.
+template <int HD, int RS>
+__device__ void redo_item(const AttnPagedArgs& a, const Item& it, int g, int key0, int key1, uint8_t* smem) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int group = a.nh / a.pg.nkv, T = 32 * RS / group, i0 = it.tile * T, rows = min(T, it.n - i0) * group;
+    float* qs = reinterpret_cast<float*>(smem + wave * 2048);                  // the row's q
+    float* ps = reinterpret_cast<float*>(smem + wave * 2048 + 512);            // 64 keys' probabilities
+    int64_t* at = reinterpret_cast<int64_t*>(smem + wave * 2048 + 1024);       // and pool rows
+    const uint64_t paths = a.pg.parent ? tree_path(a.pg, it.first, it.n) : 0;
+    const auto settle = [] {  // what the wave's lanes wrote is there for the others
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    };
+    for (int r = wave; r < rows; r += kWaves) {
+        const int i = i0 + r / group, hq = g * group + r % group, tok = it.first + i;
+        const uint64_t path = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i & 63) << 32) |
+                              (uint32_t)__shfl((int)(uint32_t)paths, i & 63);
+        const float* q = a.q + ((size_t)tok * a.nh + hq) * HD;
+        for (int d = lane; d < HD; d += 64) qs[d] = q[d] * a.qscale;
+        settle();
+        float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
+        const int end = min(key1, it.cached + i + 1);
+        for (int k0 = key0; k0 < end; k0 += 64) {
+            const int key = k0 + lane;
+            bool on = key < end && (key < it.cached || !a.pg.parent || (path >> ((key - it.cached) & 63) & 1));
+            const int64_t row = on ? paged_row(a.pg, it.s, key) : -1;
+            on = row >= 0;
+            float sc = -INFINITY;
+            if (on) {
+                const __half* k = a.pg.k + (row * a.pg.nkv + g) * HD;
+                sc = 0.f;
+                for (int d = 0; d < HD; ++d) sc = fmaf(qs[d], __half2float(k[d]), sc);
             }
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bh[t], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, bl[t], o[d], 0, 0, 0);
-            up = __builtin_amdgcn_mfma_f32_32x32x16_f16(pos, on[t], up, 0, 0, 0);
-            dn = __builtin_amdgcn_mfma_f32_32x32x16_f16(neg, on[t], dn, 0, 0, 0);
+            const float mx = fmaxf(m, wave_max(sc));
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mx);
+            const float p = on ? kPaScale * __builtin_amdgcn_exp2f(sc - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+            m = mx;
+            l = l * alpha + wave_sum(p);
+            ps[lane] = p;
+            at[lane] = row;
+            settle();
+            o[0] *= alpha, o[1] *= alpha;
+            for (int j = 0; j < 64; ++j) {
+                if (at[j] < 0) continue;
+                const __half* v = a.pg.v + (at[j] * a.pg.nkv + g) * HD;
+                for (int u = 0; u < 2; ++u)
+                    if (lane + 64 * u < HD) o[u] = fmaf(ps[j], __half2float(v[lane + 64 * u]), o[u]);
+            }
+            settle();
         }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            if (up[v] > 0.f) o[d][v] += INFINITY;
-            if (dn[v] > 0.f) o[d][v] -= INFINITY;
+        float* out = a.att + ((size_t)tok * a.nh + hq) * HD;
+        float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (it.splits > 1) {
+            const size_t p = ((size_t)it.slot * a.pg.nkv + g) * (32 * RS) + r;
+            out = a.part + p * HD;
+            inv = 1.f;
+            if (lane == 0) a.ml[p] = make_float2(m, l);
         }
+        for (int u = 0; u < 2; ++u)
+            if (lane + 64 * u < HD) out[lane + 64 * u] = o[u] * inv;
     }
 }
 
+// The keys a lane's row of a block attends, bit 16 t + u for key 16 t + 8 h + u
+// of the block at key kb (h: the lane's upper half).
+struct RowMask {
+    int cached, lim;  // the row's sequence's rows; its first key past (causal)
+    uint64_t path;    // its path (drafted trees)
+    bool tree;
+    __device__ __forceinline__ uint32_t operator()(int kb, int h) const {
+        uint32_t w;
+        if (tree) {
+            const int sh = kb - cached;
+            w = sh >= kTreeMax ? 0u
+                : sh >= 0      ? (uint32_t)(path >> sh)
+                : sh > -32     ? (uint32_t)(path << -sh) | ((1u << -sh) - 1u)
+                               : ~0u;
+        } else {
+            const int left = lim - kb;
+            w = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+        }
+        return w >> (8 * h);
+    }
+};
+
+// KG key groups: waves that take the same 32 keys of a stage share the rows
+// RS sets: 32-row sets, each a wave of every key group
 template <int HD, int RS>
-__global__ __launch_bounds__(kThreads, HD == 128 || (HD == 64 && RS == 2) ? 1 : 2) void attention_paged_kernel(AttnPagedArgs a) {
+__global__ __launch_bounds__(kThreads, HD == 128 && RS == 1 ? 1 : 2) void attention_paged_kernel(AttnPagedArgs a) {
     constexpr int KS = HD / 16, DB = HD / 32, NCH = HD / 8;
+    constexpr int KG = kWaves / RS, STAGE = 32 * KG;  // keys of a stage
+    constexpr int GROUPS = STAGE / 16;     // page groups of a stage
+    constexpr int OWN = GROUPS / kWaves;   // of them a wave loads
     constexpr int RPI = 64 / NCH;          // rows a load instruction brings
-    constexpr int LPG = 16 / RPI;          // load instructions per 16 rows
-    constexpr int LPB = 4 * LPG;           // per block, K and V
+    constexpr int LPG = 16 / RPI;          // load instructions per 16 rows (K or V)
+    constexpr int SLOT = 2 * STAGE * HD * 2;
+    constexpr bool PRIVATE = RS == 1;      // a wave reads the rows it loaded itself
     extern __shared__ __align__(256) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
+    const int set = RS == 1 ? 0 : wave % RS, kg = wave / RS;
     const int nkv = a.pg.nkv, group = a.nh / nkv, T = 32 * RS / group;
     const int g = blockIdx.x % nkv;
     Item it;
@@ -263,32 +313,42 @@ __global__ __launch_bounds__(kThreads, HD == 128 || (HD == 64 && RS == 2) ? 1 : 
     const int i0 = it.tile * T, ntok = min(T, it.n - i0);
     const int kend = it.cached + i0 + ntok;  // keys [0, kend) for the tile
     const int lim_min = a.pg.parent ? it.cached : it.cached + i0 + 1;  // every row attends the keys below
-    const int st0 = it.split * it.stages, st1 = min(st0 + it.stages, (kend + kStage - 1) / kStage);
-    // this wave's blocks
-    const int nb = max(min(st1, (kend - kBlock * wave + kStage - 1) / kStage) - st0, 0);
+    const int key0 = kStage * it.stages * it.split;
+    const int key1 = min(key0 + kStage * it.stages, kend);
+    const int nst = max((key1 - key0 + STAGE - 1) / STAGE, 0);
 
-    // Rows of K and V for block b, 16 of one page at a time.  Lane l holds the
-    // page of the wave's 16-row group l of a window of 32 blocks.
+    // Lane l holds the page of 16-row group l of a window of 64 groups
     const uint32_t row_b = 2u * (uint32_t)(nkv * HD), page_b = row_b << a.pg.page_shift;
     const int* table = a.pg.table + (size_t)it.s * a.pg.table_ld;
-    const auto page_ids = [&](int b0) __attribute__((always_inline)) {
-        const int row = kStage * (st0 + b0 + (lane >> 1)) + kBlock * wave + 16 * (lane & 1), p = row >> a.pg.page_shift;
+    constexpr int WIN = 64 / GROUPS;  // stages of a window
+    const auto page_ids = [&](int st) __attribute__((always_inline)) {
+        const int row = key0 + STAGE * st + 16 * lane, p = row >> a.pg.page_shift;
         int id = -1;
         if (row < kend && row >= 0 && p < a.pg.table_ld) id = table[p];
         return (unsigned)id < (unsigned)a.pg.n_pages ? id : -1;
     };
+    // (absent groups of the current stage's window, and of the one issued from)
     int ids = page_ids(0), ids_next = ids;
+    uint64_t gone_win = __ballot(ids < 0), gone_next = gone_win;
+    constexpr int AHEAD = PRIVATE ? 2 : 1;  // stages from a slot's issue to its use
+    const auto turn_window = [&](int st) __attribute__((always_inline)) {  // before st + AHEAD is issued
+        if (st % WIN == 0 && st > 0) gone_win = gone_next;
+        if ((st + AHEAD) % WIN == 0) ids = ids_next, gone_next = __ballot(ids < 0);
+        if (st % WIN == 0 && st + WIN < nst) ids_next = page_ids(st + WIN);
+    };
     const uint64_t kbase = scalar_addr(a.pg.k + g * HD), vbase = scalar_addr(a.pg.v + g * HD);
     const uint64_t zero = scalar_addr(zero_row);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem +
-                          (uint32_t)(wave * kSlots * slot_bytes(HD));
-    const int lr = lane / NCH, lc = lane % NCH;
-    const auto issue = [&](int b) __attribute__((always_inline)) {
-        const uint32_t slot = lds0 + (uint32_t)(b % kSlots) * slot_bytes(HD);
-        const int r0 = kStage * (st0 + b) + kBlock * wave;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const int lr = lane / NCH;
+    uint32_t kx = 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>(lr)), vx = 16 * (uint32_t)(lane % NCH ^ VRead<HD>::v_swz(lr));
+    // the wave's groups of stage st (16 rows of a page each)
+    const auto issue = [&](int st) __attribute__((always_inline)) {
+        const uint32_t slot = lds0 + (uint32_t)(st % kSlots) * SLOT;
+        asm volatile("" : "+v"(kx), "+v"(vx));  // (else every offset below is kept in registers)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int id = __builtin_amdgcn_readlane(ids, (2 * b + u) & 63), row = r0 + 16 * u;
+        for (int u = 0; u < OWN; ++u) {
+            const int gr = OWN * wave + u, row = key0 + STAGE * st + 16 * gr;
+            const int id = __builtin_amdgcn_readlane(ids, (GROUPS * st + gr) & 63);
             const uint32_t in = (uint32_t)(row & ((1 << a.pg.page_shift) - 1)) * row_b;
             const uint64_t off = (uint64_t)(uint32_t)id * page_b + in;
             const uint64_t kb = id < 0 ? zero : kbase + off, vb = id < 0 ? zero : vbase + off;
@@ -297,33 +357,30 @@ __global__ __launch_bounds__(kThreads, HD == 128 || (HD == 64 && RS == 2) ? 1 : 
             const int last = id < 0 ? 0 : kend - 1 - row;
 #pragma unroll
             for (int x = 0; x < LPG; ++x) {
-                const int r = x * RPI + lr, key = 16 * u + r;
-                const uint32_t ro = (uint32_t)min(r, last) * row_b;
-                const uint32_t to = slot + (uint32_t)(16 * u + x * RPI) * (2 * HD);
-                g2l_s(kb, ro + 16 * (lc ^ pa_swz<HD>(key)), to);
-                g2l_s(vb, ro + 16 * (lc ^ VRead<HD>::v_swz(key)), to + kBlock * HD * 2);
+                // (the rotation of row x RPI + lr is that of row lr and a constant)
+                const uint32_t ro = __umul24((uint32_t)min(x * RPI + lr, last), row_b);
+                const uint32_t to = slot + (uint32_t)(16 * gr + x * RPI) * (2 * HD);
+                g2l_s(kb, ro + (kx ^ (64 * x)), to);
+                g2l_s(vb, ro + (HD == 128 ? vx ^ (128 * (x & 1)) : vx), to + STAGE * HD * 2);
             }
         }
     };
-    if (nb > 0) issue(0);
-    if (nb > 1) issue(1);
+    if (nst > 0) issue(0);
+    if (PRIVATE && nst > 1) issue(1);
 
-    // this lane's query row of each set, split; its last key (causal) or path
-    f16x8 qh[RS][KS], ql[RS][KS];
-    int lim[RS];
-    uint64_t path[RS];
-    uint64_t paths = 0;
-    if (a.pg.parent) paths = tree_path(a.pg, it.first, it.n);
-#pragma unroll
-    for (int r = 0; r < RS; ++r) {
-        const int row = 32 * r + n, tl = row / group, hh = row % group;
+    // this lane's query row, split, and what it attends
+    f16x8 qh[KS], ql[KS];
+    RowMask mask;
+    {
+        const int row = 32 * set + n, tl = row / group, hh = row % group;
         const bool valid = tl < ntok;  // (the others: zeros at the tile's first token)
         const int i = i0 + (valid ? tl : 0);
-        lim[r] = it.cached + i + 1;
-        path[r] = 0;
-        if (a.pg.parent)
-            path[r] = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i) << 32) |
-                      (uint32_t)__shfl((int)(uint32_t)paths, i);
+        mask = RowMask{it.cached, it.cached + i + 1, 0, a.pg.parent != nullptr};
+        if (a.pg.parent) {
+            const uint64_t paths = tree_path(a.pg, it.first, it.n);
+            mask.path = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i) << 32) |
+                        (uint32_t)__shfl((int)(uint32_t)paths, i);
+        }
         const float* qp = a.q + ((size_t)(it.first + i) * a.nh + g * group + hh) * HD;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -337,151 +394,119 @@ __global__ __launch_bounds__(kThreads, HD == 128 || (HD == 64 && RS == 2) ? 1 : 
             for (int e = 0; e < 8; e += 2) {
                 f16x2 hi, lo;
                 pa_split(v[e] * a.qscale, v[e + 1] * a.qscale, hi, lo);
-                qh[r][ks][e] = hi[0], qh[r][ks][e + 1] = hi[1], ql[r][ks][e] = lo[0], ql[r][ks][e + 1] = lo[1];
+                qh[ks][e] = hi[0], qh[ks][e + 1] = hi[1], ql[ks][e] = lo[0], ql[ks][e + 1] = lo[1];
             }
         }
     }
 
-    float mref[RS], lrun[RS];
-    f32x16 o[RS][DB];
+    bool redo = false;  // (uniform)
+    float mref = -INFINITY, lrun = 0.f;
+    f32x16 o[DB];
 #pragma unroll
-    for (int r = 0; r < RS; ++r) {
-        mref[r] = -INFINITY, lrun[r] = 0.f;
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[r][d][v] = 0.f;
-    }
+        for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
     const VRead<HD> vr;
-    const int krow = pa_pi(n);
+    // this lane's piece 0 of its K row (every second piece from there: XOR 32 ks)
+    const uint32_t krow = (uint32_t)(pa_pi(n) * HD * 2 + 16 * (h ^ pa_swz<HD>(pa_pi(n))));
 
-    for (int b = 0; b < nb; ++b) {
-        if (b + 1 < nb) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPB) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const uint32_t k0 = lds0 + (uint32_t)(b % kSlots) * slot_bytes(HD), v0 = k0 + kBlock * HD * 2;
-        const int kb = kStage * (st0 + b) + kBlock * wave;
-        f32x16 s[RS];
-#pragma unroll
-        for (int r = 0; r < RS; ++r)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) s[r][v] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
-            const f16x8 k = *(lds_f16x8*)(uintptr_t)(k0 + krow * HD * 2 + 16 * ((2 * ks + h) ^ pa_swz<HD>(krow)));
-#pragma unroll
-            for (int r = 0; r < RS; ++r) {
-                s[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[r][ks], s[r], 0, 0, 0);
-                s[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[r][ks], s[r], 0, 0, 0);
-            }
+    for (int st = 0; st < nst; ++st) {
+        if constexpr (PRIVATE) {
+            if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LPG * OWN) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        } else {
+            // this stage has landed for every wave, and every wave is done with the
+            // slot that the next one goes to
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        const bool gone0 = __builtin_amdgcn_readlane(ids, (2 * b) & 63) < 0;
-        const bool gone1 = __builtin_amdgcn_readlane(ids, (2 * b + 1) & 63) < 0;
-        uint32_t w[RS];  // attended keys: bit 16 t + u for key 16 t + 8 h + u
-        bool special = false;
-        if (kb + kBlock > lim_min || gone0 || gone1) {
+        turn_window(st);
+        if (!PRIVATE && st + 1 < nst) issue(st + 1);
+        const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
+        if (kb < key1) {
+            const uint32_t k0 = lds0 + (uint32_t)(st % kSlots) * SLOT + 32 * kg * HD * 2, v0 = k0 + STAGE * HD * 2;
+            f32x16 s;
 #pragma unroll
-            for (int r = 0; r < RS; ++r) {
-                if (a.pg.parent) {
-                    const int sh = kb - it.cached;
-                    w[r] = sh >= kTreeMax ? 0u
-                           : sh >= 0      ? (uint32_t)(path[r] >> sh)
-                           : sh > -32     ? (uint32_t)(path[r] << -sh) | ((1u << -sh) - 1u)
-                                          : ~0u;
-                } else {
-                    const int left = lim[r] - kb;
-                    w[r] = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
-                }
-                if (gone0) w[r] &= 0xffff0000u;
-                if (gone1) w[r] &= 0xffffu;
-                w[r] >>= 8 * h;
+            for (int v = 0; v < 16; ++v) s[v] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+                const f16x8 k = *(lds_f16x8*)(uintptr_t)((k0 + krow) ^ (32 * ks));
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[ks], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[ks], s, 0, 0, 0);
+            }
+            const uint32_t gone = (uint32_t)(gone_win >> (GROUPS * (st % WIN) + 2 * kg)) & 3;
+            if (kb + 32 > lim_min || gone) {
+                uint32_t w = mask(kb, h);
+                if (gone & 1) w &= 0xffff0000u;
+                if (gone & 2) w &= 0xffffu;
 #pragma unroll
                 for (int v = 0; v < 16; ++v)
-                    if (!((w[r] >> (16 * (v >> 3) + (v & 7))) & 1)) s[r][v] = -INFINITY;
+                    if (!((w >> (16 * (v >> 3) + (v & 7))) & 1)) s[v] = -INFINITY;
+                redo |= any_special<HD>(v0);
             }
-            special = any_special<HD>(v0);
-        }
-        float mx[RS];
-        bool up = false;
+            float mx = s[0];
 #pragma unroll
-        for (int r = 0; r < RS; ++r) {
-            mx[r] = s[r][0];
-#pragma unroll
-            for (int v = 1; v < 16; ++v) mx[r] = fmaxf(mx[r], s[r][v]);
-            mx[r] = pa_pair_max(mx[r]);
-            up |= mx[r] > mref[r] + kPaSlack;  // also the first block with an attended key
-        }
-        if (__any(up)) {
-#pragma unroll
-            for (int r = 0; r < RS; ++r) {
-                const float mnew = fmaxf(mref[r], mx[r]);
+            for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
+            mx = pa_pair_max(mx);
+            if (__any(mx > mref + kPaSlack)) {  // also the first block with an attended key
+                const float mnew = fmaxf(mref, mx);
                 // (nothing attended so far: the sums are zero)
-                const float alpha = mref[r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref[r] - mnew);
-                mref[r] = mnew;
-                lrun[r] *= alpha;
+                const float alpha = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
+                mref = mnew;
+                lrun *= alpha;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) o[r][d][v] *= alpha;
+                    for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
             }
-        }
-        f16x8 bh[RS][2], bl[RS][2];
-#pragma unroll
-        for (int r = 0; r < RS; ++r) {
-            const float ref0 = mref[r] == -INFINITY ? 0.f : mref[r];
+            const float ref0 = mref == -INFINITY ? 0.f : mref;
             float p[16], ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                p[v] = kPaScale * __builtin_amdgcn_exp2f(s[r][v] - ref0);
+                p[v] = kPaScale * __builtin_amdgcn_exp2f(s[v] - ref0);
                 ps[v & 3] += p[v];
             }
-            lrun[r] += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+            lrun += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+            f16x8 bh[2], bl[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int u = 0; u < 8; u += 2) {
                     f16x2 hi, lo;
                     pa_split(p[8 * t + u], p[8 * t + u + 1], hi, lo);
-                    bh[r][t][u] = hi[0], bh[r][t][u + 1] = hi[1], bl[r][t][u] = lo[0], bl[r][t][u + 1] = lo[1];
+                    bh[t][u] = hi[0], bh[t][u + 1] = hi[1], bl[t][u] = lo[0], bl[t][u + 1] = lo[1];
                 }
-        }
-        if (special) {
-#pragma unroll
-            for (int r = 0; r < RS; ++r) blend_special<HD>(vr, v0, w[r], bh[r], bl[r], o[r]);
-        } else {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     const f16x8 v = vr(v0, t, d);
-#pragma unroll
-                    for (int r = 0; r < RS; ++r) {
-                        o[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bh[r][t], o[r][d], 0, 0, 0);
-                        o[r][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bl[r][t], o[r][d], 0, 0, 0);
-                    }
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bh[t], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bl[t], o[d], 0, 0, 0);
                 }
         }
-        // the slot's last reads are done before its next rows are requested
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        // a window's pages are requested 30 blocks ahead of their use
-        if ((b & 31) == 0 && b + 32 < nb) ids_next = page_ids(b + 32);
-        if (((b + kSlots) & 31) == 0) ids = ids_next;
-        if (b + kSlots < nb) issue(b + kSlots);
+        if constexpr (PRIVATE) {
+            // the slot's last reads are done before its next rows are requested
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (st + 2 < nst) issue(st + 2);
+        }
     }
 
     // the waves' parts meet (every load into the slots has been waited for)
-    __syncthreads();
+    if (__syncthreads_or(redo)) {
+        redo_item<HD, RS>(a, it, g, key0, key1, smem);
+        return;
+    }
     float* ms = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int r = 0; r < RS; ++r) {
-        float* mb = ms + (wave * RS + r) * merge_floats(HD);
-        const float lsum = lrun[r] + __shfl_xor(lrun[r], 32, 64);
+    {
+        float* mb = ms + wave * merge_floats(HD);
+        const float lsum = lrun + __shfl_xor(lrun, 32, 64);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) mb[(32 * d + 8 * (v >> 2) + 4 * h + (v & 3)) * 32 + n] = o[r][d][v];
+            for (int v = 0; v < 16; ++v) mb[(32 * d + 8 * (v >> 2) + 4 * h + (v & 3)) * 32 + n] = o[d][v];
         if (h == 0) {
-            mb[HD * 32 + n] = mref[r];
+            mb[HD * 32 + n] = mref;
             mb[HD * 32 + 32 + n] = lsum;
         }
     }
@@ -489,15 +514,15 @@ __global__ __launch_bounds__(kThreads, HD == 128 || (HD == 64 && RS == 2) ? 1 : 
     // thread: row 32 mr + mn, dims d0 .. d0 + ND
     constexpr int ND = HD * RS / 8;
     const int mr = RS == 2 ? (tid >> 5) & 1 : 0, mn = tid & 31, d0 = (tid >> (RS == 2 ? 6 : 5)) * ND;
-    const float* mb[kWaves];
-    float wt[kWaves], M = -INFINITY, L = 0.f;
+    const float* mb[KG];
+    float wt[KG], M = -INFINITY, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < KG; ++i) {
         mb[i] = ms + (i * RS + mr) * merge_floats(HD);
         M = fmaxf(M, mb[i][HD * 32 + mn]);
     }
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
+    for (int i = 0; i < KG; ++i) {
         const float mi = mb[i][HD * 32 + mn];
         wt[i] = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);  // (nothing attended there)
         L += wt[i] * mb[i][HD * 32 + 32 + mn];
@@ -519,10 +544,11 @@ __global__ __launch_bounds__(kThreads, HD == 128 || (HD == 64 && RS == 2) ? 1 : 
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int at = (d0 + d + e) * 32 + mn;
-            x[e] = ((wt[0] * mb[0][at] + wt[1] * mb[1][at]) + (wt[2] * mb[2][at] + wt[3] * mb[3][at])) * inv;
+            x[e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KG; ++i) x[e] += wt[i] * mb[i][(d0 + d + e) * 32 + mn];
         }
-        *reinterpret_cast<float4*>(op + d0 + d) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(op + d0 + d) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
     }
 }
 
