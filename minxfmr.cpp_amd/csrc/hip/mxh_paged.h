@@ -46,14 +46,18 @@ __device__ __forceinline__ int paged_seq_of(const PagedArgs& a, int t) {
     return s < a.n_seq && a.start[s] >= 0 && a.start[s] <= t ? s : -1;
 }
 
-// Lane i of the wave gets the bits of token i of a drafted tree and its
-// ancestors (`first`: the sequence's first token row, n of them, at most 64).
-// Every round a lane joins the mask of the token it points to and then points
-// to what that one points to: 2^r ancestors after r rounds.
-__device__ __forceinline__ uint64_t tree_path(const PagedArgs& a, int first, int n) {
+// The parent of token `lane` of a drafted tree (`first`: the sequence's first
+// token row, n of them, at most 64), -1 for a root and past the tree.
+__device__ __forceinline__ int tree_parent(const PagedArgs& a, int first, int n) {
+    const int lane = threadIdx.x & 63, p = lane < n ? a.parent[first + lane] : -1;
+    return p < -1 || p >= lane ? -1 : p;
+}
+
+// Lane i of the wave gets the bits of token i and its ancestors, from the
+// lanes' parents.  Every round a lane joins the mask of the token it points to
+// and then points to what that one points to: 2^r ancestors after r rounds.
+__device__ __forceinline__ uint64_t tree_path(int p) {
     const int lane = threadIdx.x & 63;
-    int p = lane < n ? a.parent[first + lane] : -1;
-    if (p < -1 || p >= lane) p = -1;
     uint64_t mask = 1ull << lane;
 #pragma unroll
     for (int r = 0; r < 6; ++r) {
@@ -64,6 +68,11 @@ __device__ __forceinline__ uint64_t tree_path(const PagedArgs& a, int first, int
         p = p < 0 ? -1 : next;
     }
     return mask;
+}
+
+// lane i's bits, in every lane (i below 64, any lane's own)
+__device__ __forceinline__ uint64_t path_of(uint64_t paths, int i) {
+    return ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i) << 32) | (uint32_t)__shfl((int)(uint32_t)paths, i);
 }
 
 // attention over the paged cache (mxh_paged_attn.hip)

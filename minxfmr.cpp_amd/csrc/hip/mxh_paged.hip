@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kRopeThreads) void qk_rope_append_kernel(RopeArgs a
                 bool mine = true;
                 if (a.pg.parent) {
                     const int n = min(min(a.pg.start[s + 1], a.pg.n_tokens) - first, kTreeMax);
-                    const uint64_t path = tree_path(a.pg, first, n);
+                    const uint64_t path = tree_path(tree_parent(a.pg, first, n));
                     pos = cached + __shfl((int)__popcll(path), i & 63) - 1;
                     mine = i < kTreeMax;
                 }

@@ -6,26 +6,28 @@
 // q.k / sqrt(hd), softmax softmax.cpp:4-18, weighted sum of V rows), here over
 // the rows of a sequence's pages, for drafted trees only along a token's path.
 //
-// Work: a tile is T = 32 RS / group consecutive tokens of one sequence with
-// the group = nh / nkv q heads of one kv head (row r: token r / group, head
-// r % group); an item is a tile and a split of its keys, a workgroup an item
-// and a kv head.  The lengths are on the device, so every workgroup computes
-// the same plan from them (paged_item): stages of 128 keys per split so that
-// the batch makes about `target` items.  The grid has room for the most items
-// that can come of it; the others leave at once.
+// Work: a tile is T = R / group consecutive tokens of one sequence with the
+// group = nh / nkv q heads of one kv head (row r: token r / group, head
+// r % group), R = 16, 32 or 64 rows; an item is a tile and a split of its keys,
+// a workgroup an item and a kv head.  The lengths are on the device, so every
+// workgroup computes the same plan from them (paged_item): stages of 128 keys
+// per split so that the batch makes about `target` items.  The grid has room
+// for the most items that can come of it; the others leave at once.
 //
-// Inside a workgroup nothing is shared: wave w of four walks the 32-key blocks
-// 4 st + w of its split, whose K and V rows it loads itself, straight into its
-// own two LDS slots (a block's 16 rows of a page are contiguous, so the
-// addresses are a scalar base a page and fixed lane offsets).  So there is no
-// barrier before the end, where the waves' (reference, sum, V sum) meet in LDS.
-// Per block and set of 32 rows, as in mxh_prefill_attn.hip:
+// K and V rows go straight into LDS (16 rows of a page are evenly spaced, so
+// their addresses are a scalar base and fixed lane offsets).  Per 32-key block
+// and set of 32 rows, as in mxh_prefill_attn.hip:
 //
 //   S^T = K Q^T      v_mfma_f32_32x32x16_f16; q pre-scaled by log2(e) /
 //                    sqrt(hd), fp16 hi + lo; K exact
 //   O^T += V^T P^T   P = 64 2^(S - ref) as fp16 hi + lo; V exact, its
 //                    transposed operand read from the rows by
 //                    ds_read_b64_tr_b16
+//
+// Tiles of 16 rows use v_mfma_f32_16x16x32_f16 instead: block b of a 32-key
+// block's two 16-key products takes the keys 8 (m / 4) + 4 b + m % 4 as its rows
+// m, so that lane l ends with the scores of keys 8 (l / 16) .. +8, the very
+// operand that the second product wants of it.
 //
 // Rows that a token does not attend must not reach it: their scores are
 // replaced, not added to, and since 0 times an infinity is no zero, blocks with
@@ -35,6 +37,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "mxh_attn.h"
 #include "mxh_internal.h"
@@ -45,16 +48,16 @@ namespace mxh {
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kStage = 128;                // keys that splits are made of
-constexpr int kSlots = 2;                  // stages in LDS
 
-// floats a wave leaves for the merge: V sums [hd][32], references, sums
-__host__ __device__ constexpr int merge_floats(int hd) { return hd * 32 + 64; }
-__host__ __device__ constexpr int lds_bytes(int hd, int rs) {
-    const int ring = kSlots * 2 * (kStage / rs) * hd * 2, merge = kWaves * merge_floats(hd) * 4;
+// floats a wave leaves for the merge: V sums [m][hd + 4], references, sums
+__host__ __device__ constexpr int merge_floats(int hd, int m) { return m * (hd + 6); }
+__host__ __device__ constexpr int lds_bytes(int hd, int rows) {
+    const int ring = 2 * kStage * hd * 2, merge = kWaves * merge_floats(hd, rows < 32 ? 16 : 32) * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -63,31 +66,38 @@ __device__ __align__(256) uint32_t zero_row[64];
 
 // One workgroup's share of the batch (all uniform)
 struct Item {
-    int s, first, n, cached;  // sequence: its first token row, new tokens, rows before them
+    int s, first, n, cached;          // sequence: its first token row, new tokens, rows before them
     int tile, split, splits, stages;  // stages per split
-    int slot;                 // of its part (splits > 1)
+    int slot;                         // of its part (splits > 1)
 };
 
 struct SeqPlan {
-    int first, n, cached, tiles, stages, splits;
+    uint32_t first, n, cached, tiles, stages, splits;  // stages: of a split
 };
 
-// tokens, tiles, and splits of `per` stages at most (0: one split) of sequence s
-__device__ __forceinline__ SeqPlan seq_plan(const PagedArgs& a, int s, int T, int per) {
+// x / d rounded up, for x < 2^21 and inv the rounded 1 / d (off by less than
+// half a step of x / d)
+__device__ __forceinline__ uint32_t div_up(uint32_t x, uint32_t d, float inv) {
+    return (uint32_t)(((float)(x + d - 1) + 0.5f) * inv);
+}
+
+// (t: tokens of a tile; in one split)
+__device__ __forceinline__ SeqPlan seq_plan(int start, int end, int cached, const PagedArgs& a, uint32_t t, float inv_t) {
     SeqPlan p;
-    p.first = max(a.start[s], 0);
-    p.n = max(min(a.start[s + 1], a.n_tokens) - p.first, 0);
-    if (a.parent) p.n = min(p.n, kTreeMax);
-    p.cached = min(max(a.cached[s], 0), 1 << 30);
-    p.tiles = (p.n + T - 1) / T;
+    p.first = (uint32_t)max(start, 0);
+    p.n = (uint32_t)max(min(end, a.n_tokens) - (int)p.first, 0);
+    if (a.parent) p.n = min(p.n, (uint32_t)kTreeMax);
+    p.cached = (uint32_t)min(max(cached, 0), 1 << 30);
+    p.tiles = div_up(p.n, t, inv_t);
     p.stages = (p.cached + p.n + kStage - 1) / kStage;
     p.splits = 1;
-    if (per > 0 && p.stages > per) {
-        const int eq = (p.stages + per - 1) / per;
-        p.stages = (p.stages + eq - 1) / eq;  // (evenly)
-        p.splits = ((p.cached + p.n + kStage - 1) / kStage + p.stages - 1) / p.stages;
-    }
     return p;
+}
+__device__ __forceinline__ void split_plan(SeqPlan& p, uint32_t per) {  // of `per` stages at most
+    if (p.stages <= per) return;
+    const uint32_t all = p.stages, eq = (all + per - 1) / per;
+    p.stages = (all + eq - 1) / eq;  // (evenly)
+    p.splits = (all + p.stages - 1) / p.stages;
 }
 
 __device__ __forceinline__ int wave_scan(int v) {  // inclusive
@@ -100,88 +110,98 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive
     return v;
 }
 
-// Item `index` of the batch (of its tiles alone with TILES); false past the
-// last.  target: items wanted, 0: no splits.  Lane l sums up the plans of the
-// sequences [l part, (l + 1) part); the one that holds the index is walked.
-// With per = ceil(W / target) stages a split, W = sum of tiles * stages, a
-// sequence in splits makes less than twice W_s / per items, so the parts of
-// all of them fit 2 target slots.
-template <bool TILES>
-__device__ bool paged_item(const PagedArgs& a, int T, int target, int index, Item& it) {
+// Item `index` of the batch; false past the last.  With MERGE the items are the
+// tiles in splits.  target: items wanted, 0: no splits.  Lane l sums up the
+// plans of the sequences [l part, (l + 1) part); the one that holds the index
+// is walked.  With per >= W / target stages a split, W = sum of tiles * stages,
+// a sequence in splits makes less than twice its W / per items, so the parts of
+// all of them fit 2 target slots, and the tiles in splits are target at most.
+template <bool MERGE>
+__device__ __forceinline__ bool paged_item(const PagedArgs& a, uint32_t t, int target, uint32_t index, Item& it) {
     const int lane = threadIdx.x & 63, part = (a.n_seq + 63) / 64;
     const int s0 = lane * part, s1 = min(s0 + part, a.n_seq);
-    int per = 0;
-    if (target > 0) {
-        double w = 0.0;
-        for (int s = s0; s < s1; ++s) {
-            const SeqPlan p = seq_plan(a, s, T, 0);
-            w += (double)p.tiles * p.stages;
-        }
-        per = (int)fmin(ceil(wave_sum_d_all(w) / target), 1e9);
-    }
-    int items = 0, slots = 0;
+    const float inv_t = 1.0f / (float)t;
+    SeqPlan p{0, 0, 0, 0, 0, 1};
+    float w = 0.f;
     for (int s = s0; s < s1; ++s) {
-        const SeqPlan p = seq_plan(a, s, T, per);
-        items += p.tiles * (TILES ? 1 : p.splits);
-        slots += p.splits > 1 ? p.tiles * p.splits : 0;
+        p = seq_plan(a.start[s], a.start[s + 1], a.cached[s], a, t, inv_t);
+        w += (float)p.tiles * (float)p.stages;
     }
-    const int upto = wave_scan(items), slots_upto = wave_scan(slots);
+    // (at least W / target: the sum is off by some 2^-23 a step)
+    const uint32_t per = target > 0 ? (uint32_t)fminf(wave_sum_all(w) / (float)target * 1.001f, 1e9f) + 1 : UINT32_MAX;
+    const auto items_of = [](const SeqPlan& q) { return MERGE ? (q.splits > 1 ? q.tiles : 0) : q.tiles * q.splits; };
+    const auto slots_of = [](const SeqPlan& q) { return q.splits > 1 ? q.tiles * q.splits : 0; };
+    uint32_t items = 0, slots = 0;
+    if (part == 1) {  // (one sequence a lane: its plan is still there)
+        split_plan(p, per);
+        items = items_of(p), slots = slots_of(p);
+    } else {
+        for (int s = s0; s < s1; ++s) {
+            p = seq_plan(a.start[s], a.start[s + 1], a.cached[s], a, t, inv_t);
+            split_plan(p, per);
+            items += items_of(p), slots += slots_of(p);
+        }
+    }
+    const uint32_t upto = (uint32_t)wave_scan((int)items), slots_upto = (uint32_t)wave_scan((int)slots);
     const uint64_t past = __ballot(upto > index);
     if (!past) return false;
     const int l = __ffsll((unsigned long long)past) - 1;
-    int at = __builtin_amdgcn_readlane(upto - items, l), slot = __builtin_amdgcn_readlane(slots_upto - slots, l);
-    for (int s = l * part;; ++s) {
-        const SeqPlan p = seq_plan(a, s, T, per);
-        const int here = p.tiles * (TILES ? 1 : p.splits);
-        if (index < at + here || s + 1 >= min((l + 1) * part, a.n_seq)) {
-            const int i = index - at;
-            it.s = s, it.first = p.first, it.n = p.n, it.cached = p.cached;
-            // (tiles with the most keys first)
-            it.tile = TILES ? i : p.tiles - 1 - i % p.tiles;
-            it.split = TILES ? 0 : i / p.tiles;
-            it.splits = p.splits, it.stages = p.stages;
-            it.slot = slot + it.tile * p.splits + it.split;
-            return index < at + here;
+    const auto lane_l = [l](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+    uint32_t i = index - lane_l(upto - items), slot = lane_l(slots_upto - slots);
+    it.s = l * part;
+    if (part == 1) {
+        p = SeqPlan{lane_l(p.first), lane_l(p.n), lane_l(p.cached), lane_l(p.tiles), lane_l(p.stages), lane_l(p.splits)};
+    } else {
+        for (;; ++it.s) {  // (ends within the lane's sequences: they hold the index)
+            p = seq_plan(a.start[it.s], a.start[it.s + 1], a.cached[it.s], a, t, inv_t);
+            split_plan(p, per);
+            if (i < items_of(p) || it.s + 1 >= min((l + 1) * part, a.n_seq)) break;
+            i -= items_of(p), slot += slots_of(p);
         }
-        at += here;
-        slot += p.splits > 1 ? p.tiles * p.splits : 0;
     }
+    it.first = p.first, it.n = p.n, it.cached = p.cached, it.splits = p.splits, it.stages = p.stages;
+    it.split = MERGE ? 0 : i / p.tiles;
+    // (tiles with the most keys first)
+    it.tile = MERGE ? i : p.tiles - 1 - (i - it.split * p.tiles);
+    it.slot = slot + it.tile * p.splits + it.split;
+    return true;
 }
 
 struct AttnPagedArgs {
     PagedArgs pg;
     const float* q;
     float* att;
-    float* part;  // [2 target][nkv][32 RS][HD]: V sums of the splits
-    float2* ml;   // [2 target][nkv][32 RS]: references and sums
+    float* part;  // [2 target][nkv][R][HD]: V sums of the splits
+    float2* ml;   // [2 target][nkv][R]: references and sums
     int nh, target;
     float qscale;
 };
 
-// 8 halves of V's transposed operand: keys 16 t + 8 h + 0..7 of the block (h:
-// the lane's upper half), dim 32 d + lane % 32.  One read turns 4 keys x 16
-// dims around in each 16 lanes.
+// pairs of 16-byte pieces of a V row are rotated by the key, so that the four
+// keys of a transposing read lie in different banks (the same for keys 16 apart)
 template <int HD>
+__device__ __forceinline__ int v_swz(int key) {
+    return HD == 128 ? 2 * (key & 7) : HD == 64 ? 2 * ((key >> 1) & 3) : 2 * ((key >> 2) & 1);
+}
+
+// 8 halves of V's transposed operand.  One read turns 4 keys x 16 dims around
+// in each 16 lanes.  M = 32: keys 16 t + 8 (l / 32) + 0..7 of the block, dim
+// 32 d + l % 32.  M = 16: keys 8 (l / 16) + 0..7 (t = 0), dim 16 d + l % 16.
+template <int HD, int M>
 struct VRead {
     uint32_t at;  // byte offset of t, d = 0 in the block's V rows
     __device__ __forceinline__ VRead() {
-        const int lane = threadIdx.x & 63, key = 8 * (lane >> 5) + ((lane & 15) >> 2);
-        const int piece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-        at = (uint32_t)(key * HD * 2 + 16 * (piece ^ v_swz(key)) + 8 * (lane & 1));
+        const int lane = threadIdx.x & 63, key = 8 * (M == 32 ? lane >> 5 : lane >> 4) + ((lane & 15) >> 2);
+        const int piece = (M == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+        at = (uint32_t)(key * HD * 2 + 16 * (piece ^ v_swz<HD>(key)) + 8 * (lane & 1));
     }
-    // pairs of 16-byte pieces rotated by the key, so that the four keys of a
-    // read lie in different banks (the same for keys 16 apart)
-    static __device__ __forceinline__ int v_swz(int key) {
-        return HD == 128 ? 2 * (key & 7) : HD == 64 ? 2 * ((key >> 1) & 3) : 2 * ((key >> 2) & 1);
-    }
-    // v0: the rows' place, a multiple of 256 bytes.  Dims 32 d on are 64 d bytes
+    // v0: the rows' place, a multiple of 256 bytes.  Dims M d on are 2 M d bytes
     // on; keys 4 on are 4 rows on, rotated by another HD bytes
     __device__ __forceinline__ f16x8 operator()(uint32_t v0, int t, int d) const {
         typedef short s16x8 __attribute__((ext_vector_type(8)));
-        const uint32_t p = v0 + at;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((p ^ (64 * d)) + t * 32 * HD));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4*)(uintptr_t)(((p ^ (64 * d)) ^ HD) + t * 32 * HD + 8 * HD));
+        const uint32_t p = (v0 + at) ^ (uint32_t)(2 * M * d);
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(p + t * 32 * HD));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((p ^ HD) + t * 32 * HD + 8 * HD));
         return __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
@@ -205,22 +225,21 @@ __device__ __forceinline__ bool any_special(uint32_t v0) {
 // does not attend: a key a lane for the scores, then a dim a lane (or two) for
 // the sums.  For items that found such a value among rows that only some of
 // their tokens attend; the rest of the kernel pays no register for it.
-template <int HD, int RS>
+template <int HD, int R>
 __device__ void redo_item(const AttnPagedArgs& a, const Item& it, int g, int key0, int key1, uint8_t* smem) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int group = a.nh / a.pg.nkv, T = 32 * RS / group, i0 = it.tile * T, rows = min(T, it.n - i0) * group;
+    const int group = a.nh / a.pg.nkv, T = R / group, i0 = it.tile * T, rows = min(T, it.n - i0) * group;
     float* qs = reinterpret_cast<float*>(smem + wave * 2048);                  // the row's q
     float* ps = reinterpret_cast<float*>(smem + wave * 2048 + 512);            // 64 keys' probabilities
     int64_t* at = reinterpret_cast<int64_t*>(smem + wave * 2048 + 1024);       // and pool rows
-    const uint64_t paths = a.pg.parent ? tree_path(a.pg, it.first, it.n) : 0;
+    const uint64_t paths = a.pg.parent ? tree_path(tree_parent(a.pg, it.first, it.n)) : 0;
     const auto settle = [] {  // what the wave's lanes wrote is there for the others
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
     };
     for (int r = wave; r < rows; r += kWaves) {
         const int i = i0 + r / group, hq = g * group + r % group, tok = it.first + i;
-        const uint64_t path = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i & 63) << 32) |
-                              (uint32_t)__shfl((int)(uint32_t)paths, i & 63);
+        const uint64_t path = path_of(paths, i & 63);
         const float* q = a.q + ((size_t)tok * a.nh + hq) * HD;
         for (int d = lane; d < HD; d += 64) qs[d] = q[d] * a.qscale;
         settle();
@@ -257,7 +276,7 @@ __device__ void redo_item(const AttnPagedArgs& a, const Item& it, int g, int key
         float* out = a.att + ((size_t)tok * a.nh + hq) * HD;
         float inv = l == 0.f ? 0.f : 1.0f / l;
         if (it.splits > 1) {
-            const size_t p = ((size_t)it.slot * a.pg.nkv + g) * (32 * RS) + r;
+            const size_t p = ((size_t)it.slot * a.pg.nkv + g) * R + r;
             out = a.part + p * HD;
             inv = 1.f;
             if (lane == 0) a.ml[p] = make_float2(m, l);
@@ -267,187 +286,237 @@ __device__ void redo_item(const AttnPagedArgs& a, const Item& it, int g, int key
     }
 }
 
-// The keys a lane's row of a block attends, bit 16 t + u for key 16 t + 8 h + u
-// of the block at key kb (h: the lane's upper half).
+// The keys a lane's row attends, a bit each, of the block of 32 at key kb.
 struct RowMask {
     int cached, lim;  // the row's sequence's rows; its first key past (causal)
     uint64_t path;    // its path (drafted trees)
     bool tree;
-    __device__ __forceinline__ uint32_t operator()(int kb, int h) const {
-        uint32_t w;
-        if (tree) {
-            const int sh = kb - cached;
-            w = sh >= kTreeMax ? 0u
-                : sh >= 0      ? (uint32_t)(path >> sh)
-                : sh > -32     ? (uint32_t)(path << -sh) | ((1u << -sh) - 1u)
-                               : ~0u;
-        } else {
+    __device__ __forceinline__ uint32_t operator()(int kb) const {
+        if (!tree) {
             const int left = lim - kb;
-            w = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+            return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
         }
-        return w >> (8 * h);
+        const int sh = kb - cached;
+        return sh >= kTreeMax ? 0u
+               : sh >= 0      ? (uint32_t)(path >> sh)
+               : sh > -32     ? (uint32_t)(path << -sh) | ((1u << -sh) - 1u)
+                              : ~0u;
     }
 };
 
-// KG key groups: waves that take the same 32 keys of a stage share the rows
-// RS sets: 32-row sets, each a wave of every key group
-template <int HD, int RS>
-__global__ __launch_bounds__(kThreads, HD == 128 && RS == 1 ? 1 : 2) void attention_paged_kernel(AttnPagedArgs a) {
-    constexpr int KS = HD / 16, DB = HD / 32, NCH = HD / 8;
-    constexpr int KG = kWaves / RS, STAGE = 32 * KG;  // keys of a stage
-    constexpr int GROUPS = STAGE / 16;     // page groups of a stage
-    constexpr int OWN = GROUPS / kWaves;   // of them a wave loads
-    constexpr int RPI = 64 / NCH;          // rows a load instruction brings
-    constexpr int LPG = 16 / RPI;          // load instructions per 16 rows (K or V)
+// a product of the matrix cores with M rows of the first operand and M columns
+template <int M>
+struct Mfma {
+    typedef f32x16 acc;
+    static __device__ __forceinline__ acc mul(f16x8 a, f16x8 b, acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mfma<16> {
+    typedef f32x4 acc;
+    static __device__ __forceinline__ acc mul(f16x8 a, f16x8 b, acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// the larger / the sum over the lanes that hold one row (l % M)
+template <int M>
+__device__ __forceinline__ float row_max(float v) {
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return pa_pair_max(v);
+}
+template <int M>
+__device__ __forceinline__ float row_sum(float v) {
+    if constexpr (M == 16) v += lane_xor<16>(v);
+    return v + lane_xor<32>(v);
+}
+
+// R = 16, 32: every wave takes 32 keys of a stage of 128 for all rows of the
+// tile and reads only what it loaded: no barrier before the merge.  K and V have
+// one place each; the next K comes while V is used, the next V while K is.
+// R = 64: two waves, one a set of 32 rows, take the same 32 keys of a stage of
+// 64, which all four waves load, two stages in LDS and a barrier a stage.
+template <int HD, int R>
+__global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedArgs a) {
+    constexpr int M = R == 16 ? 16 : 32, RS = R / M;  // rows of a wave; waves to a key group
+    constexpr int KS = HD * M / 512, DB = HD / M;     // products of a score and of a sum
+    constexpr int SB = 32 / M, NA = M * M / 64;       // score blocks of 32 keys, accumulators of one
+    constexpr int NP = SB * NA, TT = NP / 8;          // a lane's scores; operands they make
+    constexpr int NCH = HD / 8, KG = kWaves / RS, STAGE = 32 * KG;  // 16-byte pieces of a row; keys of a stage
+    constexpr int GROUPS = STAGE / 16, OWN = GROUPS / kWaves;       // page groups of a stage; of them a wave loads
+    constexpr int RPI = 64 / NCH, LPG = 16 / RPI;     // rows a load brings; loads of 16 rows (K or V)
     constexpr int SLOT = 2 * STAGE * HD * 2;
-    constexpr bool PRIVATE = RS == 1;      // a wave reads the rows it loaded itself
+    constexpr bool PRIVATE = RS == 1;
+    using MM = Mfma<M>;
+    using acc_t = typename MM::acc;
     extern __shared__ __align__(256) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 31, h = lane >> 5;
-    const int set = RS == 1 ? 0 : wave % RS, kg = wave / RS;
-    const int nkv = a.pg.nkv, group = a.nh / nkv, T = 32 * RS / group;
-    const int g = blockIdx.x % nkv;
+    const int n = lane % M, h = lane / M;
+    const int set = wave % RS, kg = wave / RS;
+    const uint32_t nkv = (uint32_t)a.pg.nkv, group = (uint32_t)a.nh / nkv, T = R / group;
+    const uint32_t index = blockIdx.x / nkv, g = blockIdx.x - index * nkv;
     Item it;
-    if (!paged_item<false>(a.pg, T, a.target, blockIdx.x / nkv, it)) return;
+    if (!paged_item<false>(a.pg, T, a.target, index, it)) return;
 
-    const int i0 = it.tile * T, ntok = min(T, it.n - i0);
+    const int i0 = it.tile * (int)T, ntok = min((int)T, it.n - i0);
     const int kend = it.cached + i0 + ntok;  // keys [0, kend) for the tile
     const int lim_min = a.pg.parent ? it.cached : it.cached + i0 + 1;  // every row attends the keys below
     const int key0 = kStage * it.stages * it.split;
     const int key1 = min(key0 + kStage * it.stages, kend);
     const int nst = max((key1 - key0 + STAGE - 1) / STAGE, 0);
 
+    // this lane's query row; its loads go first, those of K and V come back after them
+    const uint32_t row = 32 * set + n, tl = row / group;
+    const bool valid = (int)tl < ntok;  // (the others: zeros at the tile's first token)
+    const int i = i0 + (valid ? (int)tl : 0);
+    float4 qv[KS][2];
+    {
+        const float* qp = a.q + ((size_t)(it.first + i) * a.nh + g * group + (row - tl * group)) * HD + 8 * h;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                qv[ks][e] = valid ? *reinterpret_cast<const float4*>(qp + HD / KS * ks + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const int parent = a.pg.parent ? tree_parent(a.pg, it.first, it.n) : -1;
+
     // Lane l holds the page of 16-row group l of a window of 64 groups
-    const uint32_t row_b = 2u * (uint32_t)(nkv * HD), page_b = row_b << a.pg.page_shift;
+    const uint32_t row_b = 2u * nkv * HD, page_b = row_b << a.pg.page_shift;
     const int* table = a.pg.table + (size_t)it.s * a.pg.table_ld;
     constexpr int WIN = 64 / GROUPS;  // stages of a window
     const auto page_ids = [&](int st) __attribute__((always_inline)) {
-        const int row = key0 + STAGE * st + 16 * lane, p = row >> a.pg.page_shift;
+        const int r = key0 + STAGE * st + 16 * lane, p = r >> a.pg.page_shift;
         int id = -1;
-        if (row < kend && row >= 0 && p < a.pg.table_ld) id = table[p];
+        if (r < kend && r >= 0 && p < a.pg.table_ld) id = table[p];
         return (unsigned)id < (unsigned)a.pg.n_pages ? id : -1;
     };
-    // (absent groups of the current stage's window, and of the one issued from)
     int ids = page_ids(0), ids_next = ids;
+    // absent groups of the current stage's window, and of the one issued from
     uint64_t gone_win = __ballot(ids < 0), gone_next = gone_win;
-    constexpr int AHEAD = PRIVATE ? 2 : 1;  // stages from a slot's issue to its use
-    const auto turn_window = [&](int st) __attribute__((always_inline)) {  // before st + AHEAD is issued
+    const auto turn_window = [&](int st) __attribute__((always_inline)) {  // before stage st + 1 is issued
         if (st % WIN == 0 && st > 0) gone_win = gone_next;
-        if ((st + AHEAD) % WIN == 0) ids = ids_next, gone_next = __ballot(ids < 0);
+        if ((st + 1) % WIN == 0) ids = ids_next, gone_next = __ballot(ids < 0);
         if (st % WIN == 0 && st + WIN < nst) ids_next = page_ids(st + WIN);
     };
     const uint64_t kbase = scalar_addr(a.pg.k + g * HD), vbase = scalar_addr(a.pg.v + g * HD);
     const uint64_t zero = scalar_addr(zero_row);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
     const int lr = lane / NCH;
-    uint32_t kx = 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>(lr)), vx = 16 * (uint32_t)(lane % NCH ^ VRead<HD>::v_swz(lr));
+    uint32_t kx = 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>(lr)), vx = 16 * (uint32_t)(lane % NCH ^ v_swz<HD>(lr));
     // the wave's groups of stage st (16 rows of a page each)
-    const auto issue = [&](int st) __attribute__((always_inline)) {
-        const uint32_t slot = lds0 + (uint32_t)(st % kSlots) * SLOT;
+    const auto issue = [&](int st, bool ks, bool vs) __attribute__((always_inline)) {
+        const uint32_t slot = lds0 + (uint32_t)(PRIVATE ? 0 : st % 2) * SLOT;
         asm volatile("" : "+v"(kx), "+v"(vx));  // (else every offset below is kept in registers)
 #pragma unroll
         for (int u = 0; u < OWN; ++u) {
-            const int gr = OWN * wave + u, row = key0 + STAGE * st + 16 * gr;
+            const int gr = OWN * wave + u, r0 = key0 + STAGE * st + 16 * gr;
             const int id = __builtin_amdgcn_readlane(ids, (GROUPS * st + gr) & 63);
-            const uint32_t in = (uint32_t)(row & ((1 << a.pg.page_shift) - 1)) * row_b;
+            const uint32_t in = (uint32_t)(r0 & ((1 << a.pg.page_shift) - 1)) * row_b;
             const uint64_t off = (uint64_t)(uint32_t)id * page_b + in;
             const uint64_t kb = id < 0 ? zero : kbase + off, vb = id < 0 ? zero : vbase + off;
             // rows past the last repeat it (their scores are replaced); an absent
             // group reads the row of zeros
-            const int last = id < 0 ? 0 : kend - 1 - row;
+            const int last = id < 0 ? 0 : kend - 1 - r0;
 #pragma unroll
             for (int x = 0; x < LPG; ++x) {
                 // (the rotation of row x RPI + lr is that of row lr and a constant)
                 const uint32_t ro = __umul24((uint32_t)min(x * RPI + lr, last), row_b);
                 const uint32_t to = slot + (uint32_t)(16 * gr + x * RPI) * (2 * HD);
-                g2l_s(kb, ro + (kx ^ (64 * x)), to);
-                g2l_s(vb, ro + (HD == 128 ? vx ^ (128 * (x & 1)) : vx), to + STAGE * HD * 2);
+                if (ks) g2l_s(kb, ro + (kx ^ (64 * x)), to);
+                if (vs) g2l_s(vb, ro + (HD == 128 ? vx ^ (128 * (x & 1)) : vx), to + STAGE * HD * 2);
             }
         }
     };
-    if (nst > 0) issue(0);
-    if (PRIVATE && nst > 1) issue(1);
+    if (PRIVATE && nst > 0) issue(0, true, false), issue(0, false, true);
+    if (!PRIVATE && nst > 0) issue(0, true, true);
 
-    // this lane's query row, split, and what it attends
     f16x8 qh[KS], ql[KS];
-    RowMask mask;
-    {
-        const int row = 32 * set + n, tl = row / group, hh = row % group;
-        const bool valid = tl < ntok;  // (the others: zeros at the tile's first token)
-        const int i = i0 + (valid ? tl : 0);
-        mask = RowMask{it.cached, it.cached + i + 1, 0, a.pg.parent != nullptr};
-        if (a.pg.parent) {
-            const uint64_t paths = tree_path(a.pg, it.first, it.n);
-            mask.path = ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i) << 32) |
-                        (uint32_t)__shfl((int)(uint32_t)paths, i);
-        }
-        const float* qp = a.q + ((size_t)(it.first + i) * a.nh + g * group + hh) * HD;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (valid) {
-                const float4 x = *reinterpret_cast<const float4*>(qp + 16 * ks + 8 * h);
-                const float4 y = *reinterpret_cast<const float4*>(qp + 16 * ks + 8 * h + 4);
-                v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-            }
+    for (int ks = 0; ks < KS; ++ks) {
+        const float v[8] = {qv[ks][0].x, qv[ks][0].y, qv[ks][0].z, qv[ks][0].w,
+                            qv[ks][1].x, qv[ks][1].y, qv[ks][1].z, qv[ks][1].w};
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                f16x2 hi, lo;
-                pa_split(v[e] * a.qscale, v[e + 1] * a.qscale, hi, lo);
-                qh[ks][e] = hi[0], qh[ks][e + 1] = hi[1], ql[ks][e] = lo[0], ql[ks][e + 1] = lo[1];
-            }
+        for (int e = 0; e < 8; e += 2) {
+            f16x2 hi, lo;
+            pa_split(v[e] * a.qscale, v[e + 1] * a.qscale, hi, lo);
+            qh[ks][e] = hi[0], qh[ks][e + 1] = hi[1], ql[ks][e] = lo[0], ql[ks][e + 1] = lo[1];
         }
     }
+    RowMask mask{it.cached, it.cached + i + 1, 0, a.pg.parent != nullptr};
+    if (a.pg.parent) mask.path = path_of(tree_path(parent), i);
 
     bool redo = false;  // (uniform)
     float mref = -INFINITY, lrun = 0.f;
-    f32x16 o[DB];
+    acc_t o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) o[d][v] = 0.f;
-    const VRead<HD> vr;
-    // this lane's piece 0 of its K row (every second piece from there: XOR 32 ks)
-    const uint32_t krow = (uint32_t)(pa_pi(n) * HD * 2 + 16 * (h ^ pa_swz<HD>(pa_pi(n))));
+        for (int v = 0; v < NA; ++v) o[d][v] = 0.f;
+    const VRead<HD, M> vr;
+    // this lane's first piece of its K row; the next products' are 1024 / M bytes on
+    const int key_row = M == 32 ? pa_pi(n) : 8 * (n >> 2) + (n & 3);
+    const uint32_t krow = (uint32_t)(key_row * HD * 2 + 16 * (h ^ pa_swz<HD>(key_row)));
 
+    const auto wait_v = [&](int st) __attribute__((always_inline)) {  // (the next K's loads may be out)
+        if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
     for (int st = 0; st < nst; ++st) {
         if constexpr (PRIVATE) {
-            if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LPG * OWN) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");  // K, not yet V
         } else {
             // this stage has landed for every wave, and every wave is done with the
             // slot that the next one goes to
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
         turn_window(st);
-        if (!PRIVATE && st + 1 < nst) issue(st + 1);
+        if (!PRIVATE && st + 1 < nst) issue(st + 1, true, true);
         const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
         if (kb < key1) {
-            const uint32_t k0 = lds0 + (uint32_t)(st % kSlots) * SLOT + 32 * kg * HD * 2, v0 = k0 + STAGE * HD * 2;
-            f32x16 s;
+            const uint32_t k0 = lds0 + (uint32_t)(PRIVATE ? 0 : st % 2) * SLOT + 32 * kg * HD * 2, v0 = k0 + STAGE * HD * 2;
+            float s[NP];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) s[v] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
+            for (int b = 0; b < SB; ++b) {
                 typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
-                const f16x8 k = *(lds_f16x8*)(uintptr_t)((k0 + krow) ^ (32 * ks));
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qh[ks], s, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, ql[ks], s, 0, 0, 0);
+                acc_t sb;
+#pragma unroll
+                for (int v = 0; v < NA; ++v) sb[v] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    // (4 keys on: 4 rows on, rotated by another HD / 2 bytes)
+                    const uint32_t at = ((k0 + krow) ^ (uint32_t)(1024 / M * ks) ^ (uint32_t)(b * HD / 2)) + 8 * HD * b;
+                    const f16x8 k = *(lds_f16x8*)(uintptr_t)at;
+                    sb = MM::mul(k, qh[ks], sb);
+                    sb = MM::mul(k, ql[ks], sb);
+                }
+#pragma unroll
+                for (int v = 0; v < NA; ++v) s[NA * b + v] = sb[v];
+            }
+            if constexpr (PRIVATE) {
+                // K's rows have been read: the next ones may come.  V is older than they
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (st + 1 < nst) issue(st + 1, true, false);
             }
             const uint32_t gone = (uint32_t)(gone_win >> (GROUPS * (st % WIN) + 2 * kg)) & 3;
             if (kb + 32 > lim_min || gone) {
-                uint32_t w = mask(kb, h);
+                uint32_t w = mask(kb);
                 if (gone & 1) w &= 0xffff0000u;
                 if (gone & 2) w &= 0xffffu;
+                w >>= 8 * h;  // value v: key 8 h + 16 (v / 8) + v % 8
 #pragma unroll
-                for (int v = 0; v < 16; ++v)
+                for (int v = 0; v < NP; ++v)
                     if (!((w >> (16 * (v >> 3) + (v & 7))) & 1)) s[v] = -INFINITY;
+                if constexpr (PRIVATE) wait_v(st);
                 redo |= any_special<HD>(v0);
             }
             float mx = s[0];
 #pragma unroll
-            for (int v = 1; v < 16; ++v) mx = fmaxf(mx, s[v]);
-            mx = pa_pair_max(mx);
+            for (int v = 1; v < NP; ++v) mx = fmaxf(mx, s[v]);
+            mx = row_max<M>(mx);
             if (__any(mx > mref + kPaSlack)) {  // also the first block with an attended key
                 const float mnew = fmaxf(mref, mx);
                 // (nothing attended so far: the sums are zero)
@@ -457,209 +526,203 @@ __global__ __launch_bounds__(kThreads, HD == 128 && RS == 1 ? 1 : 2) void attent
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+                    for (int v = 0; v < NA; ++v) o[d][v] *= alpha;
             }
             const float ref0 = mref == -INFINITY ? 0.f : mref;
-            float p[16], ps[4] = {0.f, 0.f, 0.f, 0.f};
+            float p[NP], ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
+            for (int v = 0; v < NP; ++v) {
                 p[v] = kPaScale * __builtin_amdgcn_exp2f(s[v] - ref0);
                 ps[v & 3] += p[v];
             }
             lrun += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-            f16x8 bh[2], bl[2];
+            f16x8 bh[TT], bl[TT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < TT; ++t)
 #pragma unroll
                 for (int u = 0; u < 8; u += 2) {
                     f16x2 hi, lo;
                     pa_split(p[8 * t + u], p[8 * t + u + 1], hi, lo);
                     bh[t][u] = hi[0], bh[t][u + 1] = hi[1], bl[t][u] = lo[0], bl[t][u + 1] = lo[1];
                 }
+            if constexpr (PRIVATE) wait_v(st);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < TT; ++t)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     const f16x8 v = vr(v0, t, d);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bh[t], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, bl[t], o[d], 0, 0, 0);
+                    o[d] = MM::mul(v, bh[t], o[d]);
+                    o[d] = MM::mul(v, bl[t], o[d]);
                 }
         }
         if constexpr (PRIVATE) {
-            // the slot's last reads are done before its next rows are requested
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (st + 2 < nst) issue(st + 2);
+            if (st + 1 < nst) issue(st + 1, false, true);
         }
     }
 
-    // the waves' parts meet (every load into the slots has been waited for)
+    // the waves' parts meet, where no load is to come any more
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (__syncthreads_or(redo)) {
-        redo_item<HD, RS>(a, it, g, key0, key1, smem);
+        redo_item<HD, R>(a, it, (int)g, key0, key1, smem);
         return;
     }
     float* ms = reinterpret_cast<float*>(smem);
     {
-        float* mb = ms + wave * merge_floats(HD);
-        const float lsum = lrun + __shfl_xor(lrun, 32, 64);
+        float* mb = ms + wave * merge_floats(HD, M);  // V sums [M rows][HD + 4], references, sums
+        const float lsum = row_sum<M>(lrun);
+        if (valid) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) mb[(32 * d + 8 * (v >> 2) + 4 * h + (v & 3)) * 32 + n] = o[d][v];
-        if (h == 0) {
-            mb[HD * 32 + n] = mref;
-            mb[HD * 32 + 32 + n] = lsum;
+                for (int v = 0; v < NA; v += 4)
+                    *reinterpret_cast<float4*>(mb + n * (HD + 4) + M * d + 2 * v + 4 * h) =
+                        make_float4(o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]);
+            if (h == 0) {
+                mb[M * (HD + 4) + n] = mref;
+                mb[M * (HD + 5) + n] = lsum;
+            }
         }
     }
     __syncthreads();
-    // thread: row 32 mr + mn, dims d0 .. d0 + ND
-    constexpr int ND = HD * RS / 8;
-    const int mr = RS == 2 ? (tid >> 5) & 1 : 0, mn = tid & 31, d0 = (tid >> (RS == 2 ? 6 : 5)) * ND;
-    const float* mb[KG];
-    float wt[KG], M = -INFINITY, L = 0.f;
+    // a thread takes four dims of a row
+    for (int u = tid; u < ntok * (int)group * (HD / 4); u += kThreads) {
+        const int rr = u / (HD / 4), d = 4 * (u % (HD / 4)), rn = rr % M;
+        const float* mb = ms + rr / M * merge_floats(HD, M);
+        constexpr int NEXT = RS * merge_floats(HD, M);  // (the next key group's part)
+        float wt[KG], mm = -INFINITY, ll = 0.f;
 #pragma unroll
-    for (int i = 0; i < KG; ++i) {
-        mb[i] = ms + (i * RS + mr) * merge_floats(HD);
-        M = fmaxf(M, mb[i][HD * 32 + mn]);
-    }
+        for (int k = 0; k < KG; ++k) mm = fmaxf(mm, mb[k * NEXT + M * (HD + 4) + rn]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < KG; ++i) {
-        const float mi = mb[i][HD * 32 + mn];
-        wt[i] = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);  // (nothing attended there)
-        L += wt[i] * mb[i][HD * 32 + 32 + mn];
-    }
-    const int row = 32 * mr + mn, tl = row / group;
-    if (tl >= ntok) return;
-    float* op;
-    float inv = 1.f;
-    if (it.splits > 1) {
-        const size_t p = ((size_t)it.slot * nkv + g) * (32 * RS) + row;
-        op = a.part + p * HD;
-        if (d0 == 0) a.ml[p] = make_float2(M, L);
-    } else {
-        op = a.att + ((size_t)(it.first + i0 + tl) * a.nh + g * group + row % group) * HD;
-        inv = L == 0.f ? 0.f : 1.0f / L;  // (no row exists: zeros)
-    }
-#pragma unroll
-    for (int d = 0; d < ND; d += 4) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < KG; ++i) x[e] += wt[i] * mb[i][(d0 + d + e) * 32 + mn];
+        for (int k = 0; k < KG; ++k) {
+            const float mk = mb[k * NEXT + M * (HD + 4) + rn];
+            wt[k] = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - mm);  // (nothing attended there)
+            ll += wt[k] * mb[k * NEXT + M * (HD + 5) + rn];
+            const float4 v = *reinterpret_cast<const float4*>(mb + k * NEXT + rn * (HD + 4) + d);
+            x.x += wt[k] * v.x, x.y += wt[k] * v.y, x.z += wt[k] * v.z, x.w += wt[k] * v.w;
         }
-        *reinterpret_cast<float4*>(op + d0 + d) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        if (it.splits > 1) {
+            const size_t p = ((size_t)it.slot * nkv + g) * R + rr;
+            if (d == 0) a.ml[p] = make_float2(mm, ll);
+            *reinterpret_cast<float4*>(a.part + p * HD + d) = x;
+        } else {
+            const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // (no row exists: zeros)
+            const int rt = rr / (int)group;
+            *reinterpret_cast<float4*>(a.att + ((size_t)(it.first + i0 + rt) * a.nh + g * group + (rr - rt * (int)group)) * HD + d) =
+                make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        }
     }
 }
 
-// att from the splits' parts: a workgroup takes 4 rows of one tile and kv
-// head, a thread four dims of a row and every (256 / HD)-th... split
-constexpr int kMergeRows = 4, kMergeThreads = 512;
-template <int HD, int RS>
+// att from the splits' parts: a workgroup takes 16 rows of a tile and kv head,
+// a thread four dims of a row, and where there are fewer rows every LANES-th
+// split
+constexpr int kMergeRows = 16, kMergeThreads = 512;
+template <int HD, int R>
 __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(AttnPagedArgs a) {
-    constexpr int PER = kMergeRows * HD / 4, LANES = kMergeThreads / PER, AHEAD = 4;
+    constexpr int AHEAD = 8, RB = R / kMergeRows;
     __shared__ float4 acc[kMergeThreads];
     __shared__ float2 st[kMergeThreads];
-    constexpr int RB = 32 * RS / kMergeRows;
-    const int nkv = a.pg.nkv, group = a.nh / nkv, T = 32 * RS / group;
-    const int rb = blockIdx.x % RB, g = blockIdx.x / RB % nkv;
+    const int nkv = a.pg.nkv, group = a.nh / nkv, T = R / group;
+    const uint32_t rb = blockIdx.x % RB, index = blockIdx.x / RB / (uint32_t)nkv, g = blockIdx.x / RB - index * nkv;
     Item it;
-    if (!paged_item<true>(a.pg, T, a.target, blockIdx.x / RB / nkv, it) || it.splits < 2) return;
-    const int ntok = min(T, it.n - it.tile * T);
-    if (rb * kMergeRows >= ntok * group) return;
-    const int tid = threadIdx.x, d = 4 * (tid % (HD / 4)), row = rb * kMergeRows + tid / (HD / 4) % kMergeRows;
-    const int z0 = tid / PER;
-    const bool valid = row < ntok * group;
+    if (!paged_item<true>(a.pg, T, a.target, index, it)) return;
+    const int rows = min(min(T, it.n - it.tile * T) * group - (int)rb * kMergeRows, kMergeRows);
+    if (rows <= 0) return;
+    const int tid = threadIdx.x, per = rows * (HD / 4), lanes = kMergeThreads / per;
+    const int z0 = tid / per, u = tid % per, d = 4 * (u % (HD / 4)), row = rb * kMergeRows + u / (HD / 4);
     float M = -INFINITY, L = 0.f;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int z = z0; valid && z < it.splits; z += LANES * AHEAD) {
-        float2 t[AHEAD];
-        float4 v[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const size_t p = ((size_t)(it.slot + min(z + i * LANES, it.splits - 1)) * nkv + g) * (32 * RS) + row;
-            t[i] = a.ml[p];
-            v[i] = *reinterpret_cast<const float4*>(a.part + p * HD + d);
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (z + i * LANES >= it.splits || t[i].x == -INFINITY) continue;  // (nothing attended there)
-            const float m1 = fmaxf(M, t[i].x), a0 = __builtin_amdgcn_exp2f(M - m1), a1 = __builtin_amdgcn_exp2f(t[i].x - m1);
-            M = m1;
-            L = L * a0 + t[i].y * a1;
-            s.x = s.x * a0 + v[i].x * a1, s.y = s.y * a0 + v[i].y * a1;
-            s.z = s.z * a0 + v[i].z * a1, s.w = s.w * a0 + v[i].w * a1;
-        }
-    }
-    acc[tid] = s;
-    st[tid] = make_float2(M, L);
-    __syncthreads();
-    if (!valid || z0) return;
-    for (int i = 1; i < LANES; ++i) {
-        const float2 t = st[tid + i * PER];
-        const float4 v = acc[tid + i * PER];
-        if (t.x == -INFINITY) continue;
+    const auto join = [&](float2 t, float4 v) __attribute__((always_inline)) {
+        if (t.x == -INFINITY) return;  // (nothing attended there)
         const float m1 = fmaxf(M, t.x), a0 = __builtin_amdgcn_exp2f(M - m1), a1 = __builtin_amdgcn_exp2f(t.x - m1);
         M = m1;
         L = L * a0 + t.y * a1;
         s.x = s.x * a0 + v.x * a1, s.y = s.y * a0 + v.y * a1, s.z = s.z * a0 + v.z * a1, s.w = s.w * a0 + v.w * a1;
+    };
+    if (z0 < lanes)
+        for (int z = z0; z < it.splits; z += lanes * AHEAD) {
+            float2 t[AHEAD];
+            float4 v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const size_t p = ((size_t)(it.slot + min(z + i * lanes, it.splits - 1)) * nkv + g) * R + row;
+                t[i] = a.ml[p];
+                v[i] = *reinterpret_cast<const float4*>(a.part + p * HD + d);
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (z + i * lanes < it.splits) join(t[i], v[i]);
+        }
+    if (lanes > 1) {
+        acc[tid] = s;
+        st[tid] = make_float2(M, L);
+        __syncthreads();
     }
+    if (z0) return;
+    for (int i = 1; i < lanes; ++i) join(st[tid + i * per], acc[tid + i * per]);
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    *reinterpret_cast<float4*>(a.att + ((size_t)(it.first + it.tile * T + row / group) * a.nh + g * group + row % group) * HD + d) =
+    const size_t tok = (size_t)it.first + it.tile * T + row / group;
+    *reinterpret_cast<float4*>(a.att + (tok * a.nh + g * group + row % group) * HD + d) =
         make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
 
 // What the host can choose without the lengths: rows of a tile by the average
 // sequence, and the number of items that the splits aim at.
 struct Shape {
-    int rs, target;
-    int64_t tiles;  // at most
+    int rows, target;
+    int64_t items;  // at most
 };
 Shape attention_shape(const PagedArgs& a, int nh, int hd) {
     Shape s;
     const int group = nh / a.nkv;
-    s.rs = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group > 32 ? 2 : 1;
-    const int T = 32 * s.rs / group;
-    s.tiles = a.n_tokens / T + a.n_seq;
-    const int resident = (hd == 128 ? 1 : 2) * device_cus();
-    s.target = ((int64_t)a.table_ld << a.page_shift) > kStage ? std::max(2, resident / a.nkv) : 0;
+    const int64_t want = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group;
+    s.rows = want > 32 ? 64 : want > 16 ? 32 : 16;
+    const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq;
+    const int64_t stages = (((int64_t)a.table_ld << a.page_shift) + kStage - 1) / kStage;  // of a tile, at most
+    const int resident = (hd == 128 ? 2 : hd == 64 ? 3 : 4) * device_cus();
+    static const double mult = getenv("MXH_MULT") ? atof(getenv("MXH_MULT")) : 1.0;
+    s.target = stages > 1 ? std::max(2, (int)(mult * resident / a.nkv)) : 0;
+    s.items = std::min(s.target + tiles, tiles * stages);
     return s;
 }
 
-template <int HD, int RS>
+template <int HD, int R>
 int launch(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
     static bool attr_set = false;  // above 64 KiB of LDS needs the opt-in, once per kernel
-    if (!attr_set && lds_bytes(HD, RS) > 65536) {
-        if (hipFuncSetAttribute((const void*)attention_paged_kernel<HD, RS>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                lds_bytes(HD, RS)) != hipSuccess)
+    if (!attr_set && lds_bytes(HD, R) > 65536) {
+        if (hipFuncSetAttribute((const void*)attention_paged_kernel<HD, R>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                lds_bytes(HD, R)) != hipSuccess)
             return MXH_ERR_HIP;
         attr_set = true;
     }
-    const int64_t items = (sh.target + sh.tiles) * a.pg.nkv, merges = sh.tiles * a.pg.nkv * (32 * RS / kMergeRows);
+    const int64_t items = sh.items * a.pg.nkv, merges = (int64_t)sh.target * a.pg.nkv * (R / kMergeRows);
     if (items * kThreads > UINT32_MAX || merges * kMergeThreads > UINT32_MAX) return MXH_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((attention_paged_kernel<HD, RS>), dim3((unsigned)items), dim3(kThreads), lds_bytes(HD, RS), st, a);
+    hipLaunchKernelGGL((attention_paged_kernel<HD, R>), dim3((unsigned)items), dim3(kThreads), lds_bytes(HD, R), st, a);
     if (sh.target > 0)
-        hipLaunchKernelGGL((attention_paged_merge_kernel<HD, RS>), dim3((unsigned)merges), dim3(kMergeThreads), 0, st, a);
+        hipLaunchKernelGGL((attention_paged_merge_kernel<HD, R>), dim3((unsigned)merges), dim3(kMergeThreads), 0, st, a);
     return MXH_OK;
+}
+
+template <int HD>
+int launch_hd(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
+    return sh.rows == 64 ? launch<HD, 64>(a, sh, st) : sh.rows == 32 ? launch<HD, 32>(a, sh, st) : launch<HD, 16>(a, sh, st);
 }
 
 }  // namespace
 
 size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd) {
     const Shape s = attention_shape(a, nh, hd);
-    return (size_t)2 * s.target * a.nkv * 32 * s.rs * (hd + 2) * sizeof(float);
+    return (size_t)2 * s.target * a.nkv * s.rows * (hd + 2) * sizeof(float);
 }
 
 int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, float* att, void* work, hipStream_t st) {
     const Shape s = attention_shape(a, nh, hd);
     float* part = static_cast<float*>(work);
-    float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * s.target * a.nkv * 32 * s.rs * hd);
+    float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * s.target * a.nkv * s.rows * hd);
     const AttnPagedArgs args{a, q, att, part, ml, nh, s.target, 1.4426950408889634f / sqrtf((float)hd)};
-    switch (hd) {
-    case 32: return s.rs == 2 ? launch<32, 2>(args, s, st) : launch<32, 1>(args, s, st);
-    case 64: return s.rs == 2 ? launch<64, 2>(args, s, st) : launch<64, 1>(args, s, st);
-    default: return s.rs == 2 ? launch<128, 2>(args, s, st) : launch<128, 1>(args, s, st);
-    }
+    return hd == 32 ? launch_hd<32>(args, s, st) : hd == 64 ? launch_hd<64>(args, s, st) : launch_hd<128>(args, s, st);
 }
 
 }  // namespace mxh
