@@ -57,7 +57,8 @@ constexpr int kStage = 128;                // keys that splits are made of
 // floats a wave leaves for the merge: V sums [m][hd + 4], references, sums
 __host__ __device__ constexpr int merge_floats(int hd, int m) { return m * (hd + 6); }
 __host__ __device__ constexpr int lds_bytes(int hd, int rows) {
-    const int ring = 2 * kStage * hd * 2, merge = kWaves * merge_floats(hd, rows < 32 ? 16 : 32) * 4;
+    const int ring = 2 * kStage * hd * 2,  // R = 16: a stage, R = 64: two of half its keys
+               merge = kWaves * merge_floats(hd, rows == 16 ? 16 : 32) * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -335,11 +336,14 @@ __device__ __forceinline__ float row_sum(float v) {
     return v + lane_xor<32>(v);
 }
 
-// R = 16, 32: every wave takes 32 keys of a stage of 128 for all rows of the
-// tile and reads only what it loaded: no barrier before the merge.  K and V have
-// one place each; the next K comes while V is used, the next V while K is.
+// R = 16: every wave takes 32 keys of a stage of 128 for all rows of the tile
+// and reads only what it loaded: no barrier before the merge.  K and V have one
+// place each; the next K comes while V is used, the next V while K is.
 // R = 64: two waves, one a set of 32 rows, take the same 32 keys of a stage of
-// 64, which all four waves load, two stages in LDS and a barrier a stage.
+// 64, which all four waves load, a barrier a stage.  The scores run a stage
+// ahead, so that a wave's products of the next scores and its vector work on
+// these can overlap: at stage st there are V(st), K(st + 1), and on their way
+// V(st + 1), K(st + 2).
 template <int HD, int R>
 __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedArgs a) {
     constexpr int M = R == 16 ? 16 : 32, RS = R / M;  // rows of a wave; waves to a key group
@@ -349,8 +353,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     constexpr int NCH = HD / 8, KG = kWaves / RS, STAGE = 32 * KG;  // 16-byte pieces of a row; keys of a stage
     constexpr int GROUPS = STAGE / 16, OWN = GROUPS / kWaves;       // page groups of a stage; of them a wave loads
     constexpr int RPI = 64 / NCH, LPG = 16 / RPI;     // rows a load brings; loads of 16 rows (K or V)
-    constexpr int SLOT = 2 * STAGE * HD * 2;
     constexpr bool PRIVATE = RS == 1;
+    // LDS: K places, then V places, of a stage each; q's rows before R = 64 needs the second ones
+    constexpr int PLACE = STAGE * HD * 2, V0 = (PRIVATE ? 1 : 2) * PLACE;
     using MM = Mfma<M>;
     using acc_t = typename MM::acc;
     extern __shared__ __align__(256) uint8_t smem[];
@@ -369,13 +374,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     const int key1 = min(key0 + kStage * it.stages, kend);
     const int nst = max((key1 - key0 + STAGE - 1) / STAGE, 0);
 
-    // this lane's query row; its loads go first, those of K and V come back after them
+    // this lane's query row
     const uint32_t row = 32 * set + n, tl = row / group;
     const bool valid = (int)tl < ntok;  // (the others: zeros at the tile's first token)
     const int i = i0 + (valid ? (int)tl : 0);
+    const size_t qd = (size_t)a.nh * HD;
+    const float* q0 = a.q + (size_t)(it.first + i0) * qd + g * group * HD;  // the tile's rows
     float4 qv[KS][2];
-    {
-        const float* qp = a.q + ((size_t)(it.first + i) * a.nh + g * group + (row - tl * group)) * HD + 8 * h;
+    if constexpr (PRIVATE) {  // (few rows: their loads go first, those of K and V come back after them)
+        const float* qp = q0 + (i - i0) * qd + (row - tl * group) * HD + 8 * h;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -384,57 +391,121 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     }
     const int parent = a.pg.parent ? tree_parent(a.pg, it.first, it.n) : -1;
 
-    // Lane l holds the page of 16-row group l of a window of 64 groups
-    const uint32_t row_b = 2u * nkv * HD, page_b = row_b << a.pg.page_shift;
+    // Where the stages' rows are: lane l holds the byte offset in the pool of
+    // 16-row group l of a window of 64 groups (a page holds whole groups), the
+    // high word negative where there is none, and that of the next window
+    const uint32_t row_b = 2u * nkv * HD;
     const int* table = a.pg.table + (size_t)it.s * a.pg.table_ld;
     constexpr int WIN = 64 / GROUPS;  // stages of a window
-    const auto page_ids = [&](int st) __attribute__((always_inline)) {
-        const int r = key0 + STAGE * st + 16 * lane, p = r >> a.pg.page_shift;
+    int2 win, win_next{0, -1};
+    const auto window = [&](int w) __attribute__((always_inline)) {
+        const int r = key0 + STAGE * WIN * w + 16 * lane, p = r >> a.pg.page_shift;
         int id = -1;
         if (r < kend && r >= 0 && p < a.pg.table_ld) id = table[p];
-        return (unsigned)id < (unsigned)a.pg.n_pages ? id : -1;
+        const uint64_t row = ((uint64_t)(uint32_t)id << a.pg.page_shift) + (r & ((1 << a.pg.page_shift) - 1));
+        const uint64_t off = (unsigned)id < (unsigned)a.pg.n_pages ? row * row_b : ~0ull;
+        return make_int2((int)(uint32_t)off, (int)(uint32_t)(off >> 32));
     };
-    int ids = page_ids(0), ids_next = ids;
-    // absent groups of the current stage's window, and of the one issued from
-    uint64_t gone_win = __ballot(ids < 0), gone_next = gone_win;
-    const auto turn_window = [&](int st) __attribute__((always_inline)) {  // before stage st + 1 is issued
-        if (st % WIN == 0 && st > 0) gone_win = gone_next;
-        if ((st + 1) % WIN == 0) ids = ids_next, gone_next = __ballot(ids < 0);
-        if (st % WIN == 0 && st + WIN < nst) ids_next = page_ids(st + WIN);
+    win = window(0);
+    if (nst > WIN) win_next = window(1);
+    uint64_t gone_win = __ballot(win.y < 0);
+    // the wave's groups of a stage, and which of all its groups are absent (a bit each)
+    struct Place {
+        int lo[OWN], hi[OWN];
+        int r0;  // key of the first row
+        uint32_t gone;
     };
-    const uint64_t kbase = scalar_addr(a.pg.k + g * HD), vbase = scalar_addr(a.pg.v + g * HD);
-    const uint64_t zero = scalar_addr(zero_row);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    const int lr = lane / NCH;
-    uint32_t kx = 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>(lr)), vx = 16 * (uint32_t)(lane % NCH ^ v_swz<HD>(lr));
-    // the wave's groups of stage st (16 rows of a page each)
-    const auto issue = [&](int st, bool ks, bool vs) __attribute__((always_inline)) {
-        const uint32_t slot = lds0 + (uint32_t)(PRIVATE ? 0 : st % 2) * SLOT;
-        asm volatile("" : "+v"(kx), "+v"(vx));  // (else every offset below is kept in registers)
+    const auto look_up = [&](int st) __attribute__((always_inline)) {  // stages in their order
+        if (st % WIN == 0 && st > 0) {
+            win = win_next;
+            gone_win = __ballot(win.y < 0);
+            if (st + WIN < nst) win_next = window(st / WIN + 1);
+        }
+        Place p;
 #pragma unroll
         for (int u = 0; u < OWN; ++u) {
-            const int gr = OWN * wave + u, r0 = key0 + STAGE * st + 16 * gr;
-            const int id = __builtin_amdgcn_readlane(ids, (GROUPS * st + gr) & 63);
-            const uint32_t in = (uint32_t)(r0 & ((1 << a.pg.page_shift) - 1)) * row_b;
-            const uint64_t off = (uint64_t)(uint32_t)id * page_b + in;
-            const uint64_t kb = id < 0 ? zero : kbase + off, vb = id < 0 ? zero : vbase + off;
-            // rows past the last repeat it (their scores are replaced); an absent
-            // group reads the row of zeros
-            const int last = id < 0 ? 0 : kend - 1 - r0;
+            p.lo[u] = __builtin_amdgcn_readlane(win.x, (GROUPS * st + OWN * wave + u) & 63);
+            p.hi[u] = __builtin_amdgcn_readlane(win.y, (GROUPS * st + OWN * wave + u) & 63);
+        }
+        p.r0 = key0 + STAGE * st + 16 * OWN * wave;
+        p.gone = (uint32_t)(gone_win >> (GROUPS * st & 63)) & ((1u << GROUPS) - 1);
+        return p;
+    };
+    const uint64_t kbase = scalar_addr(a.pg.k + g * HD), vbase = scalar_addr(a.pg.v + g * HD);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const auto k_place = [&](int st) { return lds0 + (PRIVATE ? 0 : (uint32_t)(st & 1) * PLACE); };
+    const auto v_place = [&](int st) { return lds0 + V0 + (PRIVATE ? 0 : (uint32_t)(st & 1) * PLACE); };
+    // lane offsets of the loads of 16 rows: row, and the row's piece that belongs
+    // in the lane's place of the LDS row
+    const uint32_t lr = (uint32_t)(lane / NCH);
+    uint32_t koff[LPG], voff[LPG];
 #pragma unroll
-            for (int x = 0; x < LPG; ++x) {
-                // (the rotation of row x RPI + lr is that of row lr and a constant)
-                const uint32_t ro = __umul24((uint32_t)min(x * RPI + lr, last), row_b);
-                const uint32_t to = slot + (uint32_t)(16 * gr + x * RPI) * (2 * HD);
-                if (ks) g2l_s(kb, ro + (kx ^ (64 * x)), to);
-                if (vs) g2l_s(vb, ro + (HD == 128 ? vx ^ (128 * (x & 1)) : vx), to + STAGE * HD * 2);
+    for (int x = 0; x < LPG; ++x) {
+        const uint32_t r = x * RPI + lr;
+        koff[x] = r * row_b + 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>((int)r));
+        voff[x] = r * row_b + 16 * (uint32_t)(lane % NCH ^ v_swz<HD>((int)r));
+    }
+    // the wave's rows of a stage into K's or V's place
+    const auto issue = [&](const Place& p, uint32_t place, bool is_v) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < OWN; ++u) {
+            const uint32_t to = place + 32 * (OWN * wave + u) * HD;
+            const uint32_t(&off)[LPG] = is_v ? voff : koff;
+            const uint64_t from = (is_v ? vbase : kbase) + (((uint64_t)(uint32_t)p.hi[u] << 32) | (uint32_t)p.lo[u]);
+            if (p.hi[u] >= 0 && p.r0 + 16 * u + 15 < kend) {
+#pragma unroll
+                for (int x = 0; x < LPG; ++x) g2l_s(from, off[x], to + 1024 * x);
+            } else {
+                // rows past the last repeat it (their scores are replaced); an absent
+                // group reads the row of zeros
+                const bool none = p.hi[u] < 0;
+                const uint32_t last = none ? 0 : (uint32_t)(kend - 1 - p.r0 - 16 * u);
+                const uint64_t at = none ? scalar_addr(zero_row) : from;
+#pragma unroll
+                for (int x = 0; x < LPG; ++x) {
+                    const uint32_t r = x * RPI + lr;
+                    g2l_s(at, off[x] - (r - min(r, last)) * row_b, to + 1024 * x);
+                }
             }
         }
     };
-    if (PRIVATE && nst > 0) issue(0, true, false), issue(0, false, true);
-    if (!PRIVATE && nst > 0) issue(0, true, true);
-
+    Place ahead;  // of the next rows to come
     f16x8 qh[KS], ql[KS];
+    uint32_t gone = 0, gone_next = 0;  // of the current stage, and of the next
+    if (nst > 0) ahead = look_up(0), gone = ahead.gone;
+    if constexpr (PRIVATE) {
+        if (nst > 0) issue(ahead, k_place(0), false), issue(ahead, v_place(0), true);
+    } else {
+        // q's rows through LDS, in the places of K(1) and V(1), 16-byte pieces
+        // rotated by the row (a lane reads its row, not its load's neighbour's)
+        constexpr int QP = HD / 4, QR = 64 / QP;  // pieces of a row, rows a load brings
+        const uint64_t from = scalar_addr(q0);
+#pragma unroll
+        for (int x = 0; x < R / QR / kWaves; ++x) {
+            const uint32_t r0 = (uint32_t)(R / kWaves * wave + QR * x), r = r0 + lane / QP;
+            const uint32_t t = min(r / group, (uint32_t)ntok - 1);
+            const uint32_t off = 4 * (t * (uint32_t)qd + (r - r / group * group) * HD) + 16 * ((lane % QP) ^ (r & 7));
+            const uint32_t at = r0 * 4 * HD;
+            g2l_s(from, off, lds0 + (at < PLACE ? PLACE + at : V0 + at));
+        }
+        if (nst > 0) issue(ahead, k_place(0), false), issue(ahead, v_place(0), true);
+        if (nst > 0) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LPG * OWN) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+        const uint32_t at = row * 4 * HD, q = lds0 + (at < PLACE ? PLACE + at : V0 + at);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const f32x4 x = *(lds_f32x4*)(uintptr_t)(q + 16 * ((4 * ks + 2 * h + e) ^ (row & 7)));
+                qv[ks][e] = valid ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (nst > 1) {
+            ahead = look_up(1), gone_next = ahead.gone;
+            issue(ahead, k_place(1), false);
+        }
+    }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const float v[8] = {qv[ks][0].x, qv[ks][0].y, qv[ks][0].z, qv[ks][0].w,
@@ -461,103 +532,185 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     const int key_row = M == 32 ? pa_pi(n) : 8 * (n >> 2) + (n & 3);
     const uint32_t krow = (uint32_t)(key_row * HD * 2 + 16 * (h ^ pa_swz<HD>(key_row)));
 
-    const auto wait_v = [&](int st) __attribute__((always_inline)) {  // (the next K's loads may be out)
-        if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    };
-    for (int st = 0; st < nst; ++st) {
-        if constexpr (PRIVATE) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");  // K, not yet V
-        } else {
-            // this stage has landed for every wave, and every wave is done with the
-            // slot that the next one goes to
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // scores of the wave's keys with K's rows at k0
+    const auto score = [&](uint32_t k0, acc_t (&s)[SB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < SB; ++b) {
+            typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+#pragma unroll
+            for (int v = 0; v < NA; ++v) s[b][v] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                // (4 keys on: 4 rows on, rotated by another HD / 2 bytes)
+                const uint32_t at = ((k0 + krow) ^ (uint32_t)(1024 / M * ks) ^ (uint32_t)(b * HD / 2)) + 8 * HD * b;
+                const f16x8 k = *(lds_f16x8*)(uintptr_t)at;
+                s[b] = MM::mul(k, qh[ks], s[b]);
+                s[b] = MM::mul(k, ql[ks], s[b]);
+            }
         }
-        turn_window(st);
-        if (!PRIVATE && st + 1 < nst) issue(st + 1, true, true);
-        const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
-        if (kb < key1) {
-            const uint32_t k0 = lds0 + (uint32_t)(PRIVATE ? 0 : st % 2) * SLOT + 32 * kg * HD * 2, v0 = k0 + STAGE * HD * 2;
-            float s[NP];
+    };
+    // masks, and the reference moved where a score exceeds it by far
+    const auto settle = [&](int kb, uint32_t v0, acc_t (&s)[SB], auto&& v_there) __attribute__((always_inline)) {
+        if (kb + 32 > lim_min || gone) {
+            uint32_t w = mask(kb);
+            if (gone >> (2 * kg) & 1) w &= 0xffff0000u;
+            if (gone >> (2 * kg) & 2) w &= 0xffffu;
+            w >>= 8 * h;  // value v: key 8 h + 16 (v / 8) + v % 8
 #pragma unroll
-            for (int b = 0; b < SB; ++b) {
-                typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
-                acc_t sb;
+            for (int v = 0; v < NP; ++v)
+                if (!((w >> (16 * (v >> 3) + (v & 7))) & 1)) s[v / NA][v % NA] = -INFINITY;
+            v_there();
+            redo |= any_special<HD>(v0);
+        }
+        float mx = s[0][0];
 #pragma unroll
-                for (int v = 0; v < NA; ++v) sb[v] = 0.f;
+        for (int v = 1; v < NP; ++v) mx = fmaxf(mx, s[v / NA][v % NA]);
+        mx = row_max<M>(mx);
+        if (__any(mx > mref + kPaSlack)) {  // also the first block with an attended key
+            const float mnew = fmaxf(mref, mx);
+            // (nothing attended so far: the sums are zero)
+            const float alpha = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
+            mref = mnew;
+            lrun *= alpha;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    // (4 keys on: 4 rows on, rotated by another HD / 2 bytes)
-                    const uint32_t at = ((k0 + krow) ^ (uint32_t)(1024 / M * ks) ^ (uint32_t)(b * HD / 2)) + 8 * HD * b;
-                    const f16x8 k = *(lds_f16x8*)(uintptr_t)at;
-                    sb = MM::mul(k, qh[ks], sb);
-                    sb = MM::mul(k, ql[ks], sb);
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int v = 0; v < NA; ++v) o[d][v] *= alpha;
+        }
+    };
+    f16x8 bh[TT], bl[TT];
+    const auto weigh = [&](const acc_t (&s)[SB]) __attribute__((always_inline)) {
+        const float ref0 = mref == -INFINITY ? 0.f : mref;
+        float p[NP], ps[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < NP; ++v) {
+            p[v] = kPaScale * __builtin_amdgcn_exp2f(s[v / NA][v % NA] - ref0);
+            ps[v & 3] += p[v];
+        }
+        lrun += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int u = 0; u < 8; u += 2) {
+                f16x2 hi, lo;
+                pa_split(p[8 * t + u], p[8 * t + u + 1], hi, lo);
+                bh[t][u] = hi[0], bh[t][u + 1] = hi[1], bl[t][u] = lo[0], bl[t][u + 1] = lo[1];
+            }
+    };
+    const auto sum = [&](uint32_t v0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const f16x8 v = vr(v0, t, d);
+                o[d] = MM::mul(v, bh[t], o[d]);
+                o[d] = MM::mul(v, bl[t], o[d]);
+            }
+    };
+
+    // R = 64: weigh, the next score and sum with the first two's work interleaved
+    // as written (a product keeps the matrix cores busy for 32 cycles, in which a
+    // wave can issue seven vector instructions; left to itself the scheduler puts
+    // one behind the other)
+    const auto weigh_and_score = [&](uint32_t k0, uint32_t v0, const acc_t (&s)[SB], acc_t (&next)[SB]) __attribute__((always_inline)) {
+        if constexpr (!PRIVATE) {
+            constexpr int VALS = NP / (2 * KS), AHEAD = KS < 3 ? KS : 3;  // scores of a product; operands on their way
+            typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+            const float ref0 = mref == -INFINITY ? 0.f : mref;
+            f16x8 kf[KS], vf[TT * DB];
+            const auto k_read = [&](int ks) { kf[ks] = *(lds_f16x8*)(uintptr_t)((k0 + krow) ^ (uint32_t)(32 * ks)); };
+#pragma unroll
+            for (int ks = 0; ks < AHEAD; ++ks) k_read(ks);
+#pragma unroll
+            for (int v = 0; v < NA; ++v) next[0][v] = 0.f;
+            float ps[4] = {0.f, 0.f, 0.f, 0.f};
+            __builtin_amdgcn_sched_barrier(0);
+            float p[NP];
+            const auto halves = [&](int u) {  // of values u and u + 1
+                f16x2 hi, lo;
+                pa_split(p[u], p[u + 1], hi, lo);
+                bh[u / 8][u % 8] = hi[0], bh[u / 8][u % 8 + 1] = hi[1];
+                bl[u / 8][u % 8] = lo[0], bl[u / 8][u % 8 + 1] = lo[1];
+            };
+#pragma unroll
+            for (int j = 0; j < 2 * KS; ++j) {
+                const int ks = j / 2;
+                next[0] = MM::mul(kf[ks], j & 1 ? ql[ks] : qh[ks], next[0]);
+                if (j & 1) {
+                    if (ks + AHEAD < KS) k_read(ks + AHEAD);
+                    else if (ks + AHEAD - KS < TT * DB) vf[ks + AHEAD - KS] = vr(v0, (ks + AHEAD - KS) / DB, (ks + AHEAD - KS) % DB);
                 }
 #pragma unroll
-                for (int v = 0; v < NA; ++v) s[NA * b + v] = sb[v];
-            }
-            if constexpr (PRIVATE) {
-                // K's rows have been read: the next ones may come.  V is older than they
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                if (st + 1 < nst) issue(st + 1, true, false);
-            }
-            const uint32_t gone = (uint32_t)(gone_win >> (GROUPS * (st % WIN) + 2 * kg)) & 3;
-            if (kb + 32 > lim_min || gone) {
-                uint32_t w = mask(kb);
-                if (gone & 1) w &= 0xffff0000u;
-                if (gone & 2) w &= 0xffffu;
-                w >>= 8 * h;  // value v: key 8 h + 16 (v / 8) + v % 8
-#pragma unroll
-                for (int v = 0; v < NP; ++v)
-                    if (!((w >> (16 * (v >> 3) + (v & 7))) & 1)) s[v] = -INFINITY;
-                if constexpr (PRIVATE) wait_v(st);
-                redo |= any_special<HD>(v0);
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int v = 1; v < NP; ++v) mx = fmaxf(mx, s[v]);
-            mx = row_max<M>(mx);
-            if (__any(mx > mref + kPaSlack)) {  // also the first block with an attended key
-                const float mnew = fmaxf(mref, mx);
-                // (nothing attended so far: the sums are zero)
-                const float alpha = mref == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mref - mnew);
-                mref = mnew;
-                lrun *= alpha;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int v = 0; v < NA; ++v) o[d][v] *= alpha;
-            }
-            const float ref0 = mref == -INFINITY ? 0.f : mref;
-            float p[NP], ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int v = 0; v < NP; ++v) {
-                p[v] = kPaScale * __builtin_amdgcn_exp2f(s[v] - ref0);
-                ps[v & 3] += p[v];
+                for (int u = VALS * j; u < VALS * (j + 1); ++u) {
+                    p[u] = kPaScale * __builtin_amdgcn_exp2f(s[0][u] - ref0);
+                    ps[u & 3] += p[u];
+                    if (u & 1) halves(u - 1);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
             lrun += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-            f16x8 bh[TT], bl[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-#pragma unroll
-                for (int u = 0; u < 8; u += 2) {
-                    f16x2 hi, lo;
-                    pa_split(p[8 * t + u], p[8 * t + u + 1], hi, lo);
-                    bh[t][u] = hi[0], bh[t][u + 1] = hi[1], bl[t][u] = lo[0], bl[t][u + 1] = lo[1];
-                }
-            if constexpr (PRIVATE) wait_v(st);
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const f16x8 v = vr(v0, t, d);
-                    o[d] = MM::mul(v, bh[t], o[d]);
-                    o[d] = MM::mul(v, bl[t], o[d]);
-                }
+            for (int y = 0; y < TT * DB; ++y) {
+                o[y % DB] = MM::mul(vf[y], bh[y / DB], o[y % DB]);
+                o[y % DB] = MM::mul(vf[y], bl[y / DB], o[y % DB]);
+                if (y + AHEAD < TT * DB) vf[y + AHEAD] = vr(v0, (y + AHEAD) / DB, (y + AHEAD) % DB);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        if constexpr (PRIVATE) {
+    };
+
+    if constexpr (PRIVATE) {
+        for (int st = 0; st < nst; ++st) {
+            const uint32_t k0 = k_place(st) + 64 * kg * HD, v0 = v_place(st) + 64 * kg * HD;
+            const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
+            const auto v_there = [&] {  // (the next K's loads may be out)
+                if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            };
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");  // K, not yet V
+            acc_t s[SB];
+            score(k0, s);
+            // K's rows have been read: the next ones may come
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (st + 1 < nst) issue(st + 1, false, true);
+            if (st + 1 < nst) {
+                ahead = look_up(st + 1);
+                issue(ahead, k_place(0), false);
+            }
+            if (kb < key1) {
+                settle(kb, v0, s, v_there);
+                weigh(s);
+                v_there();
+                sum(v0);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (st + 1 < nst) issue(ahead, v_place(0), true), gone = ahead.gone;
+        }
+    } else {
+        acc_t s[SB], next[SB];
+        if (nst > 0) {
+            // K(0) has landed for every wave (V(0) with it; K(1) may be out)
+            if (nst > 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(LPG * OWN) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            score(k_place(0) + 64 * kg * HD, s);
+        }
+        for (int st = 0; st < nst; ++st) {
+            // V(st) and K(st + 1) have landed for every wave, and every wave is done
+            // with V(st - 1) and K(st)
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (st + 1 < nst) issue(ahead, v_place(st + 1), true);
+            if (st + 2 < nst) {
+                ahead = look_up(st + 2);
+                issue(ahead, k_place(st), false);
+            }
+            const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
+            const uint32_t v0 = v_place(st) + 64 * kg * HD;
+            // (a block behind the last key has every score replaced)
+            settle(kb, v0, s, [] {});
+            // (past the last stage the scores of whatever lies there, unused)
+            weigh_and_score(k_place(st + 1) + 64 * kg * HD, v0, s, next);
+#pragma unroll
+            for (int b = 0; b < SB; ++b) s[b] = next[b];
+            gone = gone_next, gone_next = ahead.gone;
         }
     }
 
@@ -678,7 +831,7 @@ Shape attention_shape(const PagedArgs& a, int nh, int hd) {
     Shape s;
     const int group = nh / a.nkv;
     const int64_t want = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group;
-    s.rows = want > 32 ? 64 : want > 16 ? 32 : 16;
+    s.rows = want > 16 ? 64 : 16;
     const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq;
     const int64_t stages = (((int64_t)a.table_ld << a.page_shift) + kStage - 1) / kStage;  // of a tile, at most
     const int resident = (hd == 128 ? 2 : hd == 64 ? 3 : 4) * device_cus();
@@ -707,7 +860,7 @@ int launch(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
 
 template <int HD>
 int launch_hd(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
-    return sh.rows == 64 ? launch<HD, 64>(a, sh, st) : sh.rows == 32 ? launch<HD, 32>(a, sh, st) : launch<HD, 16>(a, sh, st);
+    return sh.rows == 64 ? launch<HD, 64>(a, sh, st) : launch<HD, 16>(a, sh, st);
 }
 
 }  // namespace
