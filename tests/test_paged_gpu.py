@@ -263,6 +263,27 @@ def test_infinite_values_come_through_where_attended(mxh):
     c.close()
 
 
+@pytest.mark.parametrize("seqs,tree", [([(300, 1)], False), ([(40, 30), (700, 50)], False), ([(130, 20), (5, 1)], True)])
+def test_nan_reaches_the_outputs_that_read_it(mxh, seqs, tree):
+    """A NaN in a token's q is its head's; NaN in a cached key is everybody's who attends it, in its kv head."""
+    c = Case(seqs, nh=4, nkv=2, hd=128, page=16, tree=tree, seed=31)
+    q = c.q.reshape(c.tokens, 4, 128)
+    q[0, 1, 77] = np.nan
+    last = int(c.start[-1]) - 1
+    q[last, 2, :] = np.nan
+    s = len(seqs) - 1
+    c.row(c.k, s, 3)[5] = np.nan  # kv head 0: q heads 0 and 1 of sequence s
+    c.upload()
+    got = c.attention()
+    for b, (_, n) in enumerate(seqs):
+        for i in range(n):
+            t = int(c.start[b]) + i
+            for h in range(4):
+                bad = (t, h) in ((0, 1), (last, 2)) or (b == s and h < 2 and (seqs[s][0] > 3 or 3 in c.before(s, i)))
+                assert np.all(np.isnan(got[t, h])) if bad else np.all(np.isfinite(got[t, h])), (b, i, h)
+    c.close()
+
+
 @pytest.mark.parametrize("name", ["decode", "tree", "prompt"])
 def test_bad_pages_and_parents_stay_inside(mxh, name):
     """Ids outside the pool and rows past the table are absent; bad parents are roots; trees end at 64 tokens."""
