@@ -44,120 +44,113 @@ __device__ __forceinline__ double head_sum(double v) {
 // One workgroup per token.  HD / 8 lanes hold a head, lane j its dims
 // 4 j .. +4 and HD / 2 + 4 j .. +4: whole 16-byte pieces either way, and both
 // halves of every pair in one lane for either pairing.  Wave 0 finds the
-// token's place and turns the angles (one pair a lane) while the heads' loads
-// are in flight.
-constexpr int kRopeThreads = 256, kRopeAhead = 4;
+// token's place and turns the angles (one pair a lane) while the first heads'
+// loads are in flight; from there on a lane works on one head with the next two
+// on their way, in few registers, so that six workgroups fit a CU.  Bound by its
+// bytes: 6,410 tokens of 32/8 heads of 128, both norms, 59 us = 4.9 TB/s read
+// and written; four heads unrolled held 201 registers, so two workgroups a CU,
+// and took 90.  One token takes 5 us, little over an empty launch.
+constexpr int kRopeThreads = 256;
 
 template <int HD>
-__global__ __launch_bounds__(kRopeThreads) void qk_rope_append_kernel(RopeArgs a) {
+__global__ __launch_bounds__(kRopeThreads, 6) void qk_rope_append_kernel(RopeArgs a) {
     constexpr int LPH = HD / 8, STEP = kRopeThreads / LPH;  // heads per pass over the workgroup
     __shared__ double2 cs[HD / 2];
     __shared__ int64_t place;  // the token's cache row, -1: none; -2: the token is no sequence's
-    const int tid = threadIdx.x, j = tid % LPH, sub = tid / LPH;
-    const int nkv = a.pg.nkv, heads = a.nh + 2 * nkv;
+    const int tid = threadIdx.x, j = tid % LPH;
+    const int nkv = a.pg.nkv, heads = a.nh + 2 * nkv, t = blockIdx.x;
     const int d0 = 4 * j, d1 = HD / 2 + 4 * j;
-    // (rows are walked by a grid as wide as it may be)
-    for (int t = blockIdx.x; t < a.pg.n_tokens; t += gridDim.x) {
-        const float* row = a.qkv + (size_t)t * a.ld;
-        float4 v[kRopeAhead][2];
-        const auto load = [&](int h0) __attribute__((always_inline)) {
-#pragma unroll
-            for (int u = 0; u < kRopeAhead; ++u) {
-                const int h = h0 + u * STEP + sub;
-                if (h >= heads) continue;
-                v[u][0] = *reinterpret_cast<const float4*>(row + (size_t)h * HD + d0);
-                v[u][1] = *reinterpret_cast<const float4*>(row + (size_t)h * HD + d1);
+    const float* row = a.qkv + (size_t)t * a.ld;
+    struct Head {
+        float4 lo, hi;
+    };
+    const auto load = [&](int h) __attribute__((always_inline)) {  // (past the last head: the last again, unused)
+        const float* p = row + (size_t)min(h, heads - 1) * HD;
+        return Head{*reinterpret_cast<const float4*>(p + d0), *reinterpret_cast<const float4*>(p + d1)};
+    };
+    Head cur = load(tid / LPH), next = load(tid / LPH + STEP);
+    if (tid < 64) {
+        const int s = paged_seq_of(a.pg, t);
+        int64_t at = -2;
+        int pos = 0;
+        if (s >= 0) {
+            const int first = a.pg.start[s], i = t - first;
+            const int cached = min(max(a.pg.cached[s], 0), 1 << 30);
+            pos = cached + i;
+            bool mine = true;
+            if (a.pg.parent) {
+                const int n = min(min(a.pg.start[s + 1], a.pg.n_tokens) - first, kTreeMax);
+                const uint64_t path = tree_path(tree_parent(a.pg, first, n));
+                pos = cached + __shfl((int)__popcll(path), i & 63) - 1;
+                mine = i < kTreeMax;
             }
-        };
-        load(0);
-        if (tid < 64) {
-            const int s = paged_seq_of(a.pg, t);
-            int64_t at = -2;
-            int pos = 0;
-            if (s >= 0) {
-                const int first = a.pg.start[s], i = t - first;
-                const int cached = min(max(a.pg.cached[s], 0), 1 << 30);
-                pos = cached + i;
-                bool mine = true;
-                if (a.pg.parent) {
-                    const int n = min(min(a.pg.start[s + 1], a.pg.n_tokens) - first, kTreeMax);
-                    const uint64_t path = tree_path(tree_parent(a.pg, first, n));
-                    pos = cached + __shfl((int)__popcll(path), i & 63) - 1;
-                    mine = i < kTreeMax;
-                }
-                if (mine) at = paged_row(a.pg, s, cached + i);
-            }
-            if (tid < HD / 2) {
-                double sn, c;
-                sincospi((double)pos * a.inv_freq[tid] * 0.31830988618379067154, &sn, &c);
-                cs[tid] = make_double2(c, sn);
-            }
-            if (tid == 0) place = at;
+            if (mine) at = paged_row(a.pg, s, cached + i);
         }
-        __syncthreads();
-        const int64_t at = place;
-        if (at != -2) {
-            // the lane's pairs: of elements e and e + 4 (neox), or (0, 1), (2, 3) of both pieces
-            double2 turn[4];
+        if (tid < HD / 2) {
+            double sn, c;
+            sincospi((double)pos * a.inv_freq[tid] * 0.31830988618379067154, &sn, &c);
+            cs[tid] = make_double2(c, sn);
+        }
+        if (tid == 0) place = at;
+    }
+    __syncthreads();
+    const int64_t at = place;
+    if (at == -2) return;
+    // the lane's pairs: of elements e and e + 4 (neox), or (0, 1), (2, 3) of both pieces
+    double2 turn[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                turn[e] = cs[a.neox ? 4 * j + e : (e < 2 ? 2 * j + e : HD / 4 + 2 * j + e - 2)];
-            for (int h0 = 0; h0 < heads; h0 += kRopeAhead * STEP) {
-                if (h0) load(h0);
+    for (int e = 0; e < 4; ++e) turn[e] = cs[a.neox ? 4 * j + e : (e < 2 ? 2 * j + e : HD / 4 + 2 * j + e - 2)];
+#pragma unroll 1
+    for (int h = tid / LPH; h < heads; h += STEP) {  // (whole heads: their lanes stay together)
+        float x[8] = {cur.lo.x, cur.lo.y, cur.lo.z, cur.lo.w, cur.hi.x, cur.hi.y, cur.hi.z, cur.hi.w};
+        cur = next;
+        next = load(h + 2 * STEP);
+        if (a.bias) {
+            const float4 b0 = *reinterpret_cast<const float4*>(a.bias + h * HD + d0);
+            const float4 b1 = *reinterpret_cast<const float4*>(a.bias + h * HD + d1);
+            x[0] += b0.x, x[1] += b0.y, x[2] += b0.z, x[3] += b0.w;
+            x[4] += b1.x, x[5] += b1.y, x[6] += b1.z, x[7] += b1.w;
+        }
+        if (h < a.nh + nkv) {
+            const float* w = h < a.nh ? a.q_norm : a.k_norm;
+            if (w) {
+                double ss = 0.0;
 #pragma unroll
-                for (int u = 0; u < kRopeAhead; ++u) {
-                    const int h = h0 + u * STEP + sub;
-                    if (h >= heads) continue;  // (whole heads: their lanes stay together)
-                    float x[8] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w,
-                                  v[u][1].x, v[u][1].y, v[u][1].z, v[u][1].w};
-                    if (a.bias) {
-                        const float4 b0 = *reinterpret_cast<const float4*>(a.bias + h * HD + d0);
-                        const float4 b1 = *reinterpret_cast<const float4*>(a.bias + h * HD + d1);
-                        x[0] += b0.x, x[1] += b0.y, x[2] += b0.z, x[3] += b0.w;
-                        x[4] += b1.x, x[5] += b1.y, x[6] += b1.z, x[7] += b1.w;
-                    }
-                    if (h < a.nh + nkv) {
-                        const float* w = h < a.nh ? a.q_norm : a.k_norm;
-                        if (w) {
-                            double ss = 0.0;
+                for (int e = 0; e < 8; ++e) ss += (double)x[e] * x[e];
+                const double inv = 1.0 / sqrt(head_sum<LPH>(ss) / (double)HD + (double)a.eps);
+                const float4 w0 = *reinterpret_cast<const float4*>(w + d0);
+                const float4 w1 = *reinterpret_cast<const float4*>(w + d1);
+                const float g[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) ss += (double)x[e] * x[e];
-                            const double inv = 1.0 / sqrt(head_sum<LPH>(ss) / (double)HD + (double)a.eps);
-                            const float4 w0 = *reinterpret_cast<const float4*>(w + d0);
-                            const float4 w1 = *reinterpret_cast<const float4*>(w + d1);
-                            const float g[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+                for (int e = 0; e < 8; ++e) x[e] = (float)((double)x[e] * inv) * g[e];
+            }
+            const auto rotate = [&](float& p, float& q, const double2& c) {
+                const double x0 = p, x1 = q;
+                p = (float)(x0 * c.x - x1 * c.y);
+                q = (float)(x0 * c.y + x1 * c.x);
+            };
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) x[e] = (float)((double)x[e] * inv) * g[e];
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int p = a.neox ? e : 2 * e, q = a.neox ? e + 4 : 2 * e + 1;
-                            const double x0 = x[p], x1 = x[q];
-                            x[p] = (float)(x0 * turn[e].x - x1 * turn[e].y);
-                            x[q] = (float)(x0 * turn[e].y + x1 * turn[e].x);
-                        }
-                    }
-                    if (h < a.nh) {
-                        float* out = a.q + ((size_t)t * a.nh + h) * HD;
-                        *reinterpret_cast<float4*>(out + d0) = make_float4(x[0], x[1], x[2], x[3]);
-                        *reinterpret_cast<float4*>(out + d1) = make_float4(x[4], x[5], x[6], x[7]);
-                    } else if (at >= 0) {
-                        const int g = h - a.nh;
-                        __half* out = (g < nkv ? a.pg.k + ((size_t)at * nkv + g) * HD
-                                               : a.pg.v + ((size_t)at * nkv + g - nkv) * HD);
-                        union {
-                            __half2 h2[4];
-                            uint2 u2[2];
-                        } o;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o.h2[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-                        *reinterpret_cast<uint2*>(out + d0) = o.u2[0];
-                        *reinterpret_cast<uint2*>(out + d1) = o.u2[1];
-                    }
-                }
+            for (int e = 0; e < 4; ++e) {
+                if (a.neox) rotate(x[e], x[e + 4], turn[e]);
+                else rotate(x[2 * e], x[2 * e + 1], turn[e]);
             }
         }
-        __syncthreads();
+        if (h < a.nh) {
+            float* out = a.q + ((size_t)t * a.nh + h) * HD;
+            *reinterpret_cast<float4*>(out + d0) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(out + d1) = make_float4(x[4], x[5], x[6], x[7]);
+        } else if (at >= 0) {
+            const int g = h - a.nh;
+            __half* out = (g < nkv ? a.pg.k + ((size_t)at * nkv + g) * HD : a.pg.v + ((size_t)at * nkv + g - nkv) * HD);
+            union {
+                __half2 h2[4];
+                uint2 u2[2];
+            } o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.h2[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+            *reinterpret_cast<uint2*>(out + d0) = o.u2[0];
+            *reinterpret_cast<uint2*>(out + d1) = o.u2[1];
+        }
     }
 }
 
@@ -165,7 +158,7 @@ __global__ __launch_bounds__(kRopeThreads) void qk_rope_append_kernel(RopeArgs a
 
 // Lists travel in the kernel's arguments (at most 4 KiB of them): no copy to
 // the device before the launch, and a recorded call holds its own.
-constexpr int kCopyPairs = 448, kMoves = 320;
+constexpr int kCopyPairs = 448;
 constexpr int kCopyThreads = 256, kCopyUnroll = 4;
 
 struct CopyArgs {
@@ -175,49 +168,64 @@ struct CopyArgs {
     int src[kCopyPairs], dst[kCopyPairs];
 };
 
-// Workgroup (chunk and K or V, layer, pair)
+// Workgroup (chunk and K or V, pair, layer): 16 KB, four 16-byte loads a thread
+// in flight before its first store.  Bound by its bytes: 256 pages of 16 rows
+// of 8 heads of 128 in 36 layers 236 us = 5.1 TB/s (a large copy 5.2); one in
+// 28 layers 9.5 us, most of it the cold misses of 56 scattered regions.  With the
+// loads behind the test for the page's end, one after the other, 245 us.
 __global__ __launch_bounds__(kCopyThreads) void kv_copy_pages_kernel(CopyArgs a) {
     const int chunk = blockIdx.x >> 1;
-    uint4* base = (blockIdx.x & 1 ? a.v : a.k) + blockIdx.y * a.layer16;
-    const uint4* s = base + (int64_t)a.src[blockIdx.z] * a.page16;
-    uint4* d = base + (int64_t)a.dst[blockIdx.z] * a.page16;
+    uint4* base = (blockIdx.x & 1 ? a.v : a.k) + blockIdx.z * a.layer16;
+    const uint4* s = base + (int64_t)a.src[blockIdx.y] * a.page16;
+    uint4* d = base + (int64_t)a.dst[blockIdx.y] * a.page16;
     const int i0 = chunk * kCopyThreads * kCopyUnroll + threadIdx.x;
     uint4 x[kCopyUnroll];
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
-        if (i0 + u * kCopyThreads < a.page16) x[u] = s[i0 + u * kCopyThreads];
+    for (int u = 0; u < kCopyUnroll; ++u) x[u] = s[min(i0 + u * kCopyThreads, a.page16 - 1)];  // (all in flight at once)
 #pragma unroll
     for (int u = 0; u < kCopyUnroll; ++u)
         if (i0 + u * kCopyThreads < a.page16) d[i0 + u * kCopyThreads] = x[u];
 }
 
+// A move is 16 bits for the row it reads and 16 for the one it writes: 6 for
+// one of its sequence's pages, 10 for the row of the page.
+constexpr int kMoves = 480, kKeepPages = 300, kKeepGroups = 190, kKeepSlots = 64;
 struct KeepArgs {
     uint4 *k, *v;
     int64_t layer16;
-    int row16, columns;  // 16-byte pieces of a row; of all layers' K and V rows together
-    int src[kMoves], dst[kMoves];
-    uint16_t first[kMoves + 1];  // sequence g's moves: first[g] .. first[g + 1] - 1
+    int row16, page_rows, columns;  // 16-byte pieces of a row; columns: of all layers' K and V rows together
+    uint32_t moves[kMoves];
+    int pages[kKeepPages];
+    uint16_t first[kKeepGroups + 1], page0[kKeepGroups];  // group g: moves first[g] .. first[g + 1] - 1, its first page
 };
+static_assert(sizeof(KeepArgs) <= 4096 && sizeof(CopyArgs) <= 4096, "");
 
 // A thread moves one 16-byte column of one sequence's rows.  The moves go in
 // ascending order with dst <= src, so a row is written only after it was read
 // (dst of a move is below the src of every later one), however many loads of
-// later moves come before a store.
+// later moves come before a store.  Bound by its bytes and, before them, by
+// three dependent reads of the argument block: 64 paths of 6 rows of 2 KB in 36
+// layers, K and V, 38 us = 3.2 TB/s; one path 6.2 us.  Two or four columns to a
+// thread, with as many more loads in flight, took 40.9 and 41.0 us.
 constexpr int kKeepAhead = 8;
 __global__ __launch_bounds__(256) void kv_keep_rows_kernel(KeepArgs a) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
+    const int g = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;  // (the sequences of a layer next to each other)
     if (c >= a.columns) return;
-    const int per = 2 * a.row16, layer = c / per, in = c % per;
+    const int per = 2 * a.row16, layer = c / per, in = c - layer * per;
     uint4* base = (in < a.row16 ? a.k + in : a.v + in - a.row16) + layer * a.layer16;
-    const int end = a.first[blockIdx.y + 1];
-    for (int m = a.first[blockIdx.y]; m < end; m += kKeepAhead) {
+    const int end = a.first[g + 1];
+    const int* pages = a.pages + a.page0[g];
+    const auto at = [&](uint32_t code) {
+        return ((int64_t)pages[code >> 10] * a.page_rows + (code & 1023)) * a.row16;
+    };
+    for (int m = a.first[g]; m < end; m += kKeepAhead) {
         uint4 x[kKeepAhead];
 #pragma unroll
-        for (int u = 0; u < kKeepAhead; ++u)
-            if (m + u < end) x[u] = base[(int64_t)a.src[m + u] * a.row16];
+        for (int u = 0; u < kKeepAhead; ++u)  // (past the end the last again: all loads are in flight at once)
+            x[u] = base[at(a.moves[min(m + u, end - 1)] & 0xffff)];
 #pragma unroll
         for (int u = 0; u < kKeepAhead; ++u)
-            if (m + u < end) base[(int64_t)a.dst[m + u] * a.row16] = x[u];
+            if (m + u < end) base[at(a.moves[m + u] >> 16)] = x[u];
     }
 }
 
@@ -243,6 +251,7 @@ int check_pool(const char* who, const mxh_kv_pool* p) {
     if (p->page_rows < 16 || p->page_rows > 1024 || (p->page_rows & (p->page_rows - 1)))
         return set_error(MXH_ERR_ARG, "%s: page_rows %d is not a power of two from 16 to 1024", who, p->page_rows);
     if (p->n_layer < 1 || p->n_layer > 65535 || p->n_pages < 1 || p->n_kv < 1 || p->n_kv > 1024 ||
+        (int64_t)p->n_layer * p->n_kv * p->head_dim > 65535 * 1024 ||  // (kv_keep_rows' grid)
         (int64_t)p->n_pages * p->page_rows > INT_MAX)
         return set_error(MXH_ERR_ARG, "%s: unsupported pool of %d layers, %d pages of %d rows, %d kv heads", who,
                          p->n_layer, p->n_pages, p->page_rows, p->n_kv);
@@ -292,44 +301,37 @@ bool mark_pages(const int* ids, int n, std::vector<uint64_t>& seen) {
     return true;
 }
 
-// the moves of mxh_kv_keep_rows, with every fault of its arguments refused
-int plan_keep(const mxh_kv_pool* p, const int* table, int table_ld, const int* cached, const int* keep_start,
-              const int* keep, int n_seq, std::vector<int>& src, std::vector<int>& dst, std::vector<int>& ends) {
+// every fault of mxh_kv_keep_rows' arguments
+int check_keep(const mxh_kv_pool* p, const int* table, int table_ld, const int* cached, const int* keep_start,
+               const int* keep, int n_seq) {
     const char* who = "kv_keep_rows";
     const int pr = p->page_rows;
     std::vector<int> pages;  // every page that holds a kept row, of all sequences
     for (int s = 0; s < n_seq; ++s) {
         const int n = keep_start[s + 1] - keep_start[s];
         if (n < 0) return set_error(MXH_ERR_ARG, "%s: keep_start decreases at sequence %d", who, s);
+        if (n == 0) continue;
         const int* kept = keep + keep_start[s];
-        if (n > 0) {
-            if (kept[0] < 0) return set_error(MXH_ERR_ARG, "%s: sequence %d keeps token %d", who, s, kept[0]);
-            for (int i = 1; i < n; ++i)
-                if (kept[i] <= kept[i - 1])
-                    return set_error(MXH_ERR_ARG, "%s: the kept tokens of sequence %d do not ascend", who, s);
-            if (cached[s] < 0 || (int64_t)cached[s] + kept[n - 1] >= std::min((int64_t)table_ld * pr, (int64_t)INT_MAX))
-                return set_error(MXH_ERR_ARG, "%s: row %lld of sequence %d is past its table", who,
-                                 (long long)cached[s] + kept[n - 1], s);
-            const int* ids = table + (size_t)s * table_ld;
-            int last = -1;  // pages are met in ascending order: dst's, then src's
-            for (int pass = 0; pass < 2; ++pass)
-                for (int i = 0; i < n; ++i) {
-                    const int q = (cached[s] + (pass ? kept[i] : i)) / pr;
-                    if (q <= last) continue;
-                    last = q;
-                    if (ids[q] < 0 || ids[q] >= p->n_pages)
-                        return set_error(MXH_ERR_ARG, "%s: page %d of sequence %d is %d, not in the pool", who, q, s,
-                                         ids[q]);
-                    pages.push_back(ids[q]);
-                }
+        if (kept[0] < 0) return set_error(MXH_ERR_ARG, "%s: sequence %d keeps token %d", who, s, kept[0]);
+        for (int i = 1; i < n; ++i)
+            if (kept[i] <= kept[i - 1])
+                return set_error(MXH_ERR_ARG, "%s: the kept tokens of sequence %d do not ascend", who, s);
+        if (cached[s] < 0 || (int64_t)cached[s] + kept[n - 1] >= std::min((int64_t)table_ld * pr, (int64_t)INT_MAX))
+            return set_error(MXH_ERR_ARG, "%s: row %lld of sequence %d is past its table", who,
+                             (long long)cached[s] + kept[n - 1], s);
+        const int* ids = table + (size_t)s * table_ld;
+        // the pages of the rows written, one after the other, then those of rows
+        // that are only read
+        int last = -1;
+        for (int pass = 0; pass < 2; ++pass)
             for (int i = 0; i < n; ++i) {
-                if (kept[i] == i) continue;  // in place
-                const int from = cached[s] + kept[i], to = cached[s] + i;
-                src.push_back(ids[from / pr] * pr + from % pr);
-                dst.push_back(ids[to / pr] * pr + to % pr);
+                const int q = (cached[s] + (pass ? kept[i] : i)) / pr;
+                if (q <= last) continue;
+                last = q;
+                if (ids[q] < 0 || ids[q] >= p->n_pages)
+                    return set_error(MXH_ERR_ARG, "%s: page %d of sequence %d is %d, not in the pool", who, q, s, ids[q]);
+                pages.push_back(ids[q]);
             }
-        }
-        if (ends.empty() ? !src.empty() : (int)src.size() > ends.back()) ends.push_back((int)src.size());
     }
     std::sort(pages.begin(), pages.end());
     const auto twice = std::adjacent_find(pages.begin(), pages.end());
@@ -368,7 +370,7 @@ int mxh_qk_rope_append(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* b
         return set_error(MXH_ERR_ARG, "%s: q overlaps qkv", who);
     if (!mxh_is_available()) return MXH_ERR_NODEV;
     const RopeArgs a{paged_args(pool, layer, batch), qkv, bias, q_norm, k_norm, inv_freq, q, ld, eps, neox, nh};
-    const dim3 grid((unsigned)std::min(batch->n_tokens, 65535)), block(kRopeThreads);
+    const dim3 grid((unsigned)batch->n_tokens), block(kRopeThreads);
     switch (pool->head_dim) {
     case 32: hipLaunchKernelGGL(qk_rope_append_kernel<32>, grid, block, 0, lib_stream(), a); break;
     case 64: hipLaunchKernelGGL(qk_rope_append_kernel<64>, grid, block, 0, lib_stream(), a); break;
@@ -420,6 +422,7 @@ int mxh_kv_copy_pages(const mxh_kv_pool* pool, const int* src, const int* dst, i
     for (int i = 0; i < n; ++i)
         if (seen[(size_t)src[i] >> 6] >> (src[i] & 63) & 1)
             return set_error(MXH_ERR_ARG, "%s: page %d is read and written", who, src[i]);
+    if (n == 0) return MXH_OK;
     if (!mxh_is_available()) return MXH_ERR_NODEV;
     CopyArgs a{};
     a.k = static_cast<uint4*>(pool->k), a.v = static_cast<uint4*>(pool->v);
@@ -430,7 +433,7 @@ int mxh_kv_copy_pages(const mxh_kv_pool* pool, const int* src, const int* dst, i
         const int m = std::min(kCopyPairs, n - i);
         std::copy(src + i, src + i + m, a.src);
         std::copy(dst + i, dst + i + m, a.dst);
-        hipLaunchKernelGGL(kv_copy_pages_kernel, dim3(2u * (unsigned)a.chunks, (unsigned)pool->n_layer, (unsigned)m),
+        hipLaunchKernelGGL(kv_copy_pages_kernel, dim3(2u * (unsigned)a.chunks, (unsigned)m, (unsigned)pool->n_layer),
                            dim3(kCopyThreads), 0, lib_stream(), a);
     }
     return check_hip(hipGetLastError(), "kv_copy_pages launch");
@@ -446,34 +449,49 @@ int mxh_kv_keep_rows(const mxh_kv_pool* pool, const int* table, int table_ld, co
     if (n_seq == 0) return MXH_OK;
     if (!table || table_ld < 1 || !cached || !keep_start || (!keep && keep_start[n_seq] > keep_start[0]))
         return set_error(MXH_ERR_ARG, "%s: null array", who);
-    std::vector<int> src, dst, ends;
-    if (int rc = plan_keep(pool, table, table_ld, cached, keep_start, keep, n_seq, src, dst, ends)) return rc;
-    if (src.empty()) return MXH_OK;
-    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    if (int rc = check_keep(pool, table, table_ld, cached, keep_start, keep, n_seq)) return rc;
     KeepArgs a{};
     a.k = static_cast<uint4*>(pool->k), a.v = static_cast<uint4*>(pool->v);
     a.layer16 = layer_elems(pool) / 8;
-    a.row16 = pool->n_kv * pool->head_dim / 8;
+    a.row16 = pool->n_kv * pool->head_dim / 8, a.page_rows = pool->page_rows;
     a.columns = pool->n_layer * 2 * a.row16;
-    // a launch takes whole sequences while they fit, and a long one in parts
-    // (its moves stay in order: launches of a stream do)
-    size_t at = 0, g = 0;
-    while (at < src.size()) {
-        int groups = 0, m = 0;
-        while (g < ends.size() && m < kMoves) {
-            const int left = ends[g] - (int)at, take = std::min(left, kMoves - m);
-            if (take < left && groups) break;
-            a.first[groups++] = (uint16_t)m;
-            std::copy(src.begin() + (ptrdiff_t)at, src.begin() + (ptrdiff_t)at + take, a.src + m);
-            std::copy(dst.begin() + (ptrdiff_t)at, dst.begin() + (ptrdiff_t)at + take, a.dst + m);
-            m += take, at += (size_t)take;
-            if (take < left) break;
-            ++g;
-        }
-        a.first[groups] = (uint16_t)m;
-        hipLaunchKernelGGL(kv_keep_rows_kernel, dim3((unsigned)((a.columns + 255) / 256), (unsigned)groups), dim3(256),
+    int moves = 0, pages = 0, groups = 0;
+    const auto flush = [&] {
+        if (!groups) return;
+        a.first[groups] = (uint16_t)moves;
+        hipLaunchKernelGGL(kv_keep_rows_kernel, dim3((unsigned)groups, (unsigned)((a.columns + 255) / 256)), dim3(256),
                            0, lib_stream(), a);
+        moves = pages = groups = 0;
+    };
+    bool ready = false;
+    for (int s = 0; s < n_seq; ++s) {
+        const int* ids = table + (size_t)s * table_ld;
+        bool open = false;  // a group of this sequence, in the launch to come
+        int page0 = 0, src_q = -1, dst_q = -1, src_slot = 0, dst_slot = 0;
+        for (int i = 0; i < keep_start[s + 1] - keep_start[s]; ++i) {
+            const int kept = keep[keep_start[s] + i];
+            if (kept == i) continue;  // in place
+            if (!ready && !mxh_is_available()) return MXH_ERR_NODEV;
+            ready = true;
+            // a sequence that does not fit goes on in another launch (in order, as
+            // launches of a stream are), in a group of its own
+            if (moves == kMoves || pages + 2 > kKeepPages || (open ? pages - page0 + 2 > kKeepSlots : groups == kKeepGroups))
+                flush(), open = false;
+            if (!open) {
+                open = true;
+                a.first[groups] = (uint16_t)moves, a.page0[groups] = (uint16_t)pages;
+                ++groups;
+                page0 = pages, src_q = dst_q = -1;
+            }
+            const int from = cached[s] + kept, to = cached[s] + i, pr = pool->page_rows;
+            if (to / pr != dst_q) dst_q = to / pr, dst_slot = pages - page0, a.pages[pages++] = ids[dst_q];
+            if (from / pr == dst_q) src_q = dst_q, src_slot = dst_slot;
+            if (from / pr != src_q) src_q = from / pr, src_slot = pages - page0, a.pages[pages++] = ids[src_q];
+            a.moves[moves++] = (uint32_t)(src_slot << 10 | from % pr) | (uint32_t)(dst_slot << 10 | to % pr) << 16;
+        }
     }
+    if (!ready) return MXH_OK;
+    flush();
     return check_hip(hipGetLastError(), "kv_keep_rows launch");
 } catch (const std::bad_alloc&) {
     return set_error(MXH_ERR_OOM, "kv_keep_rows: out of host memory");

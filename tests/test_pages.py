@@ -259,6 +259,7 @@ def test_copies_refuse():
             mxhip.kv_copy_pages(pool(), src, dst)
     with pytest.raises(ValueError):
         mxhip.kv_copy_pages(pool(), [0, 1], [2])
+    mxhip.kv_copy_pages(pool(), [], [])  # nothing to do
     assert mxhip.lib.mxh_kv_copy_pages(C.byref(pool()), None, None, 1) == ERR_ARG
     assert mxhip.lib.mxh_kv_copy_pages(C.byref(pool()), None, None, -1) == ERR_ARG
 
