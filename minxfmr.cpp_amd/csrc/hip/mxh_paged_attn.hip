@@ -33,9 +33,9 @@
 // operand that the second product wants of it.
 //
 // Rows that a token does not attend must not reach it: their scores are
-// replaced, not added to, and since 0 times an infinity is no zero, blocks with
-// unattended rows look their V values over; an item that meets an infinity or a
-// NaN there is computed again without products over such rows (redo_item).
+// replaced, not added to, and since 0 times an infinity is no zero, an item whose
+// sums met an infinity or a NaN in V is computed again without products over
+// rows that a token does not attend (redo_item).
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -60,11 +60,11 @@ __host__ __device__ constexpr int stage_keys(int rows) { return rows == 16 ? 128
 // a tile's cost beside its stages, in stages
 __host__ __device__ constexpr int tile_lead(int rows) { return rows == 16 ? 2 : 4; }
 
-// floats a wave leaves for the merge: V sums [m][hd + 4], references, sums
+// floats a wave leaves for the merge: V sums [m][hd + 4], references, sums (and a flag, behind all of theirs)
 __host__ __device__ constexpr int merge_floats(int hd, int m) { return m * (hd + 6); }
 __host__ __device__ constexpr int lds_bytes(int hd, int rows) {
     const int ring = 2 * 128 * hd * 2,  // R = 16: a stage, R = 64: two
-               merge = kWaves * merge_floats(hd, rows == 16 ? 16 : 32) * 4;
+               merge = kWaves * (merge_floats(hd, rows == 16 ? 16 : 32) + 1) * 4;
     return ring > merge ? ring : merge;
 }
 
@@ -208,25 +208,10 @@ struct VRead {
     }
 };
 
-typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-
-// whether any V value of the block is infinite or NaN
-template <int HD>
-__device__ __forceinline__ bool any_special(uint32_t v0, int lane) {
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < HD / 16; ++i) {
-        const u32x4 x = *(lds_u32x4*)(uintptr_t)(v0 + 1024 * i + 16 * lane);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) bad |= (x[e] & 0x7c00u) == 0x7c00u || (x[e] & 0x7c000000u) == 0x7c000000u;
-    }
-    return __any(bad);
-}
-
 // The item again with a wave a row and no product that meets a value its row
 // does not attend: a key a lane for the scores, then a dim a lane (or two) for
-// the sums.  For items that found such a value among rows that only some of
-// their tokens attend; the rest of the kernel pays no register for it.
+// the sums.  For items whose sums met an infinity or a NaN; the rest of the
+// kernel pays no register for it.
 template <int HD, int R>
 __device__ void redo_item(const AttnPagedArgs& a, const Segment& it, int g, int key0, int key1, uint8_t* smem) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -539,7 +524,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         RowMask mask{cached, cached + i + 1, 0, a.pg.parent != nullptr};
         if (a.pg.parent) mask.path = path_of(tree_path(parent), i);
 
-        bool redo = false;  // (uniform)
         float mref = -INFINITY, lrun = 0.f;
         acc_t o[DB];
 #pragma unroll
@@ -552,7 +536,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         const uint32_t krow = (uint32_t)(key_row * HD * 2 + 16 * (h ^ pa_swz<HD>(key_row)));
 
         // what the rows do not attend, out of the scores of the block at key kb
-        const auto unmask = [&](int kb, uint32_t v0, acc_t (&s)[SB]) __attribute__((always_inline)) {
+        const auto unmask = [&](int kb, acc_t (&s)[SB]) __attribute__((always_inline)) {
             uint32_t w = mask(kb);
             if (gone >> (2 * kg) & 1) w &= 0xffff0000u;
             if (gone >> (2 * kg) & 2) w &= 0xffffu;
@@ -560,7 +544,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
 #pragma unroll
             for (int v = 0; v < NP; ++v)
                 if (!((w >> (16 * (v >> 3) + (v & 7))) & 1)) s[v / NA][v % NA] = -INFINITY;
-            redo |= any_special<HD>(v0, lane);
         };
         const auto largest = [&](const acc_t (&s)[SB]) __attribute__((always_inline)) {
             float mx = s[0][0];
@@ -716,10 +699,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             for (int st = 0; st < nst; ++st) {
                 const uint32_t k0 = k_place(st) + 64 * kg * HD, v0 = v_place(st) + 64 * kg * HD;
                 const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
-                const auto v_there = [&] {  // (the next K's loads may be out)
-                    if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");
-                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                };
                 asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");  // K, not yet V
                 acc_t s[SB];
                 score(k0, s);
@@ -730,13 +709,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                     issue(ahead, k_place(0), false);
                 }
                 if (kb < key1) {
-                    if (kb + 32 > lim_min || gone) {
-                        v_there();
-                        unmask(kb, v0, s);
-                    }
+                    if (kb + 32 > lim_min || gone) unmask(kb, s);
                     move_reference(largest(s), s);
                     weigh(s);
-                    v_there();
+                    if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");  // V, not the next K
+                    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     sum(v0);
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -764,7 +741,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                 const int kb = key0 + STAGE * st + 32 * kg;  // first key of this wave's block
                 const uint32_t v0 = v_place(st) + 64 * kg * HD;
                 if (kb + 32 > lim_min || gone) {  // (a block behind the last key has every score replaced)
-                    unmask(kb, v0, s);
+                    unmask(kb, s);
                     mx = largest(s);
                 }
                 move_reference(mx, s);
@@ -776,32 +753,47 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         }
 
         // the waves' parts meet, where no load is to come any more
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         float* ms = reinterpret_cast<float*>(smem);
-        const bool again = __syncthreads_or(redo);
-        if (again) {
-            redo_item<HD, R>(a, it, (int)g, key0, key1, smem);
-        } else {
+        uint32_t* flags = reinterpret_cast<uint32_t*>(ms + kWaves * merge_floats(HD, M));
+        {
             float* mb = ms + wave * merge_floats(HD, M);  // V sums [M rows][HD + 4], references, sums
             const float lsum = row_sum<M>(lrun);
+            float bad = 0.f;
             if (valid) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
-                    for (int v = 0; v < NA; v += 4)
+                    for (int v = 0; v < NA; v += 4) {
                         *reinterpret_cast<float4*>(mb + n * (HD + 4) + M * d + 2 * v + 4 * h) =
                             make_float4(o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) bad = fmaf(o[d][v + e], 0.f, bad);
+                    }
                 if (h == 0) {
                     mb[M * (HD + 4) + n] = mref;
                     mb[M * (HD + 5) + n] = lsum;
                 }
             }
+            // An infinity or a NaN in a V row makes sums of infinities and NaN, of rows
+            // that attend it and, as 0 times it, of rows that do not.  (Where the sum of
+            // probabilities is NaN, what was attended makes the output NaN.)
+            const uint64_t redo = __ballot(valid && !(bad == 0.f) && lsum == lsum);
+            if (lane == 0) flags[wave] = redo != 0;
         }
         __syncthreads();
-        // a thread takes four dims of a row
-        for (int u = tid; u < ntok * (int)group * (HD / 4) && !again; u += kThreads) {
-            const int rr = u / (HD / 4), d = 4 * (u % (HD / 4)), rn = rr % M;
-            const float* mb = ms + rr / M * merge_floats(HD, M);
+        const bool again = flags[0] | flags[1] | flags[2] | flags[3];
+        if (again) {  // (uniform)
+            __syncthreads();
+            redo_item<HD, R>(a, it, (int)g, key0, key1, smem);
+        }
+        // a thread takes four dims of every PASS-th row (past the tile's last: whatever lies there, not stored)
+        constexpr int PASS = kThreads / (HD / 4);
+        const int d = 4 * (tid % (HD / 4)), rows = again ? 0 : ntok * (int)group;
+#pragma unroll
+        for (int r0 = 0; r0 < R; r0 += PASS) {
+            const int rr = r0 + tid / (HD / 4), rn = rr % M;
+            const float* mb = ms + (rr / M % RS) * merge_floats(HD, M);
             constexpr int NEXT = RS * merge_floats(HD, M);  // (the next key group's part)
             float wt[KG], mm = -INFINITY, ll = 0.f;
 #pragma unroll
@@ -815,6 +807,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                 const float4 v = *reinterpret_cast<const float4*>(mb + k * NEXT + rn * (HD + 4) + d);
                 x4.x += wt[k] * v.x, x4.y += wt[k] * v.y, x4.z += wt[k] * v.z, x4.w += wt[k] * v.w;
             }
+            if (rr >= rows) continue;
             if (it.slot >= 0) {
                 const size_t p = ((size_t)it.slot * nkv + g) * R + rr;
                 if (d == 0) a.ml[p] = make_float2(mm, ll);

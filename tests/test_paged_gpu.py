@@ -263,6 +263,24 @@ def test_infinite_values_come_through_where_attended(mxh):
     c.close()
 
 
+@pytest.mark.parametrize("n", [1, 3, 30])
+@pytest.mark.parametrize("cached,rows", [(40, 16), (700, 32), (5000, 16)])
+def test_infinite_values_among_rows_that_all_attend(mxh, cached, rows, n):
+    """V infinities deep in the cached rows are every token's: +-inf in their columns, NaN where both meet."""
+    c = Case([(cached, n)], nh=4, nkv=2, hd=64, page=rows, seed=12)
+    want = {(0, 5): np.inf, (0, 9): -np.inf, (0, 11): np.nan, (1, 63): np.inf}
+    for (g, d), x in want.items():
+        for r, y in ((2, np.inf), (cached // 2, -np.inf)) if np.isnan(x) else ((cached // 3, x),):
+            c.row(c.v, 0, r)[64 * g + d] = y
+    c.upload()
+    got = c.attention()
+    for h in range(4):
+        for d in range(64):
+            x, w = got[:, h, d], want.get((h // 2, d), 0.0)
+            assert (np.isnan(x) if np.isnan(w) else x == w if np.isinf(w) else np.isfinite(x)).all(), (h, d)
+    c.close()
+
+
 @pytest.mark.parametrize("seqs,tree", [([(300, 1)], False), ([(40, 30), (700, 50)], False), ([(130, 20), (5, 1)], True)])
 def test_nan_reaches_the_outputs_that_read_it(mxh, seqs, tree):
     """A NaN in a token's q is its head's; NaN in a cached key is everybody's who attends it, in its kv head."""
