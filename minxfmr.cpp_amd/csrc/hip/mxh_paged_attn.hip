@@ -74,7 +74,7 @@ __device__ __align__(256) uint32_t zero_row[64];
 // A sequence as the plan sees it
 struct Seq {
     uint32_t first, n, cached;  // first token row, new tokens, rows before them
-    uint32_t tiles, stages;     // stages of a tile, at most
+    uint32_t tiles, stages;     // stages of its last tile
 };
 
 // A tile, or some of its stages
@@ -96,14 +96,38 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive
     return (uint32_t)v;
 }
 
-// The batch as a line of units: the stages of all tiles, sequence by sequence,
-// `lead` units before each tile's (target > 0), or the tiles themselves.  The
-// lead is what a tile costs beside its stages (its q, the merge of the waves),
-// so an item that goes on into another tile does as many stages less.  All
-// uniform but what a lane says of its sequences.
+// whether `target` items of a batch of `all` units finish before its whole tiles
+// do, the longest of `longest` units (Plan)
+__host__ __device__ constexpr bool cut_pays(int rows, float longest, float all, float target) {
+    return rows == 64 ? longest * target > 13.f * target + 1.8f * all : longest > 12.f || 2.f * longest * target > all;
+}
+
+// The batch as a line of units, cut into items.  Where tiles are cut, the units
+// are the stages of all tiles, sequence by sequence, `lead` units before each
+// tile's; elsewhere the tiles themselves.  The lead is what a tile costs beside
+// its stages (its q, the merge of the waves), so an item that goes on into
+// another tile does as many stages less.
+//
+// A prompt's earlier tiles have fewer stages.  `block` tiles have at most the
+// tokens of one stage, so those of block b need no more stages than the cached
+// rows and b + 1; the line gives them that many, and all of the sequence's to
+// the tiles from the block on where this reaches them (ramp).
+//
+// Cut or not: with M units the longest tile and U all of them, in us of a head
+// group of 128 dims on 256 CUs:
+//   R = 64: whole tiles take 4 + 1.07 M while they are few, `target` items of
+//   the cut ones (two resident a CU) 18 + 1.95 U / target.  A prompt of 256 at
+//   4,096 cached rows 82 whole, 54 cut; of 1,024 150 and 168; 16 drafted trees
+//   of up to 33 tokens at up to 8,000 rows 151 and 80, 20 of up to 60 at up to
+//   1,000 33 and 38.  Half the items where they would have less than 8 units:
+//   a prompt of 64 at 4,096 28.5 and 25.2.
+//   R = 16: cut unless all tiles are short and there are many: 200 single tokens
+//   at up to 300 rows 29 whole, 43 cut, at up to 1,000 83 and 89, at up to 6,000
+//   437 and 406; 64 at up to 2,000 61 and 53.
+// All uniform but what a lane says of its sequences.
 struct Plan {
     const PagedArgs& a;
-    uint32_t t, key_shift, lead;  // tokens of a tile; a stage has 1 << key_shift keys
+    uint32_t t, key_shift, lead, block;  // tokens of a tile; a stage has 1 << key_shift keys
     float inv_t;
     bool cut;
     uint32_t total, per;    // units of the batch (the launch sees to it that they fit), of an item
@@ -122,9 +146,44 @@ struct Plan {
         q.stages = (rows + (1u << key_shift) - 1) >> key_shift;
         return q;
     }
-    __device__ __forceinline__ uint32_t units(const Seq& q) const { return cut ? lead + q.stages : 1; }  // of a tile
+    __device__ __forceinline__ uint32_t cached_stages(const Seq& q) const {
+        return (q.cached + (1u << key_shift) - 1) >> key_shift;
+    }
+    // blocks of tiles with fewer stages than the sequence
+    __device__ __forceinline__ uint32_t ramp(const Seq& q) const {
+        const int r = (int)q.stages - (int)cached_stages(q) - 1;  // (below the blocks that q.n fills)
+        return a.parent ? 0 : (uint32_t)max(r, 0);
+    }
+    // units of the first b <= ramp blocks
+    __device__ __forceinline__ uint32_t before(const Seq& q, uint32_t b) const {
+        return block * (b * (lead + cached_stages(q) + 1) + b * (b - 1) / 2);
+    }
+    __device__ __forceinline__ uint32_t units(const Seq& q) const {
+        if (!cut) return q.tiles;
+        const uint32_t r = ramp(q);  // (block b < r has r - b stages less)
+        return q.tiles * (lead + q.stages) - (r > 0 ? block * (r * (r + 1) / 2) : 0);
+    }
+    // unit x of a sequence: its tile, the units of the tile and those before x
+    struct Spot {
+        uint32_t tile, units, at;
+    };
+    __device__ __forceinline__ Spot spot(const Seq& q, uint32_t x) const {
+        if (!cut) return Spot{x, 1, 0};
+        const uint32_t r = ramp(q);
+        uint32_t b = r, len = lead + q.stages, done = r > 0 ? before(q, r) : 0;
+        if (x < done) {
+            // the root of before(b) = x, put right by whole blocks
+            const float c = (float)(lead + cached_stages(q)) + 0.5f;
+            b = min((uint32_t)max(sqrtf(c * c + 2.0f * (float)x / (float)block) - c, 0.f), r - 1);
+            while (b > 0 && before(q, b) > x) --b;
+            while (b + 1 < r && before(q, b + 1) <= x) ++b;
+            len = lead + cached_stages(q) + 1 + b, done = before(q, b);
+        }
+        const uint32_t i = (x - done) / len;
+        return Spot{b * block + i, len, x - done - i * len};
+    }
 
-    // Lane l's sequences are [l part, (l + 1) part), of `upto - sum` to `upto` units
+    // Lane l's sequences are [l part, (l + 1) part), units `upto - sum` to `upto`
     int part;
     uint32_t sum, upto;
     Seq mine;  // (part == 1: the lane's sequence)
@@ -132,17 +191,30 @@ struct Plan {
     __device__ __forceinline__ Plan(const PagedArgs& args, int rows, uint32_t tokens, int target)
         : a(args), t(tokens), key_shift(rows == 16 ? 7 : 6), lead(tile_lead(rows)), inv_t(1.0f / (float)t),
           cut(target > 0) {
+        block = (uint32_t)(((float)stage_keys(rows) + 0.5f) * inv_t);
         const int lane = threadIdx.x & 63;
         part = (a.n_seq + 63) / 64;
         sum = 0;
         mine = Seq{0, 0, 0, 0, 0};
+        uint32_t tiles = 0, longest = 0;
         for (int s = lane * part; s < min((lane + 1) * part, a.n_seq); ++s) {
             mine = seq(s);
-            sum += mine.tiles * units(mine);
+            tiles += mine.tiles;
+            if (cut && mine.tiles > 0) sum += units(mine), longest = max(longest, lead + mine.stages);
         }
-        upto = wave_scan(sum);
-        total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-        per = cut ? (total + (uint32_t)target - 1) / (uint32_t)target : 1;
+        per = 1;
+        if (cut) {
+            upto = wave_scan(sum);
+            total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            cut = __any(cut_pays(rows, (float)longest, (float)total, (float)target));
+            const uint32_t items = (uint32_t)(rows == 64 && (int64_t)total < 8 * (int64_t)target ? target / 2 : target);
+            per = cut ? (total + items - 1) / items : 1;
+        }
+        if (!cut) {
+            sum = tiles;
+            upto = wave_scan(sum);
+            total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        }
     }
     // the sequence of unit x (< total), and x from its first unit on
     __device__ __forceinline__ int find(uint32_t& x, Seq& q) const {
@@ -156,7 +228,7 @@ struct Plan {
         int s = l * part;
         for (;; ++s) {  // (ends within the lane's sequences: they hold x)
             q = seq(s);
-            const uint32_t here = q.tiles * units(q);
+            const uint32_t here = units(q);
             if (x < here || s + 1 >= min((l + 1) * part, a.n_seq)) return s;
             x -= here;
         }
@@ -169,7 +241,7 @@ struct AttnPagedArgs {
     float* att;
     float* part;  // [2 target][nkv][R][HD]: V sums of the parts of tiles
     float2* ml;   // [2 target][nkv][R]: references and sums
-    int nh, target;  // target: items that the stages are cut into; 0: an item is a tile
+    int nh, target;  // target: items that stages are cut into, at most; 0: an item is a tile
     float qscale;
     uint32_t group, tokens;  // q heads of a kv head; tokens of a tile, R / group
     uint32_t group_inv;      // 2^16 / group rounded up
@@ -363,12 +435,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         asm volatile("" : "+v"(tid));  // (else what follows from it is kept in registers from tile to tile)
         const int lane = tid & 63, n = lane % M, h = lane / M;
         {
-            const uint32_t units = plan.units(seq), tile = r_unit / units, st = r_unit - tile * units, len = min(units - st, x1 - x);
+            const Plan::Spot spot = plan.spot(seq, r_unit);
+            const uint32_t len = min(spot.units - spot.at, x1 - x), end = spot.at + len;
             it.first = seq.first, it.n = seq.n, it.cached = seq.cached;
-            it.tile = plan.cut ? tile : seq.tiles - 1 - tile;  // (the most keys first)
-            it.st0 = plan.cut ? max(st, plan.lead) - plan.lead : 0;
-            it.st1 = plan.cut ? max(st + len, plan.lead) - plan.lead : seq.stages;
-            it.slot = it.st0 == 0 && it.st1 == seq.stages ? -1 : (int)(2 * index + (it.st0 == 0));
+            it.tile = plan.cut ? spot.tile : seq.tiles - 1 - spot.tile;  // (the most keys first)
+            it.st0 = plan.cut ? max(spot.at, plan.lead) - plan.lead : 0;
+            it.st1 = plan.cut ? max(end, plan.lead) - plan.lead : seq.stages;
+            it.slot = !plan.cut || (it.st0 == 0 && end == spot.units) ? -1 : (int)(2 * index + (it.st0 == 0));
             x += len, r_unit += len;
         }
         if (it.st0 < it.st1 || it.slot < 0) {  // (else only units of the lead)
@@ -822,7 +895,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         }
         if (x >= x1) return;
         // the item's next tile
-        while (r_unit >= seq.tiles * plan.units(seq)) {
+        while (r_unit >= plan.units(seq)) {
             r_unit = 0;
             if (++it.s >= a.pg.n_seq) return;  // (the line ends with the last sequence)
             seq = plan.seq(it.s);
@@ -847,7 +920,8 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
     if (x >= plan.total) return;
     Seq seq;
     plan.find(x, seq);
-    const uint32_t units = plan.units(seq), tile = x / units, cut = x - tile * units;
+    const Plan::Spot spot = plan.spot(seq, x);
+    const uint32_t units = spot.units, tile = spot.tile, cut = spot.at;
     if (cut <= plan.lead || cut > plan.lead + plan.per) return;  // (no stage before it; not the first of the tile's)
     const int rows = min((int)(min(T, seq.n - tile * T) * group) - (int)rb * kMergeRows, kMergeRows);
     if (rows <= 0) return;
@@ -892,8 +966,12 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
         make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
 
-// What the host can choose without the lengths: rows of a tile by the average
-// sequence, and whether tiles are cut.
+// What the host chooses without the lengths: rows of a tile, by the average
+// sequence, and how many items there can be; whether tiles are cut the plan
+// decides.  16-row tiles re-read the keys where a sequence has several of them,
+// 64-row ones leave rows empty: 16 sequences of 2 tokens (8 rows) at up to 4,000
+// keys took 25 us with 16 and 31 with 64, of up to 12 tokens 36 and 32; one of 4
+// tokens at 8,192 16 and 20, of 27 28 and 24, at 40,000 173 and 69.
 struct Shape {
     int rows, target;
     int64_t items;  // at most
@@ -901,13 +979,18 @@ struct Shape {
 Shape attention_shape(const PagedArgs& a, int nh, int hd) {
     Shape s;
     const int group = nh / a.nkv;
-    const int64_t want = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group;
-    s.rows = want > 16 ? 64 : 16;
-    const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq;
-    const int64_t stages = (((int64_t)a.table_ld << a.page_shift) + stage_keys(s.rows) - 1) / stage_keys(s.rows);  // of a tile, at most
-    const int target = std::max(2, device_cus() / a.nkv);
-    s.target = stages > 1 && (s.rows == 16 || a.n_tokens / (s.rows / group) < 4 * target) && tiles * (stages + tile_lead(s.rows)) < INT_MAX ? target : 0;
-    s.items = s.target ? std::min((int64_t)s.target, tiles * (stages + tile_lead(s.rows))) : tiles;
+    s.rows = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group > 16 ? 64 : 16;
+    const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq, keys = stage_keys(s.rows);
+    const int64_t stages = (((int64_t)a.table_ld << a.page_shift) + keys - 1) / keys;  // of a tile, at most
+    const int target = (s.rows == 64 ? 2 : 1) * std::max(2, device_cus() / a.nkv);
+    // no second kernel where no lengths could make it worth its 4 us: a table of so
+    // few keys, and tiles of one stage at least (no sequence empty)
+    const int64_t tiles_min = std::max(a.n_tokens / (s.rows / group), std::min(a.n_seq, a.n_tokens));
+    const int least = 1 + tile_lead(s.rows), most = (int)std::min(stages, (int64_t)INT_MAX / 2) + tile_lead(s.rows);
+    const bool may_cut = stages > 1 && tiles * most < INT_MAX &&
+                         cut_pays(s.rows, (float)most, (float)least * (float)tiles_min, (float)target);
+    s.target = may_cut ? target : 0;
+    s.items = std::max((int64_t)s.target, tiles);
     return s;
 }
 

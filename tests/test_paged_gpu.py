@@ -384,6 +384,45 @@ def test_graph_follows_the_lengths(mxh):
     a.close(), b.close()
 
 
+# (cached, new), extra table columns: whole tiles under a wide table and under a tight one, tiles cut with
+# some, most or all of a prompt's stages behind its cached rows, items that cross many tiles
+PLANS = {
+    "whole-wide": ([(0, 90)] * 12 + [(30, 5)], 300),
+    "whole-tight": ([(0, 90)] * 12 + [(30, 5)], 0),
+    "one-long": ([(2500, 40), (0, 130), (7, 90)], 0),
+    "long-ramp": ([(900, 300)], 40),
+    "all-ramp": ([(0, 1100)], 0),
+    "prompt-among-single-tokens": ([(0, 280)] + [(i % 70, 1) for i in range(150)], 60),
+    "prompts-over-64": ([(3 * i, 33) for i in range(70)] + [(1500, 20)], 0),
+}
+
+
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32", "g1-d128"])
+@pytest.mark.parametrize("name", list(PLANS))
+def test_whole_and_cut_tiles(mxh, name, heads):
+    nh, nkv, hd = HEADS[heads]
+    seqs, extra = PLANS[name]
+    c = Case(seqs, nh=nh, nkv=nkv, hd=hd, page=32, lead=1, tail=2, seed=nh, extra_ld=extra).upload()
+    c.check(c.attention())
+    c.close()
+
+
+def test_graph_goes_from_cut_to_whole_tiles(mxh):
+    """One recorded call while a sequence's cached rows go from many to none and back."""
+    c = Case([(2000, 100), (3, 60), (0, 1)], nh=8, nkv=2, hd=64, page=16, seed=41).upload()
+    g = Graph([c.attend])
+    for cached in (2000, 0, 777, 2000):
+        c.seqs[0] = (cached, 100)
+        c.bufs["cached"].upload(np.asarray([cached, 3, 0], np.int32))
+        mxhip.memset(c.bufs["att"], 0)
+        mxhip.synchronize()
+        g.replay()
+        c.check(c.bufs["att"].download(np.float32).reshape(c.tokens, 8, 64))
+        c.check(c.attention())
+    g.close()
+    c.close()
+
+
 # ---- norms, rotation, append -----------------------------------------------------------------
 
 
@@ -572,6 +611,52 @@ def test_kept_rows(mxh, layers, page, nkv, hd, stride, kept):
 
 
 # ---- a run of them together ------------------------------------------------------------------------
+
+
+def test_offsets_past_32_bits(mxh):
+    """Rows more than 2^32 bytes and 2^31 elements into a layer: appended, attended, copied, kept."""
+    nh, nkv, hd, page, far = 16, 8, 128, 256, 9000
+    n_pages = far + 3
+    bufs = [mxhip.DeviceBuffer(n_pages * page * nkv * hd * 2) for _ in range(2)]
+    pool = mxhip.KvPool(*bufs, n_layer=1, n_pages=n_pages, page_rows=page, n_kv=nkv, head_dim=hd)
+    rng = np.random.default_rng(5)
+    pages, row = [far + 1, 2, far], nkv * hd  # of the sequence
+    cached, n = 2 * page + 20, 12
+    kv = rng.standard_normal((2, 3 * page, row)).astype(np.float16)
+    for b, x in zip(bufs, kv):
+        for i, p in enumerate(pages):
+            b.upload(x[i * page:(i + 1) * page], p * page * row * 2)
+    qkv = rng.standard_normal((n, (nh + 2 * nkv) * hd)).astype(np.float32)
+    up = mxhip.DeviceBuffer.from_array
+    dev = [up(np.asarray(x, np.int32)) for x in ([0, n], [cached], pages)] + [up(qkv), up(np.zeros(hd // 2)),
+                                                                            up(np.zeros((2, n, nh * hd), np.float32))]
+    batch = mxhip.KvBatch(1, n, *dev[:3], 3)
+    q, att = dev[5].ptr, dev[5].ptr + 4 * n * nh * hd
+    mxhip.qk_rope_append(pool, 0, batch, dev[3], qkv.shape[1], None, None, None, 1e-6, dev[4], True, nh, q)
+    work = mxhip.DeviceBuffer(max(mxhip.attention_paged_workspace(pool, batch, nh), 1))
+    mxhip.attention_paged(pool, 0, batch, q, nh, att, work, work.nbytes)
+    mxhip.kv_copy_pages(pool, [far], [far + 2])
+    mxhip.kv_keep_rows(pool, np.asarray([pages], np.int32), [cached], [0, 3], [1, 5, 11])
+    mxhip.synchronize()
+    new = qkv[:, nh * hd:].astype(np.float16).reshape(n, 2, row)  # (frequencies 0: nothing turns)
+    kv[:, cached:cached + n] = new.transpose(1, 0, 2)
+    copied = kv[:, 2 * page:].copy()
+    for b, x in zip(bufs, copied):
+        assert np.array_equal(b.download(np.float16, page * row, (far + 2) * page * row * 2), x.reshape(-1))
+    kept = kv.copy()
+    kept[:, cached:cached + 3] = kv[:, cached + np.asarray([1, 5, 11])]
+    for b, x in zip(bufs, kept):
+        for i, p in enumerate(pages):
+            assert np.array_equal(b.download(np.float16, page * row, p * page * row * 2), x[i * page:(i + 1) * page].reshape(-1))
+    got = dev[5].download(np.float32).reshape(2, n, nh, hd)[1]
+    k, v = (x.astype(np.float64).reshape(-1, nkv, hd) for x in kv)
+    for i in range(n):
+        for h in range(nh):
+            sc = k[:cached + i + 1, h // 2] @ qkv[i, h * hd:(h + 1) * hd].astype(np.float64) / np.sqrt(hd)
+            e = np.exp(sc - sc.max())
+            assert np.all(np.abs(got[i, h] - e / e.sum() @ v[:cached + i + 1, h // 2]) <= 1e-4)
+    for b in [*bufs, *dev, work]:
+        b.close()
 
 
 def test_drafting_forking_and_keeping(mxh):
