@@ -34,7 +34,8 @@ __device__ __forceinline__ float pa_pair_max(float v) {
 template <int HALF>
 __device__ __forceinline__ float pa_rest(float p, f16x2 h) {
     float d;
-    if constexpr (HALF) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(p));
+    if constexpr (HALF)
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(p));
     else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h), "v"(p));
     return d;
 }

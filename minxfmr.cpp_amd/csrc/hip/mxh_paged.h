@@ -62,7 +62,8 @@ __device__ __forceinline__ uint64_t tree_path(int p) {
 #pragma unroll
     for (int r = 0; r < 6; ++r) {
         const int from = p < 0 ? lane : p;
-        const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)mask, from), hi = (uint32_t)__shfl((int)(uint32_t)(mask >> 32), from);
+        const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)mask, from);
+        const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)(mask >> 32), from);
         const int next = __shfl(p, from);
         mask |= ((uint64_t)hi << 32) | lo;
         p = p < 0 ? -1 : next;
@@ -72,7 +73,8 @@ __device__ __forceinline__ uint64_t tree_path(int p) {
 
 // lane i's bits, in every lane (i below 64, any lane's own)
 __device__ __forceinline__ uint64_t path_of(uint64_t paths, int i) {
-    return ((uint64_t)(uint32_t)__shfl((int)(uint32_t)(paths >> 32), i) << 32) | (uint32_t)__shfl((int)(uint32_t)paths, i);
+    const uint64_t hi = (uint32_t)__shfl((int)(uint32_t)(paths >> 32), i);
+    return hi << 32 | (uint32_t)__shfl((int)(uint32_t)paths, i);
 }
 
 // attention over the paged cache (mxh_paged_attn.hip)

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kCopyThreads) void kv_copy_pages_kernel(CopyArgs a)
     const int i0 = chunk * kCopyThreads * kCopyUnroll + threadIdx.x;
     uint4 x[kCopyUnroll];
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u) x[u] = s[min(i0 + u * kCopyThreads, a.page16 - 1)];  // (all in flight at once)
+    for (int u = 0; u < kCopyUnroll; ++u) x[u] = s[min(i0 + u * kCopyThreads, a.page16 - 1)];
 #pragma unroll
     for (int u = 0; u < kCopyUnroll; ++u)
         if (i0 + u * kCopyThreads < a.page16) d[i0 + u * kCopyThreads] = x[u];
@@ -196,36 +196,35 @@ struct KeepArgs {
     int row16, page_rows, columns;  // 16-byte pieces of a row; columns: of all layers' K and V rows together
     uint32_t moves[kMoves];
     int pages[kKeepPages];
-    uint16_t first[kKeepGroups + 1], page0[kKeepGroups];  // group g: moves first[g] .. first[g + 1] - 1, its first page
+    uint32_t group[kKeepGroups + 1];  // first move (up to the next group's) | first page << 16
 };
 static_assert(sizeof(KeepArgs) <= 4096 && sizeof(CopyArgs) <= 4096, "");
 
 // A thread moves one 16-byte column of one sequence's rows.  The moves go in
 // ascending order with dst <= src, so a row is written only after it was read
 // (dst of a move is below the src of every later one), however many loads of
-// later moves come before a store.  Bound by its bytes and, before them, by
-// three dependent reads of the argument block: 64 paths of 6 rows of 2 KB in 36
-// layers, K and V, 38 us = 3.2 TB/s; one path 6.2 us.  Two or four columns to a
-// thread, with as many more loads in flight, took 40.9 and 41.0 us.
-constexpr int kKeepAhead = 8;
+// later moves come before a store.  Bound by its bytes: 337 moved rows of 64
+// sequences, 2 KB of K and of V in 36 layers, 20.4 us = 4.9 TB/s; four rows of one
+// sequence 5.5 us, little over an empty launch.  (As an array the eight pieces went to scratch memory: 38 us,
+// twice the bytes written.)
 __global__ __launch_bounds__(256) void kv_keep_rows_kernel(KeepArgs a) {
     const int g = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;  // (the sequences of a layer next to each other)
     if (c >= a.columns) return;
     const int per = 2 * a.row16, layer = c / per, in = c - layer * per;
     uint4* base = (in < a.row16 ? a.k + in : a.v + in - a.row16) + layer * a.layer16;
-    const int end = a.first[g + 1];
-    const int* pages = a.pages + a.page0[g];
+    const int first = (int)(a.group[g] & 0xffff), end = (int)(a.group[g + 1] & 0xffff);
+    const int* pages = a.pages + (a.group[g] >> 16);
     const auto at = [&](uint32_t code) {
         return ((int64_t)pages[code >> 10] * a.page_rows + (code & 1023)) * a.row16;
     };
-    for (int m = a.first[g]; m < end; m += kKeepAhead) {
-        uint4 x[kKeepAhead];
-#pragma unroll
-        for (int u = 0; u < kKeepAhead; ++u)  // (past the end the last again: all loads are in flight at once)
-            x[u] = base[at(a.moves[min(m + u, end - 1)] & 0xffff)];
-#pragma unroll
-        for (int u = 0; u < kKeepAhead; ++u)
-            if (m + u < end) base[at(a.moves[m + u] >> 16)] = x[u];
+    for (int m = first; m < end; m += 8) {
+        // (past the end the last again: all loads are in flight at once)
+        const auto get = [&](int u) { return base[at(a.moves[min(m + u, end - 1)] & 0xffff)]; };
+        const auto put = [&](int u, const uint4& x) {
+            if (m + u < end) base[at(a.moves[m + u] >> 16)] = x;
+        };
+        const uint4 x0 = get(0), x1 = get(1), x2 = get(2), x3 = get(3), x4 = get(4), x5 = get(5), x6 = get(6), x7 = get(7);
+        put(0, x0), put(1, x1), put(2, x2), put(3, x3), put(4, x4), put(5, x5), put(6, x6), put(7, x7);
     }
 }
 
@@ -329,7 +328,8 @@ int check_keep(const mxh_kv_pool* p, const int* table, int table_ld, const int* 
                 if (q <= last) continue;
                 last = q;
                 if (ids[q] < 0 || ids[q] >= p->n_pages)
-                    return set_error(MXH_ERR_ARG, "%s: page %d of sequence %d is %d, not in the pool", who, q, s, ids[q]);
+                    return set_error(MXH_ERR_ARG, "%s: page %d of sequence %d is %d, not in the pool", who, q, s,
+                                     ids[q]);
                 pages.push_back(ids[q]);
             }
     }
@@ -458,7 +458,7 @@ int mxh_kv_keep_rows(const mxh_kv_pool* pool, const int* table, int table_ld, co
     int moves = 0, pages = 0, groups = 0;
     const auto flush = [&] {
         if (!groups) return;
-        a.first[groups] = (uint16_t)moves;
+        a.group[groups] = (uint32_t)moves;
         hipLaunchKernelGGL(kv_keep_rows_kernel, dim3((unsigned)groups, (unsigned)((a.columns + 255) / 256)), dim3(256),
                            0, lib_stream(), a);
         moves = pages = groups = 0;
@@ -475,11 +475,12 @@ int mxh_kv_keep_rows(const mxh_kv_pool* pool, const int* table, int table_ld, co
             ready = true;
             // a sequence that does not fit goes on in another launch (in order, as
             // launches of a stream are), in a group of its own
-            if (moves == kMoves || pages + 2 > kKeepPages || (open ? pages - page0 + 2 > kKeepSlots : groups == kKeepGroups))
+            if (moves == kMoves || pages + 2 > kKeepPages ||
+                (open ? pages - page0 + 2 > kKeepSlots : groups == kKeepGroups))
                 flush(), open = false;
             if (!open) {
                 open = true;
-                a.first[groups] = (uint16_t)moves, a.page0[groups] = (uint16_t)pages;
+                a.group[groups] = (uint32_t)moves | (uint32_t)pages << 16;
                 ++groups;
                 page0 = pages, src_q = dst_q = -1;
             }
@@ -549,7 +550,8 @@ int mxh_pages_extend(mxh_pages* p, int seq, int rows, int* src, int* dst, int* c
     if (rows < 0 || rows > INT_MAX - p->book.length(seq))
         return set_error(MXH_ERR_ARG, "pages_extend: %d rows behind %d", rows, p->book.length(seq));
     if (!p->book.extend(seq, rows, src, dst))
-        return set_error(MXH_ERR_OOM, "pages_extend: %d free pages do not hold %d more rows", p->book.free_pages(), rows);
+        return set_error(MXH_ERR_OOM, "pages_extend: %d free pages do not hold %d more rows", p->book.free_pages(),
+                         rows);
     *copies = *src >= 0;
     return MXH_OK;
 } catch (const std::bad_alloc&) {

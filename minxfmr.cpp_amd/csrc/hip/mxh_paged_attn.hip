@@ -8,14 +8,14 @@
 //
 // Work: a tile is T = R / group consecutive tokens of one sequence with the
 // group = nh / nkv q heads of one kv head (row r: token r / group, head
-// r % group), R = 16 or 64 rows.  Where the batch has tiles enough, an item is
-// a tile, those with the most keys of a sequence first.  Elsewhere the stages
-// (128 or 64 keys) of all tiles are laid end to end and cut into `target` items
-// of equal length, whatever tiles they cross: the workgroups, all resident, end
-// together.  A tile that is cut leaves its parts in the workspace, two at most
-// an item, and a second kernel joins them.  The lengths are on the device, so
-// every workgroup makes the plan for itself (Plan); the grid is as wide as the
-// plan can be, and what is past its end leaves at once.
+// r % group), R = 16 or 64 rows.  Where the batch has tiles enough of like
+// length, an item is a tile, those with the most keys of a sequence first.
+// Elsewhere the stages (128 or 64 keys) of all tiles are laid end to end and cut
+// into items of equal length, whatever tiles they cross: the workgroups, all
+// resident, end together.  A tile that is cut leaves its parts in the workspace,
+// two at most an item, and a second kernel joins them.  The lengths are on the
+// device, so every workgroup makes the plan for itself (Plan); the grid is as
+// wide as the plan can be, and what is past its end leaves at once.
 //
 // K and V rows go straight into LDS (16 rows of a page are evenly spaced, so
 // their addresses are a scalar base and fixed lane offsets).  Per 32-key block
@@ -275,7 +275,8 @@ struct VRead {
         typedef short s16x8 __attribute__((ext_vector_type(8)));
         const uint32_t p = (v0 + at) ^ (uint32_t)(2 * M * d);
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(p + t * 32 * HD));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((p ^ HD) + t * 32 * HD + 8 * HD));
+        const uint32_t p1 = (p ^ HD) + t * 32 * HD + 8 * HD;
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)p1);
         return __builtin_bit_cast(f16x8, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
@@ -297,7 +298,8 @@ __device__ void redo_item(const AttnPagedArgs& a, const Segment& it, int g, int 
         __builtin_amdgcn_wave_barrier();
     };
     for (int r = wave; r < rows; r += kWaves) {
-        const int tl = (int)a.over_group((uint32_t)r), i = i0 + tl, hq = g * group + r - tl * group, tok = (int)it.first + i, cached = (int)it.cached;
+        const int tl = (int)a.over_group((uint32_t)r), i = i0 + tl, hq = g * group + r - tl * group;
+        const int tok = (int)it.first + i, cached = (int)it.cached;
         const uint64_t path = path_of(paths, i & 63);
         const float* q = a.q + ((size_t)tok * a.nh + hq) * HD;
         for (int d = lane; d < HD; d += 64) qs[d] = q[d] * a.qscale;
@@ -402,6 +404,18 @@ __device__ __forceinline__ float row_sum(float v) {
 // ahead, so that a wave's products of the next scores and its vector work on
 // these can overlap: at stage st there are V(st), K(st + 1), and on their way
 // V(st + 1), K(st + 2).
+//
+// Measured with 32/8 heads of 128:
+//   R = 16: 48 single tokens at up to 16,000 rows 255 us = 5.7 TB/s of K and V (a
+//   large read 6.7), bound by those; one at 8,192 15 us.  One token of 16/8 heads
+//   at 700 9.7 us: two launches, and in each the plan's and the pages' loads one
+//   after the other.
+//   R = 64: six packed prompts of 29 to 2,100 tokens behind up to 1,500 rows 264
+//   us = 468 TFLOP/s of the formula's, 940 of the products made (a large fp16
+//   product 1,184); matrix cores and vector units half busy each, and neither
+//   fewer reads nor fewer exponentials made it faster by more than 4%.  27 drafted
+//   tokens at 8,192 rows 24.7 us: 8 stages an item 12 of them, what comes before
+//   and after an item's stages 7, the second kernel 5.
 template <int HD, int R>
 __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedArgs a) {
     constexpr int M = R == 16 ? 16 : 32, RS = R / M;  // rows of a wave; waves to a key group
@@ -446,7 +460,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         }
         if (it.st0 < it.st1 || it.slot < 0) {  // (else only units of the lead)
         const int i0 = (int)(it.tile * T), ntok = min((int)T, (int)it.n - i0), cached = (int)it.cached;
-        const int kend = (int)min((int64_t)(cached + i0 + ntok), (int64_t)a.pg.table_ld << a.pg.page_shift);  // keys [0, kend) for the tile
+        // keys [0, kend) for the tile
+        const int kend = (int)min((int64_t)(cached + i0 + ntok), (int64_t)a.pg.table_ld << a.pg.page_shift);
         const int lim_min = a.pg.parent ? cached : cached + i0 + 1;  // every row attends the keys below
         const int key0 = STAGE * (int)it.st0, key1 = min(STAGE * (int)it.st1, kend);
         const int nst = max((key1 - key0 + STAGE - 1) / STAGE, 0);
@@ -464,7 +479,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    qv[ks][e] = valid ? *reinterpret_cast<const float4*>(qp + HD / KS * ks + 4 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    qv[ks][e] = valid ? *reinterpret_cast<const float4*>(qp + HD / KS * ks + 4 * e)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
         }
         const int parent = a.pg.parent ? tree_parent(a.pg, (int)it.first, (int)it.n) : -1;
 
@@ -528,7 +544,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             for (int u = 0; u < OWN; ++u) {
                 const uint32_t to = place + 32 * (OWN * wave + u) * HD;
                 const uint32_t(&off)[LPG] = is_v ? voff : koff;
-                const uint64_t from = (is_v ? vbase : kbase) + (((uint64_t)(uint32_t)p.hi[u] << 32) | (uint32_t)p.lo[u]);
+                const uint64_t at16 = ((uint64_t)(uint32_t)p.hi[u] << 32) | (uint32_t)p.lo[u];
+                const uint64_t from = (is_v ? vbase : kbase) + at16;
                 if (p.hi[u] >= 0 && p.r0 + 16 * u + 15 < kend) {
 #pragma unroll
                     for (int x = 0; x < LPG; ++x) g2l_s(from, off[x], to + 1024 * x);
@@ -561,7 +578,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             for (int x = 0; x < R / QR / kWaves; ++x) {
                 const uint32_t r0 = (uint32_t)(R / kWaves * wave + QR * x), r = r0 + lane / QP;
                 const uint32_t t = a.over_group(r);
-                const uint32_t off = 4 * (min(t, (uint32_t)ntok - 1) * (uint32_t)qd + (r - t * group) * HD) + 16 * ((lane % QP) ^ (r & 7));
+                const uint32_t off = 4 * (min(t, (uint32_t)ntok - 1) * (uint32_t)qd + (r - t * group) * HD) +
+                                     16 * ((lane % QP) ^ (r & 7));
                 const uint32_t at = r0 * 4 * HD;
                 g2l_s(from, off, lds0 + (at < PLACE ? PLACE + at : V0 + at));
             }
@@ -650,7 +668,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             const bool first = mref == -INFINITY;
             if (!__any(mx > (first ? -INFINITY : kPaSlack))) return;
             const float up = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(mx, 0.f);
-            const float alpha = first ? 0.f : __builtin_amdgcn_exp2f(-up);  // (nothing attended so far: the sums are zero)
+            const float alpha = first ? 0.f : __builtin_amdgcn_exp2f(-up);  // (first: the sums are zero)
             if (!first) mref += up;
             else if (mx > -INFINITY) mref = mx;
             lrun *= alpha;
@@ -698,21 +716,26 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         // so what they wait for is spread: beside a score's products the vector work
         // of two values for two of them, every instruction a product away from what it
         // needs; beside the sums' products the next scores' largest.  Returns that.
-        const auto weigh_and_score = [&](uint32_t k0, uint32_t v0, const acc_t (&s)[SB], acc_t (&next)[SB], auto&& load) __attribute__((always_inline)) {
+        const auto weigh_and_score = [&](uint32_t k0, uint32_t v0, const acc_t (&s)[SB],
+                                         acc_t (&next)[SB]) __attribute__((always_inline)) {
             float mx = -INFINITY;
             if constexpr (!PRIVATE) {
-                constexpr int STEPS = 2 * KS, VALS = NP / STEPS, AHEAD = KS < 3 ? KS : 3;  // products; scores beside one; operands on their way
+                constexpr int STEPS = 2 * KS, VALS = NP / STEPS;  // products; scores beside one
+                constexpr int AHEAD = KS < 3 ? KS : 3;            // operands on their way
                 constexpr int Y = TT * DB;
                 typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
                 f16x8 kf[KS], vf[Y];
-                const auto k_read = [&](int ks) { kf[ks] = *(lds_f16x8*)(uintptr_t)((k0 + krow) ^ (uint32_t)(32 * ks)); };
+                const auto k_read = [&](int ks) {
+                    kf[ks] = *(lds_f16x8*)(uintptr_t)((k0 + krow) ^ (uint32_t)(32 * ks));
+                };
 #pragma unroll
                 for (int ks = 0; ks < AHEAD; ++ks) k_read(ks);
                 float p[NP], ps[4] = {0.f, 0.f, 0.f, 0.f};
                 f16x2 hi[NP / 2];
                 float e[NP], rest[NP];
                 // a value's steps: exponential; scaled and summed; (pairs) high half; rests; low half
-                const auto work = [&](int u) __attribute__((always_inline)) {  // the u-th value's exponential and what follows from earlier ones
+                // (work(u): the u-th value's exponential and what follows from earlier ones)
+                const auto work = [&](int u) __attribute__((always_inline)) {
                     const int pr = (u - 5) / 2;
                     if (u >= 5 && (u - 5) % 2 == 0 && pr < NP / 2) {
                         rest[2 * pr] = pa_rest<0>(p[2 * pr], hi[pr]);
@@ -742,9 +765,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                     next[0] = MM::mul(kf[ks], j & 1 ? ql[ks] : qh[ks], j ? next[0] : start);
                     if (j & 1) {
                         if (ks + AHEAD < KS) k_read(ks + AHEAD);
-                        else if (ks + AHEAD - KS < Y) vf[ks + AHEAD - KS] = vr(v0, (ks + AHEAD - KS) / DB, (ks + AHEAD - KS) % DB);
+                        else if (ks + AHEAD - KS < Y)
+                            vf[ks + AHEAD - KS] = vr(v0, (ks + AHEAD - KS) / DB, (ks + AHEAD - KS) % DB);
                     }
-                    load(j);
 #pragma unroll
                     for (int u = VALS * j; u < VALS * (j + 1); ++u) work(u);
                     __builtin_amdgcn_sched_barrier(0);
@@ -758,9 +781,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                     o[y % DB] = MM::mul(vf[y], bh[y / DB], o[y % DB]);
                     o[y % DB] = MM::mul(vf[y], bl[y / DB], o[y % DB]);
                     if (y + AHEAD < Y) vf[y + AHEAD] = vr(v0, (y + AHEAD) / DB, (y + AHEAD) % DB);
-                    constexpr int Y0 = Y / 4 > 1 ? Y / 4 : 1, PER = (NP + Y - Y0 - 1) / (Y - Y0);  // (the scores are done by then)
+                    // (from Y0 on: the scores are done by then)
+                    constexpr int Y0 = Y / 4 > 1 ? Y / 4 : 1, PER = (NP + Y - Y0 - 1) / (Y - Y0);
 #pragma unroll
-                    for (int v = PER * (y - Y0); y >= Y0 && v < PER * (y - Y0 + 1) && v < NP; ++v) mx = fmaxf(mx, next[0][v]);
+                    for (int v = PER * (y - Y0); y >= Y0 && v < PER * (y - Y0 + 1) && v < NP; ++v)
+                        mx = fmaxf(mx, next[0][v]);
                     asm volatile("" : "+v"(mx));
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -785,7 +810,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                     if (kb + 32 > lim_min || gone) unmask(kb, s);
                     move_reference(largest(s), s);
                     weigh(s);
-                    if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");  // V, not the next K
+                    // V, not the next K
+                    if (st + 1 < nst) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPG * OWN) : "memory");
                     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     sum(v0);
                 }
@@ -819,7 +845,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                 }
                 move_reference(mx, s);
                 // (past the last stage the scores of whatever lies there, unused)
-                mx = row_max<M>(weigh_and_score(k_place(st + 1) + 64 * kg * HD, v0, s, next, [](int) {}));
+                mx = row_max<M>(weigh_and_score(k_place(st + 1) + 64 * kg * HD, v0, s, next));
                 s[0] = next[0];
                 gone = gone_next, gone_next = ahead.gone;
             }
@@ -888,7 +914,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             } else {
                 const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // (no row exists: zeros)
                 const int rt = (int)a.over_group((uint32_t)rr);
-                *reinterpret_cast<float4*>(a.att + ((size_t)(it.first + i0 + rt) * a.nh + g * group + (rr - rt * (int)group)) * HD + d) =
+                const size_t head = (size_t)(it.first + i0 + rt) * a.nh + g * group + (rr - rt * (int)group);
+                *reinterpret_cast<float4*>(a.att + head * HD + d) =
                     make_float4(x4.x * inv, x4.y * inv, x4.z * inv, x4.w * inv);
             }
         }
@@ -907,6 +934,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
 // att from the parts of the tiles that were cut: a workgroup takes 8 rows of a
 // tile and kv head, a thread four dims of a row, and where there are fewer rows
 // every `lanes`-th part.  A tile is found at its first cut, the start of item i.
+// Bound by its launch and the chain of loads from lengths to parts: 3.2 us after
+// one token at 700 rows, 5.4 us after 27 drafted ones at 8,192 (8 MB of parts).
 constexpr int kMergeRows = 8, kMergeThreads = 256;
 template <int HD, int R>
 __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(AttnPagedArgs a) {
@@ -1004,7 +1033,8 @@ int launch(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
         attr_set = true;
     }
     const unsigned nkv = (unsigned)a.pg.nkv, items = (unsigned)sh.items, y = std::min(items, 32768u);
-    hipLaunchKernelGGL((attention_paged_kernel<HD, R>), dim3(nkv, y, (items + y - 1) / y), dim3(kThreads), lds_bytes(HD, R), st, a);
+    hipLaunchKernelGGL((attention_paged_kernel<HD, R>), dim3(nkv, y, (items + y - 1) / y), dim3(kThreads),
+                       lds_bytes(HD, R), st, a);
     if (sh.target > 0)
         hipLaunchKernelGGL((attention_paged_merge_kernel<HD, R>), dim3(nkv, R / kMergeRows, (unsigned)sh.target - 1),
                            dim3(kMergeThreads), 0, st, a);
