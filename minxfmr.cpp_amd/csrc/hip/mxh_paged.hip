@@ -159,7 +159,7 @@ __global__ __launch_bounds__(kRopeThreads, 6) void qk_rope_append_kernel(RopeArg
 // Lists travel in the kernel's arguments (at most 4 KiB of them): no copy to
 // the device before the launch, and a recorded call holds its own.
 constexpr int kCopyPairs = 448;
-constexpr int kCopyThreads = 256, kCopyUnroll = 4;
+constexpr int kCopyThreads = 256;
 
 struct CopyArgs {
     uint4 *k, *v;
@@ -168,23 +168,16 @@ struct CopyArgs {
     int src[kCopyPairs], dst[kCopyPairs];
 };
 
-// Workgroup (chunk and K or V, pair, layer): 16 KB, four 16-byte loads a thread
-// in flight before its first store.  Bound by its bytes: 256 pages of 16 rows
-// of 8 heads of 128 in 36 layers 236 us = 5.1 TB/s (a large copy 5.2); one in
-// 28 layers 9.5 us, most of it the cold misses of 56 scattered regions.  With the
-// loads behind the test for the page's end, one after the other, 245 us.
+// Workgroup (chunk and K or V, pair, layer): 4 KB, a 16-byte piece a thread.  Bound
+// by its bytes: 256 pages of 16 rows of 8 heads of 128 in 36 layers 231 us = 5.2
+// TB/s, a large copy's rate; one in 28 layers 5 us, little over an empty launch.
+// Two, four and eight pieces a thread, all in flight before its first store, took
+// 235, 237 and 314 us, for 16 pages 23.5, 24.7 and 28.7 (one piece 13.6).
 __global__ __launch_bounds__(kCopyThreads) void kv_copy_pages_kernel(CopyArgs a) {
-    const int chunk = blockIdx.x >> 1;
-    uint4* base = (blockIdx.x & 1 ? a.v : a.k) + blockIdx.z * a.layer16;
-    const uint4* s = base + (int64_t)a.src[blockIdx.y] * a.page16;
-    uint4* d = base + (int64_t)a.dst[blockIdx.y] * a.page16;
-    const int i0 = chunk * kCopyThreads * kCopyUnroll + threadIdx.x;
-    uint4 x[kCopyUnroll];
-#pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u) x[u] = s[min(i0 + u * kCopyThreads, a.page16 - 1)];
-#pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
-        if (i0 + u * kCopyThreads < a.page16) d[i0 + u * kCopyThreads] = x[u];
+    const int chunk = blockIdx.x >> 1, i = chunk * kCopyThreads + threadIdx.x;
+    if (i >= a.page16) return;
+    uint4* base = (blockIdx.x & 1 ? a.v : a.k) + blockIdx.z * a.layer16 + i;
+    base[(int64_t)a.dst[blockIdx.y] * a.page16] = base[(int64_t)a.src[blockIdx.y] * a.page16];
 }
 
 // A move is 16 bits for the row it reads and 16 for the one it writes: 6 for
@@ -428,7 +421,7 @@ int mxh_kv_copy_pages(const mxh_kv_pool* pool, const int* src, const int* dst, i
     a.k = static_cast<uint4*>(pool->k), a.v = static_cast<uint4*>(pool->v);
     a.layer16 = layer_elems(pool) / 8;
     a.page16 = pool->page_rows * pool->n_kv * pool->head_dim / 8;
-    a.chunks = (a.page16 + kCopyThreads * kCopyUnroll - 1) / (kCopyThreads * kCopyUnroll);
+    a.chunks = (a.page16 + kCopyThreads - 1) / kCopyThreads;
     for (int i = 0; i < n; i += kCopyPairs) {
         const int m = std::min(kCopyPairs, n - i);
         std::copy(src + i, src + i + m, a.src);
