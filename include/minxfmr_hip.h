@@ -198,7 +198,8 @@ int mxh_attention_prefill(const float *q, const void *kc, const void *vc, float 
 /* K and V in HBM: fp16, [n_layer][n_pages][page_rows][n_kv * head_dim] each,
  * layer_stride elements from one layer to the next (0: dense).  page_rows a
  * power of two from 16 to 1024; head_dim 32, 64 or 128; k and v 16-byte
- * aligned, layer_stride a multiple of 8. */
+ * aligned, layer_stride a multiple of 8; up to 65,535 layers and 1,024 kv heads,
+ * n_layer * n_kv * head_dim up to 65535 * 1024, n_pages * page_rows below 2^31. */
 typedef struct {
     void *k, *v;
     int64_t layer_stride;
@@ -219,7 +220,8 @@ typedef struct {
  * (never attended, never written), a parent that is not smaller than its token
  * counts as -1, tokens past the 64th of a drafted tree and token rows outside
  * start[0] .. start[n_seq]-1 or past n_tokens are left alone, lengths below
- * zero count as zero.  start must not decrease. */
+ * zero count as zero, a sequence that starts below 0 has no tokens.  start must
+ * not decrease (where it does, nothing is attended and att is left alone). */
 typedef struct {
     int n_seq, n_tokens;
     const int *start;  /* [n_seq + 1] */
@@ -257,8 +259,10 @@ int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *b
  * their parts in `work`: mxh_attention_paged_workspace sets *bytes to what a
  * batch of this n_seq, n_tokens and table_ld needs at most, whatever its
  * device arrays hold.  Calls that may run at the same time (a replayed graph
- * beside the library stream) need work of their own.  q, att and work 16-byte
- * aligned, not overlapping; nh as above. */
+ * beside the library stream) need work of their own.  q and the probabilities
+ * enter the matrix cores as two fp16 halves (about 22 bits), K and V as they
+ * are; |q| must stay below 65504 sqrt(head_dim) / log2(e) (256,000 at head_dim
+ * 32).  q, att and work 16-byte aligned, not overlapping; nh as above. */
 int mxh_attention_paged(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const float *q, int nh,
                         float *att, void *work, size_t work_bytes);
 int mxh_attention_paged_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, int nh, size_t *bytes);
@@ -273,8 +277,9 @@ int mxh_kv_copy_pages(const mxh_kv_pool *pool, const int *src, const int *dst, i
  * tokens keep[keep_start[s]] < ... < keep[keep_start[s+1] - 1] (indices within
  * its new tokens); their cache rows move to rows cached[s], cached[s] + 1, ...
  * Host arrays (table [n_seq][table_ld] as in mxh_kv_batch); kept indices
- * ascending from 0 on, their rows in pages of the pool, and no row written
- * that another move reads or writes, or MXH_ERR_ARG. */
+ * ascending from 0 on, their rows in pages of the pool, and no page with a
+ * sequence's kept rows, before or after, in a second place of the table (what
+ * mxh_pages_extend made a sequence's own is that), or MXH_ERR_ARG. */
 int mxh_kv_keep_rows(const mxh_kv_pool *pool, const int *table, int table_ld, const int *cached,
                      const int *keep_start, const int *keep, int n_seq);
 

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(kRopeThreads, 6) void qk_rope_append_kernel(RopeArg
             pos = cached + i;
             bool mine = true;
             if (a.pg.parent) {
-                const int n = min(min(a.pg.start[s + 1], a.pg.n_tokens) - first, kTreeMax);
+                const int n = min(max(min(a.pg.start[s + 1], a.pg.n_tokens), first) - first, kTreeMax);
                 const uint64_t path = tree_path(tree_parent(a.pg, first, n));
                 pos = cached + __shfl((int)__popcll(path), i & 63) - 1;
                 mine = i < kTreeMax;
@@ -496,7 +496,7 @@ int mxh_kv_keep_rows(const mxh_kv_pool* pool, const int* table, int table_ld, co
 int mxh_pages_create(int n_pages, int page_rows, int max_seqs, mxh_pages** out) try {
     if (!out) return set_error(MXH_ERR_ARG, "pages_create: null output pointer");
     *out = nullptr;
-    if (n_pages < 1 || max_seqs < 1 || page_rows < 16 || page_rows > 1024 || (page_rows & (page_rows - 1)) ||
+    if (n_pages < 1 || max_seqs < 1 || max_seqs > 1 << 20 || page_rows < 16 || page_rows > 1024 || (page_rows & (page_rows - 1)) ||
         (int64_t)n_pages * page_rows > INT_MAX)
         return set_error(MXH_ERR_ARG, "pages_create: unsupported %d pages of %d rows for %d sequences", n_pages,
                          page_rows, max_seqs);

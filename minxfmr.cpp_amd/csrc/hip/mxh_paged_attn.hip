@@ -135,8 +135,9 @@ struct Plan {
     // sequence s.  Rows past the table do not exist, so no tile has stages there
     __device__ __forceinline__ Seq seq(int s) const {
         Seq q;
-        q.first = (uint32_t)max(a.start[s], 0);
-        q.n = (uint32_t)max(min(a.start[s + 1], a.n_tokens) - (int)q.first, 0);
+        const int first = a.start[s], end = min(a.start[s + 1], a.n_tokens);
+        q.first = (uint32_t)first;
+        q.n = first >= 0 && end > first ? (uint32_t)(end - first) : 0;
         if (a.parent) q.n = min(q.n, (uint32_t)kTreeMax);
         q.cached = (uint32_t)min(max(a.cached[s], 0), 1 << 30);
         // (n up to 2^20: the quotient is off by less than 2^-3 / t, and n + t - 1/2 is
@@ -197,8 +198,10 @@ struct Plan {
         sum = 0;
         mine = Seq{0, 0, 0, 0, 0};
         uint32_t tiles = 0, longest = 0;
+        bool falls = false;
         for (int s = lane * part; s < min((lane + 1) * part, a.n_seq); ++s) {
             mine = seq(s);
+            falls |= a.start[s + 1] < a.start[s];
             tiles += mine.tiles;
             if (cut && mine.tiles > 0) sum += units(mine), longest = max(longest, lead + mine.stages);
         }
@@ -215,6 +218,7 @@ struct Plan {
             upto = wave_scan(sum);
             total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
         }
+        if (__any(falls)) total = 0;  // (sequences that overlap: their units need not fit 32 bits)
     }
     // the sequence of unit x (< total), and x from its first unit on
     __device__ __forceinline__ int find(uint32_t& x, Seq& q) const {

@@ -351,6 +351,41 @@ def test_lengths_below_zero_and_trees_past_64(mxh):
     c.close()
 
 
+LOW, HIGH = -2**31, 2**31 - 1
+
+
+@pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
+@pytest.mark.parametrize("start", [[0, LOW, 9], [5, LOW, LOW], [3, 1, 9], [0, HIGH, 9], [HIGH, HIGH, HIGH], [LOW, LOW, HIGH],
+                                   [-4, 2, 9], [0, 0, HIGH], [9, 9, 9], [12, 13, 14], [0, 4, HIGH]])
+def test_starts_that_make_no_sense_stay_inside(mxh, start, tree):
+    """Falling starts attend nothing; a sequence from below 0 has no tokens; ends past n_tokens end there."""
+    c = Case([(40, 4), (20, 5)], nh=4, nkv=2, hd=64, page=16, seed=6, tree=tree).upload()
+    c.bufs["start"].upload(np.asarray(start, np.int32))
+    got = c.attention()
+    falls = any(b < a for a, b in zip(start, start[1:]))
+    mine = [range(a, min(b, c.tokens)) if a >= 0 and not falls else [] for a, b in zip(start, start[1:])]
+    written = sorted(t for r in mine for t in r)
+    left = np.all(got == FILL, axis=(1, 2))
+    assert [t for t in range(c.tokens) if not left[t]] == written
+    qkv, _, _ = rope_inputs(c, 1)
+    dq, df = mxhip.DeviceBuffer.from_array(qkv), mxhip.DeviceBuffer.from_array(mxhip.rope_frequencies(1e4, 64))
+    out = mxhip.DeviceBuffer.from_array(np.full((c.tokens, 256), FILL))
+    mxhip.qk_rope_append(c.pool, 0, c.batch, dq, 512, None, None, None, 1e-6, df, True, 4, out)
+    mxhip.synchronize()
+    q = out.download(np.float32).reshape(c.tokens, 256)
+    if not falls:
+        assert [t for t in range(c.tokens) if np.any(q[t] != FILL)] == written
+    # only rows of the two sequences' pages may have changed, none before their cached rows
+    pool = c.bufs["k"].download(np.uint16).reshape(-1, 128)
+    old = c.k.view(np.uint16).reshape(-1, 128)
+    for s, (n_c, _) in enumerate(c.seqs):
+        for r in range(n_c):
+            assert np.array_equal(c.row(pool.reshape(1, -1), s, r), c.row(old.reshape(1, -1), s, r))
+    for b in (dq, df, out):
+        b.close()
+    c.close()
+
+
 def test_attention_needs_its_work(mxh):
     c = Case([(5000, 1)], nh=8, nkv=2, hd=128, page=16, seed=1).upload()
     if c.work_bytes:

@@ -290,3 +290,13 @@ def test_keeping_refuses():
     # nothing to move: no GPU needed either
     keep(pool(), [[0, 1]], [3], [0, 3], [0, 1, 2])
     keep(pool(), [[0, 1], [1, 0]], [3, 7], [0, 0, 0], [])
+
+
+def test_sizes_past_the_limits_are_refused():
+    h = C.c_void_p()
+    assert mxhip.lib.mxh_pages_create(4, 16, (1 << 20) + 1, C.byref(h)) == ERR_ARG and not h.value
+    wide = pool(n_layer=65535, n_kv=512, head_dim=32, n_pages=1, page_rows=16)  # a row of 128 MB
+    fits = pool(n_layer=65535, n_kv=32, head_dim=32, n_pages=1, page_rows=16)
+    with pytest.raises(mxhip.MxhError, match="unsupported pool"):
+        mxhip.kv_copy_pages(wide, [], [])
+    mxhip.kv_copy_pages(fits, [], [])
