@@ -261,8 +261,9 @@ int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *b
  * device arrays hold.  Calls that may run at the same time (a replayed graph
  * beside the library stream) need work of their own.  q and the probabilities
  * enter the matrix cores as two fp16 halves (about 22 bits), K and V as they
- * are; |q| must stay below 65504 sqrt(head_dim) / log2(e) (256,000 at head_dim
- * 32).  q, att and work 16-byte aligned, not overlapping; nh as above. */
+ * are; rows that meet infinities or NaN, or a |q| from 65504 sqrt(head_dim) /
+ * log2(e) on, are computed again in fp32 (slowly, milliseconds for thousands of
+ * keys).  q, att and work 16-byte aligned, not overlapping; nh as above. */
 int mxh_attention_paged(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const float *q, int nh,
                         float *att, void *work, size_t work_bytes);
 int mxh_attention_paged_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, int nh, size_t *bytes);

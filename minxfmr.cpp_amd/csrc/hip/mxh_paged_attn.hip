@@ -34,8 +34,9 @@
 //
 // Rows that a token does not attend must not reach it: their scores are
 // replaced, not added to, and since 0 times an infinity is no zero, an item whose
-// sums met an infinity or a NaN in V is computed again without products over
-// rows that a token does not attend (redo_item).
+// sums met an infinity or a NaN is computed again in fp32, without products over
+// rows that a token does not attend (redo_item).  That takes in what fp16 halves
+// cannot say: a q past 65504, an infinite score.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -879,10 +880,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                 }
             }
             // An infinity or a NaN in a V row makes sums of infinities and NaN, of rows
-            // that attend it and, as 0 times it, of rows that do not.  (Where the sum of
-            // probabilities is NaN, what was attended makes the output NaN.)
-            const uint64_t redo = __ballot(valid && !(bad == 0.f) && lsum == lsum);
-            if (lane == 0) flags[wave] = redo != 0;
+            // that attend it and, as 0 times it, of rows that do not; one in K, or a q
+            // past fp16, a NaN of what may be an infinite or an ordinary score (its two
+            // halves meet).  Nothing else helps a row whose q is not finite.
+            bool redo = valid && !(bad == 0.f);
+            if (redo && !(lsum == lsum)) {
+                const float* qp = q0 + (i - i0) * qd + (row - tl * group) * HD;
+                float rest = 0.f;
+#pragma unroll 1
+                for (int d = 0; d < HD; ++d) rest = fmaf(qp[d], 0.f, rest);
+                redo = rest == 0.f;
+            }
+            const uint64_t any = __ballot(redo);
+            if (lane == 0) flags[wave] = any != 0;
         }
         __syncthreads();
         const bool again = flags[0] | flags[1] | flags[2] | flags[3];

@@ -281,6 +281,44 @@ def test_infinite_values_among_rows_that_all_attend(mxh, cached, rows, n):
     c.close()
 
 
+@pytest.mark.parametrize("seqs,tree", [([(300, 1), (20, 2)], False), ([(700, 45)], False), ([(100, 30), (9, 4)], True)])
+def test_scores_of_minus_infinity(mxh, seqs, tree):
+    """An attended K value of an infinity: nothing of that row where the score is -inf, NaN where it is +inf."""
+    c = Case(seqs, nh=4, nkv=2, hd=64, page=16, tree=tree, seed=14)
+    for s, (n_c, n) in enumerate(seqs):
+        for r in (3, n_c - 1, n_c + n - 1):
+            c.row(c.k, s, r)[7 + r % 3] = -np.inf  # (kv head 0)
+    q = c.q.reshape(c.tokens, 4, 64)
+    q[:, 0, 7:10] = np.abs(q[:, 0, 7:10])  # q head 0: -inf every time; q head 1: by its signs
+    c.upload()
+    got = c.attention()
+    for s, (n_c, n) in enumerate(seqs):
+        k, v = (np.array([c.row(x, s, r) for r in range(n_c + n)], np.float64).reshape(-1, 2, 64) for x in (c.k, c.v))
+        for i in range(n):
+            t, at = int(c.start[s]) + i, list(range(n_c)) + [n_c + j for j in c.before(s, i)]
+            for h in range(4):
+                sc = k[at, h // 2] @ q[t, h].astype(np.float64) / 8
+                if np.any(sc == np.inf):
+                    assert np.all(np.isnan(got[t, h])), (s, i, h)
+                    continue
+                p = np.exp(sc - sc.max())
+                want = p @ v[at, h // 2] / p.sum()
+                assert np.all(np.abs(got[t, h] - want) <= 1e-4), (s, i, h)
+    c.close()
+
+
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32"])
+def test_q_past_fp16(mxh, heads):
+    """q of millions over a K of millionths."""
+    nh, nkv, hd = HEADS[heads]
+    c = Case([(300, 1), (150, 40), (3, 2)], nh=nh, nkv=nkv, hd=hd, page=16, seed=15)
+    c.q *= 2e6
+    c.k = (c.k.astype(np.float32) * 1e-5).astype(np.float16)
+    c.upload()
+    c.check(c.attention())
+    c.close()
+
+
 @pytest.mark.parametrize("seqs,tree", [([(300, 1)], False), ([(40, 30), (700, 50)], False), ([(130, 20), (5, 1)], True)])
 def test_nan_reaches_the_outputs_that_read_it(mxh, seqs, tree):
     """A NaN in a token's q is its head's; NaN in a cached key is everybody's who attends it, in its kv head."""
@@ -646,6 +684,57 @@ def test_kept_rows(mxh, layers, page, nkv, hd, stride, kept):
 
 
 # ---- a run of them together ------------------------------------------------------------------------
+
+
+def test_a_recorded_step_holds_its_lists(mxh):
+    """Append, attention of trees, copy and kept rows in one graph: the host lists may go, device arrays are followed."""
+    nh, nkv, hd, page = 8, 2, 128, 16
+    c = Case([(30, 20), (100, 9)], nh=nh, nkv=nkv, hd=hd, page=page, tree=True, seed=51, spare=4).upload()
+    qkv, b, w = rope_inputs(c, 7)
+    freq = mxhip.rope_frequencies(1e4, hd)
+    put = mxhip.DeviceBuffer.from_array
+    dev = [put(qkv), put(b), put(w[0]), put(w[1]), put(freq)]
+    spare = sorted(set(range(c.n_pages)) - set(c.table[c.table >= 0].tolist()))
+    src, dst = np.asarray([c.table[0, 0], c.table[1, 3]], np.int32), np.asarray(spare[:2], np.int32)
+    cached = np.asarray([30, 100], np.int32)
+    keep, keep_start, table = np.asarray([1, 4, 19, 0, 8], np.int32), np.asarray([0, 3, 5], np.int32), c.table.copy()
+    g = Graph([lambda: mxhip.qk_rope_append(c.pool, 0, c.batch, dev[0], qkv.shape[1], dev[1], dev[2], dev[3], 1e-6,
+                                            dev[4], True, nh, c.bufs["q"]),
+               c.attend,
+               lambda: mxhip.kv_copy_pages(c.pool, src, dst),
+               lambda: mxhip.kv_keep_rows(c.pool, table, cached, keep_start, keep)])
+    kept = [(0, [1, 4, 19]), (1, [0, 8])]
+    moved = list(zip(src.tolist(), dst.tolist()))
+    src[:], dst[:], cached[:], keep[:], keep_start[:], table[:] = 0, 0, 0, 0, 0, -1
+    rows = page * nkv * hd
+    for r in range(3):
+        if r == 2:
+            c.parents = [bush(n, c.rng) for _, n in c.seqs]
+            c.bufs["parent"].upload(c.parent_array())
+        c.bufs["k"].upload(c.k), c.bufs["v"].upload(c.v)
+        mxhip.memset(c.bufs["att"], 0)
+        mxhip.synchronize()
+        g.replay()
+        got = c.bufs["att"].download(np.float32).reshape(c.tokens, nh, hd)
+        after = [c.bufs[n].download(np.float16) for n in ("k", "v")]
+        # the same step eagerly, call by call
+        c.bufs["k"].upload(c.k), c.bufs["v"].upload(c.v)
+        mxhip.qk_rope_append(c.pool, 0, c.batch, dev[0], qkv.shape[1], dev[1], dev[2], dev[3], 1e-6, dev[4], True, nh,
+                             c.bufs["q"])
+        assert np.array_equal(c.attention(), got)
+        for n, x in zip(("k", "v"), after):
+            want = c.bufs[n].download(np.uint16).reshape(1, -1)
+            for a, z in moved:
+                want[0, z * rows:(z + 1) * rows] = want[0, a * rows:(a + 1) * rows]
+            old = want.copy()
+            for s, new in kept:
+                for i, j in enumerate(new):
+                    c.row(want, s, c.seqs[s][0] + i)[:] = c.row(old, s, c.seqs[s][0] + j)
+            assert np.array_equal(x.view(np.uint16), want.reshape(-1)), (r, n)
+    g.close()
+    for x in dev:
+        x.close()
+    c.close()
 
 
 def test_offsets_past_32_bits(mxh):
