@@ -246,6 +246,7 @@ struct AttnPagedArgs {
     float* att;
     float* part;  // [2 target][nkv][R][HD]: V sums of the parts of tiles
     float2* ml;   // [2 target][nkv][R]: references and sums
+    int4* cuts;   // [target]: of the tile that is cut first where item i starts, its first token, rows, parts (0: none)
     int nh, target;  // target: items that stages are cut into, at most; 0: an item is a tile
     float qscale;
     uint32_t group, tokens;  // q heads of a kv head; tokens of a tile, R / group
@@ -443,8 +444,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     const Plan plan(a.pg, R, T, a.target);
     static_assert(STAGE == stage_keys(R), "");
     uint32_t x = index * plan.per;  // (units of the plan that fit 32 bits: target items at most)
-    if (x >= plan.total) return;
-    const uint32_t x1 = min(x + plan.per, plan.total);
+    const bool tells = g == 0 && threadIdx.x == 0 && index < (uint32_t)a.target;  // (for the second kernel)
+    if (x >= plan.total) {
+        if (tells) a.cuts[index] = make_int4(0, 0, 0, 0);
+        return;
+    }
+    const uint32_t x0 = x, x1 = min(x + plan.per, plan.total);
     Seq seq;
     uint32_t r_unit = x;
     Segment it;
@@ -461,6 +466,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             it.st0 = plan.cut ? max(spot.at, plan.lead) - plan.lead : 0;
             it.st1 = plan.cut ? max(end, plan.lead) - plan.lead : seq.stages;
             it.slot = !plan.cut || (it.st0 == 0 && end == spot.units) ? -1 : (int)(2 * index + (it.st0 == 0));
+            if (tells && x == x0) {
+                // (no stage before the lead's end; not the tile's first cut a whole item after it)
+                const bool first = plan.cut && spot.at > plan.lead && spot.at <= plan.lead + plan.per;
+                const int i0 = (int)(spot.tile * T), parts = 1 + (int)((spot.units - spot.at + plan.per - 1) / plan.per);
+                a.cuts[index] = make_int4((int)seq.first + i0, min((int)T, (int)seq.n - i0) * (int)group, first ? parts : 0, 0);
+            }
             x += len, r_unit += len;
         }
         if (it.st0 < it.st1 || it.slot < 0) {  // (else only units of the lead)
@@ -956,19 +967,11 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
     constexpr int AHEAD = 8;
     __shared__ float4 acc[kMergeThreads];
     __shared__ float2 st[kMergeThreads];
-    const uint32_t nkv = (uint32_t)a.pg.nkv, group = a.group, T = a.tokens;
+    const uint32_t nkv = (uint32_t)a.pg.nkv, group = a.group;
     const uint32_t rb = blockIdx.y, g = blockIdx.x, item = blockIdx.z + 1;
-    const Plan plan(a.pg, R, T, a.target);
-    uint32_t x = item * plan.per;
-    if (x >= plan.total) return;
-    Seq seq;
-    plan.find(x, seq);
-    const Plan::Spot spot = plan.spot(seq, x);
-    const uint32_t units = spot.units, tile = spot.tile, cut = spot.at;
-    if (cut <= plan.lead || cut > plan.lead + plan.per) return;  // (no stage before it; not the first of the tile's)
-    const int rows = min((int)(min(T, seq.n - tile * T) * group) - (int)rb * kMergeRows, kMergeRows);
-    if (rows <= 0) return;
-    const int parts = 1 + (int)((units - cut + plan.per - 1) / plan.per);  // items item - 1, item, ...
+    const int4 cut = a.cuts[item];
+    const int rows = min(cut.y - (int)rb * kMergeRows, kMergeRows), parts = cut.z;  // parts: of items item - 1, item, ...
+    if (parts == 0 || rows <= 0) return;
     const auto slot = [&](int z) { return z ? 2 * (item - 1 + (uint32_t)z) : 2 * (item - 1) + 1; };
     const int tid = threadIdx.x, per = rows * (HD / 4), lanes = kMergeThreads / per;
     const int z0 = tid / per, u = tid - z0 * per, d = 4 * (u % (HD / 4)), row = (int)rb * kMergeRows + u / (HD / 4);
@@ -1004,7 +1007,7 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
     for (int i = 1; i < lanes; ++i) join(st[tid + i * per], acc[tid + i * per]);
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     const uint32_t tl = a.over_group((uint32_t)row);
-    const size_t tok = (size_t)seq.first + tile * T + tl;
+    const size_t tok = (size_t)cut.x + tl;
     *reinterpret_cast<float4*>(a.att + (tok * a.nh + g * group + ((uint32_t)row - tl * group)) * HD + d) =
         make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
@@ -1064,7 +1067,7 @@ int launch_hd(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
 
 size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd) {
     const Shape s = attention_shape(a, nh, hd);
-    return (size_t)2 * s.target * a.nkv * s.rows * (hd + 2) * sizeof(float);
+    return (size_t)2 * s.target * a.nkv * s.rows * (hd + 2) * sizeof(float) + s.target * sizeof(int4);
 }
 
 int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, float* att, void* work, hipStream_t st) {
@@ -1072,7 +1075,8 @@ int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, f
     float* part = static_cast<float*>(work);
     float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * s.target * a.nkv * s.rows * hd);
     const uint32_t group = (uint32_t)(nh / a.nkv);
-    const AttnPagedArgs args{a, q, att, part, ml, nh, s.target, 1.4426950408889634f / sqrtf((float)hd),
+    int4* cuts = reinterpret_cast<int4*>(ml + (size_t)2 * s.target * a.nkv * s.rows);
+    const AttnPagedArgs args{a, q, att, part, ml, cuts, nh, s.target, 1.4426950408889634f / sqrtf((float)hd),
                              group, (uint32_t)s.rows / group, (65536 + group - 1) / group};
     return hd == 32 ? launch_hd<32>(args, s, st) : hd == 64 ? launch_hd<64>(args, s, st) : launch_hd<128>(args, s, st);
 }
