@@ -412,16 +412,17 @@ __device__ __forceinline__ float row_sum(float v) {
 // V(st + 1), K(st + 2).
 //
 // Measured with 32/8 heads of 128:
-//   R = 16: 48 single tokens at up to 16,000 rows 255 us = 5.7 TB/s of K and V (a
+//   R = 16: 48 single tokens at up to 16,000 rows 254 us = 5.7 TB/s of K and V (a
 //   large read 6.7), bound by those; one at 8,192 15 us.  One token of 16/8 heads
-//   at 700 9.7 us: two launches, and in each the plan's and the pages' loads one
-//   after the other.
+//   at 700 9.5 us: two launches, and in the first the plan's, the pages' and the
+//   rows' loads one after the other.
 //   R = 64: six packed prompts of 29 to 2,100 tokens behind up to 1,500 rows 264
 //   us = 468 TFLOP/s of the formula's, 940 of the products made (a large fp16
 //   product 1,184); matrix cores and vector units half busy each, and neither
 //   fewer reads nor fewer exponentials made it faster by more than 4%.  27 drafted
-//   tokens at 8,192 rows 24.7 us: 8 stages an item 12 of them, what comes before
-//   and after an item's stages 7, the second kernel 5.
+//   tokens at 8,192 rows 24.3 us: 8 stages an item 12 of them (a stage's loads are
+//   one stage ahead and HBM is 1.4 us away), what comes before and after an item's
+//   stages 7, the second kernel 4.
 template <int HD, int R>
 __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedArgs a) {
     constexpr int M = R == 16 ? 16 : 32, RS = R / M;  // rows of a wave; waves to a key group
@@ -958,9 +959,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
 
 // att from the parts of the tiles that were cut: a workgroup takes 8 rows of a
 // tile and kv head, a thread four dims of a row, and where there are fewer rows
-// every `lanes`-th part.  A tile is found at its first cut, the start of item i.
-// Bound by its launch and the chain of loads from lengths to parts: 3.2 us after
-// one token at 700 rows, 5.4 us after 27 drafted ones at 8,192 (8 MB of parts).
+// every `lanes`-th part.  A tile is found at its first cut, the start of item i,
+// where that item left word of it (the plan made again here took 0.3 to 0.9 us
+// more).  Bound by its launch and two loads in a row: 3.8 us after one token at
+// 700 rows, 4.4 us after 27 drafted ones at 8,192 (8 MB of parts).
 constexpr int kMergeRows = 8, kMergeThreads = 256;
 template <int HD, int R>
 __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(AttnPagedArgs a) {
