@@ -256,8 +256,8 @@ int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *b
  * attend has no effect on it, infinities and NaN included; a token none of
  * whose rows exist gets zeros.  Takes whole prompts, single tokens and drafted
  * trees, mixed as they come.  Long rows of keys are split among workgroups,
- * their parts in `work`: mxh_attention_paged_workspace sets *bytes to what a
- * batch of this n_seq, n_tokens and table_ld needs at most, whatever its
+ * their parts in `work`: mxh_attention_paged_workspace sets *bytes to what any
+ * batch of up to this n_seq, n_tokens and table_ld needs at most, whatever its
  * device arrays hold.  Calls that may run at the same time (a replayed graph
  * beside the library stream) need work of their own.  q and the probabilities
  * enter the matrix cores as two fp16 halves (about 22 bits), K and V as they

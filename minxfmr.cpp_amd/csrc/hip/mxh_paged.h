@@ -78,7 +78,8 @@ __device__ __forceinline__ uint64_t path_of(uint64_t paths, int i) {
 }
 
 // attention over the paged cache (mxh_paged_attn.hip)
-size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd);
+size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd);  // of this batch
+size_t attention_paged_work_bound(const PagedArgs& a, int nh, int hd);  // of any up to its n_seq, n_tokens, table_ld
 int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, float* att, void* work, hipStream_t st);
 
 }  // namespace mxh

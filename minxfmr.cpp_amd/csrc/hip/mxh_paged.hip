@@ -216,7 +216,8 @@ __global__ __launch_bounds__(256) void kv_keep_rows_kernel(KeepArgs a) {
         const auto put = [&](int u, const uint4& x) {
             if (m + u < end) base[at(a.moves[m + u] >> 16)] = x;
         };
-        const uint4 x0 = get(0), x1 = get(1), x2 = get(2), x3 = get(3), x4 = get(4), x5 = get(5), x6 = get(6), x7 = get(7);
+        const uint4 x0 = get(0), x1 = get(1), x2 = get(2), x3 = get(3);
+        const uint4 x4 = get(4), x5 = get(5), x6 = get(6), x7 = get(7);
         put(0, x0), put(1, x1), put(2, x2), put(3, x3), put(4, x4), put(5, x5), put(6, x6), put(7, x7);
     }
 }
@@ -378,7 +379,7 @@ int mxh_attention_paged_workspace(const mxh_kv_pool* pool, const mxh_kv_batch* b
     if (int rc = check_step("attention_paged_workspace", pool, 0, batch, nh)) return rc;
     if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
     if (!mxh_is_available()) return MXH_ERR_NODEV;
-    *bytes = attention_paged_work_bytes(paged_args(pool, 0, batch), nh, pool->head_dim);
+    *bytes = attention_paged_work_bound(paged_args(pool, 0, batch), nh, pool->head_dim);
     return MXH_OK;
 }
 
@@ -496,7 +497,8 @@ int mxh_kv_keep_rows(const mxh_kv_pool* pool, const int* table, int table_ld, co
 int mxh_pages_create(int n_pages, int page_rows, int max_seqs, mxh_pages** out) try {
     if (!out) return set_error(MXH_ERR_ARG, "pages_create: null output pointer");
     *out = nullptr;
-    if (n_pages < 1 || max_seqs < 1 || max_seqs > 1 << 20 || page_rows < 16 || page_rows > 1024 || (page_rows & (page_rows - 1)) ||
+    if (n_pages < 1 || max_seqs < 1 || max_seqs > 1 << 20 || page_rows < 16 || page_rows > 1024 ||
+        (page_rows & (page_rows - 1)) ||
         (int64_t)n_pages * page_rows > INT_MAX)
         return set_error(MXH_ERR_ARG, "pages_create: unsupported %d pages of %d rows for %d sequences", n_pages,
                          page_rows, max_seqs);

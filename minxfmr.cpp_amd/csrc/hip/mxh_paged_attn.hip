@@ -417,8 +417,8 @@ __device__ __forceinline__ float row_sum(float v) {
 //   at 700 9.5 us: two launches, and in the first the plan's, the pages' and the
 //   rows' loads one after the other.
 //   R = 64: six packed prompts of 29 to 2,100 tokens behind up to 1,500 rows 264
-//   us = 468 TFLOP/s of the formula's, 940 of the products made (a large fp16
-//   product 1,184); matrix cores and vector units half busy each, and neither
+//   us (276 on another card) = 468 TFLOP/s of the formula's, 940 of the products
+//   made (a large fp16 product 1,184); matrix cores and vector units half busy each, and neither
 //   fewer reads nor fewer exponentials made it faster by more than 4%.  27 drafted
 //   tokens at 8,192 rows 24.3 us: 8 stages an item 12 of them (a stage's loads are
 //   one stage ahead and HBM is 1.4 us away), what comes before and after an item's
@@ -470,8 +470,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
             if (tells && x == x0) {
                 // (no stage before the lead's end; not the tile's first cut a whole item after it)
                 const bool first = plan.cut && spot.at > plan.lead && spot.at <= plan.lead + plan.per;
-                const int i0 = (int)(spot.tile * T), parts = 1 + (int)((spot.units - spot.at + plan.per - 1) / plan.per);
-                a.cuts[index] = make_int4((int)seq.first + i0, min((int)T, (int)seq.n - i0) * (int)group, first ? parts : 0, 0);
+                const int i0 = (int)(spot.tile * T), rows = min((int)T, (int)seq.n - i0) * (int)group;
+                const int parts = 1 + (int)((spot.units - spot.at + plan.per - 1) / plan.per);
+                a.cuts[index] = make_int4((int)seq.first + i0, rows, first ? parts : 0, 0);
             }
             x += len, r_unit += len;
         }
@@ -972,7 +973,7 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
     const uint32_t nkv = (uint32_t)a.pg.nkv, group = a.group;
     const uint32_t rb = blockIdx.y, g = blockIdx.x, item = blockIdx.z + 1;
     const int4 cut = a.cuts[item];
-    const int rows = min(cut.y - (int)rb * kMergeRows, kMergeRows), parts = cut.z;  // parts: of items item - 1, item, ...
+    const int rows = min(cut.y - (int)rb * kMergeRows, kMergeRows), parts = cut.z;  // of items item - 1, item, ...
     if (parts == 0 || rows <= 0) return;
     const auto slot = [&](int z) { return z ? 2 * (item - 1 + (uint32_t)z) : 2 * (item - 1) + 1; };
     const int tid = threadIdx.x, per = rows * (HD / 4), lanes = kMergeThreads / per;
@@ -1024,20 +1025,30 @@ struct Shape {
     int rows, target;
     int64_t items;  // at most
 };
-Shape attention_shape(const PagedArgs& a, int nh, int hd) {
+// items of R-row tiles; stages of a tile, at most
+int most_items(int rows, int nkv) { return (rows == 64 ? 2 : 1) * std::max(2, device_cus() / nkv); }
+int64_t most_stages(const PagedArgs& a, int rows) {
+    const int64_t keys = stage_keys(rows);
+    return (((int64_t)a.table_ld << a.page_shift) + keys - 1) / keys;
+}
+// whether some lengths could make cut tiles worth the second kernel's 4 us: the
+// longest tile that the table allows, and `tiles` of one stage
+bool cut_may_pay(const PagedArgs& a, int rows, int64_t tiles) {
+    const int64_t stages = most_stages(a, rows);
+    return stages > 1 && cut_pays(rows, (float)(stages + tile_lead(rows)), (float)(1 + tile_lead(rows)) * (float)tiles,
+                                  (float)most_items(rows, a.nkv));
+}
+size_t work_bytes(int rows, int target, int nkv, int hd) {
+    return (size_t)2 * target * nkv * rows * (hd + 2) * sizeof(float) + target * sizeof(int4);
+}
+Shape attention_shape(const PagedArgs& a, int nh) {
     Shape s;
     const int group = nh / a.nkv;
     s.rows = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group > 16 ? 64 : 16;
-    const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq, keys = stage_keys(s.rows);
-    const int64_t stages = (((int64_t)a.table_ld << a.page_shift) + keys - 1) / keys;  // of a tile, at most
-    const int target = (s.rows == 64 ? 2 : 1) * std::max(2, device_cus() / a.nkv);
-    // no second kernel where no lengths could make it worth its 4 us: a table of so
-    // few keys, and tiles of one stage at least (no sequence empty)
-    const int64_t tiles_min = std::max(a.n_tokens / (s.rows / group), std::min(a.n_seq, a.n_tokens));
-    const int least = 1 + tile_lead(s.rows), most = (int)std::min(stages, (int64_t)INT_MAX / 2) + tile_lead(s.rows);
-    const bool may_cut = stages > 1 && tiles * most < INT_MAX &&
-                         cut_pays(s.rows, (float)most, (float)least * (float)tiles_min, (float)target);
-    s.target = may_cut ? target : 0;
+    const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq;
+    const int64_t tiles_min = std::max(a.n_tokens / (s.rows / group), std::min(a.n_seq, a.n_tokens));  // (none empty)
+    const bool fits = tiles * (most_stages(a, s.rows) + tile_lead(s.rows)) < INT_MAX;  // (the plan's units)
+    s.target = fits && cut_may_pay(a, s.rows, tiles_min) ? most_items(s.rows, a.nkv) : 0;
     s.items = std::max((int64_t)s.target, tiles);
     return s;
 }
@@ -1068,12 +1079,20 @@ int launch_hd(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
 }  // namespace
 
 size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd) {
-    const Shape s = attention_shape(a, nh, hd);
-    return (size_t)2 * s.target * a.nkv * s.rows * (hd + 2) * sizeof(float) + s.target * sizeof(int4);
+    const Shape s = attention_shape(a, nh);
+    return work_bytes(s.rows, s.target, a.nkv, hd);
+}
+
+size_t attention_paged_work_bound(const PagedArgs& a, int nh, int hd) {
+    size_t most = 0;
+    for (const int rows : {16, 64})
+        if ((rows == 16 || (int64_t)a.n_tokens * (nh / a.nkv) > 16) && cut_may_pay(a, rows, 1))
+            most = std::max(most, work_bytes(rows, most_items(rows, a.nkv), a.nkv, hd));
+    return most;
 }
 
 int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, float* att, void* work, hipStream_t st) {
-    const Shape s = attention_shape(a, nh, hd);
+    const Shape s = attention_shape(a, nh);
     float* part = static_cast<float*>(work);
     float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * s.target * a.nkv * s.rows * hd);
     const uint32_t group = (uint32_t)(nh / a.nkv);

@@ -434,6 +434,32 @@ def test_attention_needs_its_work(mxh):
     c.close()
 
 
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (32, 8, 64), (3, 1, 32)])
+def test_the_largest_batchs_work_is_enough(mxh, nh, nkv, hd):
+    """Workspaces grow with n_seq, n_tokens and table_ld, and a small batch runs in a large one's."""
+    pool = mxhip.KvPool(1 << 20, 1 << 21, n_layer=1, n_pages=4000, page_rows=16, n_kv=nkv, head_dim=hd)
+    size = lambda s, t, ld: mxhip.attention_paged_workspace(  # noqa: E731
+        pool, mxhip.KvBatch(s, t, 1 << 20, 1 << 20, 1 << 20, ld, None), nh)
+    steps = [(1, 4, 64, 4096), (1, 3, 5, 9, 64, 1000, 1 << 20), (1, 3, 5, 9, 30, 40, 70, 600, 4000)]
+    for s in steps[0]:
+        for t in steps[1]:
+            for ld in steps[2]:
+                for up in ((4096, t, ld), (s, 1 << 20, ld), (s, t, 4000)):
+                    assert size(s, t, ld) <= size(*up), (s, t, ld, up)
+    n = size(300, 1000, 70)
+    work = mxhip.DeviceBuffer(n)
+    for seqs, tree in (([(900, 1)], False), ([(0, 200)] * 5, False), ([(1000, 40), (3, 9)], True), ([(700, 3)] * 20, True),
+                       ([(i, 1) for i in range(300)], False)):
+        c = Case(seqs, nh=nh, nkv=nkv, hd=hd, page=16, tree=tree, seed=3, extra_ld=1)
+        assert c.ld <= 70 and c.tokens <= 1000
+        c.upload()
+        mxhip.attention_paged(c.pool, 0, c.batch, c.bufs["q"], nh, c.bufs["att"], work, n)
+        mxhip.synchronize()
+        c.check(c.bufs["att"].download(np.float32).reshape(c.tokens, nh, hd))
+        c.close()
+    work.close()
+
+
 def test_graph_follows_the_lengths(mxh):
     """A recorded step replayed on another stream while lengths, tables and q change, eager work between the replays."""
     a = Case([(900, 1), (10, 1), (3000, 1)], nh=8, nkv=2, hd=128, page=16, seed=21).upload()
