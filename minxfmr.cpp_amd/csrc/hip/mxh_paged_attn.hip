@@ -100,7 +100,8 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive
 // whether `target` items of a batch of `all` units finish before its whole tiles
 // do, the longest of `longest` units (Plan)
 __host__ __device__ constexpr bool cut_pays(int rows, float longest, float all, float target) {
-    return rows == 64 ? longest * target > 13.f * target + 1.8f * all : longest > 12.f || 2.f * longest * target > all;
+    return rows == 64 ? longest * target > 13.f * target + 1.8f * all || longest * target > 7.5f * target + 3.6f * all
+                      : longest > 12.f || 2.f * longest * target > all;
 }
 
 // The batch as a line of units, cut into items.  Where tiles are cut, the units
@@ -117,11 +118,12 @@ __host__ __device__ constexpr bool cut_pays(int rows, float longest, float all, 
 // Cut or not: with M units the longest tile and U all of them, in us of a head
 // group of 128 dims on 256 CUs:
 //   R = 64: whole tiles take 4 + 1.07 M while they are few, `target` items of
-//   the cut ones (two resident a CU) 18 + 1.95 U / target.  A prompt of 256 at
-//   4,096 cached rows 82 whole, 54 cut; of 1,024 150 and 168; 16 drafted trees
-//   of up to 33 tokens at up to 8,000 rows 151 and 80, 20 of up to 60 at up to
-//   1,000 33 and 38.  Half the items where they would have less than 8 units:
-//   a prompt of 64 at 4,096 28.5 and 25.2.
+//   the cut ones (two resident a CU) 18 + 1.95 U / target, half as many 12 + 3.8
+//   U / target.  A prompt of 256 at 4,096 cached rows 82 whole, 54 cut; of 1,024
+//   150 and 168; of 8 at 500 15.7 and 12.8; 16 drafted trees of up to 33 tokens
+//   at up to 8,000 rows 151 and 80, 20 of up to 60 at up to 1,000 33 and 38.
+//   Half the items where they would have less than 8 units: a prompt of 64 at
+//   4,096 28.5 and 25.2.
 //   R = 16: cut unless all tiles are short and there are many: 200 single tokens
 //   at up to 300 rows 29 whole, 43 cut, at up to 1,000 83 and 89, at up to 6,000
 //   437 and 406; 64 at up to 2,000 61 and 53.
