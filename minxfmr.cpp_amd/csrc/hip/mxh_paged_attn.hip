@@ -242,6 +242,25 @@ struct Plan {
     }
 };
 
+// N loads of g2l_s, to lds, lds + 1024, ...: an instruction's offset counts for both
+// of its addresses, so off[i] is 1024 i less than where lane i's bytes are.  (One M0
+// for all: as LDS addresses of their own they filled the scalar registers and were
+// read back from spilled lanes at every load.)
+template <int N>
+__device__ __forceinline__ void g2l_rows(uint64_t base, const uint32_t (&off)[N], uint32_t lds) {
+    static_assert(N == 1 || N == 2 || N == 4, "");
+    if constexpr (N == 4)
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:%6\n\t"
+                     "global_load_lds_dwordx4 %2, %4 offset:%7\n\tglobal_load_lds_dwordx4 %3, %4 offset:%8" ::"v"(off[0]),
+                     "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "{m0}"(lds), "n"(1024), "n"(2 * 1024), "n"(3 * 1024)
+                     : "memory");
+    else if constexpr (N == 2)
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" ::"v"(off[0]),
+                     "v"(off[1]), "s"(base), "{m0}"(lds), "n"(1024)
+                     : "memory");
+    else g2l_s(base, off[0], lds);
+}
+
 struct AttnPagedArgs {
     PagedArgs pg;
     const float* q;
@@ -555,8 +574,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
 #pragma unroll
         for (int x = 0; x < LPG; ++x) {
             const uint32_t r = x * RPI + lr;
-            koff[x] = r * row_b + 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>((int)r));
-            voff[x] = r * row_b + 16 * (uint32_t)(lane % NCH ^ v_swz<HD>((int)r));
+            const uint32_t at = r * row_b - 1024 * x;  // (not below zero: x * RPI rows have 1024 x bytes of one head)
+            koff[x] = at + 16 * (uint32_t)(lane % NCH ^ pa_swz<HD>((int)r));
+            voff[x] = at + 16 * (uint32_t)(lane % NCH ^ v_swz<HD>((int)r));
         }
         // the wave's rows of a stage into K's or V's place
         const auto issue = [&](const Place& p, uint32_t place, bool is_v) __attribute__((always_inline)) {
@@ -567,8 +587,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
                 const uint64_t at16 = ((uint64_t)(uint32_t)p.hi[u] << 32) | (uint32_t)p.lo[u];
                 const uint64_t from = (is_v ? vbase : kbase) + at16;
                 if (p.hi[u] >= 0 && p.r0 + 16 * u + 15 < kend) {
-#pragma unroll
-                    for (int x = 0; x < LPG; ++x) g2l_s(from, off[x], to + 1024 * x);
+                    g2l_rows(from, off, to);
                 } else {
                     // rows past the last repeat it (their scores are replaced); an absent
                     // group reads the row of zeros
@@ -578,7 +597,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
 #pragma unroll
                     for (int x = 0; x < LPG; ++x) {
                         const uint32_t r = x * RPI + lr;
-                        g2l_s(at, off[x] - (r - min(r, last)) * row_b, to + 1024 * x);
+                        g2l_s(at, off[x] + 1024 * x - (r - min(r, last)) * row_b, to + 1024 * x);
                     }
                 }
             }
