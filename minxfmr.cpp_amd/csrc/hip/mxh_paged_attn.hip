@@ -134,6 +134,7 @@ struct Plan {
     float inv_t;
     bool cut;
     uint32_t total, per;    // units of the batch (the launch sees to it that they fit), of an item
+    uint32_t all;           // stages and leads of the batch (0: not counted, target == 0)
 
     // sequence s.  Rows past the table do not exist, so no tile has stages there
     __device__ __forceinline__ Seq seq(int s) const {
@@ -208,10 +209,10 @@ struct Plan {
             tiles += mine.tiles;
             if (cut && mine.tiles > 0) sum += units(mine), longest = max(longest, lead + mine.stages);
         }
-        per = 1;
+        per = 1, all = 0;
         if (cut) {
             upto = wave_scan(sum);
-            total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            all = total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
             cut = __any(cut_pays(rows, (float)longest, (float)total, (float)target));
             const uint32_t items = (uint32_t)(rows == 64 && (int64_t)total < 8 * (int64_t)target ? target / 2 : target);
             per = cut ? (total + items - 1) / items : 1;
@@ -246,20 +247,33 @@ struct Plan {
 // of its addresses, so off[i] is 1024 i less than where lane i's bytes are.  (One M0
 // for all: as LDS addresses of their own they filled the scalar registers and were
 // read back from spilled lanes at every load.)
+#define MXH_G2L_ROWS(HINT)                                                                                             \
+    if constexpr (N == 4)                                                                                              \
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %4" HINT                                                  \
+                     "\n\tglobal_load_lds_dwordx4 %1, %4 offset:%6" HINT                                               \
+                     "\n\tglobal_load_lds_dwordx4 %2, %4 offset:%7" HINT                                               \
+                     "\n\tglobal_load_lds_dwordx4 %3, %4 offset:%8" HINT ::"v"(off[0]),                                \
+                     "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "{m0}"(lds), "n"(1024), "n"(2 * 1024),          \
+                     "n"(3 * 1024)                                                                                     \
+                     : "memory");                                                                                      \
+    else if constexpr (N == 2)                                                                                         \
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %2" HINT                                                  \
+                     "\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" HINT ::"v"(off[0]),                                \
+                     "v"(off[1]), "s"(base), "{m0}"(lds), "n"(1024)                                                    \
+                     : "memory");                                                                                      \
+    else                                                                                                               \
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" HINT ::"v"(off[0]), "s"(base), "{m0}"(lds) : "memory")
 template <int N>
 __device__ __forceinline__ void g2l_rows(uint64_t base, const uint32_t (&off)[N], uint32_t lds) {
     static_assert(N == 1 || N == 2 || N == 4, "");
-    if constexpr (N == 4)
-        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:%6\n\t"
-                     "global_load_lds_dwordx4 %2, %4 offset:%7\n\tglobal_load_lds_dwordx4 %3, %4 offset:%8" ::"v"(off[0]),
-                     "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "{m0}"(lds), "n"(1024), "n"(2 * 1024), "n"(3 * 1024)
-                     : "memory");
-    else if constexpr (N == 2)
-        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" ::"v"(off[0]),
-                     "v"(off[1]), "s"(base), "{m0}"(lds), "n"(1024)
-                     : "memory");
-    else g2l_s(base, off[0], lds);
+    MXH_G2L_ROWS("");
 }
+// of rows that nothing else will read: their lines are the next to leave the caches
+template <int N>
+__device__ __forceinline__ void g2l_rows_once(uint64_t base, const uint32_t (&off)[N], uint32_t lds) {
+    MXH_G2L_ROWS(" nt");
+}
+#undef MXH_G2L_ROWS
 
 struct AttnPagedArgs {
     PagedArgs pg;
@@ -433,7 +447,7 @@ __device__ __forceinline__ float row_sum(float v) {
 // V(st + 1), K(st + 2).
 //
 // Measured with 32/8 heads of 128:
-//   R = 16: 48 single tokens at up to 16,000 rows 254 us = 5.7 TB/s of K and V (a
+//   R = 16: 48 single tokens at up to 16,000 rows 229 us = 6.3 TB/s of K and V (a
 //   large read 6.7), bound by those; one at 8,192 15 us.  One token of 16/8 heads
 //   at 700 9.5 us: two launches, and in the first the plan's, the pages' and the
 //   rows' loads one after the other.
@@ -541,6 +555,21 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         win = window(0);
         if (nst > WIN) win_next = window(1);
         uint64_t gone_win = __ballot(win.y < 0);
+        // Whether the rows are read once: the batch's are more than the 256 MB that the
+        // last cache holds, so none stay for the next call, the sequence has no other
+        // tile, and none of the 63 sequences around it has the first row's page in the
+        // same place, as forks would.  Then the loads say so, and the caches do not fill
+        // with them: 48 single tokens at up to 16,000 rows 255 us without, 228 with;
+        // 64 at up to 9,000 rows, 8,000 of them shared, 158 and 205.
+        bool once = false;
+        if constexpr (PRIVATE) {
+            if (nst > 0 && seq.tiles == 1 && (float)plan.all * (float)(STAGE * 4 * HD) * (float)nkv > 256e6f) {
+                const int page = key0 >> a.pg.page_shift, s = max(min(it.s - 32, a.pg.n_seq - 64), 0) + lane;
+                int other = -2;
+                if (s < a.pg.n_seq && s != it.s) other = a.pg.table[(size_t)s * a.pg.table_ld + page];
+                once = !__any(other == table[page]);
+            }
+        }
         // the wave's groups of a stage, and which of all its groups are absent (a bit each)
         struct Place {
             int lo[OWN], hi[OWN];
@@ -580,24 +609,32 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         }
         // the wave's rows of a stage into K's or V's place
         const auto issue = [&](const Place& p, uint32_t place, bool is_v) __attribute__((always_inline)) {
+            const uint32_t(&off)[LPG] = is_v ? voff : koff;
+            const auto from = [&](int u) {
+                return (is_v ? vbase : kbase) + (((uint64_t)(uint32_t)p.hi[u] << 32) | (uint32_t)p.lo[u]);
+            };
+            const auto to = [&](int u) { return place + 32 * (OWN * wave + u) * HD; };
+            bool all = p.r0 + 16 * OWN - 1 < kend;
 #pragma unroll
-            for (int u = 0; u < OWN; ++u) {
-                const uint32_t to = place + 32 * (OWN * wave + u) * HD;
-                const uint32_t(&off)[LPG] = is_v ? voff : koff;
-                const uint64_t at16 = ((uint64_t)(uint32_t)p.hi[u] << 32) | (uint32_t)p.lo[u];
-                const uint64_t from = (is_v ? vbase : kbase) + at16;
-                if (p.hi[u] >= 0 && p.r0 + 16 * u + 15 < kend) {
-                    g2l_rows(from, off, to);
-                } else {
-                    // rows past the last repeat it (their scores are replaced); an absent
-                    // group reads the row of zeros
+            for (int u = 0; u < OWN; ++u) all &= p.hi[u] >= 0;
+            if (all && PRIVATE && once) {
+#pragma unroll
+                for (int u = 0; u < OWN; ++u) g2l_rows_once(from(u), off, to(u));
+            } else if (all) {
+#pragma unroll
+                for (int u = 0; u < OWN; ++u) g2l_rows(from(u), off, to(u));
+            } else {
+                // rows past the last repeat it (their scores are replaced); an absent
+                // group reads the row of zeros
+#pragma unroll
+                for (int u = 0; u < OWN; ++u) {
                     const bool none = p.hi[u] < 0;
-                    const uint32_t last = none ? 0 : (uint32_t)(kend - 1 - p.r0 - 16 * u);
-                    const uint64_t at = none ? scalar_addr(zero_row) : from;
+                    const uint32_t last = none ? 0 : (uint32_t)max(min(kend - 1 - p.r0 - 16 * u, 15), 0);
+                    const uint64_t at = none ? scalar_addr(zero_row) : from(u);
 #pragma unroll
                     for (int x = 0; x < LPG; ++x) {
                         const uint32_t r = x * RPI + lr;
-                        g2l_s(at, off[x] + 1024 * x - (r - min(r, last)) * row_b, to + 1024 * x);
+                        g2l_s(at, off[x] + 1024 * x - (r - min(r, last)) * row_b, to(u) + 1024 * x);
                     }
                 }
             }

@@ -506,6 +506,53 @@ def test_whole_and_cut_tiles(mxh, name, heads):
     c.close()
 
 
+@pytest.mark.parametrize("shared", [False, True])
+def test_batches_larger_than_the_caches(mxh, shared):
+    """Single tokens over more than 256 MB of rows, apart and of one prompt: each the same as by itself."""
+    nh, nkv, hd, page, n, rows = 16, 4, 128, 64, 40, 4000
+    rng = np.random.default_rng(61)
+    per = rows // page + 1
+    kept = 3500 // page if shared else 0
+    table = np.arange(n * per, dtype=np.int32).reshape(n, per)
+    table[:, :kept] = table[0, :kept]
+    cached = np.asarray([rows - 13 * (i % 9) for i in range(n)], np.int32)
+    pages = rng.standard_normal((97, page * nkv * hd)).astype(np.float16)  # page p holds pages[p % 97], V those 5 on
+    bufs = [mxhip.DeviceBuffer(n * per * pages[0].nbytes) for _ in range(2)]
+    for p in range(n * per):
+        bufs[0].upload(pages[p % 97], p * pages[0].nbytes), bufs[1].upload(pages[(p + 5) % 97], p * pages[0].nbytes)
+    assert 2 * n * rows * nkv * hd * 2 > 256e6
+    pool = mxhip.KvPool(*bufs, n_layer=1, n_pages=n * per, page_rows=page, n_kv=nkv, head_dim=hd)
+    q = rng.standard_normal((n, nh * hd)).astype(np.float32)
+    put = mxhip.DeviceBuffer.from_array
+    dev = [put(np.arange(n + 1, dtype=np.int32)), put(cached), put(table), put(q), put(np.zeros_like(q)), put(np.zeros_like(q)),
+           put(np.asarray([0, 1], np.int32))]
+    batch = mxhip.KvBatch(n, n, dev[0], dev[1], dev[2], per, None)
+    size = mxhip.attention_paged_workspace(pool, batch, nh)
+    work = mxhip.DeviceBuffer(max(size, 1))
+    mxhip.attention_paged(pool, 0, batch, dev[3], nh, dev[4], work, size)
+    for i in range(n):
+        one = mxhip.KvBatch(1, 1, dev[6], dev[1].ptr + 4 * i, dev[2].ptr + 4 * i * per, per, None)
+        mxhip.attention_paged(pool, 0, one, dev[3].ptr + 4 * i * nh * hd, nh, dev[5].ptr + 4 * i * nh * hd, work, size)
+    mxhip.synchronize()
+    got, alone = (b.download(np.float32).reshape(n, nh, hd) for b in dev[4:6])
+    for i in range(0, n, 3):
+        r = np.arange(cached[i] + 1)
+        p = table[i, r // page]
+        k = pages[p % 97].reshape(-1, page, nkv, hd)[r, r % page].astype(np.float64)
+        v = pages[(p + 5) % 97].reshape(-1, page, nkv, hd)[r, r % page].astype(np.float64)
+        for h in range(nh):
+            x, kk, vv = q[i, h * hd:(h + 1) * hd].astype(np.float64), k[:, h // 4], v[:, h // 4]
+            sc = kk @ x / np.sqrt(hd)
+            e = np.exp(sc - sc.max())
+            e /= e.sum()
+            d = (2.0**-21 + 2 * hd * U) * (np.abs(kk) @ np.abs(x)).max() / np.sqrt(hd)
+            bound = (2 * d + 2.0**-20 + 2 * len(r) * U) * (e @ np.abs(vv))
+            for y in (got[i, h], alone[i, h]):
+                assert np.all(np.abs(y - e @ vv) <= bound), (i, h)
+    for b in [*bufs, *dev, work]:
+        b.close()
+
+
 def test_graph_goes_from_cut_to_whole_tiles(mxh):
     """One recorded call while a sequence's cached rows go from many to none and back."""
     c = Case([(2000, 100), (3, 60), (0, 1)], nh=8, nkv=2, hd=64, page=16, seed=41).upload()
