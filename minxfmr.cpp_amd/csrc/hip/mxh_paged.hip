@@ -168,16 +168,24 @@ struct CopyArgs {
     int src[kCopyPairs], dst[kCopyPairs];
 };
 
+typedef uint32_t piece __attribute__((ext_vector_type(4)));  // 16 bytes
+
 // Workgroup (chunk and K or V, pair, layer): 4 KB, a 16-byte piece a thread.  Bound
-// by its bytes: 256 pages of 16 rows of 8 heads of 128 in 36 layers 231 us = 5.2
-// TB/s, a large copy's rate; one in 28 layers 5 us, little over an empty launch.
-// Two, four and eight pieces a thread, all in flight before its first store, took
-// 235, 237 and 314 us, for 16 pages 23.5, 24.7 and 28.7 (one piece 13.6).
+// by its bytes; one page in 28 layers 5 us, little over an empty launch.  Two, four
+// and eight pieces a thread, all in flight before its first store, took 235, 237 and
+// 314 us for 256 pages of 16 rows of 8 heads of 128 in 36 layers (one 230), for 16
+// pages 23.5, 24.7 and 28.7 (13.6).
+// ONCE: copies larger than the 256 MB of the last cache do not fill it: 256 pages 216
+// us = 5.6 TB/s; 16 pages whose rows it may hold 16.0 (13.8).
+template <bool ONCE>
 __global__ __launch_bounds__(kCopyThreads) void kv_copy_pages_kernel(CopyArgs a) {
     const int chunk = blockIdx.x >> 1, i = chunk * kCopyThreads + threadIdx.x;
     if (i >= a.page16) return;
     uint4* base = (blockIdx.x & 1 ? a.v : a.k) + blockIdx.z * a.layer16 + i;
-    base[(int64_t)a.dst[blockIdx.y] * a.page16] = base[(int64_t)a.src[blockIdx.y] * a.page16];
+    const piece* from = reinterpret_cast<const piece*>(base + (int64_t)a.src[blockIdx.y] * a.page16);
+    piece* to = reinterpret_cast<piece*>(base + (int64_t)a.dst[blockIdx.y] * a.page16);
+    if (ONCE) __builtin_nontemporal_store(__builtin_nontemporal_load(from), to);
+    else *to = *from;
 }
 
 // A move is 16 bits for the row it reads and 16 for the one it writes: 6 for
@@ -197,14 +205,15 @@ static_assert(sizeof(KeepArgs) <= 4096 && sizeof(CopyArgs) <= 4096, "");
 // ascending order with dst <= src, so a row is written only after it was read
 // (dst of a move is below the src of every later one), however many loads of
 // later moves come before a store.  Bound by its bytes: 337 moved rows of 64
-// sequences, 2 KB of K and of V in 36 layers, 20.4 us = 4.9 TB/s; four rows of one
-// sequence 5.5 us, little over an empty launch.  (As an array the eight pieces went to scratch memory: 38 us,
-// twice the bytes written.)
+// sequences, 2 KB of K and of V in 36 layers, 18 us = 5.5 TB/s (20.4 with stores that
+// fill the caches, 23.5 with such loads as well); four rows of one sequence 5.5 us,
+// little over an empty launch.  (As an array the eight pieces went to scratch memory:
+// 38 us, twice the bytes written.)
 __global__ __launch_bounds__(256) void kv_keep_rows_kernel(KeepArgs a) {
     const int g = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;  // (the sequences of a layer next to each other)
     if (c >= a.columns) return;
     const int per = 2 * a.row16, layer = c / per, in = c - layer * per;
-    uint4* base = (in < a.row16 ? a.k + in : a.v + in - a.row16) + layer * a.layer16;
+    piece* base = reinterpret_cast<piece*>((in < a.row16 ? a.k + in : a.v + in - a.row16) + layer * a.layer16);
     const int first = (int)(a.group[g] & 0xffff), end = (int)(a.group[g + 1] & 0xffff);
     const int* pages = a.pages + (a.group[g] >> 16);
     const auto at = [&](uint32_t code) {
@@ -213,11 +222,11 @@ __global__ __launch_bounds__(256) void kv_keep_rows_kernel(KeepArgs a) {
     for (int m = first; m < end; m += 8) {
         // (past the end the last again: all loads are in flight at once)
         const auto get = [&](int u) { return base[at(a.moves[min(m + u, end - 1)] & 0xffff)]; };
-        const auto put = [&](int u, const uint4& x) {
-            if (m + u < end) base[at(a.moves[m + u] >> 16)] = x;
+        const auto put = [&](int u, piece x) {
+            if (m + u < end) __builtin_nontemporal_store(x, base + at(a.moves[m + u] >> 16));
         };
-        const uint4 x0 = get(0), x1 = get(1), x2 = get(2), x3 = get(3);
-        const uint4 x4 = get(4), x5 = get(5), x6 = get(6), x7 = get(7);
+        const piece x0 = get(0), x1 = get(1), x2 = get(2), x3 = get(3);
+        const piece x4 = get(4), x5 = get(5), x6 = get(6), x7 = get(7);
         put(0, x0), put(1, x1), put(2, x2), put(3, x3), put(4, x4), put(5, x5), put(6, x6), put(7, x7);
     }
 }
@@ -423,12 +432,14 @@ int mxh_kv_copy_pages(const mxh_kv_pool* pool, const int* src, const int* dst, i
     a.layer16 = layer_elems(pool) / 8;
     a.page16 = pool->page_rows * pool->n_kv * pool->head_dim / 8;
     a.chunks = (a.page16 + kCopyThreads - 1) / kCopyThreads;
+    const bool once = 4.0 * 16 * a.page16 * n * pool->n_layer > 256e6;  // read and written, K and V
     for (int i = 0; i < n; i += kCopyPairs) {
         const int m = std::min(kCopyPairs, n - i);
         std::copy(src + i, src + i + m, a.src);
         std::copy(dst + i, dst + i + m, a.dst);
-        hipLaunchKernelGGL(kv_copy_pages_kernel, dim3(2u * (unsigned)a.chunks, (unsigned)m, (unsigned)pool->n_layer),
-                           dim3(kCopyThreads), 0, lib_stream(), a);
+        const dim3 grid(2u * (unsigned)a.chunks, (unsigned)m, (unsigned)pool->n_layer);
+        if (once) hipLaunchKernelGGL(kv_copy_pages_kernel<true>, grid, dim3(kCopyThreads), 0, lib_stream(), a);
+        else hipLaunchKernelGGL(kv_copy_pages_kernel<false>, grid, dim3(kCopyThreads), 0, lib_stream(), a);
     }
     return check_hip(hipGetLastError(), "kv_copy_pages launch");
 } catch (const std::bad_alloc&) {

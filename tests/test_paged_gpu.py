@@ -722,6 +722,10 @@ def test_copied_pages(mxh, layers, n_pages, page, nkv, hd, pairs, stride):
         b.close()
 
 
+def test_copies_larger_than_the_caches(mxh):
+    test_copied_pages(mxh, 3, 91, 256, 8, 128, 45, 8)  # 283 MB read and written
+
+
 @pytest.mark.parametrize("layers,page,nkv,hd,stride,kept", [
     (1, 16, 1, 32, 0, {0: (5, [1])}),
     (3, 16, 2, 64, 16, {0: (14, [0, 3, 4, 9]), 1: (40, []), 2: (0, [2, 3, 4]), 3: (7, [0, 1, 2])}),
