@@ -449,13 +449,13 @@ __device__ __forceinline__ float row_sum(float v) {
 // Measured with 32/8 heads of 128:
 //   R = 16: 48 single tokens at up to 16,000 rows 229 us = 6.3 TB/s of K and V (a
 //   large read 6.7), bound by those; one at 8,192 15 us.  One token of 16/8 heads
-//   at 700 9.5 us: two launches, and in the first the plan's, the pages' and the
+//   at 700 9.8 us: two launches, and in the first the plan's, the pages' and the
 //   rows' loads one after the other.
 //   R = 64: six packed prompts of 29 to 2,100 tokens behind up to 1,500 rows 264
 //   us (276 on another card) = 468 TFLOP/s of the formula's, 940 of the products
 //   made (a large fp16 product 1,184); matrix cores and vector units half busy each, and neither
 //   fewer reads nor fewer exponentials made it faster by more than 4%.  27 drafted
-//   tokens at 8,192 rows 24.3 us: 8 stages an item 12 of them (a stage's loads are
+//   tokens at 8,192 rows 23.7 us: 8 stages an item 12 of them (a stage's loads are
 //   one stage ahead and HBM is 1.4 us away), what comes before and after an item's
 //   stages 7, the second kernel 4.
 template <int HD, int R>
