@@ -506,6 +506,25 @@ def test_whole_and_cut_tiles(mxh, name, heads):
     c.close()
 
 
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32"])
+def test_trees_of_many_sequences(mxh, heads):
+    """More trees than a wave has lanes, empty ones among them, one behind a long cache; then the most sequences."""
+    nh, nkv, hd = HEADS[heads]
+    seqs = [(3 * i % 200, i % 20) for i in range(100)] + [(1500, 30)] + [(7, 64), (0, 1)]
+    c = Case(seqs, nh=nh, nkv=nkv, hd=hd, page=16, tree=True, lead=2, tail=1, seed=71, extra_ld=3).upload()
+    c.check(c.attention())
+    c.close()
+
+
+def test_4096_sequences(mxh):
+    c = Case([(i % 37 if i % 500 else 900, 1 - i % 7 // 6) for i in range(4096)], nh=4, nkv=1, hd=32, page=16, lead=1, seed=72,
+             extra_ld=1).upload()
+    c.check(c.attention())
+    qkv, _, _ = rope_inputs(c, 5)
+    run_rope(c, qkv, None, [None, None], mxhip.rope_frequencies(1e4, 32), True)
+    c.close()
+
+
 @pytest.mark.parametrize("shared", [False, True])
 def test_batches_larger_than_the_caches(mxh, shared):
     """Single tokens over more than 256 MB of rows, apart and of one prompt: each the same as by itself."""
