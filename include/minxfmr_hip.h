@@ -277,7 +277,8 @@ int mxh_kv_copy_pages(const mxh_kv_pool *pool, const int *src, const int *dst, i
  * every sequence together, K and V, in every layer.  Sequence s keeps the new
  * tokens keep[keep_start[s]] < ... < keep[keep_start[s+1] - 1] (indices within
  * its new tokens); their cache rows move to rows cached[s], cached[s] + 1, ...
- * Host arrays (table [n_seq][table_ld] as in mxh_kv_batch); kept indices
+ * Host arrays (table [n_seq][table_ld] as in mxh_kv_batch); keep_start from 0
+ * or above and never falling (else keep is not read), kept indices
  * ascending from 0 on, their rows in pages of the pool, and no page with a
  * sequence's kept rows, before or after, in a second place of the table (what
  * mxh_pages_extend made a sequence's own is that), or MXH_ERR_ARG. */

@@ -303,15 +303,20 @@ bool mark_pages(const int* ids, int n, std::vector<uint64_t>& seen) {
     return true;
 }
 
-// every fault of mxh_kv_keep_rows' arguments
+// every fault of mxh_kv_keep_rows' lists; keep is read only where all of
+// keep_start makes sense
 int check_keep(const mxh_kv_pool* p, const int* table, int table_ld, const int* cached, const int* keep_start,
                const int* keep, int n_seq) {
     const char* who = "kv_keep_rows";
     const int pr = p->page_rows;
+    if (keep_start[0] < 0) return set_error(MXH_ERR_ARG, "%s: keep_start begins at %d", who, keep_start[0]);
+    for (int s = 0; s < n_seq; ++s)
+        if (keep_start[s + 1] < keep_start[s])
+            return set_error(MXH_ERR_ARG, "%s: keep_start decreases at sequence %d", who, s);
+    if (!keep && keep_start[n_seq] > keep_start[0]) return set_error(MXH_ERR_ARG, "%s: null array", who);
     std::vector<int> pages;  // every page that holds a kept row, of all sequences
     for (int s = 0; s < n_seq; ++s) {
         const int n = keep_start[s + 1] - keep_start[s];
-        if (n < 0) return set_error(MXH_ERR_ARG, "%s: keep_start decreases at sequence %d", who, s);
         if (n == 0) continue;
         const int* kept = keep + keep_start[s];
         if (kept[0] < 0) return set_error(MXH_ERR_ARG, "%s: sequence %d keeps token %d", who, s, kept[0]);
@@ -452,7 +457,7 @@ int mxh_kv_keep_rows(const mxh_kv_pool* pool, const int* table, int table_ld, co
     if (int rc = check_pool(who, pool)) return rc;
     if (n_seq < 0 || n_seq > kPagedSeqMax) return set_error(MXH_ERR_ARG, "%s: %d sequences", who, n_seq);
     if (n_seq == 0) return MXH_OK;
-    if (!table || table_ld < 1 || !cached || !keep_start || (!keep && keep_start[n_seq] > keep_start[0]))
+    if (!table || table_ld < 1 || !cached || !keep_start)
         return set_error(MXH_ERR_ARG, "%s: null array", who);
     if (int rc = check_keep(pool, table, table_ld, cached, keep_start, keep, n_seq)) return rc;
     KeepArgs a{};

@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes as C
 import random
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -300,3 +302,33 @@ def test_sizes_past_the_limits_are_refused():
     with pytest.raises(mxhip.MxhError, match="unsupported pool"):
         mxhip.kv_copy_pages(wide, [], [])
     mxhip.kv_copy_pages(fits, [], [])
+
+
+# (starts, kept or None) that begin below zero, fall, or rise past a list that is not there
+BAD_STARTS = [([-1, 0], [2]), ([-1, 1], [2]), ([-(1 << 30), 0], [2]), ([-(2**31), 2**31 - 1], [2]),
+              ([1 << 30, (1 << 30) + 1, 0], [2]), ([0, 5, 0], None), ([0, 1, 0], None), ([0, 1], None),
+              ([0, 2**31 - 1, -(2**31)], [2]), ([3, 3, 2], [2])]
+
+
+@pytest.mark.parametrize("case", range(len(BAD_STARTS)))
+def test_kept_lists_are_read_only_where_their_starts_make_sense(case):
+    """In a process of its own: the call is refused, and reads nothing outside its lists on the way."""
+    starts, kept = BAD_STARTS[case]
+    code = f"""
+import ctypes as C, sys
+sys.path[:0] = {sys.path!r}
+import mxhip
+from test_pages import pool
+n = {len(starts) - 1}
+ints = lambda a: None if a is None else (C.c_int * len(a))(*a)
+rc = mxhip.lib.mxh_kv_keep_rows(C.byref(pool()), ints([0, 1] * n), 2, ints([3] * n), ints({starts!r}), ints({kept!r}), n)
+sys.exit(0 if rc == {ERR_ARG} else 3)
+"""
+    assert subprocess.run([sys.executable, "-c", code], timeout=300).returncode == 0
+
+
+def test_starts_of_kept_lists_need_not_begin_at_zero():
+    """A slice of a longer list: the entries before the first start are not looked at."""
+    mxhip.kv_keep_rows(pool(), [[0, 1]], [3], [2, 4], [-9, 99, 0, 1])
+    assert mxhip.lib.mxh_kv_keep_rows(C.byref(pool()), (C.c_int * 2)(0, 1), 2, (C.c_int * 1)(3), (C.c_int * 2)(0, 0),
+                                      None, 1) == 0
