@@ -215,13 +215,13 @@ typedef struct {
  * after (smaller than its own; -1: the last cached token), at most 64 new
  * tokens a sequence; parent NULL: every token follows the one before it, any
  * number of them.  The arrays are device memory that no call checks on the
- * host, but no value in them makes a kernel leave the pool or the token
- * arrays: rows of a page id outside 0 .. n_pages-1 or past table_ld are absent
- * (never attended, never written), a parent that is not smaller than its token
- * counts as -1, tokens past the 64th of a drafted tree and token rows outside
- * start[0] .. start[n_seq]-1 or past n_tokens are left alone, lengths below
- * zero count as zero, a sequence that starts below 0 has no tokens.  start must
- * not decrease (where it does, nothing is attended and att is left alone). */
+ * host, but no value in them makes a kernel leave the pool, the token arrays or
+ * a workspace: rows of a page id outside 0 .. n_pages-1 or past table_ld are
+ * absent (never attended, never written), a parent that is not smaller than its
+ * token counts as -1, tokens past the 64th of a drafted tree and token rows
+ * outside start[0] .. start[n_seq]-1 or past n_tokens are left alone, lengths
+ * below zero count as zero, a sequence that starts below 0 has no tokens.  start
+ * must not decrease (where it does, nothing is attended and att is left alone). */
 typedef struct {
     int n_seq, n_tokens;
     const int *start;  /* [n_seq + 1] */

@@ -7,11 +7,9 @@
 #include <stdint.h>
 
 #include "mxh_device.h"
+#include "mxh_paged_plan.h"
 
 namespace mxh {
-
-constexpr int kTreeMax = 64;       // new tokens of a drafted tree (one lane, one mask bit each)
-constexpr int kPagedSeqMax = 4096;  // sequences of a batch
 
 // One layer of the pool and the batch; device pointers.  Nothing that the
 // arrays hold is trusted: ids, lengths and parents are bounded where they are read.

@@ -14,8 +14,9 @@
 // into items of equal length, whatever tiles they cross: the workgroups, all
 // resident, end together.  A tile that is cut leaves its parts in the workspace,
 // two at most an item, and a second kernel joins them.  The lengths are on the
-// device, so every workgroup makes the plan for itself (Plan); the grid is as
-// wide as the plan can be, and what is past its end leaves at once.
+// device, so every workgroup makes the plan for itself (Plan; its integers are in
+// mxh_paged_plan.h); the grid is as wide as the plan can be, and what is past its
+// end leaves at once.
 //
 // K and V rows go straight into LDS (16 rows of a page are evenly spaced, so
 // their addresses are a scalar base and fixed lane offsets).  Per 32-key block
@@ -56,11 +57,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 constexpr int kThreads = 256, kWaves = 4;
-// keys of a stage: 32 for every group of waves that share them
-__host__ __device__ constexpr int stage_keys(int rows) { return rows == 16 ? 128 : 64; }
-// a tile's cost beside its stages, in stages (64 rows: 3 to 6 are within 5% of one
-// another; without it items that cross tiles end late)
-__host__ __device__ constexpr int tile_lead(int rows) { return rows == 16 ? 2 : 4; }
 
 // floats a wave leaves for the merge: V sums [m][hd + 4], references, sums (and a flag, behind all of theirs)
 __host__ __device__ constexpr int merge_floats(int hd, int m) { return m * (hd + 6); }
@@ -72,12 +68,6 @@ __host__ __device__ constexpr int lds_bytes(int hd, int rows) {
 
 // what absent rows read
 __device__ __align__(256) uint32_t zero_row[64];
-
-// A sequence as the plan sees it
-struct Seq {
-    uint32_t first, n, cached;  // first token row, new tokens, rows before them
-    uint32_t tiles, stages;     // stages of its last tile
-};
 
 // A tile, or some of its stages
 struct Segment {
@@ -98,110 +88,26 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive
     return (uint32_t)v;
 }
 
-// whether `target` items of a batch of `all` units finish before its whole tiles
-// do, the longest of `longest` units (Plan)
-__host__ __device__ constexpr bool cut_pays(int rows, float longest, float all, float target) {
-    return rows == 64 ? longest * target > 13.f * target + 1.8f * all || longest * target > 7.5f * target + 3.6f * all
-                      : longest > 12.f || 2.f * longest * target > all;
-}
-
-// The batch as a line of units, cut into items.  Where tiles are cut, the units
-// are the stages of all tiles, sequence by sequence, `lead` units before each
-// tile's; elsewhere the tiles themselves.  The lead is what a tile costs beside
-// its stages (its q, the merge of the waves), so an item that goes on into
-// another tile does as many stages less.
-//
-// A prompt's earlier tiles have fewer stages.  `block` tiles have at most the
-// tokens of one stage, so those of block b need no more stages than the cached
-// rows and b + 1; the line gives them that many, and all of the sequence's to
-// the tiles from the block on where this reaches them (ramp).
-//
-// Cut or not: with M units the longest tile and U all of them, in us of a head
-// group of 128 dims on 256 CUs:
-//   R = 64: whole tiles take 4 + 1.07 M while they are few, `target` items of
-//   the cut ones (two resident a CU) 18 + 1.95 U / target, half as many 12 + 3.8
-//   U / target.  A prompt of 256 at 4,096 cached rows 82 whole, 54 cut; of 1,024
-//   150 and 168; of 8 at 500 15.7 and 12.8; 16 drafted trees of up to 33 tokens
-//   at up to 8,000 rows 151 and 80, 20 of up to 60 at up to 1,000 33 and 38.
-//   Half the items where they would have less than 8 units: a prompt of 64 at
-//   4,096 28.5 and 25.2.
-//   R = 16: cut unless all tiles are short and there are many: 200 single tokens
-//   at up to 300 rows 29 whole, 43 cut, at up to 1,000 83 and 89, at up to 6,000
-//   437 and 406; 64 at up to 2,000 61 and 53.
-// All uniform but what a lane says of its sequences.
-struct Plan {
+// The line of the batch's units (mxh_paged_plan.h), made by a wave from the
+// lengths.  All uniform but what a lane says of its sequences.
+struct Plan : PagedLine {
     const PagedArgs& a;
-    uint32_t t, key_shift, lead, block;  // tokens of a tile; a stage has 1 << key_shift keys
-    float inv_t;
-    bool cut;
-    uint32_t total, per;    // units of the batch (the launch sees to it that they fit), of an item
-    uint32_t all;           // stages and leads of the batch (0: not counted, target == 0)
 
-    // sequence s.  Rows past the table do not exist, so no tile has stages there
-    __device__ __forceinline__ Seq seq(int s) const {
-        Seq q;
-        const int first = a.start[s], end = min(a.start[s + 1], a.n_tokens);
-        q.first = (uint32_t)first;
-        q.n = first >= 0 && end > first ? (uint32_t)(end - first) : 0;
-        if (a.parent) q.n = min(q.n, (uint32_t)kTreeMax);
-        q.cached = (uint32_t)min(max(a.cached[s], 0), 1 << 30);
-        // (n up to 2^20: the quotient is off by less than 2^-3 / t, and n + t - 1/2 is
-        // at least half a token from a multiple of t)
-        q.tiles = (uint32_t)(((float)(q.n + t) - 0.5f) * inv_t);
-        const uint32_t rows = (uint32_t)min((uint64_t)(q.cached + q.n), (uint64_t)a.table_ld << a.page_shift);
-        q.stages = (rows + (1u << key_shift) - 1) >> key_shift;
-        return q;
-    }
-    __device__ __forceinline__ uint32_t cached_stages(const Seq& q) const {
-        return (q.cached + (1u << key_shift) - 1) >> key_shift;
-    }
-    // blocks of tiles with fewer stages than the sequence
-    __device__ __forceinline__ uint32_t ramp(const Seq& q) const {
-        const int r = (int)q.stages - (int)cached_stages(q) - 1;  // (below the blocks that q.n fills)
-        return a.parent ? 0 : (uint32_t)max(r, 0);
-    }
-    // units of the first b <= ramp blocks
-    __device__ __forceinline__ uint32_t before(const Seq& q, uint32_t b) const {
-        return block * (b * (lead + cached_stages(q) + 1) + b * (b - 1) / 2);
-    }
-    __device__ __forceinline__ uint32_t units(const Seq& q) const {
-        if (!cut) return q.tiles;
-        const uint32_t r = ramp(q);  // (block b < r has r - b stages less)
-        return q.tiles * (lead + q.stages) - (r > 0 ? block * (r * (r + 1) / 2) : 0);
-    }
-    // unit x of a sequence: its tile, the units of the tile and those before x
-    struct Spot {
-        uint32_t tile, units, at;
-    };
-    __device__ __forceinline__ Spot spot(const Seq& q, uint32_t x) const {
-        if (!cut) return Spot{x, 1, 0};
-        const uint32_t r = ramp(q);
-        uint32_t b = r, len = lead + q.stages, done = r > 0 ? before(q, r) : 0;
-        if (x < done) {
-            // the root of before(b) = x, put right by whole blocks
-            const float c = (float)(lead + cached_stages(q)) + 0.5f;
-            b = min((uint32_t)max(sqrtf(c * c + 2.0f * (float)x / (float)block) - c, 0.f), r - 1);
-            while (b > 0 && before(q, b) > x) --b;
-            while (b + 1 < r && before(q, b + 1) <= x) ++b;
-            len = lead + cached_stages(q) + 1 + b, done = before(q, b);
-        }
-        const uint32_t i = (x - done) / len;
-        return Spot{b * block + i, len, x - done - i * len};
+    __device__ __forceinline__ PagedSeq seq(int s) const {
+        return PagedLine::seq(a.start[s], a.start[s + 1], a.cached[s], a.n_tokens, (uint64_t)a.table_ld << a.page_shift);
     }
 
     // Lane l's sequences are [l part, (l + 1) part), units `upto - sum` to `upto`
     int part;
     uint32_t sum, upto;
-    Seq mine;  // (part == 1: the lane's sequence)
+    PagedSeq mine;  // (part == 1: the lane's sequence)
 
     __device__ __forceinline__ Plan(const PagedArgs& args, int rows, uint32_t tokens, int target)
-        : a(args), t(tokens), key_shift(rows == 16 ? 7 : 6), lead(tile_lead(rows)), inv_t(1.0f / (float)t),
-          cut(target > 0) {
-        block = (uint32_t)(((float)stage_keys(rows) + 0.5f) * inv_t);
+        : PagedLine(rows, tokens, args.parent != nullptr, target), a(args) {
         const int lane = threadIdx.x & 63;
         part = (a.n_seq + 63) / 64;
         sum = 0;
-        mine = Seq{0, 0, 0, 0, 0};
+        mine = PagedSeq{0, 0, 0, 0, 0};
         uint32_t tiles = 0, longest = 0;
         bool falls = false;
         for (int s = lane * part; s < min((lane + 1) * part, a.n_seq); ++s) {
@@ -210,28 +116,26 @@ struct Plan {
             tiles += mine.tiles;
             if (cut && mine.tiles > 0) sum += units(mine), longest = max(longest, lead + mine.stages);
         }
-        per = 1, all = 0;
         if (cut) {
             upto = wave_scan(sum);
-            all = total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-            cut = __any(cut_pays(rows, (float)longest, (float)total, (float)target));
-            const uint32_t items = (uint32_t)(rows == 64 && (int64_t)total < 8 * (int64_t)target ? target / 2 : target);
-            per = cut ? (total + items - 1) / items : 1;
+            const uint32_t units = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            settle_cut(units, __any(cut_pays(rows, (float)longest, (float)units, (float)target)), rows, target);
         }
         if (!cut) {
             sum = tiles;
             upto = wave_scan(sum);
-            total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            settle_whole((uint32_t)__builtin_amdgcn_readlane((int)upto, 63));
         }
         if (__any(falls)) total = 0;  // (sequences that overlap: their units need not fit 32 bits)
     }
     // the sequence of unit x (< total), and x from its first unit on
-    __device__ __forceinline__ int find(uint32_t& x, Seq& q) const {
+    __device__ __forceinline__ int find(uint32_t& x, PagedSeq& q) const {
         const int l = __ffsll((unsigned long long)__ballot(upto > x)) - 1;
         const auto lane_l = [l](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
         x -= lane_l(upto - sum);
         if (part == 1) {
-            q = Seq{lane_l(mine.first), lane_l(mine.n), lane_l(mine.cached), lane_l(mine.tiles), lane_l(mine.stages)};
+            q = PagedSeq{lane_l(mine.first), lane_l(mine.n), lane_l(mine.cached), lane_l(mine.tiles),
+                         lane_l(mine.stages)};
             return l;
         }
         int s = l * part;
@@ -480,14 +384,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     const uint32_t index = item_index(), g = blockIdx.x;
     const Plan plan(a.pg, R, T, a.target);
     static_assert(STAGE == stage_keys(R), "");
-    uint32_t x = index * plan.per;  // (units of the plan that fit 32 bits: target items at most)
+    uint32_t x = plan.first_unit(index);
     const bool tells = g == 0 && threadIdx.x == 0 && index < (uint32_t)a.target;  // (for the second kernel)
     if (x >= plan.total) {
         if (tells) a.cuts[index] = make_int4(0, 0, 0, 0);
         return;
     }
     const uint32_t x0 = x, x1 = min(x + plan.per, plan.total);
-    Seq seq;
+    PagedSeq seq;
     uint32_t r_unit = x;
     Segment it;
     it.s = plan.find(r_unit, seq);
@@ -497,20 +401,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         const int lane = tid & 63, n = lane % M, h = lane / M;
         {
             const Plan::Spot spot = plan.spot(seq, r_unit);
-            const uint32_t len = min(spot.units - spot.at, x1 - x), end = spot.at + len;
+            const PagedPiece p = plan.piece(seq, spot, x1 - x, index);
             it.first = seq.first, it.n = seq.n, it.cached = seq.cached;
-            it.tile = plan.cut ? spot.tile : seq.tiles - 1 - spot.tile;  // (the most keys first)
-            it.st0 = plan.cut ? max(spot.at, plan.lead) - plan.lead : 0;
-            it.st1 = plan.cut ? max(end, plan.lead) - plan.lead : seq.stages;
-            it.slot = !plan.cut || (it.st0 == 0 && end == spot.units) ? -1 : (int)(2 * index + (it.st0 == 0));
+            it.tile = p.tile, it.st0 = p.st0, it.st1 = p.st1, it.slot = p.slot;
             if (tells && x == x0) {
-                // (no stage before the lead's end; not the tile's first cut a whole item after it)
-                const bool first = plan.cut && spot.at > plan.lead && spot.at <= plan.lead + plan.per;
                 const int i0 = (int)(spot.tile * T), rows = min((int)T, (int)seq.n - i0) * (int)group;
-                const int parts = 1 + (int)((spot.units - spot.at + plan.per - 1) / plan.per);
-                a.cuts[index] = make_int4((int)seq.first + i0, rows, first ? parts : 0, 0);
+                a.cuts[index] = make_int4((int)seq.first + i0, rows, (int)plan.parts(spot), 0);
             }
-            x += len, r_unit += len;
+            x += p.len, r_unit += p.len;
         }
         if (it.st0 < it.st1 || it.slot < 0) {  // (else only units of the lead)
         const int i0 = (int)(it.tile * T), ntok = min((int)T, (int)it.n - i0), cached = (int)it.cached;
@@ -1034,7 +932,7 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
     const int4 cut = a.cuts[item];
     const int rows = min(cut.y - (int)rb * kMergeRows, kMergeRows), parts = cut.z;  // of items item - 1, item, ...
     if (parts == 0 || rows <= 0) return;
-    const auto slot = [&](int z) { return z ? 2 * (item - 1 + (uint32_t)z) : 2 * (item - 1) + 1; };
+    const auto slot = [&](int z) { return PagedLine::part_slot(item, (uint32_t)z); };
     const int tid = threadIdx.x, per = rows * (HD / 4), lanes = kMergeThreads / per;
     const int z0 = tid / per, u = tid - z0 * per, d = 4 * (u % (HD / 4)), row = (int)rb * kMergeRows + u / (HD / 4);
     float M = -INFINITY, L = 0.f;
@@ -1074,46 +972,12 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
         make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
 
-// What the host chooses without the lengths: rows of a tile, by the average
-// sequence, and how many items there can be; whether tiles are cut the plan
-// decides.  16-row tiles re-read the keys where a sequence has several of them,
-// 64-row ones leave rows empty: 16 sequences of 2 tokens (8 rows) at up to 4,000
-// keys took 25 us with 16 and 31 with 64, of up to 12 tokens 36 and 32; one of 4
-// tokens at 8,192 16 and 20, of 27 28 and 24, at 40,000 173 and 69.
-struct Shape {
-    int rows, target;
-    int64_t items;  // at most
-};
-// items of R-row tiles; stages of a tile, at most
-int most_items(int rows, int nkv) { return (rows == 64 ? 2 : 1) * std::max(2, device_cus() / nkv); }
-int64_t most_stages(const PagedArgs& a, int rows) {
-    const int64_t keys = stage_keys(rows);
-    return (((int64_t)a.table_ld << a.page_shift) + keys - 1) / keys;
-}
-// whether some lengths could make cut tiles worth the second kernel's 4 us: the
-// longest tile that the table allows, and `tiles` of one stage
-bool cut_may_pay(const PagedArgs& a, int rows, int64_t tiles) {
-    const int64_t stages = most_stages(a, rows);
-    return stages > 1 && cut_pays(rows, (float)(stages + tile_lead(rows)), (float)(1 + tile_lead(rows)) * (float)tiles,
-                                  (float)most_items(rows, a.nkv));
-}
-size_t work_bytes(int rows, int target, int nkv, int hd) {
-    return (size_t)2 * target * nkv * rows * (hd + 2) * sizeof(float) + target * sizeof(int4);
-}
-Shape attention_shape(const PagedArgs& a, int nh) {
-    Shape s;
-    const int group = nh / a.nkv;
-    s.rows = (int64_t)((a.n_tokens + a.n_seq - 1) / a.n_seq) * group > 16 ? 64 : 16;
-    const int64_t tiles = a.n_tokens / (s.rows / group) + a.n_seq;
-    const int64_t tiles_min = std::max(a.n_tokens / (s.rows / group), std::min(a.n_seq, a.n_tokens));  // (none empty)
-    const bool fits = tiles * (most_stages(a, s.rows) + tile_lead(s.rows)) < INT_MAX;  // (the plan's units)
-    s.target = fits && cut_may_pay(a, s.rows, tiles_min) ? most_items(s.rows, a.nkv) : 0;
-    s.items = std::max((int64_t)s.target, tiles);
-    return s;
+PagedSize paged_size(const PagedArgs& a, int nh) {
+    return PagedSize{a.n_seq, a.n_tokens, (int64_t)a.table_ld << a.page_shift, a.nkv, nh / a.nkv, device_cus()};
 }
 
 template <int HD, int R>
-int launch(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
+int launch(const AttnPagedArgs& a, const PagedShape& sh, hipStream_t st) {
     static bool attr_set = false;  // above 64 KiB of LDS needs the opt-in, once per kernel
     if (!attr_set && lds_bytes(HD, R) > 65536) {
         if (hipFuncSetAttribute((const void*)attention_paged_kernel<HD, R>, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -1131,27 +995,21 @@ int launch(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
 }
 
 template <int HD>
-int launch_hd(const AttnPagedArgs& a, const Shape& sh, hipStream_t st) {
+int launch_hd(const AttnPagedArgs& a, const PagedShape& sh, hipStream_t st) {
     return sh.rows == 64 ? launch<HD, 64>(a, sh, st) : launch<HD, 16>(a, sh, st);
 }
 
 }  // namespace
 
 size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd) {
-    const Shape s = attention_shape(a, nh);
-    return work_bytes(s.rows, s.target, a.nkv, hd);
+    const PagedShape s = paged_shape(paged_size(a, nh));
+    return paged_work_bytes(s.rows, s.target, a.nkv, hd);
 }
 
-size_t attention_paged_work_bound(const PagedArgs& a, int nh, int hd) {
-    size_t most = 0;
-    for (const int rows : {16, 64})
-        if ((rows == 16 || (int64_t)a.n_tokens * (nh / a.nkv) > 16) && cut_may_pay(a, rows, 1))
-            most = std::max(most, work_bytes(rows, most_items(rows, a.nkv), a.nkv, hd));
-    return most;
-}
+size_t attention_paged_work_bound(const PagedArgs& a, int nh, int hd) { return paged_work_bound(paged_size(a, nh), hd); }
 
 int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, float* att, void* work, hipStream_t st) {
-    const Shape s = attention_shape(a, nh);
+    const PagedShape s = paged_shape(paged_size(a, nh));
     float* part = static_cast<float*>(work);
     float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * s.target * a.nkv * s.rows * hd);
     const uint32_t group = (uint32_t)(nh / a.nkv);
