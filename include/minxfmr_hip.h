@@ -260,10 +260,13 @@ int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *b
  * batch of up to this n_seq, n_tokens and table_ld needs at most, whatever its
  * device arrays hold.  Calls that may run at the same time (a replayed graph
  * beside the library stream) need work of their own.  q and the probabilities
- * enter the matrix cores as two fp16 halves (about 22 bits), K and V as they
- * are; rows that meet infinities or NaN, or a |q| from 65504 sqrt(head_dim) /
- * log2(e) on, are computed again in fp32 (slowly, milliseconds for thousands of
- * keys).  q, att and work 16-byte aligned, not overlapping; nh as above. */
+ * enter the matrix cores as two fp16 halves, K and V as they are: q to 2^-22 of
+ * the row's largest |q| (rows outside the halves' range are scaled by a power of
+ * two), a probability to 2^-22 of its own and 2^-31 of the row's largest, so a
+ * key 21 nats below the largest counts in the sum of probabilities alone.  Rows
+ * that meet infinities or NaN are computed again in fp32 (slowly, milliseconds
+ * for thousands of keys).  q, att and work 16-byte aligned, not overlapping; nh
+ * as above. */
 int mxh_attention_paged(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const float *q, int nh,
                         float *att, void *work, size_t work_bytes);
 int mxh_attention_paged_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, int nh, size_t *bytes);

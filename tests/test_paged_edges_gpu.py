@@ -46,3 +46,96 @@ def test_most_sequences_behind_long_tables(mxh):
         assert np.all(np.abs(got[t] - want) <= bound), t
     for b in [*bufs, *dev, work]:
         b.close()
+
+
+HEADS = {"g4-d128": (8, 2, 128), "g3-d64": (6, 2, 64), "g8-d32": (8, 1, 32), "g1-d128": (2, 2, 128)}
+
+
+def check_precision(c, got):
+    """got against float64, with what the pairs of fp16 halves promise (q' = q log2(e) / sqrt(hd), in fp32):
+
+    - q' is off by u of itself and its halves by 2^-22 of the row's largest |q'| (rows outside [2^-3, 2^15) are
+      scaled by a power of two first; inside, the halves end at 2^-25 absolute, which is no more).  A score's
+      products are exact; sums of those that are not zero and of minus the reference round at most once each:
+      |d score| <= D = (2^-22 max|q| sum_d |k_d| + (2 z + 4) u max_j sum_d |q_d k_jd|) / sqrt(hd), z products.
+    - a probability is off by 2 D of its value (its score, the sum's), 2^-20 for the exponential, its scale and its
+      halves, 2 L u for the sums of L keys, and by 2^-31 of the row's largest, where its halves end."""
+    group, worst = c.nh // c.nkv, 0.0
+    q = c.q.astype(np.float64).reshape(c.tokens, c.nh, c.hd)
+    for s, (n_c, n) in enumerate(c.seqs):
+        k, v = (np.array([c.row(x, s, r) for r in range(n_c + n)], np.float64).reshape(-1, c.nkv, c.hd) for x in (c.k, c.v))
+        for i in range(n):
+            t, at = int(c.start[s]) + i, list(range(n_c)) + [n_c + j for j in c.before(s, i)]
+            for h in range(c.nh):
+                kk, vv, x = k[at, h // group], v[at, h // group], q[t, h]
+                sc = kk @ x / np.sqrt(c.hd)
+                p = np.exp(sc - sc.max())
+                p /= p.sum()
+                z = int(((kk != 0) & (x != 0)).sum(1).max())
+                d = (2.0**-22 * np.abs(x).max() * np.abs(kk).sum(1).max() +
+                     (2 * z + 4) * U * (np.abs(kk) @ np.abs(x)).max()) / np.sqrt(c.hd)
+                bound = (2 * d + 2.0**-20 + 2 * len(at) * U) * (p @ np.abs(vv)) + \
+                    2.0**-31 * p.max() * np.abs(vv).sum(0) + 2.0**-100
+                err = np.abs(got[t, h] - p @ vv)
+                assert np.all(err <= bound), (s, i, h, float((err / bound).max()))
+                worst = max(worst, float((err / bound).max()))
+    return worst
+
+
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("new,tree", [(1, False), (3, True), (40, False), (40, True)])
+def test_q_of_every_size(mxh, heads, new, tree):
+    """Scores of up to 6 from one product, of q from 10^-5 up over K down from the largest fp16: two cached keys of
+    opposite sign, zeros in the new ones.  Every fifth token has a second, ordinary element that meets no K."""
+    nh, nkv, hd = HEADS[heads]
+    sizes = [65504.0, 40000.0, 5000.0, 300.0, 20.0, 1.0, 2.0**-5, 2.0**-11, 2.0**-20]
+    c = Case([(2, new) for _ in sizes], nh=nh, nkv=nkv, hd=hd, page=16, tree=tree, seed=new + nh)
+    q = c.q.reshape(c.tokens, nh, hd)
+    keep = c.rng.uniform(0.5, 2, c.tokens)
+    y = c.rng.uniform(-6, 6, (c.tokens, nh))
+    q[:] = 0
+    for s, size in enumerate(sizes):
+        for r in range(2 + new):
+            row = c.row(c.k, s, r).reshape(nkv, hd)
+            row[:] = 0
+            if r < 2:
+                row[:, 5] = size if r == 0 else -0.75 * size
+        q[c.start[s]:c.start[s + 1], :, 5] = y[c.start[s]:c.start[s + 1]] / size * np.sqrt(hd)
+    q[::5, :, 9] = keep[::5, None]
+    c.upload()
+    check_precision(c, c.attention())
+    c.close()
+
+
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32"])
+@pytest.mark.parametrize("small,large", [(1e-2, 100.0), (1e-4, 6e3), (1e-5, 1e4), (1e-7, 1.2e4), (1e-37, 1e4), (1e33, 1e-6)])
+def test_small_q_over_large_k(mxh, heads, small, large):
+    """Dense rows of q and K of far apart sizes, few and many keys, 16- and 64-row tiles; every fourth token ordinary."""
+    nh, nkv, hd = HEADS[heads]
+    for seqs, tree in (([(2, 1), (0, 2), (1, 1), (300, 1)], False), ([(1, 40), (150, 33)], False), ([(0, 30), (700, 20)], True)):
+        c = Case(seqs, nh=nh, nkv=nkv, hd=hd, page=16, tree=tree, seed=19)
+        c.k = np.clip(c.k.astype(np.float32) * large, -65504, 65504).astype(np.float16)
+        c.q *= np.float32(small)
+        if large > 1:
+            c.q[3::4] /= np.float32(small * large)
+        c.upload()
+        check_precision(c, c.attention())
+        c.close()
+
+
+@pytest.mark.parametrize("below", [5.0, 10.0, 15.0, 18.0, 22.0, 30.0])
+@pytest.mark.parametrize("new", [1, 40])
+def test_keys_far_below_the_largest(mxh, below, new):
+    """One key whose V is zero, 1,000 others `below` nats under it: what the halves of a probability still say of them."""
+    c = Case([(1000, new)], nh=8, nkv=2, hd=64, page=16, seed=23)
+    q = c.q.reshape(c.tokens, 8, 64)
+    q[:] = 0
+    q[..., 0] = 8.0
+    for r in range(1000 + new):
+        row = c.row(c.k, 0, r).reshape(2, 64)
+        row[:] = 0
+        row[:, 0] = below if r == 333 else 0.0
+    c.row(c.v, 0, 333)[:] = 0
+    c.upload()
+    check_precision(c, c.attention())
+    c.close()
