@@ -254,7 +254,8 @@ int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *b
  * of the new tokens it follows and its own (all already in the cache), then
  * the weighted sum of V rows into att, same shape as q.  What a token does not
  * attend has no effect on it, infinities and NaN included; a token none of
- * whose rows exist gets zeros.  Takes whole prompts, single tokens and drafted
+ * whose rows exist gets zeros, as does a head all of whose scores are minus
+ * infinity.  Takes whole prompts, single tokens and drafted
  * trees, mixed as they come.  Long rows of keys are split among workgroups,
  * their parts in `work`: mxh_attention_paged_workspace sets *bytes to what any
  * batch of up to this n_seq, n_tokens and table_ld needs at most, whatever its

@@ -139,3 +139,33 @@ def test_keys_far_below_the_largest(mxh, below, new):
     c.upload()
     check_precision(c, c.attention())
     c.close()
+
+
+@pytest.mark.parametrize("seqs,tree", [([(0, 1), (300, 1)], False), ([(5000, 2)], False), ([(700, 45), (3, 1)], False),
+                                       ([(100, 30), (9, 4)], True)])
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_rows_whose_scores_are_all_minus_infinity(mxh, hd, seqs, tree):
+    """They get zeros, as tokens none of whose rows exist do; a q of zero there makes NaN; other heads see nothing."""
+    c = Case(seqs, nh=4, nkv=2, hd=hd, page=16, tree=tree, seed=33)
+    for s, (n_c, n) in enumerate(seqs):
+        for r in range(n_c + n):
+            c.row(c.k, s, r)[7] = -np.inf  # (kv head 0)
+    q = c.q.reshape(c.tokens, 4, hd)
+    q[:, 0, 7] = np.abs(q[:, 0, 7]) + 0.01
+    q[:, 1, 7] = 0
+    c.upload()
+    got = c.attention()
+    assert np.all(got[:, 0] == 0)
+    assert np.all(np.isnan(got[:, 1]))
+    for s, (n_c, n) in enumerate(seqs):
+        k, v = (np.array([c.row(x, s, r) for r in range(n_c + n)], np.float64).reshape(-1, 2, hd)[:, 1] for x in (c.k, c.v))
+        for i in range(n):
+            t, at = int(c.start[s]) + i, list(range(n_c)) + [n_c + j for j in c.before(s, i)]
+            for h in (2, 3):
+                sc = k[at] @ q[t, h].astype(np.float64) / np.sqrt(hd)
+                p = np.exp(sc - sc.max())
+                p /= p.sum()
+                d = (2.0**-21 + (2 * hd + 4) * U) * (np.abs(k[at]) @ np.abs(q[t, h].astype(np.float64))).max() / np.sqrt(hd)
+                bound = (2 * d + 2.0**-20 + 2 * len(at) * U) * (p @ np.abs(v[at])) + 2.0**-31 * np.abs(v[at]).sum(0)
+                assert np.all(np.abs(got[t, h] - p @ v[at]) <= bound), (s, i, h)
+    c.close()
