@@ -213,15 +213,19 @@ typedef struct {
  * r % page_rows of page table[s * table_ld + r / page_rows].  parent[t] is the
  * index, within its sequence's new tokens, of the token that t was drafted
  * after (smaller than its own; -1: the last cached token), at most 64 new
- * tokens a sequence; parent NULL: every token follows the one before it, any
- * number of them.  The arrays are device memory that no call checks on the
- * host, but no value in them makes a kernel leave the pool, the token arrays or
- * a workspace: rows of a page id outside 0 .. n_pages-1 or past table_ld are
- * absent (never attended, never written), a parent that is not smaller than its
- * token counts as -1, tokens past the 64th of a drafted tree and token rows
- * outside start[0] .. start[n_seq]-1 or past n_tokens are left alone, lengths
- * below zero count as zero, a sequence that starts below 0 has no tokens.  start
- * must not decrease (where it does, nothing is attended and att is left alone). */
+ * tokens a sequence, of every sequence of the batch; parent NULL: every token
+ * follows the one before it, any number of them.  So a prompt of more than 64
+ * tokens beside drafted trees goes in a batch of its own: two calls over the same
+ * token arrays, start (and cached and table) of the second at its sequences, each
+ * leaving the other's rows alone.  The arrays are device memory that no call
+ * checks on the host, but no value in them makes a kernel leave the pool, the
+ * token arrays or a workspace: rows of a page id outside 0 .. n_pages-1 or past
+ * table_ld are absent (never attended, never written), a parent that is not
+ * smaller than its token counts as -1, tokens past the 64th of a drafted tree and
+ * token rows outside start[0] .. start[n_seq]-1 or past n_tokens are left alone,
+ * lengths below zero count as zero, a sequence that starts below 0 has no tokens.
+ * start must not decrease (where it does, nothing is attended and att is left
+ * alone). */
 typedef struct {
     int n_seq, n_tokens;
     const int *start;  /* [n_seq + 1] */
@@ -255,19 +259,19 @@ int mxh_qk_rope_append(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *b
  * the weighted sum of V rows into att, same shape as q.  What a token does not
  * attend has no effect on it, infinities and NaN included; a token none of
  * whose rows exist gets zeros, as does a head all of whose scores are minus
- * infinity.  Takes whole prompts, single tokens and drafted
- * trees, mixed as they come.  Long rows of keys are split among workgroups,
- * their parts in `work`: mxh_attention_paged_workspace sets *bytes to what any
- * batch of up to this n_seq, n_tokens and table_ld needs at most, whatever its
- * device arrays hold.  Calls that may run at the same time (a replayed graph
- * beside the library stream) need work of their own.  q and the probabilities
- * enter the matrix cores as two fp16 halves, K and V as they are: q to 2^-22 of
- * the row's largest |q| (rows outside the halves' range are scaled by a power of
- * two), a probability to 2^-22 of its own and 2^-31 of the row's largest, so a
- * key 21 nats below the largest counts in the sum of probabilities alone.  Rows
- * that meet infinities or NaN are computed again in fp32 (slowly, milliseconds
- * for thousands of keys).  q, att and work 16-byte aligned, not overlapping; nh
- * as above. */
+ * infinity.  Takes whole prompts and single tokens, mixed as they come, or
+ * drafted trees and what else has at most 64 new tokens.  Long rows of keys are
+ * split among workgroups, their parts in `work`: mxh_attention_paged_workspace
+ * sets *bytes to what any batch of up to this n_seq, n_tokens and table_ld needs
+ * at most, whatever its device arrays hold.  Calls that may run at the same time
+ * (a replayed graph beside the library stream) need work of their own.  q and the
+ * probabilities enter the matrix cores as two fp16 halves, K and V as they are: q
+ * to 2^-22 of the row's largest |q| (rows outside the halves' range are scaled by
+ * a power of two), a probability to 2^-22 of its own and 2^-31 of the row's
+ * largest, so a key 21 nats below the largest counts in the sum of probabilities
+ * alone.  Rows that meet infinities or NaN are computed again in fp32 (slowly,
+ * milliseconds for thousands of keys).  q, att and work 16-byte aligned, not
+ * overlapping; nh as above. */
 int mxh_attention_paged(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const float *q, int nh,
                         float *att, void *work, size_t work_bytes);
 int mxh_attention_paged_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, int nh, size_t *bytes);

@@ -286,7 +286,7 @@ def attention_paged_workspace(pool: KvPool, batch: KvBatch, nh: int) -> int:
 
 
 def attention_paged(pool: KvPool, layer: int, batch: KvBatch, q, nh: int, att, work=None, work_bytes: int = 0) -> None:
-    """Attention of packed prompts, single tokens and drafted trees over the paged cache."""
+    """Attention of packed prompts and single tokens, or of drafted trees, over the paged cache."""
     check(lib.mxh_attention_paged(C.byref(pool), layer, C.byref(batch), addr(q), nh, addr(att), addr(work),
                                   work_bytes), "mxh_attention_paged")
 

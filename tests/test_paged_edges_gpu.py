@@ -9,7 +9,7 @@ import numpy as np
 import pytest
 
 import mxhip
-from test_paged_gpu import U, Case
+from test_paged_gpu import Case, U, chain, rope_expected, rope_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -168,4 +168,50 @@ def test_rows_whose_scores_are_all_minus_infinity(mxh, hd, seqs, tree):
                 d = (2.0**-21 + (2 * hd + 4) * U) * (np.abs(k[at]) @ np.abs(q[t, h].astype(np.float64))).max() / np.sqrt(hd)
                 bound = (2 * d + 2.0**-20 + 2 * len(at) * U) * (p @ np.abs(v[at])) + 2.0**-31 * np.abs(v[at]).sum(0)
                 assert np.all(np.abs(got[t, h] - p @ v[at]) <= bound), (s, i, h)
+    c.close()
+
+
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32"])
+def test_long_prompts_beside_drafted_trees_go_in_a_call_of_their_own(mxh, heads):
+    """One packed step, two batches over its arrays: trees with parents, then prompts and single tokens without.  Each
+    call leaves the other's token rows, and the pool's other rows, alone."""
+    nh, nkv, hd = HEADS[heads]
+    trees, rest = [(300, 20), (7, 64), (0, 5)], [(40, 100), (900, 1), (0, 130), (63, 1)]
+    c = Case(trees + rest, nh=nh, nkv=nkv, hd=hd, page=16, tree=True, lead=1, tail=2, seed=81, extra_ld=1)
+    for s in range(len(trees), len(c.seqs)):
+        c.parents[s] = chain(c.seqs[s][1])
+    c.upload()
+    n, b = len(trees), c.bufs
+    qkv, bias, w = rope_inputs(c, 4)
+    freq = mxhip.rope_frequencies(1e4, hd)
+    dev = [mxhip.DeviceBuffer.from_array(x) for x in (qkv, bias, w[0], w[1], freq)]
+    first = mxhip.KvBatch(n, c.tokens, b["start"], b["cached"], b["table"], c.ld, b["parent"])
+    second = mxhip.KvBatch(len(rest), c.tokens, b["start"].ptr + 4 * n, b["cached"].ptr + 4 * n,
+                           b["table"].ptr + 4 * n * c.ld, c.ld)
+    mxhip.memset(b["q"], 0)
+    for batch in (first, second):
+        mxhip.qk_rope_append(c.pool, 0, batch, dev[0], qkv.shape[1], dev[1], dev[2], dev[3], 1e-6, dev[4], True, nh, b["q"])
+    mxhip.synchronize()
+    q, k, v = (b[x].download(t) for x, t in (("q", np.float32), ("k", np.float16), ("v", np.float16)))
+    want, bound = rope_expected(c, qkv, bias, list(w), 1e-6, freq, True)
+    inside = slice(int(c.start[0]), int(c.start[-1]))
+    c.q = q.reshape(c.tokens, -1)
+    assert np.all(np.abs(q.reshape(c.tokens, nh, hd)[inside] - want[0][inside]) <= bound[0][inside] + 2.0**-140)
+    assert not c.q[:inside.start].any() and not c.q[inside.stop:].any()
+    c.k, c.v = k.reshape(c.k.shape), v.reshape(c.v.shape)
+    for s, (n_c, m) in enumerate(c.seqs):
+        for i in range(m):
+            t = int(c.start[s]) + i
+            for pool, x, e in ((c.k, want[1], bound[1]), (c.v, want[2], bound[2])):
+                y = x[t].reshape(-1)
+                assert np.all(np.abs(c.row(pool, s, n_c + i) - y) <= (np.abs(y) + e[t].reshape(-1)) * 2.0**-11 +
+                              e[t].reshape(-1) + 2.0**-25)
+    for batch in (first, second):
+        size = mxhip.attention_paged_workspace(c.pool, batch, nh)
+        assert size <= c.work_bytes  # (the whole step's is enough for its parts)
+        mxhip.attention_paged(c.pool, 0, batch, b["q"], nh, b["att"], b["work"], c.work_bytes)
+    mxhip.synchronize()
+    c.check(b["att"].download(np.float32).reshape(c.tokens, nh, hd))
+    for x in dev:
+        x.close()
     c.close()
