@@ -54,7 +54,8 @@ class SynthArch(C.Structure):
 
 
 class KvPool(C.Structure):
-    """K and V pages in HBM (mxh_kv_pool): fp16, [n_layer][n_pages][page_rows][n_kv * head_dim] each, by address."""
+    """K and V pages in HBM (mxh_kv_pool): fp16, [n_layer][n_pages][page_rows][n_kv * head_dim] each, by buffer or
+    address.  Buffers live as long as this does."""
 
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("layer_stride", C.c_int64)] + \
                [(n, C.c_int) for n in ("n_layer", "n_pages", "page_rows", "n_kv", "head_dim")]
@@ -62,16 +63,19 @@ class KvPool(C.Structure):
     def __init__(self, k, v, *, n_layer: int, n_pages: int, page_rows: int, n_kv: int, head_dim: int,
                  layer_stride: int = 0):
         super().__init__(addr(k), addr(v), layer_stride, n_layer, n_pages, page_rows, n_kv, head_dim)
+        self.buffers = k, v
 
 
 class KvBatch(C.Structure):
-    """A step's packed tokens (mxh_kv_batch); int32 device arrays, by buffer or address."""
+    """A step's packed tokens (mxh_kv_batch); int32 device arrays, by buffer or address.  Buffers live as
+    long as this does."""
 
     _fields_ = [("n_seq", C.c_int), ("n_tokens", C.c_int), ("start", C.c_void_p), ("cached", C.c_void_p),
                 ("table", C.c_void_p), ("table_ld", C.c_int), ("parent", C.c_void_p)]
 
     def __init__(self, n_seq: int, n_tokens: int, start, cached, table, table_ld: int, parent=None):
         super().__init__(n_seq, n_tokens, addr(start), addr(cached), addr(table), table_ld, addr(parent))
+        self.buffers = start, cached, table, parent
 
 
 def addr(b):

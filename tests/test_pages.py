@@ -11,6 +11,7 @@ import ctypes as C
 import random
 import subprocess
 import sys
+import weakref
 
 import numpy as np
 import pytest
@@ -332,3 +333,26 @@ def test_starts_of_kept_lists_need_not_begin_at_zero():
     mxhip.kv_keep_rows(pool(), [[0, 1]], [3], [2, 4], [-9, 99, 0, 1])
     assert mxhip.lib.mxh_kv_keep_rows(C.byref(pool()), (C.c_int * 2)(0, 1), 2, (C.c_int * 1)(3), (C.c_int * 2)(0, 0),
                                       None, 1) == 0
+
+
+def test_pools_and_batches_hold_their_buffers():
+    """A buffer that only a pool or a batch was given is not freed under it."""
+    def buffer():
+        b = object.__new__(mxhip.DeviceBuffer)  # (no GPU here: an address that is never freed)
+        b.ptr, b.nbytes, b.close = AT, 64, lambda: None
+        return b
+
+    made = []
+
+    def new():
+        b = buffer()
+        made.append(weakref.ref(b))
+        return b
+
+    pl = mxhip.KvPool(new(), new(), n_layer=1, n_pages=1, page_rows=16, n_kv=1, head_dim=32)
+    ba = mxhip.KvBatch(1, 1, new(), new(), new(), 1, new())
+    assert (pl.k, pl.v, ba.start, ba.cached, ba.table, ba.parent) == (AT,) * 6
+    assert all(r() is not None for r in made)
+    del pl, ba
+    assert all(r() is None for r in made)
+    assert mxhip.KvBatch(1, 1, AT, AT, AT, 1).parent is None
