@@ -369,7 +369,9 @@ class Pages:
 
     @property
     def free(self) -> int:
-        return lib.mxh_pages_free(self.h)
+        n = lib.mxh_pages_free(self.h)
+        check(min(n, 0), "mxh_pages_free")
+        return n
 
     def table(self, seqs, table_ld: int) -> tuple[np.ndarray, np.ndarray]:
         """(page ids [n][table_ld], lengths [n]) of the sequences, for a KvBatch."""

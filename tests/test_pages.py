@@ -356,3 +356,13 @@ def test_pools_and_batches_hold_their_buffers():
     del pl, ba
     assert all(r() is None for r in made)
     assert mxhip.KvBatch(1, 1, AT, AT, AT, 1).parent is None
+
+
+def test_closed_bookkeeping_refuses():
+    p = mxhip.Pages(4, 16, 1)
+    p.close()
+    p.close()
+    for call in (p.open, lambda: p.free, lambda: p.length(0), lambda: p.fork(0), lambda: p.release(0), lambda: p.extend(0, 1),
+                 lambda: p.set_length(0, 0), lambda: p.table([0], 1)):
+        with pytest.raises(mxhip.MxhError):
+            call()
