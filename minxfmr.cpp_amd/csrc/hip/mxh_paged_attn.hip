@@ -376,16 +376,18 @@ __device__ __forceinline__ float inverse_power(float x) { return __uint_as_float
 //
 // Measured with 32/8 heads of 128:
 //   R = 16: 48 single tokens at up to 16,000 rows 229 us = 6.3 TB/s of K and V (a
-//   large read 6.7), bound by those; one at 8,192 15 us.  One token of 16/8 heads
-//   at 700 9.8 us: two launches, and in the first the plan's, the pages' and the
+//   large read 6.7), bound by those; one at 8,192 14 us.  One token of 16/8 heads
+//   at 700 10.0 us: two launches, and in the first the plan's, the pages' and the
 //   rows' loads one after the other.
-//   R = 64: six packed prompts of 29 to 2,100 tokens behind up to 1,500 rows 264
-//   us (276 on another card) = 468 TFLOP/s of the formula's, 940 of the products
-//   made (a large fp16 product 1,184); matrix cores and vector units half busy each, and neither
-//   fewer reads nor fewer exponentials made it faster by more than 4%.  27 drafted
-//   tokens at 8,192 rows 23.7 us: 8 stages an item 12 of them (a stage's loads are
-//   one stage ahead and HBM is 1.4 us away), what comes before and after an item's
-//   stages 7, the second kernel 4.
+//   R = 64: six packed prompts of 29 to 2,100 tokens behind up to 1,500 rows 267
+//   us (263 to 270 card to card) = 464 TFLOP/s of the formula's, 930 of the products
+//   made (a large fp16 product 1,184); matrix cores and vector units half busy
+//   each, and neither fewer reads nor fewer exponentials made it faster by more
+//   than 4%.  27 drafted tokens at 8,192 rows 24.2 us: 8 stages an item 12 of them
+//   (a stage's loads are one stage ahead and HBM is 1.4 us away), what comes before
+//   and after an item's stages 8, the second kernel 4.
+// Many sequences: every workgroup plans for itself, so 1,024 single tokens at up to
+// 300 rows take 282 us (their rows 78) and 4,096 2,980 (304); 256 take 41 (19).
 template <int HD, int R>
 __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedArgs a) {
     constexpr int M = R == 16 ? 16 : 32, RS = R / M;  // rows of a wave; waves to a key group

@@ -73,6 +73,18 @@ struct PagedPiece {
 //   R = 16: cut unless all tiles are short and there are many: 200 single tokens
 //   at up to 300 rows 29 whole, 43 cut, at up to 1,000 83 and 89, at up to 6,000
 //   437 and 406; 64 at up to 2,000 61 and 53.
+//   (Shorter ones beside the longest: 64 at up to 2,000 40 and 45.)
+// Heads of 64 and 32 go by the same numbers, which suit them less where the times
+// are short.  Whole and cut, 32/8 heads of 64; 32/8 of 32; 8/1 of 32:
+//   whole: a prompt of 1,024 21 and 35; 18 and 27.  200 single tokens at up to 300
+//   21 and 35; 17 and 33; and at up to 1,000 34 and 51; 31 and 43 (45 and 34 with
+//   the second kernel that the table's width asks for)
+//   cut: a prompt of 256 at 4,096 59 and 36; 52 and 32; 52 and 19.  16 trees of up
+//   to 33 at up to 8,000 105 and 41; 93 and 36; 93 and 20, 20 of up to 60 at up to
+//   1,000 23 and 26; 20 and 22; 18 and 15.  Single tokens: 200 at up to 6,000 229
+//   and 172; 170 and 159; 36 and 27, 64 at up to 2,000 23 and 27; 22 and 25; 15 and
+//   11, 200 at up to 300 with 8/1 heads of 32 8.5 and 12, one at 8,192 53 and 11; 47
+//   and 11; 46 and 11.
 struct PagedLine {
     uint32_t t, key_shift, lead, block;  // tokens of a tile; a stage has 1 << key_shift keys
     float inv_t;
@@ -181,6 +193,11 @@ struct PagedLine {
 // 64-row ones leave rows empty: 16 sequences of 2 tokens (8 rows) at up to 4,000
 // keys took 25 us with 16 and 31 with 64, of up to 12 tokens 36 and 32; one of 4
 // tokens at 8,192 16 and 20, of 27 28 and 24, at 40,000 173 and 69.
+// One height for all, so the average costs where sequences differ: 200 single tokens
+// at up to 2,000 rows and a prompt of 2,000 226 us (119 and 91 apart), of 500 155
+// (119 and 18); a tree of 27 at 40,000 beside 20 single tokens 168 (68 and 16).
+// Empty sequences count: that tree in a batch of 16 whose others are empty 167, at
+// 8,192 30 (25 by itself).
 struct PagedShape {
     int rows, target;  // target: items that stages are cut into, at most; 0: an item is a tile
     int64_t items;     // at most
