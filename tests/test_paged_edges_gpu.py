@@ -215,3 +215,66 @@ def test_long_prompts_beside_drafted_trees_go_in_a_call_of_their_own(mxh, heads)
     for x in dev:
         x.close()
     c.close()
+
+
+def test_more_items_than_a_grid_axis_takes(mxh):
+    """4,096 prompts of 60 tokens of 8/1 heads: 34,816 tiles at most, over two axes of the grid."""
+    n, m, nh, hd, page = 4096, 60, 8, 32, 64
+    rng = np.random.default_rng(6)
+    tokens = n * m
+    q = rng.standard_normal((tokens, nh * hd), dtype=np.float32)
+    kv = rng.standard_normal((2, n * page, hd), dtype=np.float32).astype(np.float16)
+    put = mxhip.DeviceBuffer.from_array
+    order = rng.permutation(n).astype(np.int32)
+    dev = [put(np.arange(0, tokens + 1, m, dtype=np.int32)), put(np.zeros(n, np.int32)), put(order[:, None]), put(q),
+           put(np.full_like(q, -1.5)), put(kv[0]), put(kv[1])]
+    pool = mxhip.KvPool(dev[5], dev[6], n_layer=1, n_pages=n, page_rows=page, n_kv=1, head_dim=hd)
+    batch = mxhip.KvBatch(n, tokens, dev[0], dev[1], dev[2], 1)
+    size = mxhip.attention_paged_workspace(pool, batch, nh)
+    work = mxhip.DeviceBuffer(max(size, 1))
+    mxhip.attention_paged(pool, 0, batch, dev[3], nh, dev[4], work, size)
+    mxhip.synchronize()
+    got = dev[4].download(np.float32).reshape(tokens, nh, hd)
+    for s in list(range(0, n, 97)) + [n - 1]:
+        k, v = (x[order[s] * page:order[s] * page + m].astype(np.float64) for x in kv)
+        for i in (0, 7, 8, 33, m - 1):
+            t = s * m + i
+            x = q[t].reshape(nh, hd).astype(np.float64)
+            sc = x @ k[:i + 1].T / np.sqrt(hd)
+            p = np.exp(sc - sc.max(-1, keepdims=True))
+            p /= p.sum(-1, keepdims=True)
+            d = (2.0**-21 + (2 * hd + 4) * U) * (np.abs(x) @ np.abs(k[:i + 1]).T).max(-1, keepdims=True) / np.sqrt(hd)
+            bound = (2 * d + 2.0**-20 + 2 * (i + 1) * U) * (p @ np.abs(v[:i + 1])) + 2.0**-31 * np.abs(v[:i + 1]).sum(0)
+            assert np.all(np.abs(got[t] - p @ v[:i + 1]) <= bound), (s, i)
+    for b in [*dev, work]:
+        b.close()
+
+
+@pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
+def test_k_and_v_of_a_layer_side_by_side(mxh, tree):
+    """One buffer [layer][K, V][page][row]: v begins a layer's K into it and a layer's stride is two of them."""
+    nh, nkv, hd, page, layers = 6, 2, 64, 32, 3
+    c = Case([(70, 3), (0, 40), (10, 9)], nh=nh, nkv=nkv, hd=hd, page=page, tree=tree, layers=layers, layer=1, seed=91)
+    c.upload()
+    dense = c.k.shape[1]
+    both = np.stack([c.k, c.v], 1)  # [layer][K, V][...]
+    buf = mxhip.DeviceBuffer.from_array(both)
+    pool = mxhip.KvPool(buf, buf.ptr + 2 * dense, n_layer=layers, n_pages=c.n_pages, page_rows=page, n_kv=nkv, head_dim=hd,
+                        layer_stride=2 * dense)
+    mxhip.attention_paged(pool, c.layer, c.batch, c.bufs["q"], nh, c.bufs["att"], c.bufs["work"], c.work_bytes)
+    mxhip.synchronize()
+    c.check(c.bufs["att"].download(np.float32).reshape(c.tokens, nh, hd))
+    spare = sorted(set(range(c.n_pages)) - set(c.table[c.table >= 0].tolist()))
+    mxhip.kv_copy_pages(pool, c.table[1, :1], spare[:1])
+    cached = [n for n, _ in c.seqs]
+    mxhip.kv_keep_rows(pool, c.table, cached, [0, 1, 3, 3], [2, 5, 33])
+    mxhip.synchronize()
+    want = both.view(np.uint16).reshape(layers, 2, c.n_pages, page, nkv * hd).copy()
+    want[:, :, spare[0]] = want[:, :, c.table[1, 0]]
+    old = want.copy()
+    for s, i, kept in ((0, 0, 2), (1, 0, 5), (1, 1, 33)):
+        to, frm = cached[s] + i, cached[s] + kept
+        want[:, :, c.table[s, to // page], to % page] = old[:, :, c.table[s, frm // page], frm % page]
+    assert np.array_equal(buf.download(np.uint16).reshape(want.shape), want)
+    buf.close()
+    c.close()
