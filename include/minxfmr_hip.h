@@ -276,6 +276,34 @@ int mxh_attention_paged(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *
                         float *att, void *work, size_t work_bytes);
 int mxh_attention_paged_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, int nh, size_t *bytes);
 
+/* Sequences of a batch that begin with the same rows: group g is the sequences
+ * start[g] .. start[g+1]-1, in whose tables the first shared[g] rows are the same
+ * pages (forks of one sequence: mxh_pages_common), rounded down to whole pages.
+ * Sequences outside start[0] .. start[n_groups]-1 share nothing, and no group is
+ * nested in another.  Device memory that no call checks: a group's rows in common
+ * are no more than any of its sequences with new tokens has cached, nor than the
+ * table's; start that falls, or leaves 0 .. n_seq, makes no groups. */
+typedef struct {
+    int n_groups;      /* 0 .. n_seq */
+    const int *start;  /* [n_groups + 1] */
+    const int *shared; /* [n_groups] */
+} mxh_kv_groups;
+
+/* mxh_attention_paged where sequences have their first rows in common: the same
+ * result (but for fp32 rounding), with K and V of a group's prefix read once for
+ * the tokens of all its sequences, from the pages of the group's first sequence
+ * that has new tokens, instead of once a sequence.  (A group of one sequence, or
+ * none, is correct and takes about a plan and a third kernel longer than
+ * mxh_attention_paged.)  Takes the same batches, drafted trees among them; what a
+ * token does not attend, absent rows, infinities and precision are as there, and so
+ * are the rules for q, att and work; mxh_attention_shared_workspace says what any
+ * batch of up to this n_seq, n_tokens, n_groups and table_ld needs (every token's
+ * parts lie there: twice att at least). */
+int mxh_attention_shared(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const mxh_kv_groups *groups,
+                         const float *q, int nh, float *att, void *work, size_t work_bytes);
+int mxh_attention_shared_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, const mxh_kv_groups *groups,
+                                   int nh, size_t *bytes);
+
 /* Copies page src[i] to page dst[i], K and V, in every layer (what a fork
  * needs before both sequences write the page they share).  Host arrays; page
  * ids in range, every dst once and no dst among the src, or MXH_ERR_ARG. */
@@ -318,6 +346,10 @@ int mxh_pages_extend(mxh_pages *p, int seq, int rows, int *src, int *dst, int *c
 int mxh_pages_set_length(mxh_pages *p, int seq, int rows);
 /* Rows of a sequence (MXH_ERR_ARG: no such sequence). */
 int mxh_pages_length(const mxh_pages *p, int seq);
+/* Rows that all n sequences have in the same pages, from the first on: whole
+ * pages, within each one's length (what mxh_kv_groups takes; MXH_ERR_ARG: no such
+ * sequence). */
+int mxh_pages_common(const mxh_pages *p, const int *seqs, int n);
 /* Pages that no sequence holds. */
 int mxh_pages_free(const mxh_pages *p);
 /* The batch's table and cached arrays (host): row i of `table` gets the page

@@ -80,4 +80,10 @@ size_t attention_paged_work_bytes(const PagedArgs& a, int nh, int hd);  // of th
 size_t attention_paged_work_bound(const PagedArgs& a, int nh, int hd);  // of any up to its n_seq, n_tokens, table_ld
 int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, float* att, void* work, hipStream_t st);
 
+// attention where groups of sequences have their first rows in common (mxh_shared_attn.hip)
+size_t attention_shared_work_bytes(const PagedArgs& a, int n_groups, int nh, int hd);
+size_t attention_shared_work_bound(const PagedArgs& a, int n_groups, int nh, int hd);
+int attention_shared_launch(const PagedArgs& a, int n_groups, const int* group_start, const int* group_shared,
+                            const float* q, int nh, int hd, float* att, void* work, hipStream_t st);
+
 }  // namespace mxh

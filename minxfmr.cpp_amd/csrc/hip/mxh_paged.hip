@@ -292,6 +292,38 @@ PagedArgs paged_args(const mxh_kv_pool* p, int layer, const mxh_kv_batch* b) {
     return a;
 }
 
+int check_groups(const char* who, const mxh_kv_batch* b, const mxh_kv_groups* g) {
+    if (!g) return set_error(MXH_ERR_ARG, "%s: null groups", who);
+    if (g->n_groups < 0 || g->n_groups > b->n_seq)
+        return set_error(MXH_ERR_ARG, "%s: %d groups of %d sequences", who, g->n_groups, b->n_seq);
+    if (g->n_groups > 0 && (!g->start || !g->shared)) return set_error(MXH_ERR_ARG, "%s: null array", who);
+    return MXH_OK;
+}
+
+// of q and of att
+size_t batch_bytes(const mxh_kv_pool* p, const mxh_kv_batch* b, int nh) {
+    return sizeof(float) * (size_t)b->n_tokens * nh * p->head_dim;
+}
+
+int check_attention(const char* who, const mxh_kv_pool* p, const mxh_kv_batch* b, const float* q, int nh,
+                    const float* att, const void* work) {
+    if (!q || !att || !al16(q) || !al16(att) || !al16(work))
+        return set_error(MXH_ERR_ARG, "%s: q and att must be non-null, every array aligned to 16 bytes", who);
+    const size_t bytes = batch_bytes(p, b, nh);
+    if (overlap(q, bytes, att, bytes)) return set_error(MXH_ERR_ARG, "%s: att overlaps q", who);
+    return MXH_OK;
+}
+
+// x and y: what work must not overlap, `bytes` each
+int check_work(const char* who, size_t need, const void* work, size_t work_bytes, const void* x, const void* y,
+               size_t bytes) {
+    if (need && (!work || work_bytes < need))
+        return set_error(MXH_ERR_ARG, "%s: %zu bytes of work, %zu needed", who, work ? work_bytes : 0, need);
+    if (need && (overlap(work, need, x, bytes) || overlap(work, need, y, bytes)))
+        return set_error(MXH_ERR_ARG, "%s: work overlaps q or att", who);
+    return MXH_OK;
+}
+
 // marks ids (a bit a page); false where one is marked already
 bool mark_pages(const int* ids, int n, std::vector<uint64_t>& seen) {
     for (int i = 0; i < n; ++i) {
@@ -402,20 +434,44 @@ int mxh_attention_paged(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* 
     const char* who = "attention_paged";
     if (int rc = check_step(who, pool, layer, batch, nh)) return rc;
     if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
-    if (!q || !att || !al16(q) || !al16(att) || !al16(work))
-        return set_error(MXH_ERR_ARG, "%s: q and att must be non-null, every array aligned to 16 bytes", who);
-    const size_t bytes = sizeof(float) * (size_t)batch->n_tokens * nh * pool->head_dim;
-    if (overlap(q, bytes, att, bytes)) return set_error(MXH_ERR_ARG, "%s: att overlaps q", who);
+    if (int rc = check_attention(who, pool, batch, q, nh, att, work)) return rc;
     if (!mxh_is_available()) return MXH_ERR_NODEV;
     const PagedArgs a = paged_args(pool, layer, batch);
     const size_t need = attention_paged_work_bytes(a, nh, pool->head_dim);
-    if (need && (!work || work_bytes < need))
-        return set_error(MXH_ERR_ARG, "%s: %zu bytes of work, %zu needed", who, work ? work_bytes : 0, need);
-    if (need && (overlap(work, need, q, bytes) || overlap(work, need, att, bytes)))
-        return set_error(MXH_ERR_ARG, "%s: work overlaps q or att", who);
+    if (int rc = check_work(who, need, work, work_bytes, q, att, batch_bytes(pool, batch, nh))) return rc;
     if (int rc = attention_paged_launch(a, q, nh, pool->head_dim, att, work, lib_stream()))
         return set_error(rc, "%s: launch", who);
     return check_hip(hipGetLastError(), "attention_paged launch");
+}
+
+int mxh_attention_shared_workspace(const mxh_kv_pool* pool, const mxh_kv_batch* batch, const mxh_kv_groups* groups,
+                                   int nh, size_t* bytes) {
+    const char* who = "attention_shared_workspace";
+    if (!bytes) return set_error(MXH_ERR_ARG, "%s: null output pointer", who);
+    *bytes = 0;
+    if (int rc = check_step(who, pool, 0, batch, nh)) return rc;
+    if (int rc = check_groups(who, batch, groups)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    *bytes = attention_shared_work_bound(paged_args(pool, 0, batch), groups->n_groups, nh, pool->head_dim);
+    return MXH_OK;
+}
+
+int mxh_attention_shared(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* batch, const mxh_kv_groups* groups,
+                         const float* q, int nh, float* att, void* work, size_t work_bytes) {
+    const char* who = "attention_shared";
+    if (int rc = check_step(who, pool, layer, batch, nh)) return rc;
+    if (int rc = check_groups(who, batch, groups)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    if (int rc = check_attention(who, pool, batch, q, nh, att, work)) return rc;
+    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    const PagedArgs a = paged_args(pool, layer, batch);
+    const size_t need = attention_shared_work_bytes(a, groups->n_groups, nh, pool->head_dim);
+    if (int rc = check_work(who, need, work, work_bytes, q, att, batch_bytes(pool, batch, nh))) return rc;
+    if (int rc = attention_shared_launch(a, groups->n_groups, groups->start, groups->shared, q, nh, pool->head_dim,
+                                         att, work, lib_stream()))
+        return set_error(rc, "%s: launch", who);
+    return check_hip(hipGetLastError(), "attention_shared launch");
 }
 
 int mxh_kv_copy_pages(const mxh_kv_pool* pool, const int* src, const int* dst, int n) try {
@@ -580,6 +636,13 @@ int mxh_pages_set_length(mxh_pages* p, int seq, int rows) {
 int mxh_pages_length(const mxh_pages* p, int seq) {
     if (int rc = check_seq("pages_length", p, seq)) return rc;
     return p->book.length(seq);
+}
+
+int mxh_pages_common(const mxh_pages* p, const int* seqs, int n) {
+    if (!p || n < 0 || (n > 0 && !seqs)) return set_error(MXH_ERR_ARG, "pages_common: bad arguments");
+    for (int i = 0; i < n; ++i)
+        if (int rc = check_seq("pages_common", p, seqs[i])) return rc;
+    return p->book.common(seqs, n);
 }
 
 int mxh_pages_free(const mxh_pages* p) {

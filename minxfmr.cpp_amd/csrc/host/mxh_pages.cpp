@@ -84,6 +84,18 @@ bool PageBook::extend(int seq, int rows, int* src, int* dst) {
     return true;
 }
 
+int PageBook::common(const int* seqs, int n) const {
+    if (n == 0) return 0;
+    const std::vector<int>& a = pages(seqs[0]);
+    size_t same = (size_t)length(seqs[0]) / (size_t)page_rows_;
+    for (int i = 1; i < n; ++i) {
+        const std::vector<int>& b = pages(seqs[i]);
+        same = std::min(same, (size_t)length(seqs[i]) / (size_t)page_rows_);
+        same = (size_t)(std::mismatch(a.begin(), a.begin() + (std::ptrdiff_t)same, b.begin()).first - a.begin());
+    }
+    return (int)same * page_rows_;
+}
+
 void PageBook::set_length(int seq, int rows) {
     Seq& s = seqs_[(size_t)seq];
     s.length = s.reserved = rows;

@@ -29,6 +29,8 @@ public:
     // false (and nothing changed) when there are too few free pages; *src = -1
     // without a copy
     bool extend(int seq, int rows, int* src, int* dst);
+    // rows, whole pages of them, that the sequences have in the same pages
+    int common(const int* seqs, int n) const;
     // rows at most max(length, reserved)
     void set_length(int seq, int rows);
 

@@ -78,6 +78,17 @@ class KvBatch(C.Structure):
         self.buffers = start, cached, table, parent
 
 
+class KvGroups(C.Structure):
+    """Sequences of a batch that begin with the same pages (mxh_kv_groups); int32 device arrays, by buffer or address.
+    Buffers live as long as this does."""
+
+    _fields_ = [("n_groups", C.c_int), ("start", C.c_void_p), ("shared", C.c_void_p)]
+
+    def __init__(self, n_groups: int, start, shared):
+        super().__init__(n_groups, addr(start), addr(shared))
+        self.buffers = start, shared
+
+
 def addr(b):
     """The device address of a DeviceBuffer, or an address as it is (None: null)."""
     return b.ptr if isinstance(b, DeviceBuffer) else b
@@ -142,6 +153,8 @@ def _load() -> C.CDLL:
         "mxh_qk_rope_append": (ip, [vp, ip, vp, vp, i64, vp, vp, vp, C.c_float, vp, ip, ip, vp]),
         "mxh_attention_paged": (ip, [vp, ip, vp, vp, ip, vp, vp, sz]),
         "mxh_attention_paged_workspace": (ip, [vp, vp, ip, C.POINTER(sz)]),
+        "mxh_attention_shared": (ip, [vp, ip, vp, vp, vp, ip, vp, vp, sz]),
+        "mxh_attention_shared_workspace": (ip, [vp, vp, vp, ip, C.POINTER(sz)]),
         "mxh_kv_copy_pages": (ip, [vp, vp, vp, ip]),
         "mxh_kv_keep_rows": (ip, [vp, vp, ip, vp, vp, vp, ip]),
         "mxh_pages_create": (ip, [ip, ip, ip, C.POINTER(vp)]),
@@ -152,6 +165,7 @@ def _load() -> C.CDLL:
         "mxh_pages_extend": (ip, [vp, ip, ip, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int)]),
         "mxh_pages_set_length": (ip, [vp, ip, ip]),
         "mxh_pages_length": (ip, [vp, ip]),
+        "mxh_pages_common": (ip, [vp, vp, ip]),
         "mxh_pages_free": (ip, [vp]),
         "mxh_pages_table": (ip, [vp, vp, ip, vp, ip, vp]),
         "mxh_write_synthetic_gguf": (ip, [C.c_char_p, C.POINTER(SynthArch), C.c_uint64, ip]),
@@ -173,7 +187,8 @@ EXPORTED = (
     "mxh_write_synthetic_gguf mxh_model_decode mxh_model_set_token mxh_model_bench_gemv mxh_model_bench_attention "
     "mxh_qk_rope_append mxh_attention_paged mxh_attention_paged_workspace mxh_kv_copy_pages mxh_kv_keep_rows "
     "mxh_pages_create mxh_pages_destroy mxh_pages_open mxh_pages_fork mxh_pages_close mxh_pages_extend "
-    "mxh_pages_set_length mxh_pages_length mxh_pages_free mxh_pages_table"
+    "mxh_pages_set_length mxh_pages_length mxh_pages_free mxh_pages_table "
+    "mxh_attention_shared mxh_attention_shared_workspace mxh_pages_common"
 ).split()
 
 
@@ -295,6 +310,21 @@ def attention_paged(pool: KvPool, layer: int, batch: KvBatch, q, nh: int, att, w
                                   work_bytes), "mxh_attention_paged")
 
 
+def attention_shared_workspace(pool: KvPool, batch: KvBatch, groups: KvGroups, nh: int) -> int:
+    """Bytes of work that attention_shared needs for batches of this n_seq, n_tokens, n_groups and table_ld."""
+    n = C.c_size_t()
+    check(lib.mxh_attention_shared_workspace(C.byref(pool), C.byref(batch), C.byref(groups), nh, C.byref(n)),
+          "mxh_attention_shared_workspace")
+    return n.value
+
+
+def attention_shared(pool: KvPool, layer: int, batch: KvBatch, groups: KvGroups, q, nh: int, att, work,
+                     work_bytes: int) -> None:
+    """attention_paged with the rows that groups of sequences have in common read once for each group."""
+    check(lib.mxh_attention_shared(C.byref(pool), layer, C.byref(batch), C.byref(groups), addr(q), nh, addr(att),
+                                   addr(work), work_bytes), "mxh_attention_shared")
+
+
 def _ints(a) -> np.ndarray:
     return np.ascontiguousarray(a, np.int32)
 
@@ -365,6 +395,13 @@ class Pages:
     def length(self, seq: int) -> int:
         n = lib.mxh_pages_length(self.h, seq)
         check(min(n, 0), "mxh_pages_length")
+        return n
+
+    def common(self, seqs) -> int:
+        """Rows (whole pages) that the sequences have in the same pages."""
+        seqs = _ints(seqs)
+        n = lib.mxh_pages_common(self.h, seqs.ctypes.data, seqs.size)
+        check(min(n, 0), "mxh_pages_common")
         return n
 
     @property
