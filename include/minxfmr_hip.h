@@ -304,6 +304,65 @@ int mxh_attention_shared(const mxh_kv_pool *pool, int layer, const mxh_kv_batch 
 int mxh_attention_shared_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, const mxh_kv_groups *groups,
                                    int nh, size_t *bytes);
 
+/* Attention that reads, of a long context, the blocks of rows that promise most.
+ * A block is block_rows rows of a page (a power of two from 16 to page_rows);
+ * block b of a sequence has its rows b * block_rows and on, and a sequence at most
+ * 262,144 blocks (table_ld * page_rows / block_rows).  bounds holds of each block
+ * and kv head the least and the greatest key, dimension by dimension: fp16,
+ * [n_layer][n_pages][page_rows / block_rows][n_kv][2][head_dim], layer_stride
+ * elements from one layer to the next (0: dense; else a multiple of 8), 16-byte
+ * aligned.  A token takes n_select blocks (1..1024) for each kv head, among them its
+ * sequence's first n_first and its last n_last (>= 1: its own row's block is one of
+ * them). */
+typedef struct {
+    void *bounds;
+    int64_t layer_stride;
+    int block_rows, n_first, n_last, n_select;
+} mxh_kv_blocks;
+
+/* The bounds of the blocks in which the batch's new rows lie (cached[s] and on),
+ * from all rows that a block has then: to be called after mxh_qk_rope_append, and
+ * again, with a batch that says which rows, where rows changed otherwise
+ * (mxh_kv_keep_rows; a block of a copied page that the sequence does not append
+ * to).  Keys that are NaN do not count.  Blocks of absent pages are left out.
+ * n_first, n_last and n_select do not matter (n_select within its range); as in
+ * mxh_attention_paged's batches, tokens past the 64th of a drafted tree have no
+ * rows.  start that falls: some blocks may be left out. */
+int mxh_kv_block_bounds(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks);
+
+/* Which blocks each of a batch's tokens (q: [n_tokens][nh * head_dim] fp32) takes:
+ * chosen, int [n_tokens][n_kv][n_select], gets them ascending, -1 behind them.  Of
+ * the blocks up to the one of the token's own row (cached[s] and its index; the last
+ * of the table's at most) those are the first n_first, the last n_last, and the
+ * best of the others; all where there are no more than n_select.  A block's score is
+ * the largest, over the kv head's q heads, of
+ *     sum_d max(q_d, 0) greatest_d + min(q_d, 0) least_d,
+ * no score q.k of its rows being larger; scores are in 64 bits, so that a choice
+ * does not depend on the batch around it; of equal ones the earlier block is taken,
+ * a score that is not a number comes before all others, absent blocks come last.
+ * Rows of chosen of tokens that no sequence has are left alone (so may others be
+ * where start falls).  parent only counts in that tokens past the 64th have no
+ * rows.  q and work 16-byte aligned; work: mxh_kv_select_workspace, for any batch of
+ * up to this n_tokens and table_ld; nothing may overlap. */
+int mxh_kv_select_blocks(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks,
+                         const float *q, int nh, int *chosen, void *work, size_t work_bytes);
+int mxh_kv_select_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks, int nh,
+                            size_t *bytes);
+
+/* mxh_attention_paged over the rows of chosen blocks alone: of the rows that a
+ * token attends there, those of the blocks that chosen (as above, device memory)
+ * lists for it and the kv head.  A list is a set: its order does not matter, nor
+ * that it names a block twice, and what is negative or behind the token's own block
+ * is not in it; bounds are not read.  What a token does not attend, absent rows (a
+ * token none of whose listed rows exist gets zeros), infinities and precision are
+ * as in mxh_attention_paged, and so are the rules for q, att and work;
+ * mxh_attention_blocks_workspace says what any batch needs with these blocks.
+ * start that falls: some tokens may be left alone. */
+int mxh_attention_blocks(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks,
+                         const int *chosen, const float *q, int nh, float *att, void *work, size_t work_bytes);
+int mxh_attention_blocks_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks,
+                                   int nh, size_t *bytes);
+
 /* Copies page src[i] to page dst[i], K and V, in every layer (what a fork
  * needs before both sequences write the page they share).  Host arrays; page
  * ids in range, every dst once and no dst among the src, or MXH_ERR_ARG. */

@@ -1,0 +1,67 @@
+// mxh_blocks.h — how the operators over blocks of the paged cache share their
+// work out: the integers, on the host.  Plain C++ without HIP.
+//
+// A block is block_rows rows of a sequence that lie in one page; block b of a
+// sequence holds its rows [b block_rows, (b + 1) block_rows).
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace mxh {
+
+constexpr int kSelectMax = 1024;      // blocks that a token attends
+constexpr int kBlocksMax = 1 << 18;   // blocks of a sequence: a bit each of a token's in LDS
+constexpr int kListMax = 1024;        // blocks of a tile's list in LDS
+constexpr int kBitBytes = 32768;      // bits of a tile's tokens
+
+struct BlockSize {
+    int n_seq, n_tokens;
+    int64_t n_blocks;  // of a row of the table
+    int nkv, group, n_select, block_rows, cus;
+};
+
+// Tokens that share a tile of 16 rows.  Those of one sequence attend many of the
+// same blocks, and rows of absent tokens cost what others do; single tokens of
+// sequences (up to two each on average) share nothing and go by themselves.
+inline int block_tokens(const BlockSize& a) {
+    if (a.n_tokens <= 2 * (int64_t)a.n_seq) return 1;
+    const int64_t words = (a.n_blocks + 31) / 32;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({16 / a.group, kListMax / a.n_select, kBitBytes / (4 * words)}));
+}
+inline int64_t block_tiles(const BlockSize& a) {
+    const int t = block_tokens(a);
+    return (a.n_tokens + t - 1) / t;
+}
+// Workgroups that share a tile's list, for two a CU, with at least two stages of
+// 128 keys each
+inline int block_splits(const BlockSize& a) {
+    const int64_t items = block_tiles(a) * a.nkv, stages = ((int64_t)a.n_select * a.block_rows + 127) / 128;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)a.cus / items, stages / 2, 64}));
+}
+// the workspace: parts of the tiles that are split
+inline size_t block_part_bytes(int64_t parts, int nkv, int hd) {
+    return (size_t)parts * nkv * 16 * (hd + 2) * sizeof(float);
+}
+inline size_t block_work_bytes(const BlockSize& a, int hd) {
+    const int s = block_splits(a);
+    return s > 1 ? block_part_bytes(block_tiles(a) * s, a.nkv, hd) : 0;
+}
+// ... of any batch (splits > 1: splits x items are at most two a CU)
+inline size_t block_work_bound(const BlockSize& a, int hd) {
+    const int64_t stages = ((int64_t)a.n_select * a.block_rows + 127) / 128;
+    return stages < 4 ? 0 : block_part_bytes(std::max<int64_t>(2, 2 * (int64_t)a.cus / a.nkv), a.nkv, hd);
+}
+
+// Selecting: tokens whose scores the workspace holds at a time
+inline int64_t select_tokens(int n_tokens, int64_t n_blocks, int nkv) {
+    const int64_t row = n_blocks * nkv * 8;
+    return std::min<int64_t>(n_tokens, std::max<int64_t>(16, ((256 << 20) / row) / 16 * 16));
+}
+inline size_t select_work_bytes(int n_tokens, int64_t n_blocks, int nkv) {
+    return (size_t)select_tokens(n_tokens, n_blocks, nkv) * (size_t)(n_blocks * nkv) * 8;
+}
+
+}  // namespace mxh

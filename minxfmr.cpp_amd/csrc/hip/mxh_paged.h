@@ -86,4 +86,22 @@ size_t attention_shared_work_bound(const PagedArgs& a, int n_groups, int nh, int
 int attention_shared_launch(const PagedArgs& a, int n_groups, const int* group_start, const int* group_shared,
                             const float* q, int nh, int hd, float* att, void* work, hipStream_t st);
 
+// What is attended by blocks of rows (mxh_blocks.hip): bounds of a layer's blocks,
+// rows of a block (1 << block_shift), and which blocks a token takes
+struct BlocksOf {
+    __half* bounds;
+    int block_shift, n_first, n_last, n_select;
+};
+__host__ __device__ __forceinline__ int64_t blocks_of_table(const PagedArgs& a, int block_shift) {
+    return ((int64_t)a.table_ld << a.page_shift) >> block_shift;
+}
+void block_bounds_launch(const PagedArgs& a, const BlocksOf& b, int hd, hipStream_t st);
+size_t select_blocks_work_bytes(const PagedArgs& a, const BlocksOf& b);
+void select_blocks_launch(const PagedArgs& a, const BlocksOf& b, const float* q, int nh, int hd, int* chosen,
+                          void* work, hipStream_t st);
+size_t attention_blocks_work_bytes(const PagedArgs& a, const BlocksOf& b, int nh, int hd);
+size_t attention_blocks_work_bound(const PagedArgs& a, const BlocksOf& b, int nh, int hd);  // of any batch
+int attention_blocks_launch(const PagedArgs& a, const BlocksOf& b, const int* chosen, const float* q, int nh, int hd,
+                            float* att, void* work, hipStream_t st);
+
 }  // namespace mxh

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../host/mxh_pages.h"
+#include "mxh_blocks.h"
 #include "mxh_device.h"
 #include "mxh_internal.h"
 #include "mxh_paged.h"
@@ -324,6 +325,42 @@ int check_work(const char* who, size_t need, const void* work, size_t work_bytes
     return MXH_OK;
 }
 
+int64_t bounds_elems(const mxh_kv_pool* p, const mxh_kv_blocks* b) {  // of a layer
+    return b->layer_stride ? b->layer_stride
+                           : (int64_t)p->n_pages * (p->page_rows / b->block_rows) * p->n_kv * 2 * p->head_dim;
+}
+
+int check_blocks(const char* who, const mxh_kv_pool* p, const mxh_kv_batch* batch, const mxh_kv_blocks* b, bool bounds) {
+    if (!b) return set_error(MXH_ERR_ARG, "%s: null blocks", who);
+    if (b->block_rows < 16 || b->block_rows > p->page_rows || (b->block_rows & (b->block_rows - 1)))
+        return set_error(MXH_ERR_ARG, "%s: block_rows %d is not a power of two from 16 to page_rows", who,
+                         b->block_rows);
+    if (b->n_select < 1 || b->n_select > kSelectMax)
+        return set_error(MXH_ERR_ARG, "%s: n_select %d is not 1..%d", who, b->n_select, kSelectMax);
+    if ((int64_t)batch->table_ld * (p->page_rows / b->block_rows) > kBlocksMax)
+        return set_error(MXH_ERR_ARG, "%s: rows of %d pages have more than %d blocks", who, batch->table_ld, kBlocksMax);
+    if (!bounds) return MXH_OK;
+    if (!b->bounds || !al16(b->bounds))
+        return set_error(MXH_ERR_ARG, "%s: bounds must be non-null and 16-byte aligned", who);
+    if (b->layer_stride && (b->layer_stride % 8 || b->layer_stride < (int64_t)p->n_pages * (p->page_rows / b->block_rows) *
+                                                                         p->n_kv * 2 * p->head_dim))
+        return set_error(MXH_ERR_ARG, "%s: layer_stride %lld of the bounds is less than a layer or no multiple of 8", who,
+                         (long long)b->layer_stride);
+    return MXH_OK;
+}
+
+int check_budget(const char* who, const mxh_kv_blocks* b) {
+    if (b->n_first < 0 || b->n_last < 1 || (int64_t)b->n_first + b->n_last > b->n_select)
+        return set_error(MXH_ERR_ARG, "%s: the first %d and last %d of %d blocks", who, b->n_first, b->n_last,
+                         b->n_select);
+    return MXH_OK;
+}
+
+BlocksOf blocks_of(const mxh_kv_pool* p, int layer, const mxh_kv_blocks* b) {
+    return BlocksOf{b->bounds ? static_cast<__half*>(b->bounds) + layer * bounds_elems(p, b) : nullptr,
+                    __builtin_ctz((unsigned)b->block_rows), b->n_first, b->n_last, b->n_select};
+}
+
 // marks ids (a bit a page); false where one is marked already
 bool mark_pages(const int* ids, int n, std::vector<uint64_t>& seen) {
     for (int i = 0; i < n; ++i) {
@@ -472,6 +509,87 @@ int mxh_attention_shared(const mxh_kv_pool* pool, int layer, const mxh_kv_batch*
                                          att, work, lib_stream()))
         return set_error(rc, "%s: launch", who);
     return check_hip(hipGetLastError(), "attention_shared launch");
+}
+
+int mxh_kv_block_bounds(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* batch, const mxh_kv_blocks* blocks) {
+    const char* who = "kv_block_bounds";
+    if (int rc = check_step(who, pool, layer, batch, pool ? pool->n_kv : 0)) return rc;
+    if (int rc = check_blocks(who, pool, batch, blocks, true)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    block_bounds_launch(paged_args(pool, layer, batch), blocks_of(pool, layer, blocks), pool->head_dim, lib_stream());
+    return check_hip(hipGetLastError(), "kv_block_bounds launch");
+}
+
+int mxh_kv_select_workspace(const mxh_kv_pool* pool, const mxh_kv_batch* batch, const mxh_kv_blocks* blocks, int nh,
+                            size_t* bytes) {
+    const char* who = "kv_select_workspace";
+    if (!bytes) return set_error(MXH_ERR_ARG, "%s: null output pointer", who);
+    *bytes = 0;
+    if (int rc = check_step(who, pool, 0, batch, nh)) return rc;
+    if (int rc = check_blocks(who, pool, batch, blocks, false)) return rc;
+    if (int rc = check_budget(who, blocks)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    *bytes = select_blocks_work_bytes(paged_args(pool, 0, batch), blocks_of(pool, 0, blocks));
+    return MXH_OK;
+}
+
+int mxh_kv_select_blocks(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* batch, const mxh_kv_blocks* blocks,
+                         const float* q, int nh, int* chosen, void* work, size_t work_bytes) {
+    const char* who = "kv_select_blocks";
+    if (int rc = check_step(who, pool, layer, batch, nh)) return rc;
+    if (int rc = check_blocks(who, pool, batch, blocks, true)) return rc;
+    if (int rc = check_budget(who, blocks)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    if (!q || !chosen || !al16(q) || ((uintptr_t)chosen & 3) || !al16(work))
+        return set_error(MXH_ERR_ARG, "%s: q and chosen must be non-null, q and work aligned to 16 bytes", who);
+    const PagedArgs a = paged_args(pool, layer, batch);
+    const BlocksOf b = blocks_of(pool, layer, blocks);
+    const size_t list = sizeof(int) * (size_t)batch->n_tokens * pool->n_kv * blocks->n_select;
+    if (overlap(q, batch_bytes(pool, batch, nh), chosen, list))
+        return set_error(MXH_ERR_ARG, "%s: chosen overlaps q", who);
+    const size_t need = select_blocks_work_bytes(a, b);
+    if (!work || work_bytes < need)
+        return set_error(MXH_ERR_ARG, "%s: %zu bytes of work, %zu needed", who, work ? work_bytes : 0, need);
+    if (overlap(work, need, q, batch_bytes(pool, batch, nh)) || overlap(work, need, chosen, list))
+        return set_error(MXH_ERR_ARG, "%s: work overlaps q or chosen", who);
+    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    select_blocks_launch(a, b, q, nh, pool->head_dim, chosen, work, lib_stream());
+    return check_hip(hipGetLastError(), "kv_select_blocks launch");
+}
+
+int mxh_attention_blocks_workspace(const mxh_kv_pool* pool, const mxh_kv_batch* batch, const mxh_kv_blocks* blocks,
+                                   int nh, size_t* bytes) {
+    const char* who = "attention_blocks_workspace";
+    if (!bytes) return set_error(MXH_ERR_ARG, "%s: null output pointer", who);
+    *bytes = 0;
+    if (int rc = check_step(who, pool, 0, batch, nh)) return rc;
+    if (int rc = check_blocks(who, pool, batch, blocks, false)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    *bytes = attention_blocks_work_bound(paged_args(pool, 0, batch), blocks_of(pool, 0, blocks), nh, pool->head_dim);
+    return MXH_OK;
+}
+
+int mxh_attention_blocks(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* batch, const mxh_kv_blocks* blocks,
+                         const int* chosen, const float* q, int nh, float* att, void* work, size_t work_bytes) {
+    const char* who = "attention_blocks";
+    if (int rc = check_step(who, pool, layer, batch, nh)) return rc;
+    if (int rc = check_blocks(who, pool, batch, blocks, false)) return rc;
+    if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    if (int rc = check_attention(who, pool, batch, q, nh, att, work)) return rc;
+    const size_t list = sizeof(int) * (size_t)batch->n_tokens * pool->n_kv * blocks->n_select;
+    if (!chosen || ((uintptr_t)chosen & 3) || overlap(chosen, list, att, batch_bytes(pool, batch, nh)))
+        return set_error(MXH_ERR_ARG, "%s: chosen is null, not aligned, or overlaps att", who);
+    if (!mxh_is_available()) return MXH_ERR_NODEV;
+    const PagedArgs a = paged_args(pool, layer, batch);
+    const BlocksOf b = blocks_of(pool, layer, blocks);
+    const size_t need = attention_blocks_work_bytes(a, b, nh, pool->head_dim);
+    if (int rc = check_work(who, need, work, work_bytes, q, att, batch_bytes(pool, batch, nh))) return rc;
+    if (need && overlap(work, need, chosen, list)) return set_error(MXH_ERR_ARG, "%s: work overlaps chosen", who);
+    if (int rc = attention_blocks_launch(a, b, chosen, q, nh, pool->head_dim, att, work, lib_stream()))
+        return set_error(rc, "%s: launch", who);
+    return check_hip(hipGetLastError(), "attention_blocks launch");
 }
 
 int mxh_kv_copy_pages(const mxh_kv_pool* pool, const int* src, const int* dst, int n) try {

@@ -234,55 +234,24 @@ struct SharedMergeArgs {
     int nkv, group, rows_p, rows_s;
 };
 
-// att from each token's parts.  A thread has four dims of a head of a token and
-// every kMergeLanes-th part.
-constexpr int kMergeThreads = 256, kMergeLanes = 4;
+// att from each token's parts
 template <int HD>
-__global__ __launch_bounds__(kMergeThreads) void shared_merge_kernel(SharedMergeArgs a) {
-    constexpr int UNITS = kMergeThreads / kMergeLanes, AHEAD = 4;
-    __shared__ float4 acc[kMergeThreads];
-    __shared__ float2 st[kMergeThreads];
-    const int tid = threadIdx.x, lane = tid / UNITS;
-    const int64_t u = (int64_t)blockIdx.x * UNITS + tid % UNITS;
+__global__ __launch_bounds__(kJoinThreads) void shared_merge_kernel(SharedMergeArgs a) {
+    const int64_t u = (int64_t)blockIdx.x * kJoinUnits + threadIdx.x % kJoinUnits;
     const int64_t head = min(u, a.total - 1) / (HD / 4);
     const int d = 4 * (int)(u % (HD / 4)), nh = a.nkv * a.group;
     const int64_t t = head / nh;
     const int hq = (int)(head - t * nh), g = hq / a.group, hg = hq - g * a.group;
     const int4 own = a.records[2 * t], pre = a.records[2 * t + 1];
     const bool any = u < a.total && own.z >= 0 && own.z + pre.z > 0;  // (else: no sequence's, or done)
-    const int parts = any ? own.z + pre.z : 0;
-    float M = -INFINITY, L = 0.f;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    const auto join = [&](float2 x, float4 v) __attribute__((always_inline)) {
-        if (x.y == 0.f) return;  // (nothing attended there)
-        const float m1 = fmaxf(M, x.x), a0 = __builtin_amdgcn_exp2f(M - m1), a1 = __builtin_amdgcn_exp2f(x.x - m1);
-        M = m1;
-        L = L * a0 + x.y * a1;
-        s.x = s.x * a0 + v.x * a1, s.y = s.y * a0 + v.y * a1, s.z = s.z * a0 + v.z * a1, s.w = s.w * a0 + v.w * a1;
+    const auto where = [&](int z, float2& x, float4& v) __attribute__((always_inline)) {
+        const bool p = z < pre.z;
+        const int64_t slot = p ? pre.x + (int64_t)z * pre.y : own.x + (int64_t)(z - pre.z) * own.y;
+        const int64_t at = (slot * a.nkv + g) * (p ? a.rows_p : a.rows_s) + (p ? pre.w : own.w) + hg;
+        x = (p ? a.ml_p : a.ml_s)[at];
+        v = *reinterpret_cast<const float4*>((p ? a.part_p : a.part_s) + at * HD + d);
     };
-    for (int z0 = lane; z0 < parts; z0 += AHEAD * kMergeLanes) {
-        float2 x[AHEAD];
-        float4 v[AHEAD];
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int z = min(z0 + i * kMergeLanes, parts - 1);
-            const bool p = z < pre.z;
-            const int64_t slot = p ? pre.x + (int64_t)z * pre.y : own.x + (int64_t)(z - pre.z) * own.y;
-            const int64_t at = (slot * a.nkv + g) * (p ? a.rows_p : a.rows_s) + (p ? pre.w : own.w) + hg;
-            x[i] = (p ? a.ml_p : a.ml_s)[at];
-            v[i] = *reinterpret_cast<const float4*>((p ? a.part_p : a.part_s) + at * HD + d);
-        }
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (z0 + i * kMergeLanes < parts) join(x[i], v[i]);
-    }
-    acc[tid] = s;
-    st[tid] = make_float2(M, L);
-    __syncthreads();
-    if (lane || !any) return;
-    for (int i = 1; i < kMergeLanes; ++i) join(st[tid + i * UNITS], acc[tid + i * UNITS]);
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-    *reinterpret_cast<float4*>(a.att + head * HD + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+    join_parts(own.z + pre.z, where, any ? a.att + head * HD + d : nullptr);
 }
 
 PagedSize shared_size(const PagedArgs& a, int nh) {
@@ -311,10 +280,10 @@ int launch_hd(const SharedArgs& a, const SharedShape& sh, hipStream_t st) {
                    : sh.rows_p == 64 ? launch<HD, 64, 16>(a, sh, st)
                                      : launch<HD, 16, 16>(a, sh, st);
     if (rc) return rc;
-    const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4), units = kMergeThreads / kMergeLanes;
+    const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4), units = kJoinUnits;
     const SharedMergeArgs m{a.records, a.t.part, a.part_s, a.t.ml, a.ml_s, a.t.att, total, a.t.pg.nkv,
                             (int)a.t.group, sh.rows_p, sh.rows_s};
-    hipLaunchKernelGGL(shared_merge_kernel<HD>, dim3((unsigned)((total + units - 1) / units)), dim3(kMergeThreads), 0,
+    hipLaunchKernelGGL(shared_merge_kernel<HD>, dim3((unsigned)((total + units - 1) / units)), dim3(kJoinThreads), 0,
                        st, m);
     return MXH_OK;
 }

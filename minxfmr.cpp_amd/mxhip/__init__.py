@@ -89,6 +89,19 @@ class KvGroups(C.Structure):
         self.buffers = start, shared
 
 
+class KvBlocks(C.Structure):
+    """Blocks of rows, their bounds in HBM (by buffer or address; None where no call reads or writes them) and how many
+    a token takes (mxh_kv_blocks).  The buffer lives as long as this does."""
+
+    _fields_ = [("bounds", C.c_void_p), ("layer_stride", C.c_int64)] + \
+               [(n, C.c_int) for n in ("block_rows", "n_first", "n_last", "n_select")]
+
+    def __init__(self, bounds, *, block_rows: int, n_first: int = 0, n_last: int = 1, n_select: int = 1,
+                 layer_stride: int = 0):
+        super().__init__(addr(bounds), layer_stride, block_rows, n_first, n_last, n_select)
+        self.buffers = bounds
+
+
 def addr(b):
     """The device address of a DeviceBuffer, or an address as it is (None: null)."""
     return b.ptr if isinstance(b, DeviceBuffer) else b
@@ -155,6 +168,11 @@ def _load() -> C.CDLL:
         "mxh_attention_paged_workspace": (ip, [vp, vp, ip, C.POINTER(sz)]),
         "mxh_attention_shared": (ip, [vp, ip, vp, vp, vp, ip, vp, vp, sz]),
         "mxh_attention_shared_workspace": (ip, [vp, vp, vp, ip, C.POINTER(sz)]),
+        "mxh_kv_block_bounds": (ip, [vp, ip, vp, vp]),
+        "mxh_kv_select_blocks": (ip, [vp, ip, vp, vp, vp, ip, vp, vp, sz]),
+        "mxh_kv_select_workspace": (ip, [vp, vp, vp, ip, C.POINTER(sz)]),
+        "mxh_attention_blocks": (ip, [vp, ip, vp, vp, vp, vp, ip, vp, vp, sz]),
+        "mxh_attention_blocks_workspace": (ip, [vp, vp, vp, ip, C.POINTER(sz)]),
         "mxh_kv_copy_pages": (ip, [vp, vp, vp, ip]),
         "mxh_kv_keep_rows": (ip, [vp, vp, ip, vp, vp, vp, ip]),
         "mxh_pages_create": (ip, [ip, ip, ip, C.POINTER(vp)]),
@@ -188,7 +206,9 @@ EXPORTED = (
     "mxh_qk_rope_append mxh_attention_paged mxh_attention_paged_workspace mxh_kv_copy_pages mxh_kv_keep_rows "
     "mxh_pages_create mxh_pages_destroy mxh_pages_open mxh_pages_fork mxh_pages_close mxh_pages_extend "
     "mxh_pages_set_length mxh_pages_length mxh_pages_free mxh_pages_table "
-    "mxh_attention_shared mxh_attention_shared_workspace mxh_pages_common"
+    "mxh_attention_shared mxh_attention_shared_workspace mxh_pages_common "
+    "mxh_kv_block_bounds mxh_kv_select_blocks mxh_kv_select_workspace mxh_attention_blocks "
+    "mxh_attention_blocks_workspace"
 ).split()
 
 
@@ -323,6 +343,41 @@ def attention_shared(pool: KvPool, layer: int, batch: KvBatch, groups: KvGroups,
     """attention_paged with the rows that groups of sequences have in common read once for each group."""
     check(lib.mxh_attention_shared(C.byref(pool), layer, C.byref(batch), C.byref(groups), addr(q), nh, addr(att),
                                    addr(work), work_bytes), "mxh_attention_shared")
+
+
+def kv_block_bounds(pool: KvPool, layer: int, batch: KvBatch, blocks: KvBlocks) -> None:
+    """The least and greatest keys of the blocks in which the batch's new rows lie."""
+    check(lib.mxh_kv_block_bounds(C.byref(pool), layer, C.byref(batch), C.byref(blocks)), "mxh_kv_block_bounds")
+
+
+def kv_select_workspace(pool: KvPool, batch: KvBatch, blocks: KvBlocks, nh: int) -> int:
+    """Bytes of work that kv_select_blocks needs for batches of this n_tokens and table_ld."""
+    n = C.c_size_t()
+    check(lib.mxh_kv_select_workspace(C.byref(pool), C.byref(batch), C.byref(blocks), nh, C.byref(n)),
+          "mxh_kv_select_workspace")
+    return n.value
+
+
+def kv_select_blocks(pool: KvPool, layer: int, batch: KvBatch, blocks: KvBlocks, q, nh: int, chosen, work,
+                     work_bytes: int) -> None:
+    """For each token and kv head the first, the last and the most promising blocks, ascending, -1 behind them."""
+    check(lib.mxh_kv_select_blocks(C.byref(pool), layer, C.byref(batch), C.byref(blocks), addr(q), nh, addr(chosen),
+                                   addr(work), work_bytes), "mxh_kv_select_blocks")
+
+
+def attention_blocks_workspace(pool: KvPool, batch: KvBatch, blocks: KvBlocks, nh: int) -> int:
+    """Bytes of work that attention_blocks needs for any batch."""
+    n = C.c_size_t()
+    check(lib.mxh_attention_blocks_workspace(C.byref(pool), C.byref(batch), C.byref(blocks), nh, C.byref(n)),
+          "mxh_attention_blocks_workspace")
+    return n.value
+
+
+def attention_blocks(pool: KvPool, layer: int, batch: KvBatch, blocks: KvBlocks, chosen, q, nh: int, att, work=None,
+                     work_bytes: int = 0) -> None:
+    """attention_paged over the rows of the chosen blocks alone."""
+    check(lib.mxh_attention_blocks(C.byref(pool), layer, C.byref(batch), C.byref(blocks), addr(chosen), addr(q), nh,
+                                   addr(att), addr(work), work_bytes), "mxh_attention_blocks")
 
 
 def _ints(a) -> np.ndarray:
