@@ -55,13 +55,15 @@ inline size_t block_work_bound(const BlockSize& a, int hd) {
     return stages < 4 ? 0 : block_part_bytes(std::max<int64_t>(2, 2 * (int64_t)a.cus / a.nkv), a.nkv, hd);
 }
 
-// Selecting: tokens whose scores the workspace holds at a time
+// Selecting: scores of a token and kv head (whole tiles of 16 blocks), and tokens whose
+// scores the workspace holds at a time
+inline int64_t select_row(int64_t n_blocks) { return (n_blocks + 15) / 16 * 16; }
 inline int64_t select_tokens(int n_tokens, int64_t n_blocks, int nkv) {
-    const int64_t row = n_blocks * nkv * 8;
+    const int64_t row = select_row(n_blocks) * nkv * 8;
     return std::min<int64_t>(n_tokens, std::max<int64_t>(16, ((256 << 20) / row) / 16 * 16));
 }
 inline size_t select_work_bytes(int n_tokens, int64_t n_blocks, int nkv) {
-    return (size_t)select_tokens(n_tokens, n_blocks, nkv) * (size_t)(n_blocks * nkv) * 8;
+    return (size_t)select_tokens(n_tokens, n_blocks, nkv) * (size_t)(select_row(n_blocks) * nkv) * 8;
 }
 
 }  // namespace mxh

@@ -117,12 +117,18 @@ __device__ __forceinline__ uint64_t order_key(double x) {
     return u ^ (u >> 63 ? ~0ull : 1ull << 63);
 }
 
+// A block's score so far, in units of the token's and kv head's own, and how far it
+// may be off; of an absent block -infinity and 0
+struct Score {
+    float s, off;
+};
 struct SelectArgs {
     BlockArgs b;
     const float* q;
     int nh, group, tokens;  // q heads of a kv head; tokens of a tile
     int t0, t1;             // tokens of this launch
-    uint64_t* keys;         // [t1 - t0][nkv][n_blocks]
+    int ld;                 // scores of a row, n_blocks and up to a multiple of 16
+    Score* scores;          // [t1 - t0][nkv][ld]
     int* chosen;            // [n_tokens][nkv][n_select]
 };
 
@@ -138,20 +144,191 @@ __device__ __forceinline__ Rivals rivals(const BlockArgs& a, const TokenAt& x) {
     return r;
 }
 
-// Workgroup (64 `iters` blocks, kv head, tile of tokens): a wave takes 16 blocks
-// and the tile's 16 rows of q at a time, v_mfma_f64_16x16x4_f64: in 64 bits the
-// choice depends neither on how the work is split nor on the order of sums.
-constexpr int kScoreThreads = 256;
-typedef double f64x4 __attribute__((ext_vector_type(4)));
+// max over the q heads of a kv head, in the lane of its first: lanes m .. m + group - 1
+// of a row of 16.  (Two instructions a value for group 4, six as C++; a lane's value
+// may be read by its neighbours two instructions after it was written.)
+#define MXH_MAX4(PERM)                                                                                        \
+    asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 " PERM " row_mask:0xf bank_mask:0xf"                             \
+        "\n\tv_max_f32_dpp %1, %1, %1 " PERM " row_mask:0xf bank_mask:0xf"                                    \
+        "\n\tv_max_f32_dpp %2, %2, %2 " PERM " row_mask:0xf bank_mask:0xf"                                    \
+        "\n\tv_max_f32_dpp %3, %3, %3 " PERM " row_mask:0xf bank_mask:0xf"                                    \
+        : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w))
+__device__ __forceinline__ void heads_max(float4& v, int group) {
+    if ((group & (group - 1)) == 0) {
+        if (group >= 2) MXH_MAX4("quad_perm:[1,0,3,2]");  // the other of a pair
+        if (group >= 4) MXH_MAX4("quad_perm:[2,3,0,1]");  // of a quad's pairs
+        if (group >= 8) MXH_MAX4("row_half_mirror");      // of eight lanes' quads
+        return;
+    }
+    const float4 o = v;
+    for (int h = 1; h < group; ++h) {
+        v.x = fmaxf(v.x, __shfl_down(o.x, (unsigned)h)), v.y = fmaxf(v.y, __shfl_down(o.y, (unsigned)h));
+        v.z = fmaxf(v.z, __shfl_down(o.z, (unsigned)h)), v.w = fmaxf(v.w, __shfl_down(o.w, (unsigned)h));
+    }
+}
+#undef MXH_MAX4
+
+// Scores on the fp16 matrix cores, 16 blocks and the 16 rows of q of a tile of
+// tokens at a time, v_mfma_f32_16x16x32_f16: least | greatest of a block as they lie
+// there times min(q, 0) | max(q, 0), q in fp16 after the power of two that brings the
+// largest |q| of the token's kv head to [2^13, 2^14).
+//
+// What the sums may be off by: q by 2^-11 of itself and 2^-25, and up to 256
+// additions, each by 2^-23 of the sum of the magnitudes at most (were they cut
+// off).  A second product sums magnitudes, with |q| raised to 2^-3 where it is less,
+// so that 1.25 x 2^-11 of it is over all of that; block_pick_kernel decides what that
+// leaves open in 64 bits, some five blocks of a thousand.  (All scores in 64 bits,
+// v_mfma_f64_16x16x4_f64: 125 us for 512 tokens at 30,000 rows, 26 now, and 60 for 48
+// single tokens at up to 16,000, 18 now.)
+// magnitudes of halves (the sign bits of pairs at a time), and an eighth at least (as
+// integers: a maximum of halves costs an instruction more for every operand)
+__device__ __forceinline__ f16x8 magnitudes(f16x8 v) {
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(f16x8, __builtin_bit_cast(words, v) & 0x7fff7fffu);
+}
+__device__ __forceinline__ f16x8 at_least(f16x8 v, uint32_t eighth) {
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    const u16x8 y = (uint16_t)eighth;
+    return __builtin_bit_cast(f16x8, __builtin_elementwise_max(__builtin_bit_cast(u16x8, magnitudes(v)), y));
+}
+
+// SIZES: whether the magnitudes of q stay in registers
+template <int HD, bool SIZES>
+struct ScoreTile {
+    static constexpr int KS = HD / 16;  // products
+    f16x8 q[KS], q_size[SIZES ? KS : 1];
+    // the largest sum of magnitudes of a lane's column, as bits: those of infinity and
+    // above where scores are no numbers; odd: whether those of any block are
+    uint32_t size, odd;
+    // column m of the tile: token first + m / group, q head m % group; lane: dims
+    // 32 i + 8 kk + e
+    __device__ __forceinline__ void stage(const SelectArgs& a, int first, int last, int g, int m, int kk) {
+        const int u = m / a.group, tt = first + u;
+        const bool there = u < a.tokens && tt < last;
+        const float* row =
+            a.q + ((int64_t)(there ? tt : min(first, a.t1 - 1)) * a.nh + g * a.group + (there ? m % a.group : 0)) * HD;
+        const auto at = [&](int i, int e) { return *reinterpret_cast<const float4*>(row + 32 * i + 8 * kk + e); };
+        uint32_t big = 0;  // the largest magnitude's bits; past those of infinity where there is a NaN
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 y = at(i, e);
+                big = max(max(big, max(__float_as_uint(y.x) << 1, __float_as_uint(y.y) << 1)),
+                          max(__float_as_uint(y.z) << 1, __float_as_uint(y.w) << 1));
+            }
+        big = there ? big : 0;
+        big = max(big, __float_as_uint(lane_xor<16>(__uint_as_float(big))));
+        big = max(big, __float_as_uint(lane_xor<32>(__uint_as_float(big))));
+        const int c0 = u * a.group;     // the kv head's columns of the token
+        uint32_t most = 0;
+        for (int h = 0; h < a.group; ++h) most = max(most, (uint32_t)__shfl((int)big, min(c0 + h, 15)));
+        size = odd = most < 0xff000000u ? 0u : 0x7f800000u;
+        const int f = min(14 - __builtin_amdgcn_frexp_expf(__uint_as_float(most >> 1)), 120);
+        const float scale = there && odd == 0 ? __uint_as_float((uint32_t)(127 + f) << 23) : 0.f;
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 y = at(i, e);
+                const f16x2 z[2] = {__builtin_convertvector((f32x2{y.x * scale, y.y * scale}), f16x2),
+                                    __builtin_convertvector((f32x2{y.z * scale, y.w * scale}), f16x2)};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {  // least with min(q, 0), greatest with max(q, 0)
+                    const f16x2 none = {0, 0}, neg = __builtin_elementwise_min(z[c], none),
+                                pos = __builtin_elementwise_max(z[c], none);
+                    q[i][e + 2 * c] = neg[0], q[i][e + 2 * c + 1] = neg[1];
+                    q[KS / 2 + i][e + 2 * c] = pos[0], q[KS / 2 + i][e + 2 * c + 1] = pos[1];
+                }
+            }
+        if constexpr (SIZES)
+#pragma unroll
+            for (int i = 0; i < KS; ++i) q_size[i] = at_least(q[i], 0x3000);
+    }
+    // bounds(i): lane's 8 of block m of 16.  The scores of the tile's token u, the largest
+    // of its q heads', go to to[u stride], 16
+    template <class Bounds>
+    __device__ __forceinline__ void score(const SelectArgs& a, const Bounds& bounds, int place, float* to, int stride,
+                                          int m, int kk) {
+        f32x4 s = {0.f, 0.f, 0.f, 0.f}, sum = s;
+        uint32_t eighth = 0x3000;
+        if constexpr (!SIZES) asm volatile("" : "+v"(eighth));  // (else the magnitudes of q stay in registers)
+        constexpr int BATCH = KS < 4 ? KS : 4;
+        f16x8 v[BATCH];
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            if (i % BATCH == 0)
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) v[k] = bounds(i + k);
+            s = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[i % BATCH], q[i], s, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                magnitudes(v[i % BATCH]), SIZES ? q_size[SIZES ? i : 0] : at_least(q[i], eighth), sum, 0, 0, 0);
+        }
+        // lane: column m, blocks 4 kk + r.  (Absent ones' bounds are zeros, their sums too)
+        const uint32_t gone = (uint32_t)__ballot(place < 0) >> (4 * kk);
+        float4 x;
+        x.x = gone & 1 ? -INFINITY : s[0], x.y = gone & 2 ? -INFINITY : s[1];
+        x.z = gone & 4 ? -INFINITY : s[2], x.w = gone & 8 ? -INFINITY : s[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) size = max(size, __float_as_uint(sum[r]));
+        heads_max(x, a.group);
+        if (m % a.group == 0 && m / a.group < a.tokens) *reinterpret_cast<float4*>(to + m / a.group * stride + 4 * kk) = x;
+    }
+    // The scores of tokens [t, stop) of the tile, `steps` of 16 blocks b0 + apart j, out
+    // of LDS (`kept`, as score left them), with what they are off by
+    __device__ __forceinline__ void flush(const SelectArgs& a, const float* kept, int stride, int steps, int b0, int apart,
+                                          int first, int t, int stop, int g, int lane) {
+        float off = size < 0x7f800000u ? __uint_as_float(size) * (1.25f / 2048.f) : INFINITY;
+        off = fmaxf(off, lane_xor<16>(off));
+        off = fmaxf(off, lane_xor<32>(off));
+        size = odd;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+        for (int tt = t; tt < stop; ++tt) {
+            const int u = tt - first;
+            float far = 0.f;
+            for (int h = 0; h < a.group; ++h) far = fmaxf(far, __shfl(off, u * a.group + h));
+            Score* row = a.scores + ((int64_t)(tt - a.t0) * a.b.pg.nkv + g) * a.ld;
+            for (int i = lane; i < 16 * steps; i += 64) {
+                const float s = kept[u * stride + i];
+                row[b0 + apart * (i >> 4) + (i & 15)] = Score{s, s > -INFINITY ? far : 0.f};
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+
+// the lane's pieces of a block's bounds, of head g: every fourth 16 bytes from there
+__device__ uint4 no_bounds[2 * 128 / 8];  // (of absent blocks: zeros)
 template <int HD>
-__global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a, int iters, int chunks) {
-    constexpr int STEPS = HD / 2;  // products; a lane's halves of a block's bounds
-    __shared__ double qs[STEPS * 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, kk = lane >> 4;
-    const int nkv = a.b.pg.nkv;
-    const int chunk = (int)(blockIdx.x % chunks), g = (int)(blockIdx.x / chunks % nkv);
-    const int first = a.t0 + (int)(blockIdx.x / chunks / nkv) * a.tokens, last = min(first + a.tokens, a.t1);
-    const int lo = chunk * 64 * iters;
+__device__ __forceinline__ const half8* bounds_at(const SelectArgs& a, int place, int g, int kk) {
+    const half8* p = reinterpret_cast<const half8*>(a.b.bounds) + ((int64_t)place * a.b.pg.nkv + g) * (HD / 4);
+    return (place < 0 ? reinterpret_cast<const half8*>(no_bounds) : p) + kk;
+}
+
+// Places of `steps` times 16 blocks, b0 + apart j, of a wave's, into LDS before the
+// loop that reads them: a table load in there would have every step wait for it
+__device__ __forceinline__ void find_places(const SelectArgs& a, int s, int b0, int apart, int steps, int* places, int lane) {
+    for (int i = lane; i < 16 * steps; i += 64) places[i] = (int)block_place(a.b, s, b0 + apart * (i >> 4) + (i & 15));
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Few tokens: a workgroup takes a tile, its waves different blocks (16 `iters` each).
+constexpr int kScoreThreads = 256, kScoreWaves = 4;
+template <int HD>
+__global__ __launch_bounds__(kScoreThreads, 3) void block_score_kernel(SelectArgs a, int iters, int chunks) {
+    extern __shared__ __align__(16) float kept_lds[];  // [waves][tokens][16 iters], places [waves][16 iters]
+    constexpr int KS = ScoreTile<HD, false>::KS, STEP = 16 * kScoreWaves;
+    const int lane = threadIdx.x & 63, m = lane & 15, kk = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), nkv = a.b.pg.nkv;
+    const int chunk = (int)(blockIdx.x % chunks), rest = (int)(blockIdx.x / chunks), g = rest % nkv, tile = rest / nkv;
+    const int first = a.t0 + tile * a.tokens, last = min(first + a.tokens, a.t1);
+    const int lo = max(chunk * iters * STEP, a.b.n_first & ~15) + 16 * wave, top = (chunk + 1) * iters * STEP;
+    float* kept = kept_lds + wave * a.tokens * 16 * iters;
+    int* places = reinterpret_cast<int*>(kept_lds + kScoreWaves * a.tokens * 16 * iters) + wave * 16 * iters;
+    ScoreTile<HD, false> st;
     bool staged = false;
     for (int t = first; t < last;) {
         const TokenAt x = token_at(a.b.pg, t);
@@ -160,62 +337,141 @@ __global__ __launch_bounds__(kScoreThreads) void block_score_kernel(SelectArgs a
             continue;
         }
         const int stop = min(t - x.i + x.n, last);  // the run of this sequence's tokens
-        const int hi = rivals(a.b, TokenAt{x.s, x.i + stop - 1 - t, x.cached, x.n}).end;
+        const int hi = min(rivals(a.b, TokenAt{x.s, x.i + stop - 1 - t, x.cached, x.n}).end, top);
         if (hi > lo) {
-            if (!staged) {
-                // column c of the tile: token c / group, q head c % group
-                for (int i = tid; i < STEPS * 64; i += kScoreThreads) {
-                    const int c = i & 15, e = (i >> 4 & 3) * STEPS + (i >> 6), tt = first + c / a.group;
-                    float v = 0.f;
-                    if (c < a.tokens * a.group && tt < last) {
-                        v = a.q[((int64_t)tt * a.nh + g * a.group + c % a.group) * HD + e % HD];
-                        v = e < HD ? (v >= 0.f ? 0.f : v) : (v <= 0.f ? 0.f : v);
-                    }
-                    qs[i] = v;
-                }
-                __syncthreads();
-                staged = true;
+            const int steps = (hi - lo + STEP - 1) / STEP;
+            find_places(a, x.s, lo, STEP, steps, places, lane);
+            int place = places[m];
+            half8 v[KS];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) v[i] = bounds_at<HD>(a, place, g, kk)[4 * i];
+            if (!staged) st.stage(a, first, last, g, m, kk), staged = true;
+            for (int j = 0; j < steps; ++j) {
+                const int place_next = places[16 * min(j + 1, steps - 1) + m];
+                const half8* p = bounds_at<HD>(a, place_next, g, kk);
+                const auto bounds = [&](int i) __attribute__((always_inline)) {
+                    const f16x8 y = v[i];
+                    v[i] = p[4 * i];  // the next step's
+                    return y;
+                };
+                st.score(a, bounds, place, kept + 16 * j, 16 * iters, m, kk);
+                place = place_next;
             }
-            for (int b0 = lo + 16 * wave; b0 < min(lo + 64 * iters, hi); b0 += 64) {
-                const int64_t place = block_place(a.b, x.s, b0 + m);
-                half8 v[STEPS / 8];
-#pragma unroll
-                for (int i = 0; i < STEPS / 8; ++i) {
-                    const half8* p = reinterpret_cast<const half8*>(a.b.bounds + ((place < 0 ? 0 : place) * nkv + g) * 2 * HD +
-                                                                    kk * STEPS);
-                    v[i] = p[i];
-                }
-                f64x4 acc = {0., 0., 0., 0.};
-#pragma unroll
-                for (int i = 0; i < STEPS; ++i)
-                    acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)v[i / 8][i % 8], qs[64 * i + lane], acc, 0,
-                                                               0, 0);
-                // lane: column m, blocks b0 + 4 r + kk
-                const uint64_t gone = __ballot(place < 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    double best = acc[r];
-                    for (int h = 1; h < a.group; ++h) {
-                        const double o = __shfl(acc[r], min(lane + h, 63));
-                        best = o > best || o != o ? o : best;
-                    }
-                    const int b = b0 + 4 * r + kk, tt = first + m / a.group;
-                    if (gone >> (4 * r + kk) & 1) best = -INFINITY;
-                    if (m % a.group == 0 && tt >= t && tt < stop && b < hi)
-                        a.keys[((int64_t)(tt - a.t0) * nkv + g) * a.b.n_blocks + b] = order_key(best);
-                }
-            }
+            st.flush(a, kept, 16 * iters, steps, lo, STEP, first, t, stop, g, lane);
         }
         t = stop;
     }
 }
 
-// Workgroup (token, kv head): the n-th largest key, eight bits at a time, then the
-// blocks from there on in their order.
-constexpr int kPickThreads = 256;
-__global__ __launch_bounds__(kPickThreads) void block_pick_kernel(SelectArgs a) {
-    __shared__ uint32_t bins[256], wsum[kPickThreads / 64];
-    __shared__ uint32_t found[2];  // the bin, keys wanted of it
+// Many tokens: a workgroup takes four tiles, a wave each, and 16 `iters` blocks, whose
+// bounds the waves bring into LDS together, two steps ahead in registers.
+template <int HD>
+__global__ __launch_bounds__(kScoreThreads, 2) void block_score_rows_kernel(SelectArgs a, int iters, int chunks) {
+    extern __shared__ __align__(16) float kept_lds[];  // [waves][tokens][16 iters], places [waves][16 iters]
+    constexpr int KS = ScoreTile<HD, true>::KS, OWN = KS < kScoreWaves ? 1 : KS / kScoreWaves;  // pieces a wave brings
+    __shared__ half8 ring[2][KS][64];
+    const int lane = threadIdx.x & 63, m = lane & 15, kk = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), nkv = a.b.pg.nkv;
+    const int chunk = (int)(blockIdx.x % chunks), rest = (int)(blockIdx.x / chunks), g = rest % nkv, tile = rest / nkv;
+    const int first = a.t0 + kScoreWaves * tile * a.tokens, last = min(first + kScoreWaves * a.tokens, a.t1);
+    const int mine = first + wave * a.tokens;  // the wave's first token
+    const int lo = max(chunk * iters * 16, a.b.n_first & ~15), top = (chunk + 1) * iters * 16;
+    const int piece0 = min(wave * OWN, KS - OWN);  // (HD = 32: waves that bring a piece again)
+    float* kept = kept_lds + wave * a.tokens * 16 * iters;
+    int* places = reinterpret_cast<int*>(kept_lds + kScoreWaves * a.tokens * 16 * iters) + wave * 16 * iters;
+    ScoreTile<HD, true> st;
+    bool staged = false;
+    for (int t = first; t < last;) {  // (all waves together)
+        const TokenAt x = token_at(a.b.pg, t);
+        if (x.s < 0) {
+            ++t;
+            continue;
+        }
+        const int stop = min(t - x.i + x.n, last);
+        const int hi = min(rivals(a.b, TokenAt{x.s, x.i + stop - 1 - t, x.cached, x.n}).end, top);
+        if (hi > lo) {
+            const int steps = (hi - lo + 15) >> 4;
+            find_places(a, x.s, lo, 16, steps, places, lane);
+            // step `at`'s place and pieces, steps in their order (past the last the last's again)
+            int at = 0;
+            const auto fetch = [&](half8 (&v)[OWN]) __attribute__((always_inline)) {
+                const int place = places[16 * min(at++, steps - 1) + m];
+                const half8* p = bounds_at<HD>(a, place, g, kk);
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) v[i] = p[4 * (piece0 + i)];
+                return place;
+            };
+            const auto keep = [&](const half8 (&v)[OWN], int slot) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) ring[slot][piece0 + i][lane] = v[i];
+            };
+            half8 v0[OWN], v1[OWN], v2[OWN];
+            int place = fetch(v0), place1 = fetch(v1), place2 = fetch(v2);
+            if (!staged) st.stage(a, mine, min(mine + a.tokens, a.t1), g, m, kk), staged = true;
+            keep(v0, 0);
+            __syncthreads();
+            int j = 0;
+            // Three steps by name: registers that loads are on their way to cannot be moved.
+            // (And all three each time, past the last one too, unused: with ways out in
+            // between every round began by waiting for all loads.)
+            const auto step = [&](half8 (&into)[OWN], const half8 (&next)[OWN]) __attribute__((always_inline)) {
+                const int place3 = fetch(into);
+                const auto bounds = [&](int i) __attribute__((always_inline)) { return ring[j & 1][i][lane]; };
+                st.score(a, bounds, place, kept + 16 * j, 16 * iters, m, kk);
+                ++j;
+                keep(next, j & 1);
+                place = place1, place1 = place2, place2 = place3;
+                __syncthreads();
+            };
+            while (j < steps) step(v0, v1), step(v1, v2), step(v2, v0);
+            st.flush(a, kept, 16 * iters, steps, lo, 16, mine, max(t, mine), min(stop, min(mine + a.tokens, a.t1)), g, lane);
+        }
+        t = stop;
+    }
+}
+
+// A block's score in 64 bits, by 16 lanes (in all of them); q: the kv head's q heads
+template <int HD>
+__device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, int g, const float* q, int group) {
+    constexpr int PER = HD / 16;
+    typedef _Float16 piece __attribute__((ext_vector_type(PER)));
+    typedef float qpiece __attribute__((ext_vector_type(PER)));
+    const int d = (threadIdx.x & 15) * PER;
+    const int64_t place = block_place(a, s, b);
+    const __half* p = a.bounds + (max(place, (int64_t)0) * a.pg.nkv + g) * 2 * HD + d;
+    const piece least = *reinterpret_cast<const piece*>(p), greatest = *reinterpret_cast<const piece*>(p + HD);
+    double best = -INFINITY;
+    for (int h = 0; h < group; ++h) {
+        const qpiece y = *reinterpret_cast<const qpiece*>(q + h * HD + d);
+        double sum = 0.;
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            sum += (double)(y[e] <= 0.f ? 0.f : y[e]) * (double)greatest[e] +
+                   (double)(y[e] >= 0.f ? 0.f : y[e]) * (double)least[e];
+        sum += dpp_d<0xb1>(sum);  // over the row of 16 lanes
+        sum += dpp_d<0x4e>(sum);
+        sum += dpp_d<0x141>(sum);
+        sum += dpp_d<0x140>(sum);
+        best = best != best ? best : sum > best || sum != sum ? sum : best;
+    }
+    return place < 0 ? -INFINITY : best;
+}
+
+// Workgroup (token, kv head).  The scores' range in equal bins; the bin that the
+// n-th largest falls into; what lies above it by more than scores are off is taken,
+// what lies below by as much is not, and the few in between are ordered by their
+// scores in 64 bits.  Where they are not few, or scores are not finite, all of them
+// are, eight bits of the n-th largest at a time.
+constexpr int kPickThreads = 256, kPickBins = 512, kPickKeys = 4096, kOpenMax = 128;
+template <int HD>
+__global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs a) {
+    constexpr int WAVES = kPickThreads / 64;
+    __shared__ uint32_t bins[kPickBins], wsum[WAVES];
+    __shared__ float red[WAVES][3];
+    extern __shared__ float keys_lds[];  // [kPickKeys], of n_blocks at most
+    __shared__ uint32_t found[2], n_open, n_above;  // a bin, keys wanted of it; blocks that are open, taken
+    __shared__ int open[kOpenMax];
+    __shared__ uint64_t open_key[kOpenMax];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nkv = a.b.pg.nkv;
     const int t = a.t0 + (int)(blockIdx.x / nkv), g = (int)(blockIdx.x % nkv);
     const TokenAt x = token_at(a.b.pg, t);
@@ -226,36 +482,143 @@ __global__ __launch_bounds__(kPickThreads) void block_pick_kernel(SelectArgs a) 
         for (int i = tid; i < a.b.n_select; i += kPickThreads) out[i] = i <= r.own ? i : -1;
         return;
     }
-    const int n0 = a.b.n_first, want = a.b.n_select - n0 - a.b.n_last;
+    const int n0 = a.b.n_first, n = r.end - n0, want = a.b.n_select - n0 - a.b.n_last;
     for (int i = tid; i < n0; i += kPickThreads) out[i] = i;
     for (int i = tid; i < a.b.n_last; i += kPickThreads) out[n0 + want + i] = r.end + i;
     if (want == 0) return;
-    const uint64_t* keys = a.keys + ((int64_t)(t - a.t0) * nkv + g) * a.b.n_blocks;
-    uint64_t prefix = 0;
-    uint32_t need = (uint32_t)want;
-    int shift = 64;
+    Score* scores = a.scores + ((int64_t)(t - a.t0) * nkv + g) * a.ld + n0;
+    const float* q = a.q + ((int64_t)t * a.nh + g * a.group) * HD;
     const auto inclusive = [&](uint32_t v) {  // over the workgroup
-        for (int off = 1; off < 64; off <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_up((int)v, off);
-            if (lane >= off) v += o;
-        }
+        v = wave_scan(v);
         __syncthreads();
         if (lane == 63) wsum[wave] = v;
         __syncthreads();
         for (int w = 0; w < wave; ++w) v += wsum[w];
         return v;
     };
+
+    // the range of the scores, the most one is off
+    const bool held = n <= kPickKeys;
+    float least = INFINITY, most = -INFINITY, off = 0.f;
+    for (int i = tid; i < kPickBins; i += kPickThreads) bins[i] = 0;
+    if (tid == 0) n_open = n_above = 0;
+    for (int i = tid; i < n; i += kPickThreads) {
+        const Score c = scores[i];
+        if (held) keys_lds[i] = c.s;
+        if (c.s > -INFINITY) least = fminf(least, c.s);
+        most = fmaxf(most, c.s);
+        off = c.s != c.s || !(c.off < INFINITY) ? INFINITY : fmaxf(off, c.off);
+    }
+    least = -wave_max_all(-least), most = wave_max_all(most), off = wave_max_all(off);
+    if (lane == 0) red[wave][0] = least, red[wave][1] = most, red[wave][2] = off;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) least = fminf(least, red[w][0]), most = fmaxf(most, red[w][1]), off = fmaxf(off, red[w][2]);
+    const auto key = [&](int i) { return held ? keys_lds[i] : scores[i].s; };
+    bool exact = !(off < INFINITY) || !(fabsf(least) < INFINITY) || !(fabsf(most) < INFINITY);
+    float above = 0.f, below = 0.f;
+    int taken_above = 0;
+    if (!exact) {
+        const float range = most - least, scale = range > 0.f ? (float)(kPickBins - 1) / range : 0.f;
+        const auto bin = [&](float s) { return min((int)((s - least) * scale), kPickBins - 1); };
+        exact = !(scale < INFINITY) || !(range < INFINITY);
+        for (int i = tid; i < n && !exact; i += kPickThreads) {
+            const float s = key(i);
+            if (s > -INFINITY) atomicAdd(&bins[bin(s)], 1u);
+        }
+        __syncthreads();
+        // bins from the top, two a thread
+        static_assert(kPickBins == 2 * kPickThreads, "");
+        const uint32_t c0 = bins[kPickBins - 1 - 2 * tid], c1 = bins[kPickBins - 2 - 2 * tid];
+        const uint32_t upto = inclusive(c0 + c1), before = upto - c0 - c1, w = (uint32_t)want;
+        if (tid == 0) found[0] = 0xffffffffu;
+        __syncthreads();
+        if (before < w && before + c0 >= w) found[0] = (uint32_t)(kPickBins - 1 - 2 * tid);
+        else if (before + c0 < w && upto >= w) found[0] = (uint32_t)(kPickBins - 2 - 2 * tid);
+        __syncthreads();
+        if (found[0] == 0xffffffffu) exact = true;  // (fewer blocks are there than wanted)
+        else {
+            // the bin's edges, with what the sums above round
+            const float width = range / (float)(kPickBins - 1), at = least + (float)found[0] * width;
+            const float slack = 2.f * off + range * 0x1p-18f + fmaxf(fabsf(least), fabsf(most)) * 0x1p-20f;
+            above = at + width + slack, below = at - slack;
+            uint32_t mine = 0;  // (the wave's)
+            for (int i = tid; i < n; i += kPickThreads) {
+                const float s = key(i);
+                mine += (uint32_t)__popcll(__ballot(s > above));
+                if (s >= below && s <= above) {
+                    const uint32_t e = atomicAdd(&n_open, 1u);
+                    if (e < (uint32_t)kOpenMax) open[e] = i;
+                }
+            }
+            mine = (uint32_t)__builtin_amdgcn_readfirstlane((int)mine);  // (its first lane took part to the end)
+            if (lane == 0) atomicAdd(&n_above, mine);
+            __syncthreads();
+            taken_above = (int)n_above;
+            exact = n_open > (uint32_t)kOpenMax;
+        }
+    }
+    if (!exact) {
+        const int ours = (int)n_open, need = want - taken_above;
+        if (ours != need) {
+            for (int j = tid / 16; j < ours; j += kPickThreads / 16) {
+                const double s = exact_score<HD>(a.b, x.s, n0 + open[j], g, q, a.group);
+                if ((tid & 15) == 0) open_key[j] = order_key(s);
+            }
+            __syncthreads();
+            if (tid < ours) {
+                int rank = 0;
+                for (int j = 0; j < ours; ++j)
+                    rank += open_key[j] > open_key[tid] || (open_key[j] == open_key[tid] && open[j] < open[tid]);
+                const float s = rank < need ? INFINITY : -INFINITY;
+                if (held) keys_lds[open[tid]] = s;
+                else scores[open[tid]].s = s;
+            }
+            __syncthreads();
+        }
+        const bool edge = ours == need;  // (all that are open are taken)
+        // each wave a stretch of the blocks: how many it takes, then which
+        const auto take = [&](int i) {
+            if (i >= n) return false;
+            const float s = key(i);
+            return edge ? s >= below : s > above;
+        };
+        const int stretch = (n + 64 * WAVES - 1) / (64 * WAVES) * 64, i0 = wave * stretch, i1 = min(i0 + stretch, n);
+        uint32_t count = 0;
+        for (int i = i0; i < i1; i += 64) count += (uint32_t)__popcll(__ballot(i + lane < i1 && take(i + lane)));
+        if (lane == 0) wsum[wave] = count;
+        __syncthreads();
+        int at = n0;
+        for (int w = 0; w < wave; ++w) at += (int)wsum[w];
+        for (int i = i0; i < i1; i += 64) {
+            const bool on = i + lane < i1 && take(i + lane);
+            const uint64_t all = __ballot(on);
+            if (on) out[at + (int)__popcll(all & ((1ull << lane) - 1))] = n0 + i + lane;
+            at += (int)__popcll(all);
+        }
+        return;
+    }
+
+    // all scores in 64 bits, where the others were
+    uint64_t* keys = reinterpret_cast<uint64_t*>(scores);
+    for (int i = tid / 16; i < n; i += kPickThreads / 16) {
+        const double s = exact_score<HD>(a.b, x.s, n0 + i, g, q, a.group);
+        if ((tid & 15) == 0) keys[i] = order_key(s);
+    }
+    __syncthreads();
+    uint64_t prefix = 0;
+    uint32_t need = (uint32_t)want;
+    int shift = 64;
     for (;;) {
         shift -= 8;
         bins[tid] = 0;
         __syncthreads();
-        for (int b = n0 + tid; b < r.end; b += kPickThreads) {
-            const uint64_t k = keys[b];
+        for (int i = tid; i < n; i += kPickThreads) {
+            const uint64_t k = keys[i];
             if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&bins[k >> shift & 255], 1u);
         }
         __syncthreads();
-        const uint32_t n = bins[255 - tid], upto = inclusive(n);
-        if (upto >= need && upto - n < need) found[0] = 255 - tid, found[1] = need - (upto - n);
+        const uint32_t c = bins[255 - tid], upto = inclusive(c);
+        if (upto >= need && upto - c < need) found[0] = 255 - tid, found[1] = need - (upto - c);
         __syncthreads();
         prefix = prefix << 8 | found[0], need = found[1];
         const bool all = bins[found[0]] == need;
@@ -265,14 +628,14 @@ __global__ __launch_bounds__(kPickThreads) void block_pick_kernel(SelectArgs a) 
     // those above the prefix, and the first `need` of those with it
     int done = n0;
     uint32_t ties = 0;
-    for (int b0 = n0; b0 < r.end; b0 += kPickThreads) {
-        const int b = b0 + tid;
-        const uint64_t k = b < r.end ? keys[b] >> shift : 0;
-        const bool above = b < r.end && k > prefix, same = b < r.end && k == prefix;
+    for (int i0 = 0; i0 < n; i0 += kPickThreads) {
+        const int i = i0 + tid;
+        const uint64_t k = i < n ? keys[i] >> shift : 0;
+        const bool larger = i < n && k > prefix, same = i < n && k == prefix;
         const uint32_t before = inclusive(same) - same + ties;
-        const bool take = above || (same && before < need);
+        const bool take = larger || (same && before < need);
         const uint32_t upto = inclusive(take);
-        if (take) out[done + upto - 1] = b;
+        if (take) out[done + upto - 1] = n0 + i;
         __syncthreads();
         if (tid == kPickThreads - 1) found[0] = upto, found[1] = before + same;
         __syncthreads();
@@ -431,13 +794,25 @@ int launch_attention(const BlockAttnArgs& a, int64_t tiles, hipStream_t st) {
 }
 
 template <int HD>
-void launch_scores(const SelectArgs& a, int64_t tiles, hipStream_t st) {
-    // blocks of a workgroup: 64 where that leaves few workgroups
-    const int64_t few = (a.b.n_blocks + 63) / 64;
-    const int iters = few * tiles * a.b.pg.nkv > 4096 ? 4 : 1;
-    const int chunks = (a.b.n_blocks + 64 * iters - 1) / (64 * iters);
-    hipLaunchKernelGGL(block_score_kernel<HD>, dim3((unsigned)(chunks * tiles * a.b.pg.nkv)), dim3(kScoreThreads), 0, st,
-                       a, iters, chunks);
+void launch_select(const SelectArgs& a, hipStream_t st) {
+    const int64_t n = a.t1 - a.t0, tiles = (n + a.tokens - 1) / a.tokens, nkv = a.b.pg.nkv;
+    if (a.b.n_blocks > a.b.n_select) {  // (else no token has more blocks than it takes)
+        // steps of a workgroup: so many that there are some four workgroups a CU
+        const bool many = tiles >= kScoreWaves && a.tokens > 1;
+        const int64_t rows = many ? (tiles + kScoreWaves - 1) / kScoreWaves : tiles, step = many ? 16 : 16 * kScoreWaves;
+        const int64_t one = (a.b.n_blocks + step - 1) / step;
+        int64_t iters = one * rows * nkv / (many ? 512 : 1024);
+        iters = std::max<int64_t>(1, std::min<int64_t>({one, iters, 64 / a.tokens, 15}));  // (at most 20 KB of LDS)
+        if (many) iters = (iters + 2) / 3 * 3;  // (as its steps are taken)
+        const int64_t chunks = (one + iters - 1) / iters;
+        const size_t lds = sizeof(float) * kScoreWaves * (a.tokens + 1) * 16 * (size_t)iters;
+        const dim3 grid((unsigned)(chunks * rows * nkv));
+        if (many)
+            hipLaunchKernelGGL(block_score_rows_kernel<HD>, grid, dim3(kScoreThreads), lds, st, a, (int)iters, (int)chunks);
+        else hipLaunchKernelGGL(block_score_kernel<HD>, grid, dim3(kScoreThreads), lds, st, a, (int)iters, (int)chunks);
+    }
+    hipLaunchKernelGGL(block_pick_kernel<HD>, dim3((unsigned)(n * nkv)), dim3(kPickThreads),
+                       sizeof(float) * std::min(a.b.n_blocks, kPickKeys), st, a);
 }
 
 }  // namespace
@@ -458,18 +833,15 @@ size_t select_blocks_work_bytes(const PagedArgs& pg, const BlocksOf& b) {
 
 void select_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const float* q, int nh, int hd, int* chosen,
                           void* work, hipStream_t st) {
-    SelectArgs a{block_args(pg, b), q, nh, nh / pg.nkv, 0, 0, 0, static_cast<uint64_t*>(work), chosen};
+    const BlockArgs ba = block_args(pg, b);
+    SelectArgs a{ba, q, nh, nh / pg.nkv, 0, 0, 0, (int)select_row(ba.n_blocks), static_cast<Score*>(work), chosen};
     a.tokens = pg.n_tokens > 2 * (int64_t)pg.n_seq ? 16 / a.group : 1;
-    const int64_t step = select_tokens(pg.n_tokens, a.b.n_blocks, pg.nkv);
+    const int64_t step = select_tokens(pg.n_tokens, ba.n_blocks, pg.nkv);
     for (int64_t t = 0; t < pg.n_tokens; t += step) {
         a.t0 = (int)t, a.t1 = (int)std::min<int64_t>(t + step, pg.n_tokens);
-        const int64_t n = a.t1 - a.t0, tiles = (n + a.tokens - 1) / a.tokens;
-        if (a.b.n_blocks > b.n_select) {  // (else no token has more blocks than it takes)
-            if (hd == 32) launch_scores<32>(a, tiles, st);
-            else if (hd == 64) launch_scores<64>(a, tiles, st);
-            else launch_scores<128>(a, tiles, st);
-        }
-        hipLaunchKernelGGL(block_pick_kernel, dim3((unsigned)(n * pg.nkv)), dim3(kPickThreads), 0, st, a);
+        if (hd == 32) launch_select<32>(a, st);
+        else if (hd == 64) launch_select<64>(a, st);
+        else launch_select<128>(a, st);
     }
 }
 

@@ -110,6 +110,17 @@ __device__ __forceinline__ int dpp_i(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
 }
 
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive, over the wave
+    int v = (int)x;
+    v += dpp_i<0x111>(v);       // row_shr:1
+    v += dpp_i<0x112>(v);
+    v += dpp_i<0x114>(v);
+    v += dpp_i<0x118>(v);
+    v += dpp_i<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp_i<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return (uint32_t)v;
+}
+
 __device__ __forceinline__ int sum4_dpp(int v) {
     v += dpp_i<0xb1>(v);
     return v + dpp_i<0x4e>(v);

@@ -32,17 +32,6 @@ namespace mxh {
 
 namespace {
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive
-    int v = (int)x;
-    v += dpp_i<0x111>(v);       // row_shr:1
-    v += dpp_i<0x112>(v);
-    v += dpp_i<0x114>(v);
-    v += dpp_i<0x118>(v);
-    v += dpp_i<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
-    v += dpp_i<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
-    return (uint32_t)v;
-}
-
 // The line of the batch's units (mxh_paged_plan.h), made by a wave from the
 // lengths.  All uniform but what a lane says of its sequences.
 struct Plan : PagedLine {
