@@ -292,13 +292,13 @@ typedef struct {
 /* mxh_attention_paged where sequences have their first rows in common: the same
  * result (but for fp32 rounding), with K and V of a group's prefix read once for
  * the tokens of all its sequences, from the pages of the group's first sequence
- * that has new tokens, instead of once a sequence.  (A group of one sequence, or
- * none, is correct and takes about a plan and a third kernel longer than
- * mxh_attention_paged.)  Takes the same batches, drafted trees among them; what a
- * token does not attend, absent rows, infinities and precision are as there, and so
- * are the rules for q, att and work; mxh_attention_shared_workspace says what any
- * batch of up to this n_seq, n_tokens, n_groups and table_ld needs (every token's
- * parts lie there: twice att at least). */
+ * that has new tokens, instead of once a sequence.  That is done where it can pay:
+ * where the sequences have few new tokens (up to 32 rows of q a kv head on average)
+ * and rows of the table's width would be 180 MB of K and V or more for all of them;
+ * elsewhere this is mxh_attention_paged.  Takes the same batches, drafted trees among
+ * them; what a token does not attend, absent rows, infinities and precision are as
+ * there, and so are the rules for q, att and work; mxh_attention_shared_workspace
+ * says what any batch of up to this n_seq, n_tokens, n_groups and table_ld needs. */
 int mxh_attention_shared(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const mxh_kv_groups *groups,
                          const float *q, int nh, float *att, void *work, size_t work_bytes);
 int mxh_attention_shared_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, const mxh_kv_groups *groups,

@@ -732,6 +732,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockAttn
     }
 }
 
+// (splits make few tiles into some two workgroups a CU, so units are few)
+constexpr int kMergeLanes = 4, kMergeUnits = kJoinThreads / kMergeLanes;
 struct BlockMergeArgs {
     const float* part;
     const float2* ml;
@@ -742,7 +744,7 @@ struct BlockMergeArgs {
 
 template <int HD>
 __global__ __launch_bounds__(kJoinThreads) void blocks_merge_kernel(BlockMergeArgs a) {
-    const int64_t u = (int64_t)blockIdx.x * kJoinUnits + threadIdx.x % kJoinUnits;
+    const int64_t u = (int64_t)blockIdx.x * kMergeUnits + threadIdx.x % kMergeUnits;
     const int64_t head = min(u, a.total - 1) / (HD / 4);
     const int d = 4 * (int)(u % (HD / 4)), nh = a.nkv * a.group;
     const int64_t t = head / nh, tile = t / a.tokens;
@@ -755,7 +757,7 @@ __global__ __launch_bounds__(kJoinThreads) void blocks_merge_kernel(BlockMergeAr
         v = *reinterpret_cast<const float4*>(a.part + at * HD + d);
     };
     const bool any = u < a.total && !(a.ml[place(0)].y < 0.f);  // (else no sequence's)
-    join_parts(a.splits, where, any ? a.att + head * HD + d : nullptr);
+    join_parts<kMergeLanes>(a.splits, where, any ? a.att + head * HD + d : nullptr);
 }
 
 BlockSize block_size(const BlockArgs& a, int nh) {
@@ -787,7 +789,7 @@ int launch_attention(const BlockAttnArgs& a, int64_t tiles, hipStream_t st) {
     if (a.splits > 1) {
         const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4);
         const BlockMergeArgs m{a.t.part, a.t.ml, a.t.att, total, a.t.pg.nkv, (int)a.t.group, (int)a.t.tokens, a.splits};
-        hipLaunchKernelGGL(blocks_merge_kernel<HD>, dim3((unsigned)((total + kJoinUnits - 1) / kJoinUnits)),
+        hipLaunchKernelGGL(blocks_merge_kernel<HD>, dim3((unsigned)((total + kMergeUnits - 1) / kMergeUnits)),
                            dim3(kJoinThreads), 0, st, m);
     }
     return MXH_OK;

@@ -907,15 +907,16 @@ __device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, ui
 
 // The row `out` (of a thread's four dims) from its parts: where(z, x, v) reads part
 // z's reference and sum and its V sums there.  A thread of the 256 has a unit, four
-// dims of a row, u = tid % 64, and every 4th part; `out` is null where there is no
-// row to write.  Called by all threads.
-constexpr int kJoinThreads = 256, kJoinLanes = 4, kJoinUnits = kJoinThreads / kJoinLanes;
-template <class Where>
+// dims of a row, u = tid % (256 / LANES), and every LANES-th part; `out` is null where
+// there is no row to write.  Called by all threads.
+constexpr int kJoinThreads = 256;
+// lanes to a unit: four where there are few units, one where they fill the GPU (1,500
+// tokens of 32 heads of 128, two or three parts each: 57 us with four, X with one)
+inline int join_lanes(int64_t units, int cus) { return units > (int64_t)cus * 1024 ? 1 : 4; }
+template <int LANES, class Where>
 __device__ __forceinline__ void join_parts(int parts, const Where& where, float* out) {
-    constexpr int AHEAD = 4;
-    __shared__ float4 acc[kJoinThreads];
-    __shared__ float2 st[kJoinThreads];
-    const int tid = threadIdx.x, lane = tid / kJoinUnits;
+    constexpr int AHEAD = 4, UNITS = kJoinThreads / LANES;
+    const int tid = threadIdx.x, lane = tid / UNITS;
     float M = -INFINITY, L = 0.f;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
     const auto join = [&](float2 x, float4 v) __attribute__((always_inline)) {
@@ -926,20 +927,25 @@ __device__ __forceinline__ void join_parts(int parts, const Where& where, float*
         s.x = s.x * a0 + v.x * a1, s.y = s.y * a0 + v.y * a1, s.z = s.z * a0 + v.z * a1, s.w = s.w * a0 + v.w * a1;
     };
     if (out)
-        for (int z0 = lane; z0 < parts; z0 += AHEAD * kJoinLanes) {
+        for (int z0 = lane; z0 < parts; z0 += AHEAD * LANES) {
             float2 x[AHEAD];
             float4 v[AHEAD];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) where(min(z0 + i * kJoinLanes, parts - 1), x[i], v[i]);
+            for (int i = 0; i < AHEAD; ++i) where(min(z0 + i * LANES, parts - 1), x[i], v[i]);
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
-                if (z0 + i * kJoinLanes < parts) join(x[i], v[i]);
+                if (z0 + i * LANES < parts) join(x[i], v[i]);
         }
-    acc[tid] = s;
-    st[tid] = make_float2(M, L);
-    __syncthreads();
+    if constexpr (LANES > 1) {
+        __shared__ float4 acc[kJoinThreads];
+        __shared__ float2 st[kJoinThreads];
+        acc[tid] = s;
+        st[tid] = make_float2(M, L);
+        __syncthreads();
+        if (lane == 0 && out)
+            for (int i = 1; i < LANES; ++i) join(st[tid + i * UNITS], acc[tid + i * UNITS]);
+    }
     if (lane || !out) return;
-    for (int i = 1; i < kJoinLanes; ++i) join(st[tid + i * kJoinUnits], acc[tid + i * kJoinUnits]);
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     *reinterpret_cast<float4*>(out) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }

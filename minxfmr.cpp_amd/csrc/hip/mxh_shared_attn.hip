@@ -38,148 +38,157 @@ struct SharedPlanArgs {
     int4* records;  // [n_tokens][2]
 };
 
-constexpr int kPlanThreads = 1024;
-
-__device__ __forceinline__ uint64_t block_sum(uint64_t v, uint64_t* s) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) v += s[w];
-    __syncthreads();
-    return v;
+// What the plan keeps in LDS: starts and lengths of the sequences, the groups' starts,
+// rows in common and first sequences with tokens, tiles and stages of the runs, the
+// sequences' groups
+__host__ __device__ constexpr size_t plan_lds(int n_seq, int n_groups) {
+    return sizeof(int) * ((size_t)4 * n_seq + (size_t)5 * n_groups + 3) + sizeof(int16_t) * n_seq;
 }
+constexpr int kPlanWaves = 16;
 
 // Workgroup 0 writes the items, the others the records of tokens that no sequence
 // may have.  A group's rows in common are whole pages, no more than any of its
 // sequences with tokens has cached (group_start that falls or leaves the batch:
-// no rows in common).
-__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(SharedPlanArgs a) {
+// no rows in common).  Few instructions, each once: they come from memory as
+// the one workgroup gets to them (as long as X us with the runs computed three times).
+__global__ __launch_bounds__(64 * kPlanWaves) void shared_plan_kernel(SharedPlanArgs a) {
     extern __shared__ int lds[];
-    const int tid = threadIdx.x;
+    __shared__ unsigned long long sums[2][kPlanWaves];
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 63, wave = tid >> 6, waves = threads >> 6;
     if (blockIdx.x > 0) {
-        const int t = (int)(blockIdx.x - 1) * kPlanThreads + tid;
+        const int t = (int)(blockIdx.x - 1) * threads + tid;
         if (t < a.pg.n_tokens) a.records[2 * t] = make_int4(0, 0, -1, 0);
         return;
     }
-    __shared__ uint64_t sums[kPlanThreads / 64];
     const int ng = a.n_groups, ns = a.pg.n_seq, runs = ng + ns;
-    int *gstart = lds, *common = gstart + ng + 1, *lead = common + ng;  // lead: the group's first sequence with tokens
-    uint32_t* base = (uint32_t*)(lead + ng);                            // items before the run's
+    int *start = lds, *cached = start + ns + 1, *gstart = cached + ns, *common = gstart + ng + 1,
+        *lead = common + ng;
+    uint32_t *base = (uint32_t*)(lead + ng), *stages = base + runs + 1;  // base: tiles, then items before the run's
+    int16_t* group = (int16_t*)(stages + runs);
     const int64_t table_rows = (int64_t)a.pg.table_ld << a.pg.page_shift;
     const int page = ~((1 << a.pg.page_shift) - 1);
-    bool bad = false;
-    for (int g = tid; g <= ng && ng > 0; g += kPlanThreads) {
-        const int at = a.group_start[g];
-        bad |= at < 0 || at > ns || (g < ng && a.group_start[g + 1] < at);
-        gstart[g] = at;
-        if (g < ng) common[g] = (int)min((int64_t)max(a.group_shared[g], 0), table_rows) & page, lead[g] = INT_MAX;
+#pragma unroll 1
+    for (int i = tid; i <= ns; i += threads) {
+        start[i] = a.pg.start[i];
+        if (i < ns) cached[i] = min(max(a.pg.cached[i], 0), 1 << 30);
+        if (i <= ng && ng > 0) gstart[i] = a.group_start[i];  // (no more groups than sequences)
+        if (i < ng) common[i] = (int)min((int64_t)max(a.group_shared[i], 0), table_rows) & page, lead[i] = INT_MAX;
     }
-    const bool grouped = ng > 0 && !__syncthreads_or(bad);
-    const auto group_of = [&](int s) {  // -1: none
-        if (!grouped || s < gstart[0] || s >= gstart[ng]) return -1;
-        int lo = 0, hi = ng;  // gstart[lo] <= s < gstart[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (gstart[mid] <= s) lo = mid;
-            else hi = mid;
-        }
-        return lo;
-    };
-    PagedLine line(a.sh.rows_s, a.tokens_s, a.pg.parent != nullptr, 0);
-    const auto seq = [&](int s) {
-        return line.seq(a.pg.start[s], a.pg.start[s + 1], a.pg.cached[s], a.pg.n_tokens, (uint64_t)table_rows);
-    };
-    bool falls = false;
-    for (int s = tid; s < ns; s += kPlanThreads) {
-        const PagedSeq q = seq(s);
-        falls |= a.pg.start[s + 1] < a.pg.start[s];
-        const int g = group_of(s);
-        if (q.n > 0 && g >= 0) {
-            atomicMin(&common[g], (int)q.cached & page);
-            atomicMin(&lead[g], s);
-        }
+    __syncthreads();
+    int wrong = 0;  // 1: groups that make no sense, 2: starts that fall
+#pragma unroll 1
+    for (int i = tid; i < ns; i += threads) {
+        if (i < ng && (gstart[i] < 0 || gstart[i + 1] > ns || gstart[i + 1] < gstart[i])) wrong |= 1;
+        if (start[i + 1] < start[i]) wrong |= 2;
     }
-    if (__syncthreads_or(falls)) {
+    if (__syncthreads_or(wrong & 2)) {
         if (tid == 0) *a.counts = make_int2(0, 0);
         return;
     }
-    // (a group's tokens: those of all its sequences)
-    const auto prefix = [&](int g, int& first, int& n) {
-        first = max(a.pg.start[gstart[g]], 0);
-        n = max(min(a.pg.start[gstart[g + 1]], a.pg.n_tokens) - first, 0);
+    const bool grouped = !__syncthreads_or(wrong) && ng > 0;
+    const auto tokens_of = [&](int s) {
+        const int n = start[s] < 0 ? 0 : max(min(start[s + 1], a.pg.n_tokens) - start[s], 0);
+        return a.pg.parent ? min(n, kTreeMax) : n;
     };
-    const auto run = [&](int r) {
-        if (r < ng) {
-            int first, n;
-            if (!grouped || lead[r] == INT_MAX || common[r] == 0) return SharedRun{0, 0};
-            prefix(r, first, n);
-            return shared_run((uint32_t)n, (uint32_t)common[r], a.sh.rows_p, a.tokens_p);
+#pragma unroll 1
+    for (int s = tid; s < ns; s += threads) {
+        int g = -1;
+        if (grouped && s >= gstart[0] && s < gstart[ng]) {
+            int hi = ng;  // gstart[g] <= s < gstart[hi]
+            for (g = 0; hi - g > 1;) {
+                const int mid = (g + hi) >> 1;
+                if (gstart[mid] <= s) g = mid;
+                else hi = mid;
+            }
         }
-        const PagedSeq q = seq(r - ng);
-        const int g = group_of(r - ng);
-        const uint32_t rows = (uint32_t)min((int64_t)q.cached + q.n, table_rows);
-        return shared_run(q.n, rows - (uint32_t)(g >= 0 && q.n > 0 ? common[g] : 0), a.sh.rows_s, a.tokens_s);
-    };
-    uint64_t units = 0;
-    for (int r = tid; r < runs; r += kPlanThreads) units += run(r).units();
-    const uint32_t per = shared_per(block_sum(units, sums), a.sh.target);
+        group[s] = (int16_t)g;
+        if (g >= 0 && tokens_of(s) > 0) {
+            atomicMin(&common[g], cached[s] & page);
+            atomicMin(&lead[g], s);
+        }
+    }
+    __syncthreads();
+    unsigned long long units[2] = {0, 0};  // of prefixes, of own rows
+#pragma unroll 1
+    for (int r = tid; r < runs; r += threads) {
+        int n = 0, keys = 0;
+        if (r >= ng) {
+            const int s = r - ng, g = group[s];
+            n = tokens_of(s);
+            keys = (int)min((int64_t)cached[s] + n, table_rows) - (g >= 0 && n > 0 ? common[g] : 0);
+        } else if (grouped && lead[r] != INT_MAX && common[r] > 0) {  // the tokens of all the group's sequences
+            n = max(min(start[gstart[r + 1]], a.pg.n_tokens) - max(start[gstart[r]], 0), 0);
+            keys = common[r];
+        }
+        const SharedRun x = shared_run((uint32_t)n, (uint32_t)keys, r < ng ? a.sh.rows_p : a.sh.rows_s,
+                                       r < ng ? a.tokens_p : a.tokens_s);
+        base[r] = x.tiles, stages[r] = x.stages;
+        units[r >= ng] += x.units();
+    }
+#pragma unroll 1
+    for (int off = 32; off > 0; off >>= 1) {
+        units[0] += __shfl_xor(units[0], off);
+        units[1] += __shfl_xor(units[1], off);
+    }
+    if (lane == 0) sums[0][wave] = units[0], sums[1][wave] = units[1];
+    __syncthreads();
+    units[0] = units[1] = 0;
+#pragma unroll 1
+    for (int w = 0; w < waves; ++w) units[0] += sums[0][w], units[1] += sums[1][w];
+    const uint32_t per_p = shared_per(units[0], a.sh.target_p), per_s = shared_per(units[1], a.sh.target_s);
+    __syncthreads();
     // items before each run's: a thread has the runs [tid part, (tid + 1) part)
-    const int part = (runs + kPlanThreads - 1) / kPlanThreads, r0 = min(tid * part, runs), r1 = min(r0 + part, runs);
+    const int part = (runs + threads - 1) / threads, r0 = min(tid * part, runs), r1 = min(r0 + part, runs);
+    const auto count = [&](int r) { return base[r] * SharedRun{base[r], stages[r]}.parts(r < ng ? per_p : per_s); };
     uint32_t mine = 0;
-    for (int r = r0; r < r1; ++r) {
-        const SharedRun x = run(r);
-        mine += x.tiles * x.parts(per);
-    }
-    uint32_t upto = mine;
-    for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t v = (uint32_t)__shfl_up((int)upto, off);
-        if ((tid & 63) >= off) upto += v;
-    }
-    if ((tid & 63) == 63) sums[tid >> 6] = upto;
+#pragma unroll 1
+    for (int r = r0; r < r1; ++r) mine += count(r);
+    uint32_t at = wave_scan(mine);
+    if (lane == 63) sums[0][wave] = at;
+    at -= mine;
     __syncthreads();
-    uint32_t total = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w < tid >> 6) upto += (uint32_t)sums[w];
-        total += (uint32_t)sums[w];
-    }
-    uint32_t at = upto - mine;
+#pragma unroll 1
+    for (int w = 0; w < wave; ++w) at += (uint32_t)sums[0][w];
+#pragma unroll 1
     for (int r = r0; r < r1; ++r) {
-        const SharedRun x = run(r);
+        const uint32_t n = count(r);
         base[r] = at;
-        at += x.tiles * x.parts(per);
+        at += n;
     }
-    if (tid == 0) base[runs] = total;
+    if (r0 < runs && r1 == runs) base[runs] = at;
     __syncthreads();
-    const uint32_t total_p = base[ng];
+    const uint32_t total_p = base[ng], total = base[runs];
     if (tid == 0) *a.counts = make_int2((int)total_p, (int)total);
-    for (uint32_t i = (uint32_t)tid; i < total; i += kPlanThreads) {
-        int lo = 0, hi = runs;  // base[lo] <= i < base[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (base[mid] <= i) lo = mid;
+#pragma unroll 1
+    for (uint32_t i = (uint32_t)tid; i < total; i += threads) {
+        int r = 0, hi = runs;  // base[r] <= i < base[hi]
+#pragma unroll 1
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if (base[mid] <= i) r = mid;
             else hi = mid;
         }
-        const SharedRun x = run(lo);
-        const uint32_t local = i - base[lo], parts = x.parts(per);
+        const bool own = r >= ng;
+        SharedItem it;
+        it.begin = 0;
+        if (own) {
+            const int s = r - ng, g = group[s];
+            it.s = s, it.first = start[s], it.n = tokens_of(s), it.cached = cached[s];
+            if (g >= 0) it.begin = common[g];
+        } else {
+            it.s = lead[r], it.first = max(start[gstart[r]], 0), it.cached = common[r];
+            it.n = max(min(start[gstart[r + 1]], a.pg.n_tokens) - it.first, 0);
+        }
+        const uint32_t t = own ? a.tokens_s : a.tokens_p, per = own ? per_s : per_p;
+        const SharedRun x{((uint32_t)it.n + t - 1) / t, stages[r]};
+        const uint32_t len = x.length(per), local = i - base[r];
         // (the tiles of a part next to one another: they read the same rows)
         const uint32_t z = local / x.tiles, tile = local - z * x.tiles;
-        SharedItem it;
-        it.tile = (int)tile, it.begin = 0;
-        it.st0 = (int)((uint64_t)x.stages * z / parts), it.st1 = (int)((uint64_t)x.stages * (z + 1) / parts);
-        it.parts = (int)parts, it.stride = (int)x.tiles;
-        it.slot0 = (int)(base[lo] + tile), it.slot = (int)i;
-        if (lo < ng) {
-            it.s = lead[lo], it.cached = common[lo];
-            prefix(lo, it.first, it.n);
-        } else {
-            const PagedSeq q = seq(lo - ng);
-            const int g = group_of(lo - ng);
-            it.s = lo - ng, it.first = (int)q.first, it.n = (int)q.n, it.cached = (int)q.cached;
-            it.begin = g >= 0 ? common[g] : 0;
-            it.slot0 -= (int)total_p, it.slot -= (int)total_p;
-            if (it.begin == 0 && parts == 1) it.slot = -1;  // (nothing to join)
-        }
+        it.tile = (int)tile, it.parts = (int)x.parts(per), it.stride = (int)x.tiles;
+        it.st0 = (int)(z * len), it.st1 = (int)min((z + 1) * len, x.stages);
+        const uint32_t kind = own ? total_p : 0;
+        it.slot0 = (int)(base[r] + tile - kind), it.slot = (int)(i - kind);
+        if (own && it.begin == 0 && it.parts == 1) it.slot = -1;  // (nothing to join)
         a.items[i] = it;
     }
 }
@@ -235,9 +244,10 @@ struct SharedMergeArgs {
 };
 
 // att from each token's parts
-template <int HD>
+template <int HD, int LANES>
 __global__ __launch_bounds__(kJoinThreads) void shared_merge_kernel(SharedMergeArgs a) {
-    const int64_t u = (int64_t)blockIdx.x * kJoinUnits + threadIdx.x % kJoinUnits;
+    constexpr int UNITS = kJoinThreads / LANES;
+    const int64_t u = (int64_t)blockIdx.x * UNITS + threadIdx.x % UNITS;
     const int64_t head = min(u, a.total - 1) / (HD / 4);
     const int d = 4 * (int)(u % (HD / 4)), nh = a.nkv * a.group;
     const int64_t t = head / nh;
@@ -251,7 +261,7 @@ __global__ __launch_bounds__(kJoinThreads) void shared_merge_kernel(SharedMergeA
         x = (p ? a.ml_p : a.ml_s)[at];
         v = *reinterpret_cast<const float4*>((p ? a.part_p : a.part_s) + at * HD + d);
     };
-    join_parts(own.z + pre.z, where, any ? a.att + head * HD + d : nullptr);
+    join_parts<LANES>(own.z + pre.z, where, any ? a.att + head * HD + d : nullptr);
 }
 
 PagedSize shared_size(const PagedArgs& a, int nh) {
@@ -280,27 +290,36 @@ int launch_hd(const SharedArgs& a, const SharedShape& sh, hipStream_t st) {
                    : sh.rows_p == 64 ? launch<HD, 64, 16>(a, sh, st)
                                      : launch<HD, 16, 16>(a, sh, st);
     if (rc) return rc;
-    const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4), units = kJoinUnits;
+    const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4);
+    const int lanes = join_lanes(total, device_cus());
+    const dim3 grid((unsigned)((total + kJoinThreads / lanes - 1) / (kJoinThreads / lanes)));
     const SharedMergeArgs m{a.records, a.t.part, a.part_s, a.t.ml, a.ml_s, a.t.att, total, a.t.pg.nkv,
                             (int)a.t.group, sh.rows_p, sh.rows_s};
-    hipLaunchKernelGGL(shared_merge_kernel<HD>, dim3((unsigned)((total + units - 1) / units)), dim3(kJoinThreads), 0,
-                       st, m);
+    if (lanes == 1) hipLaunchKernelGGL((shared_merge_kernel<HD, 1>), grid, dim3(kJoinThreads), 0, st, m);
+    else hipLaunchKernelGGL((shared_merge_kernel<HD, 4>), grid, dim3(kJoinThreads), 0, st, m);
     return MXH_OK;
 }
 
 }  // namespace
 
 size_t attention_shared_work_bytes(const PagedArgs& a, int n_groups, int nh, int hd) {
-    return shared_work(shared_shape(shared_size(a, nh), n_groups), a.n_tokens, a.nkv, hd).bytes;
+    const PagedSize size = shared_size(a, nh);
+    if (!shared_pays(size, hd, n_groups)) return attention_paged_work_bytes(a, nh, hd);
+    return shared_work(shared_shape(size, n_groups), a.n_tokens, a.nkv, hd).bytes;
 }
 
 size_t attention_shared_work_bound(const PagedArgs& a, int n_groups, int nh, int hd) {
     const PagedSize size = shared_size(a, nh);
-    return shared_work(shared_bound(size, n_groups), shared_bound(size, a.n_seq), a.n_tokens, a.nkv, hd).bytes;
+    const size_t paged = attention_paged_work_bound(a, nh, hd);
+    // (fewer tokens may pay where these do not; fewer sequences or groups do not)
+    if (!shared_pays(PagedSize{size.n_seq, 1, size.table_rows, size.nkv, size.group, size.cus}, hd, n_groups)) return paged;
+    return std::max(paged, shared_work(shared_bound(size, n_groups), shared_bound(size, a.n_seq), shared_tokens(size),
+                                       a.nkv, hd).bytes);
 }
 
 int attention_shared_launch(const PagedArgs& a, int n_groups, const int* group_start, const int* group_shared,
                             const float* q, int nh, int hd, float* att, void* work, hipStream_t st) {
+    if (!shared_pays(shared_size(a, nh), hd, n_groups)) return attention_paged_launch(a, q, nh, hd, att, work, st);
     const SharedShape sh = shared_shape(shared_size(a, nh), n_groups);
     const SharedWork w = shared_work(sh, a.n_tokens, a.nkv, hd);
     const uint32_t group = (uint32_t)(nh / a.nkv);
@@ -308,16 +327,16 @@ int attention_shared_launch(const PagedArgs& a, int n_groups, const int* group_s
     const SharedPlanArgs plan{a, group_start, group_shared, n_groups, sh, (uint32_t)sh.rows_p / group,
                               (uint32_t)sh.rows_s / group, reinterpret_cast<int2*>(at),
                               reinterpret_cast<SharedItem*>(at + w.items), reinterpret_cast<int4*>(at + w.records)};
-    const size_t lds = sizeof(int) * ((size_t)4 * n_groups + a.n_seq + 2);
     static bool attr_set = false;
     if (!attr_set) {
         if (hipFuncSetAttribute((const void*)shared_plan_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)sizeof(int) * (5 * kPagedSeqMax + 2)) != hipSuccess)
+                                (int)plan_lds(kPagedSeqMax, kPagedSeqMax)) != hipSuccess)
             return MXH_ERR_HIP;
         attr_set = true;
     }
-    hipLaunchKernelGGL(shared_plan_kernel, dim3(1 + (unsigned)((a.n_tokens + kPlanThreads - 1) / kPlanThreads)),
-                       dim3(kPlanThreads), lds, st, plan);
+    const unsigned threads = a.n_seq + n_groups > 512 ? 64 * kPlanWaves : 256;
+    hipLaunchKernelGGL(shared_plan_kernel, dim3(1 + ((unsigned)a.n_tokens + threads - 1) / threads), dim3(threads),
+                       plan_lds(a.n_seq, n_groups), st, plan);
     const SharedArgs args{{a, q, att, reinterpret_cast<float*>(at + w.part_p), reinterpret_cast<float2*>(at + w.ml_p),
                            nh, 1.4426950408889634f / sqrtf((float)hd), group, 0, (65536 + group - 1) / group},
                           reinterpret_cast<float*>(at + w.part_s),

@@ -10,11 +10,39 @@
 
 namespace mxh {
 
+// Whether prefixes are read apart, from what the host knows: as long as the table
+// allows, the batch's K and V rows, and the rows of q that a sequence has on average.
+// Read with the sequences' own rows, a prefix comes out of the caches for all but the
+// first of them; read apart, it takes a plan, a third kernel and 10 us more.  And
+// where a sequence fills a tile of 64 rows its tiles are bound by their products.
+// 32/8 heads of 128 (4 KB of K and V a row), apart and not, us:
+//   single tokens: 4 at 1,200 rows 17 and 11, 8 at 4,500 25 and 21, 12 at 2,200 21.3
+//   and 19.5, 6 at 8,200 25.7 and 25.1 (200 MB), 32 at 1,200 22.3 and 22.8 (160 MB), 24
+//   at 2,200 23 and 25 (220 MB), 16 at 4,500 26 and 31, 64 at 8,200 (2 GB) and of their
+//   own up to 1,000 60 and 158
+//   up to 4 tokens each (12 rows of q): 12 at 6,300 30 and 34, 30 45 and 65
+//   up to 16 (43 rows): 12 at 6,300 49 and 51, 30 100 and 102; up to 64 and 128: 30
+//   at 6,300 289 and 279, 503 and 527
+constexpr int kSharedRows = 32;         // rows of q of a sequence, on average, at most
+constexpr double kSharedBytes = 180e6;  // of K and V at least
+inline bool shared_pays(const PagedSize& a, int hd, int n_groups) {
+    return n_groups > 0 && (int64_t)a.n_tokens * a.group <= (int64_t)kSharedRows * a.n_seq &&
+           (double)a.n_seq * (double)a.table_rows * a.nkv * hd * 4 >= kSharedBytes;
+}
+// tokens of a batch with prefixes read apart, at most, of those up to a's size
+inline int shared_tokens(const PagedSize& a) {
+    return (int)std::min<int64_t>(a.n_tokens, (int64_t)kSharedRows * a.n_seq / a.group);
+}
+
 // What the host chooses without the lengths: rows of the tiles over prefixes and
-// of those over the sequences' own rows, items that the stages are cut into,
-// and how many there can be of either kind.
+// of those over the sequences' own rows, items that the stages of either kind are cut
+// into, and how many there can be.  Items over prefixes are one a CU, first: two on a
+// CU take nearly twice as long, and the sequences' own rows, which wait for memory,
+// fit beside one.  64 single tokens behind 8,000 rows, up to 1,000 of their own (32/8
+// heads of 128): one a CU 45 us, 5 for 4 CUs 54, 12 for 4 59; own rows first 60, the
+// two in turn 55; either by itself 31.
 struct SharedShape {
-    int rows_p, rows_s, target;
+    int rows_p, rows_s, target_p, target_s;
     int64_t items_p, items_s;
 };
 inline SharedShape shared_shape(const PagedSize& a, int n_groups) {
@@ -22,9 +50,10 @@ inline SharedShape shared_shape(const PagedSize& a, int n_groups) {
     const auto rows = [&](int n) { return (int64_t)((a.n_tokens + n - 1) / n) * a.group > 16 ? 64 : 16; };
     s.rows_s = rows(a.n_seq);
     s.rows_p = n_groups > 0 ? std::max(rows(n_groups), s.rows_s) : s.rows_s;
-    s.target = most_items(64, a.nkv, a.cus);
-    s.items_p = n_groups > 0 ? s.target + a.n_tokens / (s.rows_p / a.group) + n_groups : 0;
-    s.items_s = s.target + a.n_tokens / (s.rows_s / a.group) + a.n_seq;
+    s.target_p = most_items(16, a.nkv, a.cus);
+    s.target_s = most_items(64, a.nkv, a.cus);
+    s.items_p = n_groups > 0 ? s.target_p + a.n_tokens / (s.rows_p / a.group) + n_groups : 0;
+    s.items_s = s.target_s + a.n_tokens / (s.rows_s / a.group) + a.n_seq;
     return s;
 }
 
@@ -33,16 +62,26 @@ struct SharedRun {
     uint32_t tiles, stages;
     // (tiles of a prompt have fewer stages the earlier they are: counted in full)
     MXH_HD uint64_t units() const { return (uint64_t)tiles * stages; }
-    // parts that each of its tiles is cut into, `per` stages at most each
-    MXH_HD uint32_t parts(uint32_t per) const { return stages > per ? (stages + per - 1) / per : 1; }
+    // Parts that each of its tiles is cut into, of at most `per` stages: as many equal
+    // ones as that takes
+    MXH_HD uint32_t length(uint32_t per) const {  // of a part
+        if (stages <= per) return stages;
+        const uint32_t n = (stages + per - 1) / per;
+        return (stages + n - 1) / n;
+    }
+    MXH_HD uint32_t parts(uint32_t per) const {
+        if (stages <= per) return 1;
+        const uint32_t len = length(per);
+        return (stages + len - 1) / len;
+    }
 };
 MXH_HD SharedRun shared_run(uint32_t n, uint32_t keys, int rows, uint32_t tokens) {
     return SharedRun{(n + tokens - 1) / tokens, (keys + (uint32_t)stage_keys(rows) - 1) / (uint32_t)stage_keys(rows)};
 }
 // stages of an item, so that `units` make no more than target items beside one a tile
 MXH_HD uint32_t shared_per(uint64_t units, int target) {
-    const uint64_t per = (units + (uint64_t)target - 1) / (uint64_t)target;
-    return per < 2 ? 2 : (uint32_t)per;
+    const double per = ceil((double)units / (double)target);  // (units fit 53 bits; a 64-bit division is slow)
+    return per < 2. ? 2 : (uint32_t)per;
 }
 
 // One item: tile `tile` of the run's, stages [st0, st1) over the rows of sequence s
@@ -59,9 +98,10 @@ struct SharedBound {
 };
 inline SharedBound shared_bound(const PagedSize& a, int runs) {
     SharedBound b;
+    const int tokens = shared_tokens(a);
     for (const int rows : {16, 64}) {
-        if (runs == 0 || (rows == 64 && (int64_t)a.n_tokens * a.group <= 16)) continue;
-        const int64_t items = most_items(64, a.nkv, a.cus) + a.n_tokens / (rows / a.group) + runs;
+        if (runs == 0 || (rows == 64 && (int64_t)tokens * a.group <= 16)) continue;
+        const int64_t items = most_items(64, a.nkv, a.cus) + tokens / (rows / a.group) + runs;
         b.items = std::max(b.items, items), b.rows = std::max(b.rows, items * rows);
     }
     return b;

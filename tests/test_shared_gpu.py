@@ -4,6 +4,11 @@ The values expected and their bound are those of attention over the paged cache
 (test_paged_gpu.py), which do not depend on what is read once: the sums over the
 keys that a row's parts share among them are covered by the bound's L u.  Pages
 that members of a group would have had of their own for the common rows hold NaN.
+
+Prefixes are read apart where the table is wide enough for the batch to be large
+(180 MB of K and V) and sequences have few tokens on average (32 rows of q): `wide`
+cases have such a table, mostly of absent pages.  Others run as attention over the
+paged cache.
 """
 from __future__ import annotations
 
@@ -20,7 +25,10 @@ pytestmark = pytest.mark.gpu
 class Shared(Case):
     """Case whose groups, (first sequence, one past the last, rows in common), have those rows in the same pages."""
 
-    def __init__(self, seqs, groups, *, told=None, starts=None, **kw):
+    def __init__(self, seqs, groups, *, told=None, starts=None, wide=True, **kw):
+        if wide:
+            row = 4 * kw["nkv"] * kw["hd"]
+            kw["extra_ld"] = kw.get("extra_ld", 0) + -(-180_000_000 // (row * kw["page"] * len(seqs)))
         super().__init__(seqs, **kw)
         self.groups = groups
         width = self.nkv * self.hd
@@ -78,22 +86,28 @@ GROUPS = {
     "nothing-in-common": ([(40, 2), (70, 1), (0, 5)], [(0, 3, 0)]),
     "no-groups": ([(40, 2), (200, 1), (0, 5)], []),
     "forty": ([(320 + 3 * s % 50, 1) for s in range(40)], [(0, 40, 320)]),
+    "prompts-among-single-tokens": ([(256 + s % 7, 70 if s in (3, 9) else 1) for s in range(34)], [(0, 20, 256), (20, 34, 192)]),
+    "few-tokens": ([(640 + s, 2 + s % 5) for s in range(12)], [(0, 5, 640), (7, 12, 576)]),
 }
 TREES = {
     "trees": ([(128, 7), (130, 12), (190, 64), (128, 1), (64, 16), (95, 33)], [(0, 4, 128)]),
     "trees-of-a-long-prompt": ([(2048, 27), (2050, 5), (2100, 13)], [(0, 3, 2048)]),
+    "trees-among-single-tokens": ([(192 + s % 9, 64 if s == 5 else 13 if s in (2, 20) else 1) for s in range(30)],
+                                  [(0, 16, 192), (16, 30, 128)]),
+    "small-trees": ([(320 + s, 1 + s % 6) for s in range(16)], [(0, 16, 320)]),
 }
 
 
+@pytest.mark.parametrize("wide", [True, False], ids=["wide", "narrow"])
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("heads", list(HEADS))
 @pytest.mark.parametrize("name", list(GROUPS) + list(TREES))
-def test_attention_matches_float64(mxh, name, heads, page):
+def test_attention_matches_float64(mxh, name, heads, page, wide):
     nh, nkv, hd = HEADS[heads]
     tree = name in TREES
     seqs, groups = (TREES if tree else GROUPS)[name]
     c = Shared(seqs, groups, nh=nh, nkv=nkv, hd=hd, page=page, tree=tree, lead=2, tail=3, seed=len(name) * 17 + nh,
-               extra_ld=2).upload()
+               extra_ld=2, wide=wide).upload()
     c.check(c.attention())
     c.close()
 
@@ -183,8 +197,9 @@ def test_absent_rows(mxh):
 @pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
 def test_what_is_not_attended_has_no_effect(mxh, tree):
     """Infinities and NaN among the new rows; a token that attends one gets what it makes."""
-    seqs, groups = [(64, 40), (80, 21), (64, 1)], [(0, 3, 64)]
+    seqs, groups = [(64, 40), (80, 21)] + [(64, 1)] * 10, [(0, 12, 64)]
     c = Shared(seqs, groups, nh=8, nkv=2, hd=64, page=16, tree=tree, seed=11)
+    assert c.tokens * 4 <= 32 * len(seqs)
     bad = {0: [7, 30, 39], 1: [20, 5]}
     for s, rows in bad.items():
         for i, r in enumerate(rows):
@@ -268,19 +283,20 @@ def test_a_recorded_call_follows_lengths_tables_and_groups(mxh):
     c.close()
 
 
-def test_the_largest_batchs_workspace_is_enough(mxh):
+@pytest.mark.parametrize("ld", [30, 30000])
+def test_the_largest_batchs_workspace_is_enough(mxh, ld):
     """Of a batch of n_seq sequences and n_tokens tokens, for all with fewer of either."""
     ns, nt, nh, nkv, hd = 40, 90, 8, 2, 64
     pool = mxhip.KvPool(256, 256, n_layer=1, n_pages=100, page_rows=16, n_kv=nkv, head_dim=hd)
     size = lambda s, t, g: mxhip.attention_shared_workspace(  # noqa: E731
-        pool, mxhip.KvBatch(s, t, 256, 256, 256, 30), mxhip.KvGroups(g, 256, 256), nh)
+        pool, mxhip.KvBatch(s, t, 256, 256, 256, ld), mxhip.KvGroups(g, 256, 256), nh)
     most = size(ns, nt, 10)
     for s in (1, 2, 7, 39, 40):
         for t in (1, 2, 3, 40, 89, 90):
             for g in (0, 1, 2, 10):
                 if g <= s:
                     assert size(s, t, g) <= most
-    c = Shared([(64, 1)] * 3 + [(64, 84)], [(0, 4, 64)], nh=nh, nkv=nkv, hd=hd, page=16, seed=1).upload()
+    c = Shared([(64, 1)] * 9 + [(64, 54)], [(0, 10, 64)], nh=nh, nkv=nkv, hd=hd, page=16, seed=1, wide=ld > 30).upload()
     c.bufs["work"].close()
     c.bufs["work"], c.work_bytes = mxhip.DeviceBuffer(most), most
     c.check(c.attention())
