@@ -35,11 +35,13 @@ inline int64_t block_tiles(const BlockSize& a) {
     const int t = block_tokens(a);
     return (a.n_tokens + t - 1) / t;
 }
-// Workgroups that share a tile's list, for two a CU, with at least two stages of
-// 128 keys each
+// Workgroups that share a tile's list, for two a CU: of one token with 2,048 rows for
+// each of 8 kv heads of 128 a stage of 128 keys each, 16 workgroups, 9.4 us, 8 11.2, 4
+// 13.3 (and 3.9 for joining their parts).  (48 tokens with 1,280, a workgroup each 53
+// us, two each 55 and 5)
 inline int block_splits(const BlockSize& a) {
     const int64_t items = block_tiles(a) * a.nkv, stages = ((int64_t)a.n_select * a.block_rows + 127) / 128;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)a.cus / items, stages / 2, 64}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)a.cus / items, stages, 64}));
 }
 // the workspace: parts of the tiles that are split
 inline size_t block_part_bytes(int64_t parts, int nkv, int hd) {
@@ -52,7 +54,7 @@ inline size_t block_work_bytes(const BlockSize& a, int hd) {
 // ... of any batch (splits > 1: splits x items are at most two a CU)
 inline size_t block_work_bound(const BlockSize& a, int hd) {
     const int64_t stages = ((int64_t)a.n_select * a.block_rows + 127) / 128;
-    return stages < 4 ? 0 : block_part_bytes(std::max<int64_t>(2, 2 * (int64_t)a.cus / a.nkv), a.nkv, hd);
+    return stages < 2 ? 0 : block_part_bytes(std::max<int64_t>(2, 2 * (int64_t)a.cus / a.nkv), a.nkv, hd);
 }
 
 // Selecting: scores of a token and kv head (whole tiles of 16 blocks), and tokens whose

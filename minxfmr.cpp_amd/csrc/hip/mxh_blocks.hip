@@ -649,7 +649,7 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
 struct BlockAttnArgs {
     TileArgs t;
     const int* chosen;  // [n_tokens][nkv][n_select]
-    int n_select, block_shift, n_blocks, splits, words;
+    int n_select, block_shift, n_blocks, splits, words, once;  // once: rows that a call reads do not stay for the next
     int lists;  // LDS bytes before the lists
 };
 
@@ -726,7 +726,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockAttn
         it.st0 = stages * (uint32_t)z / (uint32_t)a.splits, it.st1 = stages * (uint32_t)(z + 1) / (uint32_t)a.splits;
         it.slot = a.splits > 1 ? (int)index : -1;
         it.row0 = (uint32_t)(t - first) * a.t.group;
-        attend_tile<HD, 16, kListed>(a.t, it, g, tid, wave, false, smem);
+        attend_tile<HD, 16, kListed>(a.t, it, g, tid, wave, a.once, smem);
         t += n;
         if (t < last) __syncthreads();
     }
@@ -863,10 +863,13 @@ int attention_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const int* c
     const int64_t tiles = block_tiles(size);
     const uint32_t group = (uint32_t)size.group;
     float* part = static_cast<float*>(work);
+    // single tokens whose rows are more than half of the last cache's 256 MB: 48 of them
+    // with 1,280 rows for each of 8 kv heads of 128 53 us, 47 so
+    const bool once = block_tokens(size) == 1 && (double)pg.n_tokens * pg.nkv * b.n_select * size.block_rows * hd * 4 > 128e6;
     const BlockAttnArgs a{{pg, q, att, part, reinterpret_cast<float2*>(part + (size_t)tiles * splits * pg.nkv * 16 * hd),
                            nh, 1.4426950408889634f / sqrtf((float)hd), group, (uint32_t)block_tokens(size),
                            (65536 + group - 1) / group},
-                          chosen, b.n_select, b.block_shift, ba.n_blocks, splits, (ba.n_blocks + 31) / 32, 0};
+                          chosen, b.n_select, b.block_shift, ba.n_blocks, splits, (ba.n_blocks + 31) / 32, once, 0};
     return hd == 32   ? launch_attention<32>(a, tiles, st)
            : hd == 64 ? launch_attention<64>(a, tiles, st)
                       : launch_attention<128>(a, tiles, st);

@@ -415,11 +415,14 @@ __device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, ui
     // tile, and none of the 63 sequences around it has the first row's page in the
     // same place, as forks would.  Then the loads say so, and the caches do not fill
     // with them: 48 single tokens at up to 16,000 rows 255 us without, 228 with;
-    // 64 at up to 9,000 rows, 8,000 of them shared, 158 and 205.
+    // 64 at up to 9,000 rows, 8,000 of them shared, 158 and 205.  (kListed: the first
+    // listed row's page)
     bool once = false;
     if constexpr (PRIVATE) {
         if (nst > 0 && unshared) {
-            const int page = key0 >> a.pg.page_shift, s = max(min(it.s - 32, a.pg.n_seq - 64), 0) + lane;
+            int page = key0 >> a.pg.page_shift;
+            if constexpr (LISTED) page = (int)(it.blocks[0] << it.block_shift) >> a.pg.page_shift;
+            const int s = max(min(it.s - 32, a.pg.n_seq - 64), 0) + lane;
             int other = -2;
             if (s < a.pg.n_seq && s != it.s) other = a.pg.table[(size_t)s * a.pg.table_ld + page];
             once = !__any(other == table[page]);
