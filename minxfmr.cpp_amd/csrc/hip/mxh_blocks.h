@@ -23,13 +23,22 @@ struct BlockSize {
     int nkv, group, n_select, block_rows, cus;
 };
 
-// Tokens that share a tile of 16 rows.  Those of one sequence attend many of the
-// same blocks, and rows of absent tokens cost what others do; single tokens of
-// sequences (up to two each on average) share nothing and go by themselves.
-inline int block_tokens(const BlockSize& a) {
-    if (a.n_tokens <= 2 * (int64_t)a.n_seq) return 1;
+// Tokens that share a tile, and its rows.  Tokens of one sequence attend many of the
+// same blocks, whose rows are then loaded once for all of them; single tokens of
+// sequences (up to two each on average) share nothing and go by themselves.  32 rows
+// where sequences have tokens enough and lists and bits leave room for them: 512
+// tokens with 32 of 469 blocks of 64 rows each, of which four tokens together have
+// some 63 and eight some 82 (32/8 heads of 128), 121 us, in tiles of 16 rows 129.
+inline int block_tokens_of(const BlockSize& a, int rows) {
     const int64_t words = (a.n_blocks + 31) / 32;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({16 / a.group, kListMax / a.n_select, kBitBytes / (4 * words)}));
+    return (int)std::max<int64_t>(
+        1, std::min<int64_t>({rows / a.group, 16, kListMax / a.n_select, kBitBytes / (4 * words)}));
+}
+inline int block_rows_of_tile(const BlockSize& a) {
+    return a.n_tokens > 8 * (int64_t)a.n_seq && block_tokens_of(a, 32) * a.group > 16 ? 32 : 16;
+}
+inline int block_tokens(const BlockSize& a) {
+    return a.n_tokens <= 2 * (int64_t)a.n_seq ? 1 : block_tokens_of(a, block_rows_of_tile(a));
 }
 inline int64_t block_tiles(const BlockSize& a) {
     const int t = block_tokens(a);
@@ -44,17 +53,17 @@ inline int block_splits(const BlockSize& a) {
     return (int)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)a.cus / items, stages, 64}));
 }
 // the workspace: parts of the tiles that are split
-inline size_t block_part_bytes(int64_t parts, int nkv, int hd) {
-    return (size_t)parts * nkv * 16 * (hd + 2) * sizeof(float);
+inline size_t block_part_bytes(int64_t parts, int rows, int nkv, int hd) {
+    return (size_t)parts * nkv * rows * (hd + 2) * sizeof(float);
 }
 inline size_t block_work_bytes(const BlockSize& a, int hd) {
     const int s = block_splits(a);
-    return s > 1 ? block_part_bytes(block_tiles(a) * s, a.nkv, hd) : 0;
+    return s > 1 ? block_part_bytes(block_tiles(a) * s, block_rows_of_tile(a), a.nkv, hd) : 0;
 }
 // ... of any batch (splits > 1: splits x items are at most two a CU)
 inline size_t block_work_bound(const BlockSize& a, int hd) {
     const int64_t stages = ((int64_t)a.n_select * a.block_rows + 127) / 128;
-    return stages < 2 ? 0 : block_part_bytes(std::max<int64_t>(2, 2 * (int64_t)a.cus / a.nkv), a.nkv, hd);
+    return stages < 2 ? 0 : block_part_bytes(std::max<int64_t>(2, 2 * (int64_t)a.cus / a.nkv), 32, a.nkv, hd);
 }
 
 // Selecting: scores of a token and kv head (whole tiles of 16 blocks), and tokens whose

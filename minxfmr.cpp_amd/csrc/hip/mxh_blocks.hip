@@ -42,14 +42,19 @@ struct TokenAt {
     int s, i, cached, n;  // cached rows, tokens of the sequence
 };
 __device__ __forceinline__ TokenAt token_at(const PagedArgs& a, int t) {
-    TokenAt x{paged_seq_of(a, t), 0, 0, 0};
-    if (x.s < 0) return x;
-    const int first = a.start[x.s];
-    x.i = t - first;
-    x.n = min(a.start[x.s + 1], a.n_tokens) - first;
+    // (as paged_seq_of, with what is read of the sequence in flight together)
+    const int lane = threadIdx.x & 63, part = (a.n_seq + 63) / 64;
+    int s = 0;
+    if (part > 1) {
+        const int e = (lane + 1) * part;
+        s = part * (int)__popcll(__ballot(e <= a.n_seq && a.start[min(e, a.n_seq)] <= t));
+    }
+    const int e = s + lane + 1;
+    s += (int)__popcll(__ballot(a.start[min(e, a.n_seq)] <= t && e <= a.n_seq));
+    const int at = min(s, a.n_seq - 1), first = a.start[at], end = a.start[at + 1], cached = a.cached[at];
+    TokenAt x{s, t - first, min(max(cached, 0), 1 << 30), min(end, a.n_tokens) - first};
     if (a.parent) x.n = min(x.n, kTreeMax);
-    x.cached = min(max(a.cached[x.s], 0), 1 << 30);
-    if (x.i >= x.n) x.s = -1;
+    if (s >= a.n_seq || first < 0 || x.i < 0 || x.i >= x.n) x.s = -1;
     return x;
 }
 
@@ -655,7 +660,7 @@ struct BlockAttnArgs {
 
 // Workgroup (kv head, tile and split): the blocks that any of a sequence's tokens
 // in the tile has chosen, found as bits in LDS, then a share of their stages.
-template <int HD>
+template <int HD, int R>
 __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockAttnArgs a) {
     extern __shared__ __align__(256) uint8_t smem[];
     __shared__ uint32_t sums[kWaves];
@@ -672,7 +677,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockAttn
         if (x.s < 0) {  // (its rows of the part: to be left alone)
             if (a.splits > 1)
                 for (int i = tid; i < (int)a.t.group; i += kThreads)
-                    a.t.ml[(index * nkv + g) * 16 + (t - first) * (int)a.t.group + i] = make_float2(0.f, -1.f);
+                    a.t.ml[(index * nkv + g) * R + (t - first) * (int)a.t.group + i] = make_float2(0.f, -1.f);
             ++t;
             continue;
         }
@@ -726,7 +731,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockAttn
         it.st0 = stages * (uint32_t)z / (uint32_t)a.splits, it.st1 = stages * (uint32_t)(z + 1) / (uint32_t)a.splits;
         it.slot = a.splits > 1 ? (int)index : -1;
         it.row0 = (uint32_t)(t - first) * a.t.group;
-        attend_tile<HD, 16, kListed>(a.t, it, g, tid, wave, a.once, smem);
+        attend_tile<HD, R, kListed>(a.t, it, g, tid, wave, a.once, smem);
         t += n;
         if (t < last) __syncthreads();
     }
@@ -739,7 +744,7 @@ struct BlockMergeArgs {
     const float2* ml;
     float* att;
     int64_t total;  // units of four dims, of all tokens
-    int nkv, group, tokens, splits;
+    int nkv, group, tokens, splits, rows;
 };
 
 template <int HD>
@@ -750,7 +755,7 @@ __global__ __launch_bounds__(kJoinThreads) void blocks_merge_kernel(BlockMergeAr
     const int64_t t = head / nh, tile = t / a.tokens;
     const int hq = (int)(head - t * nh), g = hq / a.group;
     const int row = (int)(t - tile * a.tokens) * a.group + hq - g * a.group;
-    const auto place = [&](int z) { return ((tile * a.splits + z) * a.nkv + g) * 16 + row; };
+    const auto place = [&](int z) { return ((tile * a.splits + z) * a.nkv + g) * a.rows + row; };
     const auto where = [&](int z, float2& x, float4& v) __attribute__((always_inline)) {
         const int64_t at = place(z);
         x = a.ml[at];
@@ -769,30 +774,35 @@ BlockArgs block_args(const PagedArgs& pg, const BlocksOf& b) {
     return BlockArgs{pg, b.bounds, b.block_shift, b.n_first, b.n_last, b.n_select, (int)blocks_of_table(pg, b.block_shift)};
 }
 
-template <int HD>
-int launch_attention(const BlockAttnArgs& a, int64_t tiles, hipStream_t st) {
-    constexpr int RING = lds_bytes(HD, 16);
+template <int HD, int R>
+int launch_rows(const BlockAttnArgs& a, int64_t tiles, hipStream_t st) {
+    constexpr int RING = lds_bytes(HD, R);
     BlockAttnArgs args = a;
     args.lists = std::max(RING, (int)((a.t.tokens * (size_t)a.words * 4 + 255) / 256 * 256));
     const size_t lds = (size_t)args.lists + kListMax * 6;
     static bool attr_set = false;
     if (!attr_set) {
-        if (hipFuncSetAttribute((const void*)attention_blocks_kernel<HD>, hipFuncAttributeMaxDynamicSharedMemorySize,
+        if (hipFuncSetAttribute((const void*)attention_blocks_kernel<HD, R>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                 std::max(RING, kBitBytes) + kListMax * 6) != hipSuccess)
             return MXH_ERR_HIP;
         attr_set = true;
     }
     const int64_t items = tiles * a.splits, y = std::min<int64_t>(items, 32768);
-    hipLaunchKernelGGL(attention_blocks_kernel<HD>,
+    hipLaunchKernelGGL((attention_blocks_kernel<HD, R>),
                        dim3((unsigned)a.t.pg.nkv, (unsigned)y, (unsigned)((items + y - 1) / y)), dim3(kThreads), lds, st,
                        args);
     if (a.splits > 1) {
         const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4);
-        const BlockMergeArgs m{a.t.part, a.t.ml, a.t.att, total, a.t.pg.nkv, (int)a.t.group, (int)a.t.tokens, a.splits};
+        const BlockMergeArgs m{a.t.part, a.t.ml, a.t.att, total, a.t.pg.nkv, (int)a.t.group, (int)a.t.tokens, a.splits, R};
         hipLaunchKernelGGL(blocks_merge_kernel<HD>, dim3((unsigned)((total + kMergeUnits - 1) / kMergeUnits)),
                            dim3(kJoinThreads), 0, st, m);
     }
     return MXH_OK;
+}
+
+template <int HD>
+int launch_attention(const BlockAttnArgs& a, int rows, int64_t tiles, hipStream_t st) {
+    return rows == 32 ? launch_rows<HD, 32>(a, tiles, st) : launch_rows<HD, 16>(a, tiles, st);
 }
 
 template <int HD>
@@ -866,13 +876,14 @@ int attention_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const int* c
     // single tokens whose rows are more than half of the last cache's 256 MB: 48 of them
     // with 1,280 rows for each of 8 kv heads of 128 53 us, 47 so
     const bool once = block_tokens(size) == 1 && (double)pg.n_tokens * pg.nkv * b.n_select * size.block_rows * hd * 4 > 128e6;
-    const BlockAttnArgs a{{pg, q, att, part, reinterpret_cast<float2*>(part + (size_t)tiles * splits * pg.nkv * 16 * hd),
+    const BlockAttnArgs a{{pg, q, att, part, reinterpret_cast<float2*>(part + (size_t)tiles * splits * pg.nkv * block_rows_of_tile(size) * hd),
                            nh, 1.4426950408889634f / sqrtf((float)hd), group, (uint32_t)block_tokens(size),
                            (65536 + group - 1) / group},
                           chosen, b.n_select, b.block_shift, ba.n_blocks, splits, (ba.n_blocks + 31) / 32, once, 0};
-    return hd == 32   ? launch_attention<32>(a, tiles, st)
-           : hd == 64 ? launch_attention<64>(a, tiles, st)
-                      : launch_attention<128>(a, tiles, st);
+    const int rows = block_rows_of_tile(size);
+    return hd == 32   ? launch_attention<32>(a, rows, tiles, st)
+           : hd == 64 ? launch_attention<64>(a, rows, tiles, st)
+                      : launch_attention<128>(a, rows, tiles, st);
 }
 
 }  // namespace mxh

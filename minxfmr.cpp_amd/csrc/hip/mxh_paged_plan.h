@@ -25,7 +25,7 @@ constexpr int kTreeMax = 64;        // new tokens of a drafted tree (one lane, o
 constexpr int kPagedSeqMax = 4096;  // sequences of a batch
 
 // keys of a stage: 32 for every group of waves that share them
-constexpr int stage_keys(int rows) { return rows == 16 ? 128 : 64; }
+constexpr int stage_keys(int rows) { return rows == 64 ? 64 : 128; }
 // a tile's cost beside its stages, in stages (64 rows: 3 to 6 are within 5% of one
 // another; without it items that cross tiles end late)
 constexpr int tile_lead(int rows) { return rows == 16 ? 2 : 4; }

@@ -5,7 +5,8 @@
 //
 // A tile is T = R / group consecutive tokens of one sequence with the group =
 // nh / nkv q heads of one kv head (row r: token r / group, head r % group), R =
-// 16 or 64 rows, and a stage 128 or 64 keys.
+// 16 or 64 rows, and a stage 128 or 64 keys.  (R = 32 goes as 16 does, with the
+// products of 64.)
 //
 // K and V rows go straight into LDS (16 rows of a page are evenly spaced, so
 // their addresses are a scalar base and fixed lane offsets).  Per 32-key block
@@ -47,7 +48,7 @@ constexpr int kThreads = 256, kWaves = 4;
 // floats a wave leaves for the merge: V sums [m][hd + 4], references, sums (and a flag, behind all of theirs)
 __host__ __device__ constexpr int merge_floats(int hd, int m) { return m * (hd + 6); }
 __host__ __device__ constexpr int lds_bytes(int hd, int rows) {
-    const int ring = 2 * 128 * hd * 2,  // R = 16: a stage, R = 64: two
+    const int ring = 2 * 128 * hd * 2,  // R = 16 and 32: a stage, R = 64: two
                merge = kWaves * (merge_floats(hd, rows == 16 ? 16 : 32) + 1) * 4;
     return ring > merge ? ring : merge;
 }
@@ -61,7 +62,7 @@ __device__ __align__(256) uint32_t zero_row[64];
 //              the tokens have in common
 //   kOwnRows   as kSequence, from row `begin` on (a multiple of 16)
 //   kListed    the rows of a list of blocks, one behind the other, up to each
-//              token's own (R = 16)
+//              token's own (R = 16 and 32)
 enum Keys { kSequence, kPrefix, kOwnRows, kListed };
 
 // A tile, or some of its stages
@@ -914,7 +915,7 @@ __device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, ui
 // there is no row to write.  Called by all threads.
 constexpr int kJoinThreads = 256;
 // lanes to a unit: four where there are few units, one where they fill the GPU (1,500
-// tokens of 32 heads of 128, two or three parts each: 57 us with four, X with one)
+// tokens of 32 heads of 128, two or three parts each: 57 us with four, 27 with one)
 inline int join_lanes(int64_t units, int cus) { return units > (int64_t)cus * 1024 ? 1 : 4; }
 template <int LANES, class Where>
 __device__ __forceinline__ void join_parts(int parts, const Where& where, float* out) {

@@ -49,8 +49,9 @@ constexpr int kPlanWaves = 16;
 // Workgroup 0 writes the items, the others the records of tokens that no sequence
 // may have.  A group's rows in common are whole pages, no more than any of its
 // sequences with tokens has cached (group_start that falls or leaves the batch:
-// no rows in common).  Few instructions, each once: they come from memory as
-// the one workgroup gets to them (as long as X us with the runs computed three times).
+// no rows in common).  The lengths are read once, all at a time, and little code is
+// written twice: it comes from memory as the one workgroup gets to it.  64 sequences
+// 8 us, 9 before that.
 __global__ __launch_bounds__(64 * kPlanWaves) void shared_plan_kernel(SharedPlanArgs a) {
     extern __shared__ int lds[];
     __shared__ unsigned long long sums[2][kPlanWaves];

@@ -253,7 +253,7 @@ extern "C" int blocks(int n_seq, int n_tokens, int64_t n_blocks, int nkv, int gr
                       int cus, int hd) {
     const BlockSize a{n_seq, n_tokens, n_blocks, nkv, group, n_select, block_rows, cus};
     const int t = block_tokens(a), s = block_splits(a);
-    REQUIRE(t >= 1 && t * group <= 16 && (int64_t)t * n_select <= kListMax);
+    REQUIRE(t >= 1 && t <= 16 && t * group <= block_rows_of_tile(a) && (int64_t)t * n_select <= kListMax);
     REQUIRE(t * ((n_blocks + 31) / 32) * 4 <= kBitBytes);
     REQUIRE(block_tiles(a) * t >= n_tokens && (block_tiles(a) - 1) * t < n_tokens);
     REQUIRE(s >= 1 && block_work_bytes(a, hd) <= block_work_bound(a, hd));
