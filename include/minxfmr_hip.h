@@ -324,7 +324,9 @@ typedef struct {
  * from all rows that a block has then: to be called after mxh_qk_rope_append, and
  * again, with a batch that says which rows, where rows changed otherwise
  * (mxh_kv_keep_rows; a block of a copied page that the sequence does not append
- * to).  Keys that are NaN do not count.  Blocks of absent pages are left out.
+ * to).  A block that several of the batch's sequences have gets one's: they should
+ * end at the same row of it.  bounds must not overlap k and v.
+ * Keys that are NaN do not count.  Blocks of absent pages are left out.
  * n_first, n_last and n_select do not matter (n_select within its range); as in
  * mxh_attention_paged's batches, tokens past the 64th of a drafted tree have no
  * rows.  start that falls: some blocks may be left out. */
@@ -343,7 +345,8 @@ int mxh_kv_block_bounds(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *
  * Rows of chosen of tokens that no sequence has are left alone (so may others be
  * where start falls).  parent only counts in that tokens past the 64th have no
  * rows.  q and work 16-byte aligned; work: mxh_kv_select_workspace, for any batch of
- * up to this n_tokens and table_ld; nothing may overlap. */
+ * up to this n_tokens and table_ld, one of its own for calls that may run at the
+ * same time; nothing may overlap. */
 int mxh_kv_select_blocks(const mxh_kv_pool *pool, int layer, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks,
                          const float *q, int nh, int *chosen, void *work, size_t work_bytes);
 int mxh_kv_select_workspace(const mxh_kv_pool *pool, const mxh_kv_batch *batch, const mxh_kv_blocks *blocks, int nh,

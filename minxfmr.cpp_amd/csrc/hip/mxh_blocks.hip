@@ -814,7 +814,7 @@ void launch_select(const SelectArgs& a, hipStream_t st) {
         const int64_t rows = many ? (tiles + kScoreWaves - 1) / kScoreWaves : tiles, step = many ? 16 : 16 * kScoreWaves;
         const int64_t one = (a.b.n_blocks + step - 1) / step;
         int64_t iters = one * rows * nkv / (many ? 512 : 1024);
-        iters = std::max<int64_t>(1, std::min<int64_t>({one, iters, 64 / a.tokens, 15}));  // (at most 20 KB of LDS)
+        iters = std::max<int64_t>(1, std::min<int64_t>({one, iters, 64 / a.tokens, 15}));  // (at most 26 KB of LDS)
         if (many) iters = (iters + 2) / 3 * 3;  // (as its steps are taken)
         const int64_t chunks = (one + iters - 1) / iters;
         const size_t lds = sizeof(float) * kScoreWaves * (a.tokens + 1) * 16 * (size_t)iters;

@@ -326,8 +326,15 @@ int check_work(const char* who, size_t need, const void* work, size_t work_bytes
 }
 
 int64_t bounds_elems(const mxh_kv_pool* p, const mxh_kv_blocks* b) {  // of a layer
-    return b->layer_stride ? b->layer_stride
-                           : (int64_t)p->n_pages * (p->page_rows / b->block_rows) * p->n_kv * 2 * p->head_dim;
+    return (int64_t)p->n_pages * (p->page_rows / b->block_rows) * p->n_kv * 2 * p->head_dim;
+}
+__half* layer_bounds(const mxh_kv_pool* p, int layer, const mxh_kv_blocks* b) {
+    return b->bounds ? static_cast<__half*>(b->bounds) + layer * (b->layer_stride ? b->layer_stride : bounds_elems(p, b))
+                     : nullptr;
+}
+// whether [x, x + bytes) and a layer's bounds overlap
+bool in_bounds(const mxh_kv_pool* p, int layer, const mxh_kv_blocks* b, const void* x, size_t bytes) {
+    return overlap(layer_bounds(p, layer, b), sizeof(__half) * (size_t)bounds_elems(p, b), x, bytes);
 }
 
 int check_blocks(const char* who, const mxh_kv_pool* p, const mxh_kv_batch* batch, const mxh_kv_blocks* b, bool bounds) {
@@ -342,8 +349,7 @@ int check_blocks(const char* who, const mxh_kv_pool* p, const mxh_kv_batch* batc
     if (!bounds) return MXH_OK;
     if (!b->bounds || !al16(b->bounds))
         return set_error(MXH_ERR_ARG, "%s: bounds must be non-null and 16-byte aligned", who);
-    if (b->layer_stride && (b->layer_stride % 8 || b->layer_stride < (int64_t)p->n_pages * (p->page_rows / b->block_rows) *
-                                                                         p->n_kv * 2 * p->head_dim))
+    if (b->layer_stride && (b->layer_stride % 8 || b->layer_stride < bounds_elems(p, b)))
         return set_error(MXH_ERR_ARG, "%s: layer_stride %lld of the bounds is less than a layer or no multiple of 8", who,
                          (long long)b->layer_stride);
     return MXH_OK;
@@ -357,8 +363,8 @@ int check_budget(const char* who, const mxh_kv_blocks* b) {
 }
 
 BlocksOf blocks_of(const mxh_kv_pool* p, int layer, const mxh_kv_blocks* b) {
-    return BlocksOf{b->bounds ? static_cast<__half*>(b->bounds) + layer * bounds_elems(p, b) : nullptr,
-                    __builtin_ctz((unsigned)b->block_rows), b->n_first, b->n_last, b->n_select};
+    return BlocksOf{layer_bounds(p, layer, b), __builtin_ctz((unsigned)b->block_rows), b->n_first, b->n_last,
+                    b->n_select};
 }
 
 // marks ids (a bit a page); false where one is marked already
@@ -516,8 +522,12 @@ int mxh_kv_block_bounds(const mxh_kv_pool* pool, int layer, const mxh_kv_batch* 
     if (int rc = check_step(who, pool, layer, batch, pool ? pool->n_kv : 0)) return rc;
     if (int rc = check_blocks(who, pool, batch, blocks, true)) return rc;
     if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
+    const PagedArgs a = paged_args(pool, layer, batch);
+    const size_t rows = sizeof(__half) * (size_t)pool->n_pages * pool->page_rows * pool->n_kv * pool->head_dim;
+    if (in_bounds(pool, layer, blocks, a.k, rows) || in_bounds(pool, layer, blocks, a.v, rows))
+        return set_error(MXH_ERR_ARG, "%s: bounds overlap k or v", who);
     if (!mxh_is_available()) return MXH_ERR_NODEV;
-    block_bounds_launch(paged_args(pool, layer, batch), blocks_of(pool, layer, blocks), pool->head_dim, lib_stream());
+    block_bounds_launch(a, blocks_of(pool, layer, blocks), pool->head_dim, lib_stream());
     return check_hip(hipGetLastError(), "kv_block_bounds launch");
 }
 
@@ -553,6 +563,8 @@ int mxh_kv_select_blocks(const mxh_kv_pool* pool, int layer, const mxh_kv_batch*
         return set_error(MXH_ERR_ARG, "%s: %zu bytes of work, %zu needed", who, work ? work_bytes : 0, need);
     if (overlap(work, need, q, batch_bytes(pool, batch, nh)) || overlap(work, need, chosen, list))
         return set_error(MXH_ERR_ARG, "%s: work overlaps q or chosen", who);
+    if (in_bounds(pool, layer, blocks, chosen, list) || in_bounds(pool, layer, blocks, work, need))
+        return set_error(MXH_ERR_ARG, "%s: chosen or work overlaps the bounds", who);
     if (!mxh_is_available()) return MXH_ERR_NODEV;
     select_blocks_launch(a, b, q, nh, pool->head_dim, chosen, work, lib_stream());
     return check_hip(hipGetLastError(), "kv_select_blocks launch");

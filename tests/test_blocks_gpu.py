@@ -343,6 +343,21 @@ def test_a_token_past_the_table_counts_from_its_last_block(mxh):
     c.close()
 
 
+@pytest.mark.parametrize("new", [1, 40], ids=["few", "many"])
+@pytest.mark.parametrize("keys,queries", [(2.0**-19, 1.0), (1.0, 2.0**-140), (2.0**-19, 2.0**100), (2.0**12, 2.0**120)])
+def test_small_and_large_values(mxh, new, keys, queries):
+    """Bounds and queries of fp16's and fp32's subnormals, and large ones; a few dims of q far above the others."""
+    c = Blocks([(1500, new), (900, new)], block=16, first=1, last=2, select=12, nh=8, nkv=2, hd=64, page=64, seed=8)
+    c.k[:] = (c.k.astype(np.float32) * np.float32(keys)).astype(np.float16)
+    c.q *= np.float32(queries)
+    c.q.reshape(-1, 64)[:, ::7] *= np.float32(2.0**-16)
+    c.fill_bounds()
+    c.upload()
+    c.choose()
+    c.check_chosen(c.got_chosen())
+    c.close()
+
+
 def test_queries_of_infinities_and_nan(mxh):
     """Scores that are no numbers everywhere: the first blocks; of one q head it is the kv head's."""
     c = Blocks([(500, 2)], block=16, first=1, last=1, select=6, nh=4, nkv=2, hd=32, page=16, seed=5)

@@ -185,6 +185,24 @@ def test_arrays_are_checked():
             select(pool(), 0, batch(), **over)
 
 
+def test_bounds_overlap_nothing():
+    """Of the call's layer: 8 pages of 16 rows, 2 kv heads of 64, so 32 KB of K and of V and 4 KB of bounds."""
+    pl, b = pool(), batch()
+    size = 2 * pl.n_pages * pl.page_rows * pl.n_kv * pl.head_dim
+    own = 2 * 2 * pl.n_pages * pl.n_kv * pl.head_dim
+    for at in (pl.k, pl.v):
+        for x in (at - own + 16, at, at + size - 16):
+            with pytest.raises(mxhip.MxhError, match="bounds overlap"):
+                bounds(pl, 0, b, bl=blocks(bounds=x))
+        with pytest.raises(mxhip.MxhError, match="bounds overlap"):
+            bounds(pl, 1, b, bl=blocks(bounds=at + size - own))
+    for over in (dict(chosen=6 * AT + own - 16), dict(work=6 * AT + own - 16), dict(chosen=6 * AT - 16)):
+        with pytest.raises(mxhip.MxhError, match="overlaps the bounds"):
+            select(pl, 0, b, **over)
+    with pytest.raises(mxhip.MxhError, match="overlaps the bounds"):
+        select(pl, 1, b, chosen=6 * AT + own)
+
+
 def test_descriptions_hold_their_buffers():
     made = []
 
