@@ -122,18 +122,17 @@ __device__ __forceinline__ uint64_t order_key(double x) {
     return u ^ (u >> 63 ? ~0ull : 1ull << 63);
 }
 
-// A block's score so far, in units of the token's and kv head's own, and how far it
-// may be off; of an absent block -infinity and 0
-struct Score {
-    float s, off;
-};
+// Of a row of scores (of a token and kv head) the workspace has ld floats, the blocks'
+// scores in units of the row's own (of absent blocks -infinity), and from there one
+// for every 16 blocks, how far their scores may be off.  Where that does not decide,
+// 64-bit keys take their place.
 struct SelectArgs {
     BlockArgs b;
     const float* q;
     int nh, group, tokens;  // q heads of a kv head; tokens of a tile
     int t0, t1;             // tokens of this launch
     int ld;                 // scores of a row, n_blocks and up to a multiple of 16
-    Score* scores;          // [t1 - t0][nkv][ld]
+    float* scores;          // [t1 - t0][nkv][2 ld]
     int* chosen;            // [n_tokens][nkv][n_select]
 };
 
@@ -293,11 +292,9 @@ struct ScoreTile {
             const int u = tt - first;
             float far = 0.f;
             for (int h = 0; h < a.group; ++h) far = fmaxf(far, __shfl(off, u * a.group + h));
-            Score* row = a.scores + ((int64_t)(tt - a.t0) * a.b.pg.nkv + g) * a.ld;
-            for (int i = lane; i < 16 * steps; i += 64) {
-                const float s = kept[u * stride + i];
-                row[b0 + apart * (i >> 4) + (i & 15)] = Score{s, s > -INFINITY ? far : 0.f};
-            }
+            float* row = a.scores + ((int64_t)(tt - a.t0) * a.b.pg.nkv + g) * 2 * a.ld;
+            for (int i = lane; i < 16 * steps; i += 64) row[b0 + apart * (i >> 4) + (i & 15)] = kept[u * stride + i];
+            for (int i = lane; i < steps; i += 64) row[a.ld + ((b0 + apart * i) >> 4)] = far;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         __builtin_amdgcn_wave_barrier();
@@ -437,7 +434,7 @@ __global__ __launch_bounds__(kScoreThreads, 2) void block_score_rows_kernel(Sele
 
 // A block's score in 64 bits, by 16 lanes (in all of them); q: the kv head's q heads
 template <int HD>
-__device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, int g, const float* q, int group) {
+__device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, int g, const float4* q, int group) {
     constexpr int PER = HD / 16;
     typedef _Float16 piece __attribute__((ext_vector_type(PER)));
     typedef float qpiece __attribute__((ext_vector_type(PER)));
@@ -447,7 +444,7 @@ __device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, 
     const piece least = *reinterpret_cast<const piece*>(p), greatest = *reinterpret_cast<const piece*>(p + HD);
     double best = -INFINITY;
     for (int h = 0; h < group; ++h) {
-        const qpiece y = *reinterpret_cast<const qpiece*>(q + h * HD + d);
+        const qpiece y = *reinterpret_cast<const qpiece*>(reinterpret_cast<const float*>(q) + h * HD + d);
         double sum = 0.;
 #pragma unroll
         for (int e = 0; e < PER; ++e)
@@ -466,12 +463,12 @@ __device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, 
 // n-th largest falls into; what lies above it by more than scores are off is taken,
 // what lies below by as much is not, and the few in between are ordered by their
 // scores in 64 bits.  Where they are not few, or scores are not finite, all of them
-// are, eight bits of the n-th largest at a time.
-constexpr int kPickThreads = 256, kPickBins = 512, kPickKeys = 4096, kOpenMax = 128;
-template <int HD>
-__global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs a) {
-    constexpr int WAVES = kPickThreads / 64;
-    __shared__ uint32_t bins[kPickBins], wsum[WAVES];
+// are, a few bits of the n-th largest at a time.
+constexpr int kPickKeys = 4096, kOpenMax = 128;
+template <int HD, int THREADS>
+__global__ __launch_bounds__(THREADS, 8) void block_pick_kernel(SelectArgs a) {
+    constexpr int WAVES = THREADS / 64, BINS = 2 * THREADS, DIGIT = THREADS < 256 ? 4 : 8, DIGITS = 1 << DIGIT;
+    __shared__ uint32_t bins[BINS], wsum[WAVES];
     __shared__ float red[WAVES][3];
     extern __shared__ float keys_lds[];  // [kPickKeys], of n_blocks at most
     __shared__ uint32_t found[2], n_open, n_above;  // a bin, keys wanted of it; blocks that are open, taken
@@ -484,15 +481,24 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
     const Rivals r = rivals(a.b, x);
     int* out = a.chosen + ((int64_t)t * nkv + g) * a.b.n_select;
     if (r.end == 0) {
-        for (int i = tid; i < a.b.n_select; i += kPickThreads) out[i] = i <= r.own ? i : -1;
+        for (int i = tid; i < a.b.n_select; i += THREADS) out[i] = i <= r.own ? i : -1;
         return;
     }
     const int n0 = a.b.n_first, n = r.end - n0, want = a.b.n_select - n0 - a.b.n_last;
-    for (int i = tid; i < n0; i += kPickThreads) out[i] = i;
-    for (int i = tid; i < a.b.n_last; i += kPickThreads) out[n0 + want + i] = r.end + i;
+    for (int i = tid; i < n0; i += THREADS) out[i] = i;
+    for (int i = tid; i < a.b.n_last; i += THREADS) out[n0 + want + i] = r.end + i;
     if (want == 0) return;
-    Score* scores = a.scores + ((int64_t)(t - a.t0) * nkv + g) * a.ld + n0;
-    const float* q = a.q + ((int64_t)t * a.nh + g * a.group) * HD;
+    float* row = a.scores + ((int64_t)(t - a.t0) * nkv + g) * 2 * a.ld;
+    float* scores = row + n0;
+    // (q comes while the scores do)
+    constexpr int PIECES = 2 * HD > THREADS ? 2 * HD / THREADS : 1;
+    __shared__ float4 q[2 * HD];  // [group][HD]
+    const int q_pieces = a.group * (HD / 4);
+    float4 q_mine[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+        q_mine[i] = reinterpret_cast<const float4*>(a.q + ((int64_t)t * a.nh + g * a.group) * HD)
+            [min(tid + i * THREADS, q_pieces - 1)];
     const auto inclusive = [&](uint32_t v) {  // over the workgroup
         v = wave_scan(v);
         __syncthreads();
@@ -505,49 +511,51 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
     // the range of the scores, the most one is off
     const bool held = n <= kPickKeys;
     float least = INFINITY, most = -INFINITY, off = 0.f;
-    for (int i = tid; i < kPickBins; i += kPickThreads) bins[i] = 0;
+    for (int i = tid; i < BINS; i += THREADS) bins[i] = 0;
     if (tid == 0) n_open = n_above = 0;
-    for (int i = tid; i < n; i += kPickThreads) {
-        const Score c = scores[i];
-        if (held) keys_lds[i] = c.s;
-        if (c.s > -INFINITY) least = fminf(least, c.s);
-        most = fmaxf(most, c.s);
-        off = c.s != c.s || !(c.off < INFINITY) ? INFINITY : fmaxf(off, c.off);
+    for (int i = tid; i < n; i += THREADS) {
+        const float s = scores[i];
+        if (held) keys_lds[i] = s;
+        if (s > -INFINITY) least = fminf(least, s);
+        most = fmaxf(most, s);
+        if (s != s) off = INFINITY;
     }
+    for (int i = (n0 >> 4) + tid; i <= (r.end - 1) >> 4; i += THREADS) off = fmaxf(off, row[a.ld + i]);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) q[min(tid + i * THREADS, q_pieces - 1)] = q_mine[i];
     least = -wave_max_all(-least), most = wave_max_all(most), off = wave_max_all(off);
     if (lane == 0) red[wave][0] = least, red[wave][1] = most, red[wave][2] = off;
     __syncthreads();
     for (int w = 0; w < WAVES; ++w) least = fminf(least, red[w][0]), most = fmaxf(most, red[w][1]), off = fmaxf(off, red[w][2]);
-    const auto key = [&](int i) { return held ? keys_lds[i] : scores[i].s; };
+    const auto key = [&](int i) { return held ? keys_lds[i] : scores[i]; };
     bool exact = !(off < INFINITY) || !(fabsf(least) < INFINITY) || !(fabsf(most) < INFINITY);
     float above = 0.f, below = 0.f;
     int taken_above = 0;
     if (!exact) {
-        const float range = most - least, scale = range > 0.f ? (float)(kPickBins - 1) / range : 0.f;
-        const auto bin = [&](float s) { return min((int)((s - least) * scale), kPickBins - 1); };
+        const float range = most - least, scale = range > 0.f ? (float)(BINS - 1) / range : 0.f;
+        const auto bin = [&](float s) { return min((int)((s - least) * scale), BINS - 1); };
         exact = !(scale < INFINITY) || !(range < INFINITY);
-        for (int i = tid; i < n && !exact; i += kPickThreads) {
+        for (int i = tid; i < n && !exact; i += THREADS) {
             const float s = key(i);
             if (s > -INFINITY) atomicAdd(&bins[bin(s)], 1u);
         }
         __syncthreads();
         // bins from the top, two a thread
-        static_assert(kPickBins == 2 * kPickThreads, "");
-        const uint32_t c0 = bins[kPickBins - 1 - 2 * tid], c1 = bins[kPickBins - 2 - 2 * tid];
+            const uint32_t c0 = bins[BINS - 1 - 2 * tid], c1 = bins[BINS - 2 - 2 * tid];
         const uint32_t upto = inclusive(c0 + c1), before = upto - c0 - c1, w = (uint32_t)want;
         if (tid == 0) found[0] = 0xffffffffu;
         __syncthreads();
-        if (before < w && before + c0 >= w) found[0] = (uint32_t)(kPickBins - 1 - 2 * tid);
-        else if (before + c0 < w && upto >= w) found[0] = (uint32_t)(kPickBins - 2 - 2 * tid);
+        if (before < w && before + c0 >= w) found[0] = (uint32_t)(BINS - 1 - 2 * tid);
+        else if (before + c0 < w && upto >= w) found[0] = (uint32_t)(BINS - 2 - 2 * tid);
         __syncthreads();
         if (found[0] == 0xffffffffu) exact = true;  // (fewer blocks are there than wanted)
         else {
             // the bin's edges, with what the sums above round
-            const float width = range / (float)(kPickBins - 1), at = least + (float)found[0] * width;
+            const float width = range / (float)(BINS - 1), at = least + (float)found[0] * width;
             const float slack = 2.f * off + range * 0x1p-18f + fmaxf(fabsf(least), fabsf(most)) * 0x1p-20f;
             above = at + width + slack, below = at - slack;
             uint32_t mine = 0;  // (the wave's)
-            for (int i = tid; i < n; i += kPickThreads) {
+            for (int i = tid; i < n; i += THREADS) {
                 const float s = key(i);
                 mine += (uint32_t)__popcll(__ballot(s > above));
                 if (s >= below && s <= above) {
@@ -565,18 +573,18 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
     if (!exact) {
         const int ours = (int)n_open, need = want - taken_above;
         if (ours != need) {
-            for (int j = tid / 16; j < ours; j += kPickThreads / 16) {
+            for (int j = tid / 16; j < ours; j += THREADS / 16) {
                 const double s = exact_score<HD>(a.b, x.s, n0 + open[j], g, q, a.group);
                 if ((tid & 15) == 0) open_key[j] = order_key(s);
             }
             __syncthreads();
-            if (tid < ours) {
+            for (int i = tid; i < ours; i += THREADS) {
                 int rank = 0;
                 for (int j = 0; j < ours; ++j)
-                    rank += open_key[j] > open_key[tid] || (open_key[j] == open_key[tid] && open[j] < open[tid]);
+                    rank += open_key[j] > open_key[i] || (open_key[j] == open_key[i] && open[j] < open[i]);
                 const float s = rank < need ? INFINITY : -INFINITY;
-                if (held) keys_lds[open[tid]] = s;
-                else scores[open[tid]].s = s;
+                if (held) keys_lds[open[i]] = s;
+                else scores[open[i]] = s;
             }
             __syncthreads();
         }
@@ -604,8 +612,8 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
     }
 
     // all scores in 64 bits, where the others were
-    uint64_t* keys = reinterpret_cast<uint64_t*>(scores);
-    for (int i = tid / 16; i < n; i += kPickThreads / 16) {
+    uint64_t* keys = reinterpret_cast<uint64_t*>(row);
+    for (int i = tid / 16; i < n; i += THREADS / 16) {
         const double s = exact_score<HD>(a.b, x.s, n0 + i, g, q, a.group);
         if ((tid & 15) == 0) keys[i] = order_key(s);
     }
@@ -614,18 +622,18 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
     uint32_t need = (uint32_t)want;
     int shift = 64;
     for (;;) {
-        shift -= 8;
-        bins[tid] = 0;
+        shift -= DIGIT;
+        if (tid < DIGITS) bins[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += kPickThreads) {
+        for (int i = tid; i < n; i += THREADS) {
             const uint64_t k = keys[i];
-            if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&bins[k >> shift & 255], 1u);
+            if (shift + DIGIT == 64 || k >> (shift + DIGIT) == prefix) atomicAdd(&bins[k >> shift & (DIGITS - 1)], 1u);
         }
         __syncthreads();
-        const uint32_t c = bins[255 - tid], upto = inclusive(c);
-        if (upto >= need && upto - c < need) found[0] = 255 - tid, found[1] = need - (upto - c);
+        const uint32_t c = tid < DIGITS ? bins[DIGITS - 1 - tid] : 0, upto = inclusive(c);
+        if (upto >= need && upto - c < need) found[0] = DIGITS - 1 - tid, found[1] = need - (upto - c);
         __syncthreads();
-        prefix = prefix << 8 | found[0], need = found[1];
+        prefix = prefix << DIGIT | found[0], need = found[1];
         const bool all = bins[found[0]] == need;
         __syncthreads();
         if (all || shift == 0) break;
@@ -633,7 +641,7 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
     // those above the prefix, and the first `need` of those with it
     int done = n0;
     uint32_t ties = 0;
-    for (int i0 = 0; i0 < n; i0 += kPickThreads) {
+    for (int i0 = 0; i0 < n; i0 += THREADS) {
         const int i = i0 + tid;
         const uint64_t k = i < n ? keys[i] >> shift : 0;
         const bool larger = i < n && k > prefix, same = i < n && k == prefix;
@@ -642,7 +650,7 @@ __global__ __launch_bounds__(kPickThreads, 8) void block_pick_kernel(SelectArgs 
         const uint32_t upto = inclusive(take);
         if (take) out[done + upto - 1] = n0 + i;
         __syncthreads();
-        if (tid == kPickThreads - 1) found[0] = upto, found[1] = before + same;
+        if (tid == THREADS - 1) found[0] = upto, found[1] = before + same;
         __syncthreads();
         done += found[0], ties = found[1];
         __syncthreads();
@@ -823,8 +831,13 @@ void launch_select(const SelectArgs& a, hipStream_t st) {
             hipLaunchKernelGGL(block_score_rows_kernel<HD>, grid, dim3(kScoreThreads), lds, st, a, (int)iters, (int)chunks);
         else hipLaunchKernelGGL(block_score_kernel<HD>, grid, dim3(kScoreThreads), lds, st, a, (int)iters, (int)chunks);
     }
-    hipLaunchKernelGGL(block_pick_kernel<HD>, dim3((unsigned)(n * nkv)), dim3(kPickThreads),
-                       sizeof(float) * std::min(a.b.n_blocks, kPickKeys), st, a);
+    const dim3 rows((unsigned)(n * nkv));
+    const size_t lds = sizeof(float) * std::min(a.b.n_blocks, kPickKeys);
+    // four waves a row as long as all rows are taken at once, else two: 4,096 rows of 469
+    // blocks 26.4 and 22.2 us, 384 of up to 500 9.4 and 12.2
+    if (n * nkv > 8 * (int64_t)device_cus())
+        hipLaunchKernelGGL((block_pick_kernel<HD, 128>), rows, dim3(128), lds, st, a);
+    else hipLaunchKernelGGL((block_pick_kernel<HD, 256>), rows, dim3(256), lds, st, a);
 }
 
 }  // namespace
@@ -846,7 +859,7 @@ size_t select_blocks_work_bytes(const PagedArgs& pg, const BlocksOf& b) {
 void select_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const float* q, int nh, int hd, int* chosen,
                           void* work, hipStream_t st) {
     const BlockArgs ba = block_args(pg, b);
-    SelectArgs a{ba, q, nh, nh / pg.nkv, 0, 0, 0, (int)select_row(ba.n_blocks), static_cast<Score*>(work), chosen};
+    SelectArgs a{ba, q, nh, nh / pg.nkv, 0, 0, 0, (int)select_row(ba.n_blocks), static_cast<float*>(work), chosen};
     a.tokens = pg.n_tokens > 2 * (int64_t)pg.n_seq ? 16 / a.group : 1;
     const int64_t step = select_tokens(pg.n_tokens, ba.n_blocks, pg.nkv);
     for (int64_t t = 0; t < pg.n_tokens; t += step) {

@@ -312,6 +312,21 @@ def test_of_equal_scores_the_earlier_blocks_are_taken(mxh):
     c.close()
 
 
+def test_equal_scores_and_infinities_of_many_rows(mxh):
+    c = Blocks([(500, 300)], block=16, first=1, last=2, select=9, nh=8, nkv=8, hd=32, page=32, seed=6)
+    c.fill_bounds()
+    c.bounds[0, ::3, :, :4] = 1
+    c.bounds[0, :, :, 4:6] = 2
+    c.bounds[0][c.place(0, 9)][6, 0, 5] = np.inf
+    c.bounds[0][c.place(0, 11)][6, 1, 5] = -np.inf
+    c.q.reshape(-1, 8, 32)[:, 6, 5] = np.where(np.arange(c.tokens) % 3 == 0, -1, 1)
+    c.q.reshape(-1, 8, 32)[:, 7] = 0
+    c.upload()
+    c.choose()
+    c.check_chosen(c.got_chosen())
+    c.close()
+
+
 def test_what_is_no_number_comes_first_and_absent_blocks_last(mxh):
     c = Blocks([(800, 1), (900, 6)], block=16, first=0, last=1, select=4, nh=6, nkv=2, hd=32, page=16, seed=4)
     c.fill_bounds()
