@@ -64,7 +64,10 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
 // Workgroup (tokens [chunk x, + chunk), 64 pieces of 8 dims): the blocks that the
 // tokens are the first new rows of, one after the other; all rows of a block by
-// threads that each take every RG-th, joined through LDS.
+// threads that each take every RG-th, joined through LDS.  Seven prompts of up to
+// 6,000 tokens (35 MB of K with 8 heads of 128) 11 us, one token 4: a launch, and the
+// loads of lengths, page and rows one after the other.  (8 / 16 / 32 / 128 pieces a
+// workgroup 44 / 23 / 16 / 13 us, eight waves 13; sixteen rows at a time 12.7)
 constexpr int kBoundThreads = 256;
 __global__ __launch_bounds__(kBoundThreads) void kv_block_bounds_kernel(BlockArgs a, int chunk, int pieces, int hd8) {
     __shared__ half8 least[kBoundThreads], greatest[kBoundThreads];
@@ -91,12 +94,13 @@ __global__ __launch_bounds__(kBoundThreads) void kv_block_bounds_kernel(BlockArg
 #pragma unroll
         for (int e = 0; e < 8; ++e) lo[e] = (_Float16)INFINITY, hi[e] = -(_Float16)INFINITY;
         if (mine < rg) {
-            const half8* p = reinterpret_cast<const half8*>(a.pg.k) + ((place << a.block_shift) + mine) * pieces + col;
-#pragma unroll 8
-            for (int r = mine; r < n; r += rg, p += (int64_t)rg * pieces) {
-                const half8 v = *p;
-                lo = __builtin_elementwise_min(lo, v);
-                hi = __builtin_elementwise_max(hi, v);
+            const half8* p = reinterpret_cast<const half8*>(a.pg.k) + (place << a.block_shift) * pieces + col;
+            for (int r = mine; r < n; r += 8 * rg) {  // (past the last row the last again)
+                half8 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)min(r + i * rg, n - 1) * pieces];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) lo = __builtin_elementwise_min(lo, v[i]), hi = __builtin_elementwise_max(hi, v[i]);
             }
         }
         least[tid] = lo, greatest[tid] = hi;
@@ -318,6 +322,8 @@ __device__ __forceinline__ void find_places(const SelectArgs& a, int s, int b0, 
 }
 
 // Few tokens: a workgroup takes a tile, its waves different blocks (16 `iters` each).
+// 48 single tokens at up to 16,000 rows, blocks of 32: 18 us for 39 MB of bounds, of
+// which waves wait 56%; one at 60,000, blocks of 64, 6 us.
 constexpr int kScoreThreads = 256, kScoreWaves = 4;
 template <int HD>
 __global__ __launch_bounds__(kScoreThreads, 3) void block_score_kernel(SelectArgs a, int iters, int chunks) {
@@ -366,7 +372,9 @@ __global__ __launch_bounds__(kScoreThreads, 3) void block_score_kernel(SelectArg
 }
 
 // Many tokens: a workgroup takes four tiles, a wave each, and 16 `iters` blocks, whose
-// bounds the waves bring into LDS together, two steps ahead in registers.
+// bounds the waves bring into LDS together, two steps ahead in registers.  512 tokens,
+// 469 blocks: 26 us, of which waves wait half; bounds straight into every wave's
+// registers, as above, take 8 KB of loads a step from the L2s for each of them.
 template <int HD>
 __global__ __launch_bounds__(kScoreThreads, 2) void block_score_rows_kernel(SelectArgs a, int iters, int chunks) {
     extern __shared__ __align__(16) float kept_lds[];  // [waves][tokens][16 iters], places [waves][16 iters]
@@ -464,6 +472,9 @@ __device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, 
 // what lies below by as much is not, and the few in between are ordered by their
 // scores in 64 bits.  Where they are not few, or scores are not finite, all of them
 // are, a few bits of the n-th largest at a time.
+// One token's 8 rows of 938 blocks 10 us, one after the other: its lengths 0.7, scores
+// 2, bins 1, those that are open 0.8, their 64 bits 2.6, the list 1.4.  512 tokens' 4,096
+// rows of 469 blocks 22: some 1,000 vector instructions a wave.
 constexpr int kPickKeys = 4096, kOpenMax = 128;
 template <int HD, int THREADS>
 __global__ __launch_bounds__(THREADS, 8) void block_pick_kernel(SelectArgs a) {
