@@ -23,10 +23,23 @@ struct BlockSize {
     int nkv, group, n_select, block_rows, cus;
 };
 
+// Stages of 128 keys that a token's list has, at most
+inline int64_t block_stages(const BlockSize& a) {
+    return (std::min<int64_t>(a.n_select, a.n_blocks) * a.block_rows + 127) / 128;
+}
 // Tokens that share a tile, and its rows.  Tokens of one sequence attend many of the
 // same blocks, whose rows are then loaded once for all of them; single tokens of
-// sequences (up to two each on average) share nothing and go by themselves.  32 rows
-// where sequences have tokens enough and lists and bits leave room for them: 512
+// sequences (up to two each on average) share nothing and go by themselves, and so do
+// all where that makes little work, 16 stages a CU: a tile's tokens wait for the union
+// of their lists, and for one another's sequences.  Each by itself and in tiles, us
+// (32/8 heads of 128, stages a CU): 30 tokens of one sequence with a stage each 9 and
+// 26, of 16 34 and 38 (15), 60 of 8 25 and 35 (15), of 16 47 and 44 (30); 8 of 32 26 and
+// 24 (8), of 100 61 and 39 (25); 16 sequences of up to 8 of 5 34 and 35 (11), of 16 68
+// and 65 (36).
+inline bool block_alone(const BlockSize& a) {
+    return a.n_tokens <= 2 * (int64_t)a.n_seq || (int64_t)a.n_tokens * a.nkv * block_stages(a) <= 16 * (int64_t)a.cus;
+}
+// 32 rows where sequences have tokens enough and lists and bits leave room for them: 512
 // tokens with 32 of 469 blocks of 64 rows each, of which four tokens together have
 // some 63 and eight some 82 (32/8 heads of 128), 121 us, in tiles of 16 rows 129.
 inline int block_tokens_of(const BlockSize& a, int rows) {
@@ -35,10 +48,10 @@ inline int block_tokens_of(const BlockSize& a, int rows) {
         1, std::min<int64_t>({rows / a.group, 16, kListMax / a.n_select, kBitBytes / (4 * words)}));
 }
 inline int block_rows_of_tile(const BlockSize& a) {
-    return a.n_tokens > 8 * (int64_t)a.n_seq && block_tokens_of(a, 32) * a.group > 16 ? 32 : 16;
+    return !block_alone(a) && a.n_tokens > 8 * (int64_t)a.n_seq && block_tokens_of(a, 32) * a.group > 16 ? 32 : 16;
 }
 inline int block_tokens(const BlockSize& a) {
-    return a.n_tokens <= 2 * (int64_t)a.n_seq ? 1 : block_tokens_of(a, block_rows_of_tile(a));
+    return block_alone(a) ? 1 : block_tokens_of(a, block_rows_of_tile(a));
 }
 inline int64_t block_tiles(const BlockSize& a) {
     const int t = block_tokens(a);
@@ -49,8 +62,8 @@ inline int64_t block_tiles(const BlockSize& a) {
 // 13.3 (and 3.9 for joining their parts).  (48 tokens with 1,280, a workgroup each 53
 // us, two each 55 and 5)
 inline int block_splits(const BlockSize& a) {
-    const int64_t items = block_tiles(a) * a.nkv, stages = ((int64_t)a.n_select * a.block_rows + 127) / 128;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)a.cus / items, stages, 64}));
+    const int64_t items = block_tiles(a) * a.nkv;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({2 * (int64_t)a.cus / items, block_stages(a), 64}));
 }
 // the workspace: parts of the tiles that are split
 inline size_t block_part_bytes(int64_t parts, int rows, int nkv, int hd) {

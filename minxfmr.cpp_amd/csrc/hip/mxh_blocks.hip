@@ -899,7 +899,7 @@ int attention_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const int* c
     float* part = static_cast<float*>(work);
     // single tokens whose rows are more than half of the last cache's 256 MB: 48 of them
     // with 1,280 rows for each of 8 kv heads of 128 53 us, 47 so
-    const bool once = block_tokens(size) == 1 && (double)pg.n_tokens * pg.nkv * b.n_select * size.block_rows * hd * 4 > 128e6;
+    const bool once = pg.n_tokens <= 2 * (int64_t)pg.n_seq && (double)pg.n_tokens * pg.nkv * b.n_select * size.block_rows * hd * 4 > 128e6;
     const BlockAttnArgs a{{pg, q, att, part, reinterpret_cast<float2*>(part + (size_t)tiles * splits * pg.nkv * block_rows_of_tile(size) * hd),
                            nh, 1.4426950408889634f / sqrtf((float)hd), group, (uint32_t)block_tokens(size),
                            (65536 + group - 1) / group},

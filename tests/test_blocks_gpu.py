@@ -471,6 +471,75 @@ def test_what_is_not_listed_or_attended_has_no_effect(mxh, tree):
     c.close()
 
 
+def thin_lists(c, few=5):
+    """Lists with places for more blocks than the few that stand in them: tokens go in tiles where their lists may be
+    long (16 stages of 128 keys a CU and more)."""
+    c.random_lists(c.rng)
+    c.chosen[c.rng.random(c.chosen.shape) < 1 - few / c.select] = -1
+    assert c.tokens * c.nkv * (c.select * c.block // 128) > 16 * 256
+
+
+def tiles():
+    """Cases and the shortest lists, of 64, 128 or 256 blocks, with which they have tiles."""
+    for name in ("prompts", "tree-64", "trees", "chunks", "empty-among", "prompt"):
+        tokens = sum(n for _, n in {**SETS, **TREES, **LONG, **DRAFTS}[name])
+        for heads, (_, nkv, _) in HEADS.items():
+            for size in ((256, 128), (64, 16)):
+                enough = [s for s in (64, 128, 256) if tokens * nkv * (s * size[1] // 128) > 16 * 256]
+                if enough:
+                    yield pytest.param(name, heads, size, enough[0], id=f"{name}-{heads}-{size[0]}-{size[1]}")
+
+
+@pytest.mark.parametrize("name,heads,size,select", tiles())
+def test_tiles_of_tokens(mxh, name, heads, size, select):
+    """... of one sequence and of several, 16 and 32 rows, whole and split."""
+    c = case(name, heads, size, select=select, extra_ld=select * size[1] // size[0])
+    thin_lists(c)
+    c.upload()
+    c.check_listed(c.attention(), c.chosen)
+    c.close()
+
+
+def test_tiles_of_many_sequences(mxh):
+    rng = np.random.default_rng(9)
+    seqs = [(int(rng.integers(0, 200)), int(rng.choice([0, 0, 1, 2, 5, 12]))) for _ in range(150)]
+    c = Blocks(seqs, block=16, select=100, nh=4, nkv=2, hd=32, page=16, seed=8, lead=3, tail=5, extra_ld=100)
+    assert c.tokens > 2 * len(seqs)
+    thin_lists(c)
+    c.upload()
+    c.check_listed(c.attention(), c.chosen)
+    c.close()
+
+
+@pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
+@pytest.mark.parametrize("select", [200, 300])  # tiles of 32 and of 16 rows
+def test_in_tiles_what_is_not_listed_or_attended_has_no_effect(mxh, tree, select):
+    c = Blocks([(200, 40), (330, 21), (150, 1)], block=16, select=select, nh=16, nkv=4, hd=64, page=16, tree=tree, seed=11,
+               extra_ld=300)
+    thin_lists(c)
+    bad = {0: [207, 230, 33], 1: [350, 100], 2: [7]}
+    for s, rows in bad.items():
+        for i, r in enumerate(rows):
+            c.row(c.v, s, r)[i::3] = [np.inf, -np.inf, np.nan][i]
+            c.row(c.k, s, r)[i::5] = [-np.inf, np.nan, np.inf][i]
+    free, hit = set(), []
+    for s, (n_c, n) in enumerate(c.seqs):
+        for i in range(n):
+            t = int(c.start[s]) + i
+            at = set(range(n_c)) | {n_c + j for j in c.before(s, i)}
+            on = [{r // 16 for r in bad[s] if r in at} & set(c.chosen[t, g].tolist()) for g in range(4)]
+            if not any(on):
+                free.add(t)
+            hit += [(t, g) for g in range(4) if on[g]]
+    assert len(free) >= 5 and len(hit) >= 5
+    c.upload()
+    got = c.attention()
+    c.check_listed(got, c.chosen, rows=free)
+    for t, g in hit:
+        assert not np.all(np.isfinite(got[t, 4 * g:4 * g + 4]))
+    c.close()
+
+
 def test_rows_behind_a_sequence_do_not_matter(mxh):
     """The rest of the last page holds NaN already; of a listed block that is absent nothing is read."""
     c = Blocks([(37, 2), (100, 1)], block=32, select=4, nh=4, nkv=2, hd=128, page=64, seed=12)
