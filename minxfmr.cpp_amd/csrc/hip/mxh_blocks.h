@@ -30,14 +30,16 @@ inline int64_t block_stages(const BlockSize& a) {
 // Tokens that share a tile, and its rows.  Tokens of one sequence attend many of the
 // same blocks, whose rows are then loaded once for all of them; single tokens of
 // sequences (up to two each on average) share nothing and go by themselves, and so do
-// all where that makes little work, 16 stages a CU: a tile's tokens wait for the union
-// of their lists, and for one another's sequences.  Each by itself and in tiles, us
-// (32/8 heads of 128, stages a CU): 30 tokens of one sequence with a stage each 9 and
-// 26, of 16 34 and 38 (15), 60 of 8 25 and 35 (15), of 16 47 and 44 (30); 8 of 32 26 and
-// 24 (8), of 100 61 and 39 (25); 16 sequences of up to 8 of 5 34 and 35 (11), of 16 68
-// and 65 (36).
+// all where that makes little work, 46 stages a CU with four for a token's start: in a
+// tile they wait for the union of their lists, and for one another's sequences.  All
+// by themselves and in tiles, us (32/8 heads of 128; work): 40 tokens of two sequences,
+// a stage each 9 and 26 (6); of one sequence 30 of 16 27 and 37 (19), 60 of 16 35 and
+// 44 (38), 100 of 16 65 and 56 (63), 120 of 4 29 and 34 (30), 200 of 3.5 49 and 38 (47),
+// 8 of 100 40 and 39 (26); of 16 sequences up to 8 each of 16 57 and 65 (45), of 4 up to 30
+// 35 and 51 (45).
 inline bool block_alone(const BlockSize& a) {
-    return a.n_tokens <= 2 * (int64_t)a.n_seq || (int64_t)a.n_tokens * a.nkv * block_stages(a) <= 16 * (int64_t)a.cus;
+    return a.n_tokens <= 2 * (int64_t)a.n_seq ||
+           (int64_t)a.n_tokens * a.nkv * (block_stages(a) + 4) <= 46 * (int64_t)a.cus;
 }
 // 32 rows where sequences have tokens enough and lists and bits leave room for them: 512
 // tokens with 32 of 469 blocks of 64 rows each, of which four tokens together have

@@ -471,12 +471,17 @@ def test_what_is_not_listed_or_attended_has_no_effect(mxh, tree):
     c.close()
 
 
+def in_tiles(tokens, nkv, select, block):
+    """Whether the tokens make 46 stages of 128 keys a CU, four for a token's start among them."""
+    return tokens * nkv * (select * block // 128 + 4) > 46 * 256
+
+
 def thin_lists(c, few=5):
     """Lists with places for more blocks than the few that stand in them: tokens go in tiles where their lists may be
-    long (16 stages of 128 keys a CU and more)."""
+    long (see in_tiles)."""
     c.random_lists(c.rng)
     c.chosen[c.rng.random(c.chosen.shape) < 1 - few / c.select] = -1
-    assert c.tokens * c.nkv * (c.select * c.block // 128) > 16 * 256
+    assert in_tiles(c.tokens, c.nkv, c.select, c.block)
 
 
 def tiles():
@@ -485,7 +490,7 @@ def tiles():
         tokens = sum(n for _, n in {**SETS, **TREES, **LONG, **DRAFTS}[name])
         for heads, (_, nkv, _) in HEADS.items():
             for size in ((256, 128), (64, 16)):
-                enough = [s for s in (64, 128, 256) if tokens * nkv * (s * size[1] // 128) > 16 * 256]
+                enough = [s for s in (64, 128, 256) if in_tiles(tokens, nkv, s, size[1])]
                 if enough:
                     yield pytest.param(name, heads, size, enough[0], id=f"{name}-{heads}-{size[0]}-{size[1]}")
 
@@ -514,9 +519,9 @@ def test_tiles_of_many_sequences(mxh):
 @pytest.mark.parametrize("tree", [False, True], ids=["causal", "tree"])
 @pytest.mark.parametrize("select", [200, 300])  # tiles of 32 and of 16 rows
 def test_in_tiles_what_is_not_listed_or_attended_has_no_effect(mxh, tree, select):
-    c = Blocks([(200, 40), (330, 21), (150, 1)], block=16, select=select, nh=16, nkv=4, hd=64, page=16, tree=tree, seed=11,
+    c = Blocks([(200, 40), (330, 21), (150, 1)], block=16, select=select, nh=32, nkv=8, hd=64, page=16, tree=tree, seed=11,
                extra_ld=300)
-    thin_lists(c)
+    thin_lists(c, few=1)
     bad = {0: [207, 230, 33], 1: [350, 100], 2: [7]}
     for s, rows in bad.items():
         for i, r in enumerate(rows):
@@ -527,10 +532,10 @@ def test_in_tiles_what_is_not_listed_or_attended_has_no_effect(mxh, tree, select
         for i in range(n):
             t = int(c.start[s]) + i
             at = set(range(n_c)) | {n_c + j for j in c.before(s, i)}
-            on = [{r // 16 for r in bad[s] if r in at} & set(c.chosen[t, g].tolist()) for g in range(4)]
+            on = [{r // 16 for r in bad[s] if r in at} & set(c.chosen[t, g].tolist()) for g in range(8)]
             if not any(on):
                 free.add(t)
-            hit += [(t, g) for g in range(4) if on[g]]
+            hit += [(t, g) for g in range(8) if on[g]]
     assert len(free) >= 5 and len(hit) >= 5
     c.upload()
     got = c.attention()
