@@ -871,7 +871,14 @@ void select_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const float* q
                           void* work, hipStream_t st) {
     const BlockArgs ba = block_args(pg, b);
     SelectArgs a{ba, q, nh, nh / pg.nkv, 0, 0, 0, (int)select_row(ba.n_blocks), static_cast<float*>(work), chosen};
-    a.tokens = pg.n_tokens > 2 * (int64_t)pg.n_seq ? 16 / a.group : 1;
+    // tokens by themselves also where that makes little work (64 blocks of a token and kv
+    // head, 1.5 a CU), as those of a tile wait for one another's sequences.  Up to 8
+    // tokens of 6 sequences of 16 blocks 5.0 us, in tiles 16.9, up to 15 of 4 of 28 5.3 and
+    // 12.4; 8 of one of 469 (2) 9.4 and 8.4, 15 (4) 15.0 and 9.5, up to 30 of 4 of 156 (7)
+    // 15.5 and 12.9
+    const bool alone = pg.n_tokens <= 2 * (int64_t)pg.n_seq ||
+                       2 * (int64_t)pg.n_tokens * pg.nkv * ((ba.n_blocks + 63) / 64) <= 3 * (int64_t)device_cus();
+    a.tokens = alone ? 1 : 16 / a.group;
     const int64_t step = select_tokens(pg.n_tokens, ba.n_blocks, pg.nkv);
     for (int64_t t = 0; t < pg.n_tokens; t += step) {
         a.t0 = (int)t, a.t1 = (int)std::min<int64_t>(t + step, pg.n_tokens);

@@ -271,6 +271,20 @@ def test_chosen_blocks(mxh, name, heads, size):
     c.close()
 
 
+@pytest.mark.parametrize("heads", list(HEADS))
+@pytest.mark.parametrize("name", ["chunks", "empty-among", "prompt", "trees"])
+@pytest.mark.parametrize("size", [(16, 16), (128, 64)], ids=lambda s: f"{s[0]}-{s[1]}")
+def test_chosen_blocks_in_tiles(mxh, name, heads, size):
+    """Rows of the table wide enough that tokens share tiles (1.5 times 64 blocks of a token and kv head a CU)."""
+    c = case(name, heads, size, extra_ld=2500 * size[1] // size[0])
+    assert 2 * c.tokens * c.nkv * (c.ld * size[0] // size[1] // 64) > 3 * 256
+    c.fill_bounds()
+    c.upload()
+    c.choose()
+    c.check_chosen(c.got_chosen())
+    c.close()
+
+
 @pytest.mark.parametrize("first,last,select", [(0, 1, 1), (0, 1, 2), (3, 4, 7), (2, 1, 40), (0, 5, 64), (1, 1, 200)])
 def test_budgets(mxh, first, last, select):
     c = Blocks([(3000, 1), (1500, 20), (700, 1)], block=16, first=first, last=last, select=select, nh=8, nkv=2, hd=64,
@@ -362,7 +376,8 @@ def test_a_token_past_the_table_counts_from_its_last_block(mxh):
 @pytest.mark.parametrize("keys,queries", [(2.0**-19, 1.0), (1.0, 2.0**-140), (2.0**-19, 2.0**100), (2.0**12, 2.0**120)])
 def test_small_and_large_values(mxh, new, keys, queries):
     """Bounds and queries of fp16's and fp32's subnormals, and large ones; a few dims of q far above the others."""
-    c = Blocks([(1500, new), (900, new)], block=16, first=1, last=2, select=12, nh=8, nkv=2, hd=64, page=64, seed=8)
+    c = Blocks([(1500, new), (900, new)], block=16, first=1, last=2, select=12, nh=8, nkv=2, hd=64, page=64, seed=8,
+               extra_ld=0 if new == 1 else 300)
     c.k[:] = (c.k.astype(np.float32) * np.float32(keys)).astype(np.float16)
     c.q *= np.float32(queries)
     c.q.reshape(-1, 64)[:, ::7] *= np.float32(2.0**-16)
