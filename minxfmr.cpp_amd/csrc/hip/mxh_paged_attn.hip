@@ -117,7 +117,7 @@ __device__ __forceinline__ uint32_t item_index() { return blockIdx.y + gridDim.y
 //   us (263 to 270 card to card) = 464 TFLOP/s of the formula's, 930 of the products
 //   made (a large fp16 product 1,184); matrix cores and vector units half busy
 //   each, and neither fewer reads nor fewer exponentials made it faster by more
-//   than 4%.  27 drafted tokens at 8,192 rows 24.2 us: 8 stages an item 12 of them
+//   than 4%.  27 drafted tokens at 8,192 rows 24.8 us: 8 stages an item 12 of them
 //   (a stage's loads are one stage ahead and HBM is 1.4 us away), what comes before
 //   and after an item's stages 8, the second kernel 4.
 // Many sequences: every workgroup plans for itself, so 1,024 single tokens at up to
