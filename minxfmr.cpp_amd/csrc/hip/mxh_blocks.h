@@ -83,13 +83,20 @@ inline size_t block_work_bound(const BlockSize& a, int hd) {
 
 // Selecting: scores of a token and kv head (whole tiles of 16 blocks), and tokens whose
 // scores the workspace holds at a time
+constexpr int64_t kSelectBytes = 256 << 20;
 inline int64_t select_row(int64_t n_blocks) { return (n_blocks + 15) / 16 * 16; }
 inline int64_t select_tokens(int n_tokens, int64_t n_blocks, int nkv) {
     const int64_t row = select_row(n_blocks) * nkv * 8;
-    return std::min<int64_t>(n_tokens, std::max<int64_t>(16, ((256 << 20) / row) / 16 * 16));
+    return std::min<int64_t>(n_tokens, std::max<int64_t>(16, kSelectBytes / row / 16 * 16));
 }
 inline size_t select_work_bytes(int n_tokens, int64_t n_blocks, int nkv) {
     return (size_t)select_tokens(n_tokens, n_blocks, nkv) * (size_t)(select_row(n_blocks) * nkv) * 8;
+}
+// ... of any batch up to this n_tokens and n_blocks: tokens come in sixteens, so rows a
+// little shorter may fill more of the 256 MB
+inline size_t select_work_bound(int n_tokens, int64_t n_blocks, int nkv) {
+    const int64_t row = select_row(n_blocks) * nkv * 8;
+    return (size_t)std::min<int64_t>(n_tokens * row, std::max<int64_t>(kSelectBytes, 16 * row));
 }
 
 }  // namespace mxh

@@ -867,6 +867,10 @@ size_t select_blocks_work_bytes(const PagedArgs& pg, const BlocksOf& b) {
     return select_work_bytes(pg.n_tokens, blocks_of_table(pg, b.block_shift), pg.nkv);
 }
 
+size_t select_blocks_work_bound(const PagedArgs& pg, const BlocksOf& b) {
+    return select_work_bound(pg.n_tokens, blocks_of_table(pg, b.block_shift), pg.nkv);
+}
+
 void select_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const float* q, int nh, int hd, int* chosen,
                           void* work, hipStream_t st) {
     const BlockArgs ba = block_args(pg, b);

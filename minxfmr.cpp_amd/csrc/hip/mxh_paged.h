@@ -97,6 +97,7 @@ __host__ __device__ __forceinline__ int64_t blocks_of_table(const PagedArgs& a, 
 }
 void block_bounds_launch(const PagedArgs& a, const BlocksOf& b, int hd, hipStream_t st);
 size_t select_blocks_work_bytes(const PagedArgs& a, const BlocksOf& b);
+size_t select_blocks_work_bound(const PagedArgs& a, const BlocksOf& b);  // of any up to its n_tokens, table_ld
 void select_blocks_launch(const PagedArgs& a, const BlocksOf& b, const float* q, int nh, int hd, int* chosen,
                           void* work, hipStream_t st);
 size_t attention_blocks_work_bytes(const PagedArgs& a, const BlocksOf& b, int nh, int hd);

@@ -540,7 +540,7 @@ int mxh_kv_select_workspace(const mxh_kv_pool* pool, const mxh_kv_batch* batch, 
     if (int rc = check_blocks(who, pool, batch, blocks, false)) return rc;
     if (int rc = check_budget(who, blocks)) return rc;
     if (batch->n_seq == 0 || batch->n_tokens == 0) return MXH_OK;
-    *bytes = select_blocks_work_bytes(paged_args(pool, 0, batch), blocks_of(pool, 0, blocks));
+    *bytes = select_blocks_work_bound(paged_args(pool, 0, batch), blocks_of(pool, 0, blocks));
     return MXH_OK;
 }
 

@@ -351,7 +351,7 @@ def kv_block_bounds(pool: KvPool, layer: int, batch: KvBatch, blocks: KvBlocks) 
 
 
 def kv_select_workspace(pool: KvPool, batch: KvBatch, blocks: KvBlocks, nh: int) -> int:
-    """Bytes of work that kv_select_blocks needs for batches of this n_tokens and table_ld."""
+    """Bytes of work that kv_select_blocks needs for any batch of up to this n_tokens and table_ld."""
     n = C.c_size_t()
     check(lib.mxh_kv_select_workspace(C.byref(pool), C.byref(batch), C.byref(blocks), nh, C.byref(n)),
           "mxh_kv_select_workspace")

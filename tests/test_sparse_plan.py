@@ -203,6 +203,24 @@ def test_bounds_overlap_nothing():
         select(pl, 1, b, chosen=6 * AT + own)
 
 
+def test_the_selection_workspace_is_enough_for_shorter_tables_and_fewer_tokens():
+    """What the query says of a batch, every call up to its tokens and its table's width takes (and then refuses its
+    arrays, so that none gets to a GPU)."""
+    rng = random.Random(7)
+    wide = [(8, 2048, 2064, 2048, 2048), (8, 512, 8193, 8177, 512), (8, 40, 262144, 70000, 39)]
+    for _ in range(300):
+        nkv, tokens, ld = rng.choice([1, 2, 8, 40]), int(2 ** rng.uniform(0, 20)), int(2 ** rng.uniform(0, 18))
+        wide.append((nkv, tokens, ld, rng.randint(max(1, ld - 40), ld), rng.randint(max(1, tokens - 40), tokens)))
+        wide.append((nkv, tokens, ld, rng.randint(1, ld), rng.randint(1, tokens)))
+    for nkv, tokens, ld, less_ld, less_tokens in wide:
+        pl = pool(n_kv=nkv)
+        enough = mxhip.kv_select_workspace(pl, batch(n_tokens=tokens, table_ld=ld), blocks(), nkv)
+        b = batch(n_tokens=less_tokens, table_ld=less_ld)
+        assert mxhip.kv_select_workspace(pl, b, blocks(), nkv) <= enough
+        with pytest.raises(mxhip.MxhError, match="work overlaps"):
+            select(pl, 0, b, nh=nkv, q=1 << 45, chosen=1 << 44, work=1 << 44, nbytes=enough)
+
+
 def test_descriptions_hold_their_buffers():
     made = []
 
