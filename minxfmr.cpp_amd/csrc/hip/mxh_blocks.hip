@@ -120,10 +120,11 @@ __global__ __launch_bounds__(kBoundThreads) void kv_block_bounds_kernel(BlockArg
 
 // ---- selection -------------------------------------------------------------
 
-// Scores as 64-bit integers that order as the doubles do, NaN as +infinity
+// Scores as 64-bit integers that order as the doubles do, NaN above all of them (0 is
+// below all: absent blocks)
 __device__ __forceinline__ uint64_t order_key(double x) {
-    const uint64_t u = (uint64_t)__double_as_longlong(x == x ? x + 0.0 : (double)INFINITY);
-    return u ^ (u >> 63 ? ~0ull : 1ull << 63);
+    const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+    return x != x ? ~0ull : u ^ (u >> 63 ? ~0ull : 1ull << 63);
 }
 
 // Of a row of scores (of a token and kv head) the workspace has ld floats, the blocks'
@@ -440,9 +441,10 @@ __global__ __launch_bounds__(kScoreThreads, 2) void block_score_rows_kernel(Sele
     }
 }
 
-// A block's score in 64 bits, by 16 lanes (in all of them); q: the kv head's q heads
+// A block's score in 64 bits as order_key has it, by 16 lanes (in all of them); q: the
+// kv head's q heads
 template <int HD>
-__device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, int g, const float4* q, int group) {
+__device__ __forceinline__ uint64_t exact_key(const BlockArgs& a, int s, int b, int g, const float4* q, int group) {
     constexpr int PER = HD / 16;
     typedef _Float16 piece __attribute__((ext_vector_type(PER)));
     typedef float qpiece __attribute__((ext_vector_type(PER)));
@@ -464,7 +466,7 @@ __device__ __forceinline__ double exact_score(const BlockArgs& a, int s, int b, 
         sum += dpp_d<0x140>(sum);
         best = best != best ? best : sum > best || sum != sum ? sum : best;
     }
-    return place < 0 ? -INFINITY : best;
+    return place < 0 ? 0 : order_key(best);
 }
 
 // Workgroup (token, kv head).  The scores' range in equal bins; the bin that the
@@ -585,8 +587,8 @@ __global__ __launch_bounds__(THREADS, 8) void block_pick_kernel(SelectArgs a) {
         const int ours = (int)n_open, need = want - taken_above;
         if (ours != need) {
             for (int j = tid / 16; j < ours; j += THREADS / 16) {
-                const double s = exact_score<HD>(a.b, x.s, n0 + open[j], g, q, a.group);
-                if ((tid & 15) == 0) open_key[j] = order_key(s);
+                const uint64_t k = exact_key<HD>(a.b, x.s, n0 + open[j], g, q, a.group);
+                if ((tid & 15) == 0) open_key[j] = k;
             }
             __syncthreads();
             for (int i = tid; i < ours; i += THREADS) {
@@ -625,8 +627,8 @@ __global__ __launch_bounds__(THREADS, 8) void block_pick_kernel(SelectArgs a) {
     // all scores in 64 bits, where the others were
     uint64_t* keys = reinterpret_cast<uint64_t*>(row);
     for (int i = tid / 16; i < n; i += THREADS / 16) {
-        const double s = exact_score<HD>(a.b, x.s, n0 + i, g, q, a.group);
-        if ((tid & 15) == 0) keys[i] = order_key(s);
+        const uint64_t k = exact_key<HD>(a.b, x.s, n0 + i, g, q, a.group);
+        if ((tid & 15) == 0) keys[i] = k;
     }
     __syncthreads();
     uint64_t prefix = 0;

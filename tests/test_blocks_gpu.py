@@ -750,3 +750,40 @@ def test_workspaces_that_are_too_small_are_refused(mxh):
     mxhip.synchronize()
     assert np.all(c.bufs["att"].download(np.float32) == FILL) and np.all(c.got_chosen() == 3)
     c.close()
+
+
+@pytest.mark.parametrize("new", [1, 300], ids=["few", "many"])
+def test_no_number_comes_before_infinity(mxh, new):
+    """A score of +inf is a number: an earlier block with it stands behind a later one whose score is none."""
+    for select, want in ((2, [9]), (3, [4, 9]), (4, [4, 6, 9])):
+        c = Blocks([(800, new)], block=16, first=0, last=1, select=select, nh=8, nkv=8, hd=32, page=16, seed=4)
+        c.fill_bounds()
+        c.q[:] = 1
+        for b, x in ((4, np.inf), (6, np.inf), (9, np.nan)):
+            p, at = c.place(0, b)
+            c.bounds[0, p, at, :, 1, 5] = x
+        c.upload()
+        c.choose()
+        got = c.got_chosen()
+        for i in range(new):
+            assert np.all(got[i] == want + [(800 + i) // 16]), (i, got[i, 0])
+        c.close()
+
+
+@pytest.mark.parametrize("new", [1, 300], ids=["few", "many"])
+def test_minus_infinity_comes_before_absent_blocks(mxh, new):
+    c = Blocks([(800, new)], block=16, first=0, last=1, select=5, nh=8, nkv=8, hd=32, page=16, seed=4)
+    c.fill_bounds()
+    c.q[:] = 1
+    for b in range(50):
+        if b not in (20, 33):
+            p, at = c.place(0, b)
+            c.bounds[0, p, at, :, 1, 5] = -np.inf
+    c.table[0, :6] = c.n_pages
+    c.upload()
+    c.choose()
+    got = c.got_chosen()
+    for i in range(16):
+        if i < new:
+            assert np.all(got[i] == [6, 7, 20, 33, 50]), (i, got[i, 0])
+    c.close()
