@@ -315,9 +315,15 @@ __device__ __forceinline__ const half8* bounds_at(const SelectArgs& a, int place
 }
 
 // Places of `steps` times 16 blocks, b0 + apart j, of a wave's, into LDS before the
-// loop that reads them: a table load in there would have every step wait for it
-__device__ __forceinline__ void find_places(const SelectArgs& a, int s, int b0, int apart, int steps, int* places, int lane) {
-    for (int i = lane; i < 16 * steps; i += 64) places[i] = (int)block_place(a.b, s, b0 + apart * (i >> 4) + (i & 15));
+// loop that reads them: a table load in there would have every step wait for it.
+// Blocks below n_first and from `end` on compete for no token of the run: -1, as what
+// lies in their bounds (nothing yet, behind the sequence) is not to count in `size`
+__device__ __forceinline__ void find_places(const SelectArgs& a, int s, int b0, int apart, int steps, int end, int* places,
+                                            int lane) {
+    for (int i = lane; i < 16 * steps; i += 64) {
+        const int b = b0 + apart * (i >> 4) + (i & 15);
+        places[i] = b >= a.b.n_first && b < end ? (int)block_place(a.b, s, b) : -1;
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
 }
@@ -349,7 +355,7 @@ __global__ __launch_bounds__(kScoreThreads, 3) void block_score_kernel(SelectArg
         const int hi = min(rivals(a.b, TokenAt{x.s, x.i + stop - 1 - t, x.cached, x.n}).end, top);
         if (hi > lo) {
             const int steps = (hi - lo + STEP - 1) / STEP;
-            find_places(a, x.s, lo, STEP, steps, places, lane);
+            find_places(a, x.s, lo, STEP, steps, hi, places, lane);
             int place = places[m];
             half8 v[KS];
 #pragma unroll
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(kScoreThreads, 2) void block_score_rows_kernel(Sele
         const int hi = min(rivals(a.b, TokenAt{x.s, x.i + stop - 1 - t, x.cached, x.n}).end, top);
         if (hi > lo) {
             const int steps = (hi - lo + 15) >> 4;
-            find_places(a, x.s, lo, 16, steps, places, lane);
+            find_places(a, x.s, lo, 16, steps, hi, places, lane);
             // step `at`'s place and pieces, steps in their order (past the last the last's again)
             int at = 0;
             const auto fetch = [&](half8 (&v)[OWN]) __attribute__((always_inline)) {

@@ -787,3 +787,30 @@ def test_minus_infinity_comes_before_absent_blocks(mxh, new):
         if i < new:
             assert np.all(got[i] == [6, 7, 20, 33, 50]), (i, got[i, 0])
     c.close()
+
+
+@pytest.mark.parametrize("seqs,nh,extra_ld", [([(300, 1)], 8, 3), ([(300, 12)], 8, 70), ([(300, 40), (70, 40)], 8, 70)],
+                         ids=["tokens-alone", "a-tile", "tiles"])
+def test_bounds_of_blocks_that_do_not_compete_have_no_effect(mxh, seqs, nh, extra_ld):
+    """Behind a sequence and outside its rivals whatever lies there: not even what scores may be off by takes it in
+    (with an infinity there all scores would be made again in 64 bits).  That stands in the workspace's rows of
+    2 x (blocks of a row of the table, in sixteens) floats, in the second half, one for every 16 blocks."""
+    c = Blocks(seqs, block=16, first=1, last=2, select=6, nh=nh, nkv=2, hd=64, page=256, seed=9, extra_ld=extra_ld)
+    c.fill_bounds()
+    want = c.bounds.copy()
+    c.bounds[:] = np.nan
+    for s, (n_c, n) in enumerate(seqs):
+        p, x = zip(*(c.place(s, b) for b in range(1, (n_c + n - 1) // 16 + 1 - 2)))
+        c.bounds[0, p, x] = want[0, p, x]
+    c.upload()
+    c.choose()
+    c.check_chosen(c.got_chosen())
+    row = (c.ld * 16 + 15) // 16 * 16
+    marks = c.bufs["s_work"].download(np.float32)[:c.tokens * c.nkv * 2 * row].reshape(c.tokens, c.nkv, 2, row)[:, :, 1]
+    for s, (n_c, n) in enumerate(seqs):
+        for i in range(n):
+            end = (n_c + i) // 16 + 1 - 2
+            if (n_c + i) // 16 >= c.select:
+                m = marks[int(c.start[s]) + i, :, :(end + 15) // 16]
+                assert np.all((m > 0) & (m < 1e30)), (s, i)
+    c.close()
