@@ -15,6 +15,7 @@ import pytest
 
 import mxhip
 from test_graph_capture_gpu import Graph
+from test_paged_edges_gpu import check_precision
 from test_paged_gpu import FILL, HEADS, SETS, TREES, U, Case
 
 pytestmark = pytest.mark.gpu
@@ -814,3 +815,102 @@ def test_bounds_of_blocks_that_do_not_compete_have_no_effect(mxh, seqs, nh, extr
                 m = marks[int(c.start[s]) + i, :, :(end + 15) // 16]
                 assert np.all((m > 0) & (m < 1e30)), (s, i)
     c.close()
+
+
+@pytest.mark.parametrize("nh", [8, 32])  # a tile, and tiles enough for four a workgroup
+def test_scores_of_more_than_the_workspace_holds(mxh, nh):
+    """262,144 blocks a sequence, most of them absent, 8 kv heads: scores of 16 tokens fill the workspace, so that
+    three launches use it."""
+    c = Blocks([(900, 20), (300, 21)], block=16, select=8, nh=nh, nkv=8, hd=32, page=16, seed=6, extra_ld=262144 - 58,
+               lead=1, tail=1)
+    assert c.ld == 262144 and 32 < c.tokens <= 48 and 16 * c.ld * c.nkv * 8 == 256 << 20
+    c.fill_bounds()
+    c.upload()
+    for _ in range(2):
+        c.choose()
+        c.check_chosen(c.got_chosen())
+    c.close()
+
+
+@pytest.mark.parametrize("heads", [(64, 8, 128), (8, 8, 128), (32, 8, 64)], ids=lambda h: "-".join(map(str, h)))
+@pytest.mark.parametrize("equal", [False, True], ids=["", "equal-scores"])
+def test_many_rows(mxh, heads, equal):
+    """More rows of scores than are picked from at a time (8 a CU), where two waves take one."""
+    nh, nkv, hd = heads
+    c = Blocks([(500, 290), (340, 10)], block=16, select=9, nh=nh, nkv=nkv, hd=hd, page=32, seed=6)
+    assert c.tokens * nkv > 8 * 256
+    c.fill_bounds()
+    if equal:
+        c.bounds[0, ::3] = 1
+        c.bounds[0][c.place(0, 9)][:, 0, 5] = np.inf
+    c.upload()
+    c.choose()
+    c.check_chosen(c.got_chosen())
+    c.close()
+
+
+@pytest.mark.parametrize("equal", [False, True], ids=["", "equal-scores"])
+def test_many_rows_of_more_blocks_than_lds_holds(mxh, equal):
+    """4,300 rivals of 2,240 rows of scores: two waves a row, scores left where they are."""
+    nkv, hd, tokens, cached, first, last, select = 32, 32, 70, 16 * 4302 + 5, 1, 2, 40
+    pages = cached // 16 + 8
+    assert tokens * nkv > 8 * 256 and cached // 16 - first - last > 4096
+    rng = np.random.default_rng(3)
+    table = rng.permutation(pages).astype(np.int32)[None]
+    q = rng.standard_normal((tokens, nkv, hd)).astype(np.float32)
+    bounds = np.sort(rng.standard_normal((pages, nkv, 2, hd)).astype(np.float16), 2)
+    if equal:
+        bounds[rng.random(pages) < 0.995] = 1
+    put = mxhip.DeviceBuffer.from_array
+    b = [put(x) for x in (np.asarray([0, tokens], np.int32), np.asarray([cached], np.int32), table, bounds, q,
+                          np.full((tokens, nkv, select), LEFT, np.int32))]
+    kv = mxhip.DeviceBuffer(2 * pages * 16 * nkv * hd)  # (no row of it is read)
+    pool = mxhip.KvPool(kv, kv, n_layer=1, n_pages=pages, page_rows=16, n_kv=nkv, head_dim=hd)
+    batch = mxhip.KvBatch(1, tokens, b[0], b[1], b[2], pages)
+    what = mxhip.KvBlocks(b[3], block_rows=16, n_first=first, n_last=last, n_select=select)
+    size = mxhip.kv_select_workspace(pool, batch, what, nkv)
+    work = mxhip.DeviceBuffer(size)
+    mxhip.kv_select_blocks(pool, 0, batch, what, b[4], nkv, b[5], work, size)
+    mxhip.synchronize()
+    got = b[5].download(np.int32).reshape(tokens, nkv, select)
+    least, greatest = bounds[table[0]].astype(np.float64).transpose(2, 1, 3, 0)  # [kv heads, hd, blocks]
+    x = q.astype(np.float64).transpose(1, 0, 2)
+    score = np.maximum(x, 0) @ greatest + np.minimum(x, 0) @ least
+    if equal:  # (blocks of the same bounds: of the first one the score of all, whatever the order of a sum)
+        same = np.flatnonzero((bounds[table[0]] == 1).all((1, 2, 3)))
+        score[:, :, same] = score[:, :, same[:1]]
+    for t in range(tokens):
+        own = (cached + t) // 16
+        rivals = np.arange(first, own + 1 - last)
+        for g in range(nkv):
+            s = score[g, t, rivals]
+            order = np.argsort(-s, kind="stable")
+            k = select - first - last
+            a, z = s[order[k - 1]], s[order[k]]
+            assert a == z or a - z > 2.0**-40 * abs(a), "scores of these inputs lie next to one another"
+            want = [0, *np.sort(rivals[order[:k]]), own - 1, own]
+            assert got[t, g].tolist() == want, (t, g)
+    for y in [*b, kv, work]:
+        y.close()
+
+
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32"])
+@pytest.mark.parametrize("small,large", [(1e-2, 100.0), (1e-5, 1e4), (1e-37, 1e4), (1e33, 1e-6)])
+@pytest.mark.parametrize("tiles", [False, True], ids=["alone", "tiles"])
+def test_small_q_over_large_k(mxh, tiles, heads, small, large):
+    """q outside the range of fp16 halves, over lists of all blocks; every fourth token ordinary."""
+    nh, nkv, hd = HEADS[heads]
+    for seqs, tree in (([(150, 33), (300, 1), (0, 2)], False), ([(0, 30), (400, 20)], True)):
+        tokens = sum(n for _, n in seqs)
+        select = 32 if not tiles else next(s for s in (64, 128, 256, 512, 1024) if in_tiles(tokens, nkv, s, 64))
+        c = Blocks(seqs, block=64, select=select, nh=nh, nkv=nkv, hd=hd, page=64, tree=tree, seed=19, extra_ld=select)
+        assert in_tiles(tokens, nkv, select, 64) == tiles
+        c.chosen[:] = -1
+        c.chosen[..., :8] = np.arange(8)[::-1]
+        c.k = np.clip(c.k.astype(np.float32) * large, -65504, 65504).astype(np.float16)
+        c.q *= np.float32(small)
+        if large > 1:
+            c.q[3::4] /= np.float32(small * large)
+        c.upload()
+        check_precision(c, c.attention())
+        c.close()

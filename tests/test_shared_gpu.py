@@ -17,6 +17,7 @@ import pytest
 
 import mxhip
 from test_graph_capture_gpu import Graph
+from test_paged_edges_gpu import check_precision
 from test_paged_gpu import FILL, HEADS, Case
 
 pytestmark = pytest.mark.gpu
@@ -310,4 +311,60 @@ def test_a_workspace_that_is_too_small_is_refused(mxh):
         c.attend()
     mxhip.synchronize()
     assert np.all(c.bufs["att"].download(np.float32) == FILL)
+    c.close()
+
+
+@pytest.mark.parametrize("groups", [1, 1365, 4096])
+def test_the_most_sequences_and_groups(mxh, groups):
+    """4,096 sequences: the plan's lengths, groups and runs fill their place in LDS."""
+    n = 4096
+    size = n // groups
+    ends = [size * g for g in range(groups)] + [n]
+    rng = np.random.default_rng(groups)
+    seqs = [(16 + int(rng.integers(0, 30)), int(s % 7 != 3)) for s in range(n)]
+    c = Shared(seqs, [(a, b, 16) for a, b in zip(ends, ends[1:])], nh=2, nkv=1, hd=32, page=16, seed=groups)
+    assert len(c.common) == groups and n * c.ld * 16 * 4 * 32 >= 180e6
+    c.upload()
+    c.check(c.attention())
+    c.close()
+
+
+@pytest.mark.parametrize("heads", ["g4-d128", "g3-d64", "g8-d32"])
+@pytest.mark.parametrize("small,large", [(1e-2, 100.0), (1e-5, 1e4), (1e-37, 1e4), (1e33, 1e-6)])
+def test_small_q_over_large_k(mxh, heads, small, large):
+    """q outside the range of fp16 halves, over prefixes and the rows behind them; every fourth token ordinary."""
+    nh, nkv, hd = HEADS[heads]
+    for seqs, tree in (([(130, 1), (150, 1), (128, 1)], False), ([(140, 3), (128, 1), (133, 4)], True),
+                       ([(128, 2 if s else 20) for s in range(12)], False)):
+        c = Shared(seqs, [(0, len(seqs), 128)], nh=nh, nkv=nkv, hd=hd, page=16, tree=tree, seed=19)
+        assert c.tokens * nh // nkv <= 32 * len(seqs)
+        c.k = np.clip(c.k.astype(np.float32) * large, -65504, 65504).astype(np.float16)
+        c.q *= np.float32(small)
+        if large > 1:
+            c.q[3::4] /= np.float32(small * large)
+        c.upload()
+        check_precision(c, c.attention())
+        c.close()
+
+
+@pytest.mark.parametrize("whole", [False, True], ids=["a-row", "all-of-the-prefix"])
+def test_scores_of_minus_infinity_in_the_prefix(mxh, whole):
+    """Nothing of those rows: what is left of the prefix and the rows behind it share the weight."""
+    seqs = [(320, 1), (330, 5), (320, 1)]
+    c = Shared(seqs, [(0, 3, 320)], nh=4, nkv=2, hd=64, page=16, seed=12)
+    gone = range(320) if whole else [100, 319]
+    for r in gone:
+        c.row(c.k, 0, r)[7] = -np.inf  # (kv head 0)
+    q = c.q.reshape(c.tokens, 4, 64)
+    q[:, :2, 7] = np.abs(q[:, :2, 7])
+    c.upload()
+    got = c.attention()
+    for s, (n_c, n) in enumerate(seqs):
+        k, v = (np.array([c.row(x, s, r) for r in range(n_c + n)], np.float64).reshape(-1, 2, 64) for x in (c.k, c.v))
+        for i in range(n):
+            t = int(c.start[s]) + i
+            for h in range(4):
+                sc = k[:n_c + i + 1, h // 2] @ q[t, h].astype(np.float64) / 8
+                p = np.exp(sc - sc.max())
+                assert np.all(np.abs(got[t, h] - p @ v[:n_c + i + 1, h // 2] / p.sum()) <= 1e-4), (s, i, h)
     c.close()
