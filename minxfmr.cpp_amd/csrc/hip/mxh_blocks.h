@@ -33,17 +33,18 @@ inline int64_t block_stages(const BlockSize& a) {
 // all where that makes little work, 46 stages a CU with four for a token's start: in a
 // tile they wait for the union of their lists, and for one another's sequences.  All
 // by themselves and in tiles, us (32/8 heads of 128; work): 40 tokens of two sequences,
-// a stage each 9 and 26 (6); of one sequence 30 of 16 27 and 37 (19), 60 of 16 35 and
-// 44 (38), 100 of 16 65 and 56 (63), 120 of 4 29 and 34 (30), 200 of 3.5 49 and 38 (47),
-// 8 of 100 40 and 39 (26); of 16 sequences up to 8 each of 16 57 and 65 (45), of 4 up to 30
-// 35 and 51 (45).
+// a stage each 9 and 18 (6); of one sequence 30 of 16 24 and 29 (19), 60 of 16 31 and
+// 35 (38), 100 of 16 58 and 45 (63), 120 of 4 27 and 28 (30), 200 of 3.5 46 and 31 (47),
+// 8 of 100 38 and 39 (26); of 16 sequences up to 8 each of 16 56 and 65 (45), of 4 up to 30
+// 32 and 43 (45).
 inline bool block_alone(const BlockSize& a) {
     return a.n_tokens <= 2 * (int64_t)a.n_seq ||
            (int64_t)a.n_tokens * a.nkv * (block_stages(a) + 4) <= 46 * (int64_t)a.cus;
 }
 // 32 rows where sequences have tokens enough and lists and bits leave room for them: 512
 // tokens with 32 of 469 blocks of 64 rows each, of which four tokens together have
-// some 63 and eight some 82 (32/8 heads of 128), 121 us, in tiles of 16 rows 129.
+// some 63 and eight some 82 (32/8 heads of 128), 114 us, in tiles of 16 rows 126; 100 of
+// them 45 and 43, 200 tokens with 7 blocks 31 and 21.
 inline int block_tokens_of(const BlockSize& a, int rows) {
     const int64_t words = (a.n_blocks + 31) / 32;
     return (int)std::max<int64_t>(

@@ -758,7 +758,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_blocks_kernel(BlockAttn
         it.st0 = stages * (uint32_t)z / (uint32_t)a.splits, it.st1 = stages * (uint32_t)(z + 1) / (uint32_t)a.splits;
         it.slot = a.splits > 1 ? (int)index : -1;
         it.row0 = (uint32_t)(t - first) * a.t.group;
-        attend_tile<HD, R, kListed>(a.t, it, g, tid, wave, a.once, smem);
+        attend_tile<HD, R, kListed>(a.t, it, g, a.once, smem);
         t += n;
         if (t < last) __syncthreads();
     }
@@ -819,7 +819,7 @@ int launch_rows(const BlockAttnArgs& a, int64_t tiles, hipStream_t st) {
                        dim3((unsigned)a.t.pg.nkv, (unsigned)y, (unsigned)((items + y - 1) / y)), dim3(kThreads), lds, st,
                        args);
     if (a.splits > 1) {
-        const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4);
+        const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh() * (HD / 4);
         const BlockMergeArgs m{a.t.part, a.t.ml, a.t.att, total, a.t.pg.nkv, (int)a.t.group, (int)a.t.tokens, a.splits, R};
         hipLaunchKernelGGL(blocks_merge_kernel<HD>, dim3((unsigned)((total + kMergeUnits - 1) / kMergeUnits)),
                            dim3(kJoinThreads), 0, st, m);
@@ -920,7 +920,7 @@ int attention_blocks_launch(const PagedArgs& pg, const BlocksOf& b, const int* c
     // with 1,280 rows for each of 8 kv heads of 128 53 us, 47 so
     const bool once = pg.n_tokens <= 2 * (int64_t)pg.n_seq && (double)pg.n_tokens * pg.nkv * b.n_select * size.block_rows * hd * 4 > 128e6;
     const BlockAttnArgs a{{pg, q, att, part, reinterpret_cast<float2*>(part + (size_t)tiles * splits * pg.nkv * block_rows_of_tile(size) * hd),
-                           nh, 1.4426950408889634f / sqrtf((float)hd), group, (uint32_t)block_tokens(size),
+                           1.4426950408889634f / sqrtf((float)hd), group, (uint32_t)block_tokens(size),
                            (65536 + group - 1) / group},
                           chosen, b.n_select, b.block_shift, ba.n_blocks, splits, (ba.n_blocks + 31) / 32, once, 0};
     const int rows = block_rows_of_tile(size);

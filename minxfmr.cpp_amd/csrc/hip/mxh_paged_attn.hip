@@ -117,7 +117,7 @@ __device__ __forceinline__ uint32_t item_index() { return blockIdx.y + gridDim.y
 //   us (263 to 270 card to card) = 464 TFLOP/s of the formula's, 930 of the products
 //   made (a large fp16 product 1,184); matrix cores and vector units half busy
 //   each, and neither fewer reads nor fewer exponentials made it faster by more
-//   than 4%.  27 drafted tokens at 8,192 rows 24.8 us: 8 stages an item 12 of them
+//   than 4%.  27 drafted tokens at 8,192 rows 24.4 us: 8 stages an item 12 of them
 //   (a stage's loads are one stage ahead and HBM is 1.4 us away), what comes before
 //   and after an item's stages 8, the second kernel 4.
 // Many sequences: every workgroup plans for itself, so 1,024 single tokens at up to
@@ -125,7 +125,6 @@ __device__ __forceinline__ uint32_t item_index() { return blockIdx.y + gridDim.y
 template <int HD, int R>
 __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedArgs a) {
     extern __shared__ __align__(256) uint8_t smem[];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const uint32_t nkv = (uint32_t)a.pg.nkv, group = a.group, T = a.tokens;
     const uint32_t index = item_index(), g = blockIdx.x;
     const Plan plan(a.pg, R, T, a.target);
@@ -141,8 +140,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     Segment it;
     it.s = plan.find(r_unit, seq);
     for (;;) {
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));  // (else what follows from it is kept in registers from tile to tile)
         {
             const Plan::Spot spot = plan.spot(seq, r_unit);
             const PagedPiece p = plan.piece(seq, spot, x1 - x, index);
@@ -157,7 +154,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
         if (it.st0 < it.st1 || it.slot < 0) {  // (else only units of the lead)
             const bool unshared =
                 seq.tiles == 1 && (float)plan.all * (float)(stage_keys(R) * 4 * HD) * (float)nkv > 256e6f;
-            attend_tile<HD, R, kSequence>(a, it, g, tid, wave, unshared, smem);
+            attend_tile<HD, R, kSequence>(a, it, g, unshared, smem);
         }
         if (x >= x1) return;
         // the item's next tile
@@ -223,7 +220,7 @@ __global__ __launch_bounds__(kMergeThreads) void attention_paged_merge_kernel(At
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     const uint32_t tl = a.over_group((uint32_t)row);
     const size_t tok = (size_t)cut.x + tl;
-    *reinterpret_cast<float4*>(a.att + (tok * a.nh + g * group + ((uint32_t)row - tl * group)) * HD + d) =
+    *reinterpret_cast<float4*>(a.att + (tok * a.nh() + g * group + ((uint32_t)row - tl * group)) * HD + d) =
         make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
 
@@ -269,7 +266,7 @@ int attention_paged_launch(const PagedArgs& a, const float* q, int nh, int hd, f
     float2* ml = reinterpret_cast<float2*>(part + (size_t)2 * s.target * a.nkv * s.rows * hd);
     const uint32_t group = (uint32_t)(nh / a.nkv);
     int4* cuts = reinterpret_cast<int4*>(ml + (size_t)2 * s.target * a.nkv * s.rows);
-    const AttnPagedArgs args{{a, q, att, part, ml, nh, 1.4426950408889634f / sqrtf((float)hd), group,
+    const AttnPagedArgs args{{a, q, att, part, ml, 1.4426950408889634f / sqrtf((float)hd), group,
                               (uint32_t)s.rows / group, (65536 + group - 1) / group},
                              cuts,
                              s.target};

@@ -122,10 +122,12 @@ struct TileArgs {
     float* att;
     float* part;  // [slots][nkv][R][HD]: V sums of the parts of tiles
     float2* ml;   // [slots][nkv][R]: references and sums
-    int nh;
     float qscale;
     uint32_t group, tokens;  // q heads of a kv head; tokens of a tile, R / group
     uint32_t group_inv;      // 2^16 / group rounded up
+    // (not kept: what a kernel adds begins within the arguments' first 128 bytes so, 0.2
+    // us of the 24.4 that 27 drafted tokens at 8,192 rows take)
+    __host__ __device__ __forceinline__ int nh() const { return pg.nkv * (int)group; }
     // r / group for r up to 64
     __device__ __forceinline__ uint32_t over_group(uint32_t r) const { return (r * group_inv) >> 16; }
 };
@@ -199,7 +201,7 @@ __device__ void redo_item(const TileArgs& a, const Seg& it, int g, int key0, int
         const int tl = (int)a.over_group((uint32_t)r), i = i0 + tl, hq = g * group + r - tl * group;
         const int tok = (int)it.first + i, cached = (int)it.cached;
         const uint64_t path = path_of(paths, i & 63);
-        const float* q = a.q + ((size_t)tok * a.nh + hq) * HD;
+        const float* q = a.q + ((size_t)tok * a.nh() + hq) * HD;
         for (int d = lane; d < HD; d += 64) qs[d] = q[d] * a.qscale;
         settle();
         float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
@@ -240,7 +242,7 @@ __device__ void redo_item(const TileArgs& a, const Seg& it, int g, int key0, int
             }
             settle();
         }
-        float* out = a.att + ((size_t)tok * a.nh + hq) * HD;
+        float* out = a.att + ((size_t)tok * a.nh() + hq) * HD;
         float inv = l == 0.f ? 0.f : 1.0f / l;
         if (it.slot >= 0) {
             const size_t p = ((size_t)it.slot * a.pg.nkv + g) * R + part_row<KEYS>(it, r);
@@ -330,8 +332,14 @@ __device__ __forceinline__ float inverse_power(float x) { return __uint_as_float
 // as part it.slot, into the workspace.  unshared: the rows are more than the last
 // cache holds and the sequence has no other tile.
 template <int HD, int R, Keys KEYS, class Seg>
-__device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, uint32_t g, int tid, int wave,
-                                            bool unshared, uint8_t* smem) {
+__device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, uint32_t g, bool unshared,
+                                            uint8_t* smem) {
+    // (the thread and the wave found here: what follows from the caller's is kept in
+    // registers beside the tile and from tile to tile.  27 drafted tokens at 8,192 rows
+    // 24.6 us, with the caller's 24.9; lists with R = 32 7 registers spilled and 40)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     constexpr int M = R == 16 ? 16 : 32, RS = R / M;  // rows of a wave; waves to a key group
     constexpr int KS = HD * M / 512, DB = HD / M;     // products of a score and of a sum
     constexpr int SB = 32 / M, NA = M * M / 64;       // score blocks of 32 keys, accumulators of one
@@ -370,7 +378,7 @@ __device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, ui
     const uint32_t row = 32 * set + n, tl = a.over_group(row);
     const bool valid = (int)tl < ntok;  // (the others: zeros at the tile's first token)
     const int i = i0 + (valid ? (int)tl : 0);
-    const size_t qd = (size_t)a.nh * HD;
+    const size_t qd = (size_t)a.nh() * HD;
     const float* q0 = a.q + (size_t)(it.first + i0) * qd + g * group * HD;  // the tile's rows
     float4 qv[KS][2];
     if constexpr (PRIVATE) {  // (few rows: their loads go first, those of K and V come back after them)
@@ -902,7 +910,7 @@ __device__ __forceinline__ void attend_tile(const TileArgs& a, const Seg& it, ui
         } else {
             const float inv = ll == 0.f ? 0.f : 1.0f / ll;  // (no row exists: zeros)
             const int rt = (int)a.over_group((uint32_t)rr);
-            const size_t head = (size_t)(it.first + i0 + rt) * a.nh + g * group + (rr - rt * (int)group);
+            const size_t head = (size_t)(it.first + i0 + rt) * a.nh() + g * group + (rr - rt * (int)group);
             *reinterpret_cast<float4*>(a.att + head * HD + d) =
                 make_float4(x4.x * inv, x4.y * inv, x4.z * inv, x4.w * inv);
         }

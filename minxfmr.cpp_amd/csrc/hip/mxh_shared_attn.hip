@@ -206,7 +206,7 @@ struct SharedArgs {
 template <int HD, int RP, int RS>
 __global__ __launch_bounds__(kThreads, 2) void attention_shared_kernel(SharedArgs a) {
     extern __shared__ __align__(256) uint8_t smem[];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), tid = threadIdx.x;
+    const int tid = threadIdx.x;
     const uint32_t index = blockIdx.y + gridDim.y * blockIdx.z, g = blockIdx.x;
     const int2 counts = *a.counts;
     if (index >= (uint32_t)counts.y) return;
@@ -228,10 +228,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_shared_kernel(SharedArg
             }
     }
     if (is_prefix) {
-        attend_tile<HD, RP, kPrefix>(t, it, g, tid, wave, false, smem);
+        attend_tile<HD, RP, kPrefix>(t, it, g, false, smem);
     } else {
         t.part = a.part_s, t.ml = a.ml_s;
-        attend_tile<HD, RS, kOwnRows>(t, it, g, tid, wave, false, smem);
+        attend_tile<HD, RS, kOwnRows>(t, it, g, false, smem);
     }
 }
 
@@ -291,7 +291,7 @@ int launch_hd(const SharedArgs& a, const SharedShape& sh, hipStream_t st) {
                    : sh.rows_p == 64 ? launch<HD, 64, 16>(a, sh, st)
                                      : launch<HD, 16, 16>(a, sh, st);
     if (rc) return rc;
-    const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh * (HD / 4);
+    const int64_t total = (int64_t)a.t.pg.n_tokens * a.t.nh() * (HD / 4);
     const int lanes = join_lanes(total, device_cus());
     const dim3 grid((unsigned)((total + kJoinThreads / lanes - 1) / (kJoinThreads / lanes)));
     const SharedMergeArgs m{a.records, a.t.part, a.part_s, a.t.ml, a.ml_s, a.t.att, total, a.t.pg.nkv,
@@ -339,7 +339,7 @@ int attention_shared_launch(const PagedArgs& a, int n_groups, const int* group_s
     hipLaunchKernelGGL(shared_plan_kernel, dim3(1 + ((unsigned)a.n_tokens + threads - 1) / threads), dim3(threads),
                        plan_lds(a.n_seq, n_groups), st, plan);
     const SharedArgs args{{a, q, att, reinterpret_cast<float*>(at + w.part_p), reinterpret_cast<float2*>(at + w.ml_p),
-                           nh, 1.4426950408889634f / sqrtf((float)hd), group, 0, (65536 + group - 1) / group},
+                           1.4426950408889634f / sqrtf((float)hd), group, 0, (65536 + group - 1) / group},
                           reinterpret_cast<float*>(at + w.part_s),
                           reinterpret_cast<float2*>(at + w.ml_s),
                           plan.counts,
