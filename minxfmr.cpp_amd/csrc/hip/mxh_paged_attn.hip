@@ -117,7 +117,7 @@ __device__ __forceinline__ uint32_t item_index() { return blockIdx.y + gridDim.y
 //   us (263 to 270 card to card) = 464 TFLOP/s of the formula's, 930 of the products
 //   made (a large fp16 product 1,184); matrix cores and vector units half busy
 //   each, and neither fewer reads nor fewer exponentials made it faster by more
-//   than 4%.  27 drafted tokens at 8,192 rows 24.4 us: 8 stages an item 12 of them
+//   than 4%.  27 drafted tokens at 8,192 rows 24.2 us: 8 stages an item 12 of them
 //   (a stage's loads are one stage ahead and HBM is 1.4 us away), what comes before
 //   and after an item's stages 8, the second kernel 4.
 // Many sequences: every workgroup plans for itself, so 1,024 single tokens at up to
@@ -129,9 +129,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     const uint32_t index = item_index(), g = blockIdx.x;
     const Plan plan(a.pg, R, T, a.target);
     uint32_t x = plan.first_unit(index);
-    const bool tells = g == 0 && threadIdx.x == 0 && index < (uint32_t)a.target;  // (for the second kernel)
+    const bool tells = g == 0 && index < (uint32_t)a.target;  // (the second kernel; thread 0)
     if (x >= plan.total) {
-        if (tells) a.cuts[index] = make_int4(0, 0, 0, 0);
+        if (tells && threadIdx.x == 0) a.cuts[index] = make_int4(0, 0, 0, 0);
         return;
     }
     const uint32_t x0 = x, x1 = min(x + plan.per, plan.total);
@@ -140,12 +140,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_kernel(AttnPagedA
     Segment it;
     it.s = plan.find(r_unit, seq);
     for (;;) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // (as in attend_tile)
         {
             const Plan::Spot spot = plan.spot(seq, r_unit);
             const PagedPiece p = plan.piece(seq, spot, x1 - x, index);
             it.first = seq.first, it.n = seq.n, it.cached = seq.cached;
             it.tile = p.tile, it.st0 = p.st0, it.st1 = p.st1, it.slot = p.slot;
-            if (tells && x == x0) {
+            if (tells && tid == 0 && x == x0) {
                 const int i0 = (int)(spot.tile * T), rows = min((int)T, (int)seq.n - i0) * (int)group;
                 a.cuts[index] = make_int4((int)seq.first + i0, rows, (int)plan.parts(spot), 0);
             }

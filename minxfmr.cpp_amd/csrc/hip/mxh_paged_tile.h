@@ -126,7 +126,7 @@ struct TileArgs {
     uint32_t group, tokens;  // q heads of a kv head; tokens of a tile, R / group
     uint32_t group_inv;      // 2^16 / group rounded up
     // (not kept: what a kernel adds begins within the arguments' first 128 bytes so, 0.2
-    // us of the 24.4 that 27 drafted tokens at 8,192 rows take)
+    // us of the 24.2 that 27 drafted tokens at 8,192 rows take)
     __host__ __device__ __forceinline__ int nh() const { return pg.nkv * (int)group; }
     // r / group for r up to 64
     __device__ __forceinline__ uint32_t over_group(uint32_t r) const { return (r * group_inv) >> 16; }
