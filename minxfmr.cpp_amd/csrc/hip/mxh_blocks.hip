@@ -560,7 +560,7 @@ __global__ __launch_bounds__(THREADS, 8) void block_pick_kernel(SelectArgs a) {
         }
         __syncthreads();
         // bins from the top, two a thread
-            const uint32_t c0 = bins[BINS - 1 - 2 * tid], c1 = bins[BINS - 2 - 2 * tid];
+        const uint32_t c0 = bins[BINS - 1 - 2 * tid], c1 = bins[BINS - 2 - 2 * tid];
         const uint32_t upto = inclusive(c0 + c1), before = upto - c0 - c1, w = (uint32_t)want;
         if (tid == 0) found[0] = 0xffffffffu;
         __syncthreads();

@@ -5,8 +5,8 @@
 //
 // A tile is T = R / group consecutive tokens of one sequence with the group =
 // nh / nkv q heads of one kv head (row r: token r / group, head r % group), R =
-// 16 or 64 rows, and a stage 128 or 64 keys.  (R = 32 goes as 16 does, with the
-// products of 64.)
+// 16, 32 (lists alone) or 64 rows, and a stage 128 keys, with R = 64 half as many.
+// R = 32 goes as 16 does, with the products of 64.
 //
 // K and V rows go straight into LDS (16 rows of a page are evenly spaced, so
 // their addresses are a scalar base and fixed lane offsets).  Per 32-key block

@@ -13,16 +13,25 @@ namespace mxh {
 // Whether prefixes are read apart, from what the host knows: as long as the table
 // allows, the batch's K and V rows, and the rows of q that a sequence has on average.
 // Read with the sequences' own rows, a prefix comes out of the caches for all but the
-// first of them; read apart, it takes a plan, a third kernel and 10 us more.  And
-// where a sequence fills a tile of 64 rows its tiles are bound by their products.
-// 32/8 heads of 128 (4 KB of K and V a row), apart and not, us:
+// first of them; read apart, it takes a plan, a third kernel and 10 us more.
+// Apart and not, us, 32/8 heads of 128 (4 KB of K and V a row):
 //   single tokens: 4 at 1,200 rows 17 and 11, 8 at 4,500 25 and 21, 12 at 2,200 21.3
 //   and 19.5, 6 at 8,200 25.7 and 25.1 (200 MB), 32 at 1,200 22.3 and 22.8 (160 MB), 24
 //   at 2,200 23 and 25 (220 MB), 16 at 4,500 26 and 31, 64 at 8,200 (2 GB) and of their
 //   own up to 1,000 60 and 158
 //   up to 4 tokens each (12 rows of q): 12 at 6,300 30 and 34, 30 45 and 65
-//   up to 16 (43 rows): 12 at 6,300 49 and 51, 30 100 and 102; up to 64 and 128: 30
-//   at 6,300 289 and 279, 503 and 527
+//   More rows of q are not read apart, where it takes from a quarter less time to a
+//   third more, by how the tiles happen to fill.  Up to 16 (39 rows): 12 at 6,300 49 and
+//   53, 30 100 and 102; up to 33 (81): 80 and 84, 181 and 178; up to 64 (152): 116 and
+//   153, 302 and 293, 12 at 16,300 257 and 294; up to 90 (204): 176 and 169, 328 and 364;
+//   up to 128: 208 and 200, 503 and 527, but 30 at 1,300 (170 MB) 166 and 125
+// 16/8 heads of 128: 12 of up to 16 (20 rows of q) at 6,300 36 and 47, 30 71 and 96; 16
+// drafted trees of up to 13 at 3,200 (210 MB) 29 and 35, at 16,300 57 and 135, of up to
+// 33 (39 rows, not read apart) 124 and 157.
+// Heads of 64, 6/2 (512 bytes a row): 64 single tokens at 9,000 (300 MB) 27 and 39, at
+// 4,500 (150) 23 and 24, 16 at 16,500 (135) 32 and 24; 16 trees of up to 13 at 3,200
+// (26) 21 and 17, at 16,300 (134) 29 and 33.  Of 32, 8/1 (128 bytes): 64 at 31,000 (250
+// MB) 31 and 51, at 17,000 (140) 27 and 32, at 9,000 (74) 23 and 21.
 constexpr int kSharedRows = 32;         // rows of q of a sequence, on average, at most
 constexpr double kSharedBytes = 180e6;  // of K and V at least
 inline bool shared_pays(const PagedSize& a, int hd, int n_groups) {
