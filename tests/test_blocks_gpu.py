@@ -914,3 +914,55 @@ def test_small_q_over_large_k(mxh, tiles, heads, small, large):
         c.upload()
         check_precision(c, c.attention())
         c.close()
+
+
+def test_lists_and_attention_in_a_layer_of_strided_pools(mxh):
+    c = Blocks([(170, 3), (210, 40), (64, 1)], block=16, select=6, nh=12, nkv=6, hd=64, page=32, layers=3, layer=1,
+               stride=24, seed=5)
+    c.fill_bounds()
+    dense = int(np.prod(c.shape[1:]))
+    c.upload()
+    wide = np.full((3, dense + 40), np.nan, np.float16)
+    wide[1, :dense] = c.bounds[1].reshape(-1)
+    b = mxhip.DeviceBuffer.from_array(wide)
+    c.what = mxhip.KvBlocks(b, block_rows=16, n_first=1, n_last=2, n_select=6, layer_stride=dense + 40)
+    c.choose()
+    got = c.got_chosen()
+    c.check_chosen(got)
+    c.check_listed(c.attention(), got)
+    b.close()
+    c.close()
+
+
+@pytest.mark.parametrize("block", [16, 1024])
+def test_the_largest_pages(mxh, block):
+    c = Blocks([(5000, 1), (1500, 20), (1023, 2), (9000, 1)], block=block, first=1, last=1, select=3, nh=8, nkv=2, hd=64,
+               page=1024, seed=3, lead=1, tail=1)
+    c.upload()
+    c.find_bounds()
+    c.check_bounds(c.got_bounds())
+    c.fill_bounds()
+    c.upload()
+    c.choose()
+    got = c.got_chosen()
+    c.check_chosen(got)
+    c.check_listed(c.attention(), got)
+    c.close()
+
+
+@pytest.mark.parametrize("select", [6, 300])
+def test_drafted_trees_end_at_64_tokens(mxh, select):
+    seqs = [(300, 70), (200, 90), (100, 2)]
+    c = Blocks(seqs, block=16, select=select, nh=16, nkv=8, hd=32, page=32, tree=True, seed=7, extra_ld=150)
+    assert in_tiles(c.tokens, c.nkv, select, 16) == (select == 300)
+    c.fill_bounds()
+    c.upload()
+    c.choose()
+    got = c.got_chosen()
+    c.check_chosen(got)
+    att = c.attention()
+    past = [int(c.start[s]) + i for s, (_, n) in enumerate(seqs) for i in range(64, n)]
+    assert np.all(att[past] == FILL) and np.all(got[past] == LEFT)
+    att[past] = 0
+    c.check_listed(att, got, rows=set(range(c.tokens)) - set(past))
+    c.close()

@@ -368,3 +368,16 @@ def test_scores_of_minus_infinity_in_the_prefix(mxh, whole):
                 p = np.exp(sc - sc.max())
                 assert np.all(np.abs(got[t, h] - p @ v[:n_c + i + 1, h // 2] / p.sum()) <= 1e-4), (s, i, h)
     c.close()
+
+
+def test_drafted_trees_end_at_64_tokens(mxh):
+    seqs = [(128, 70), (130, 3)] + [(128 + s, 1) for s in range(20)]
+    c = Shared(seqs, [(0, 22, 128)], nh=8, nkv=2, hd=64, page=16, tree=True, seed=7)
+    assert c.tokens * 4 <= 32 * len(seqs)
+    c.upload()
+    got = c.attention()
+    past = list(range(64, 70))
+    assert np.all(got[past] == FILL)
+    got[past] = 0
+    c.check(got, rows=set(range(c.tokens)) - set(past))
+    c.close()
